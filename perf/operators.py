@@ -7,7 +7,8 @@ elementary torch operations in 32 bits, rounded once at the end.  Where it is
 true, ``run`` makes the calls a program makes of the ``busfill`` package.
 ``exact`` computes the same outputs from the definitions in 64 bits.
 
-Sizes are the repository's own (5120 wide, 7168 = 5120 + 2 * 1024 for a layer's
+Attention's and the experts' outputs are the fp16 rows that the next linear
+takes.  Sizes are the repository's own (5120 wide, 7168 = 5120 + 2 * 1024 for a layer's
 query, key and value projections, i.e. 40 query heads over 8 key/value heads of
 128; batches of 1, 8, 32; 2000-token prompts) or generic ones.
 """
@@ -35,19 +36,19 @@ def listed():
         {"name": "store_prompt_2000", "kind": "store", "T": 2000, "H": 8, "D": 128, "start": 37, "whole": True},
         # one stream early in its answer: the smallest call, where latency counts
         {"name": "attn_decode_1x519", "kind": "attn", "S": 1, "nq": 1, "kv": 519, "spread": False, "Hq": 40, "H": 8,
-         "D": 128, "window": 0, "out": "f16"},
+         "D": 128, "window": 0},
         # 32 concurrent streams of ragged lengths up to 8000 tokens
         {"name": "attn_decode_32x8000", "kind": "attn", "S": 32, "nq": 1, "kv": 8000, "spread": True, "Hq": 40, "H": 8,
-         "D": 128, "window": 0, "out": "f16"},
+         "D": 128, "window": 0},
         # one stream with a long document
         {"name": "attn_decode_1x131072", "kind": "attn", "S": 1, "nq": 1, "kv": 131072, "spread": False, "Hq": 32,
-         "H": 4, "D": 128, "window": 0, "out": "f16"},
+         "H": 4, "D": 128, "window": 0},
         # four drafted tokens a stream checked at once, a model with heads of 64 and a sliding window
         {"name": "attn_draft_8x4_window", "kind": "attn", "S": 8, "nq": 4, "kv": 4099, "spread": True, "Hq": 16, "H": 8,
-         "D": 64, "window": 1024, "out": "f32"},
+         "D": 64, "window": 1024},
         # a 2000-token prompt over the cache that holds it
         {"name": "attn_prompt_2000", "kind": "attn", "S": 1, "nq": 2000, "kv": 2000, "spread": False, "Hq": 40, "H": 8,
-         "D": 128, "window": 0, "out": "f16"},
+         "D": 128, "window": 0},
         # a decode step's routing: softmax scores, eight of 64
         {"name": "route_decode_32", "kind": "route", "T": 32, "E": 64, "k": 8, "score": "softmax", "biased": False,
          "groups": 1, "top": 1, "renorm": True, "factor": 1.0, "logits": "f32"},
@@ -55,14 +56,12 @@ def listed():
         {"name": "route_prompt_4096", "kind": "route", "T": 4096, "E": 256, "k": 8, "score": "sigmoid", "biased": True,
          "groups": 8, "top": 4, "renorm": True, "factor": 2.5, "logits": "f32"},
         # the experts' block for one token
-        {"name": "experts_m1", "kind": "experts", "fmt": "q4_k", "T": 1, "E": 64, "k": 8, "K": 2048, "F": 1024,
-         "out": "f32"},
+        {"name": "experts_m1", "kind": "experts", "fmt": "q4_k", "T": 1, "E": 64, "k": 8, "K": 2048, "F": 1024},
         # 32 streams, nearly every expert in use
-        {"name": "experts_m32", "kind": "experts", "fmt": "q4_k", "T": 32, "E": 64, "k": 8, "K": 5120, "F": 1280,
-         "out": "f32"},
+        {"name": "experts_m32", "kind": "experts", "fmt": "q4_k", "T": 32, "E": 64, "k": 8, "K": 5120, "F": 1280},
         # a 2000-token prompt, about 250 rows an expert
         {"name": "experts_prompt_2000", "kind": "experts", "fmt": "q4_0", "T": 2000, "E": 64, "k": 8, "K": 4096,
-         "F": 1792, "out": "f16"},
+         "F": 1792},
     ]
 
 
@@ -86,7 +85,6 @@ def draw(rng):
     if kind in ("attn", "prompt"):
         group = rng.choice([1, 2, 4, 5, 8, 16])
         window = rng.choice([0, 0, 0, rng.randint(16, 2048)])
-        out = rng.choice(["f16", "f16", "f32"])
         if kind == "prompt":
             h = min(h, max(1, 40 // group))
             nq = _log(rng, 17, min(2000, math.isqrt(2 * MOST_PAIRS // (group * h * d))))
@@ -99,7 +97,7 @@ def draw(rng):
             nq, s = rng.choice([1, 1, 1, 1, 2, 4, 7]), _log(rng, 1, 64)
             kv = _log(rng, max(nq, 16), min(131072, MOST_CACHED // (s * h * d)))
         return {"kind": "attn", "S": s, "nq": nq, "kv": kv, "spread": s > 1, "Hq": group * h, "H": h, "D": d,
-                "window": window, "out": out}
+                "window": window}
     if kind == "route":
         score = rng.choice(["softmax", "sigmoid"])
         groups = rng.choice([1, 1, 4, 8])
@@ -117,7 +115,7 @@ def draw(rng):
         e //= 2
     k = min(k, e)
     return {"kind": "experts", "fmt": fmt, "T": max(1, min(t, MOST_EXPERT // (k * width * f))), "E": e, "k": k,
-            "K": width, "F": f, "out": rng.choice(["f32", "f16"])}
+            "K": width, "F": f}
 
 
 # ------------------------------------------------------------------ inputs
@@ -329,27 +327,23 @@ def _plain_store(s):
 
 def _plain_attn(s):
     c = s["case"]
-    nq, hq, h, d = c["nq"], c["Hq"], c["H"], c["D"]
-    r = hq // h
-    out, at = [], 0
-    for i, n in enumerate(_lens(c)):
-        lo = 0 if not c["window"] else max(0, n - nq - c["window"] + 1)
-        rows = slice(at + lo, at + n)
-        k = _unpack(s["kq"][rows], s["kd"][rows]).transpose(0, 1)                # [H][n][D]
-        v = _unpack(s["vq"][rows], s["vd"][rows]).transpose(0, 1)
-        q = s["q"][i * nq:(i + 1) * nq].float().reshape(nq, h, r, d).permute(1, 2, 0, 3).reshape(h, r * nq, d)
-        x = torch.matmul(q, k.transpose(1, 2)).mul_(s["scale"]).reshape(h, r, nq, n - lo)
-        t = torch.arange(lo, n, device=DEV)[None, :]
-        p = torch.arange(n - nq, n, device=DEV)[:, None]
-        hide = t > p
-        if c["window"]:
-            hide = hide | (t <= p - c["window"])
-        x = x.masked_fill_(hide, float("-inf"))
-        x = torch.exp(x - x.amax(-1, keepdim=True))
-        o = torch.matmul(x.reshape(h, r * nq, n - lo), v) / x.reshape(h, r * nq, n - lo).sum(-1, keepdim=True)
-        out.append(o.reshape(h, r, nq, d).permute(2, 0, 1, 3).reshape(nq, hq, d))
-        at += n
-    return torch.cat(out).to(s["otype"])
+    n, nq, hq, h, d = c["S"], c["nq"], c["Hq"], c["H"], c["D"]
+    r, most = hq // h, max(_reached(c))
+    lens, first, seen = s["lens"][:, None], s["first"][:, None], torch.arange(most, device=DEV)
+    t = torch.clamp(lens - c["nq"] - c["window"] + 1, min=0) + seen if c["window"] else seen.expand(n, most)   # positions
+    at = first + torch.minimum(t, lens - 1)
+    k = _unpack(s["kq"][at], s["kd"][at]).transpose(1, 2)                        # [S][H][most][D]
+    v = _unpack(s["vq"][at], s["vd"][at]).transpose(1, 2)
+    q = s["q"].float().reshape(n, nq, h, r, d).permute(0, 2, 3, 1, 4).reshape(n, h, r * nq, d)
+    x = torch.matmul(q, k.transpose(2, 3)).mul_(s["scale"]).reshape(n, h, r, nq, most)
+    p = (lens - nq + torch.arange(nq, device=DEV))[:, :, None]                   # the queries' positions
+    hide = t[:, None, :] > p
+    if c["window"]:
+        hide = hide | (t[:, None, :] <= p - c["window"])
+    x = x.masked_fill_(hide[:, None, None], float("-inf"))
+    x = torch.exp(x - x.amax(-1, keepdim=True)).reshape(n, h, r * nq, most)
+    o = torch.matmul(x, v) / x.sum(-1, keepdim=True)
+    return o.reshape(n, h, r, nq, d).permute(0, 3, 1, 2, 4).reshape(n * nq, hq, d).to(torch.float16)
 
 
 def _plain_route(s):
@@ -401,17 +395,27 @@ def _expert(ws, i, e, n):
 
 
 def _plain_experts(s):
+    """All experts in use at once: their weights decoded, their rows side by side, padded to the longest list."""
     c = s["case"]
     t, k, width, f, fmt = c["T"], c["k"], c["K"], c["F"], c["fmt"]
-    x, ids = s["x"].float(), s["ids"]
-    y = torch.zeros(t, k, width, dtype=torch.float32, device=DEV)
-    for e in torch.unique(ids).tolist():
-        row, j = torch.nonzero(ids == e, as_tuple=True)
-        a = x[row]
-        g = a @ _dequant(fmt, *_expert(s["ws"], 0, e, f), f, width).t()
-        u = a @ _dequant(fmt, *_expert(s["ws"], 1, e, f), f, width).t()
-        y[row, j] = (g / (1 + torch.exp(-g)) * u) @ _dequant(fmt, *_expert(s["ws"], 2, e, width), width, f).t()
-    return (y * s["w"][..., None]).sum(1).to(_dtype(c))
+    used, which = torch.unique(s["ids"], return_inverse=True)
+    which, n = which.reshape(-1), used.numel()
+    order = torch.sort(which, stable=True).indices
+    count = torch.bincount(which, minlength=n)
+    place = torch.empty_like(which)
+    place[order] = torch.arange(t * k, device=DEV) - (torch.cumsum(count, 0) - count)[which[order]]
+    a = torch.zeros(n, int(count.max()), width, dtype=torch.float32, device=DEV)
+    a[which, place] = s["x"].float().repeat_interleave(k, 0)
+
+    def linear(x, i, rows, cols):
+        w, aux = s["ws"][i]
+        w = w.reshape(c["E"], rows, -1)[used].reshape(n * rows, -1)
+        aux = None if aux is None else aux.reshape(c["E"], rows, -1)[used].reshape(n * rows, -1)
+        return torch.matmul(x, _dequant(fmt, w, aux, n * rows, cols).reshape(n, rows, cols).transpose(1, 2))
+
+    g = linear(a, 0, f, width)
+    y = linear(g / (1 + torch.exp(-g)) * linear(a, 1, f, width), 2, width, f)
+    return (y[which, place].reshape(t, k, width) * s["w"][..., None]).sum(1).to(torch.float16)
 
 
 # ------------------------------------------------------------------ the four parts that are measured
@@ -423,10 +427,6 @@ def _package():
         sys.path.insert(0, path)
     import busfill
     return busfill
-
-
-def _dtype(case):
-    return torch.float16 if case["out"] == "f16" else torch.float32
 
 
 def prepare(case, seed):
@@ -441,16 +441,17 @@ def prepare(case, seed):
             s["out"] = [torch.empty_like(s["k"]), torch.empty_like(s["v"])]
     elif case["kind"] == "attn":
         g, lens, s["q"], k, v = _attn_inputs(case, seed)
-        s["scale"], s["otype"] = 1 / math.sqrt(case["D"]), _dtype(case)
+        s["scale"] = 1 / math.sqrt(case["D"])
+        s["lens"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
         if own:
             s["table"], slots, pages = _pages(case, g)
             s["data"] = torch.zeros(bf.kv4_bytes(pages, PAGE, case["H"], case["D"]), dtype=torch.uint8, device=DEV)
             s["cache"] = bf.kv4_cache(s["data"], pages, PAGE, case["H"], case["D"])
             bf.kv4_store(s["cache"], k, v, slots, sum(lens))
-            s["lens"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
             s["starts"] = torch.arange(0, (case["S"] + 1) * case["nq"], case["nq"], dtype=torch.int32, device=DEV)
-            s["o"] = torch.empty(s["q"].shape, dtype=s["otype"], device=DEV)
+            s["o"] = torch.empty(s["q"].shape, dtype=torch.float16, device=DEV)
         else:
+            s["first"] = torch.cumsum(s["lens"], 0) - s["lens"]
             (s["kq"], s["kd"]), (s["vq"], s["vd"]) = _pack(k), _pack(v)
     elif case["kind"] == "route":
         s["x"], s["bias"] = _logits(case, _gen(seed))
@@ -460,7 +461,7 @@ def prepare(case, seed):
     else:
         s["ws"], s["x"], s["ids"], s["w"] = _expert_inputs(case, _gen(seed))
         if own:
-            s["y"] = torch.empty(case["T"], case["K"], dtype=_dtype(case), device=DEV)
+            s["y"] = torch.empty(case["T"], case["K"], dtype=torch.float16, device=DEV)
     return s
 
 
@@ -482,7 +483,7 @@ def run(s):
     if kind == "attn":
         bf.kv4_attention(s["cache"], s["q"], s["o"], s["starts"], s["lens"], s["table"], S=c["S"],
                          T=c["S"] * c["nq"], q_heads=c["Hq"], max_q=c["nq"], max_kv=c["kv"], scale=s["scale"],
-                         window=c["window"], otype=bf.OUT_F16 if c["out"] == "f16" else bf.OUT_F32)
+                         window=c["window"], otype=bf.OUT_F16)
         return [s["o"]]
     if kind == "route":
         bf.moe_route(s["x"], s["out"][0], s["out"][1], c["T"], c["E"], c["k"], bias=s["bias"],
@@ -491,7 +492,7 @@ def run(s):
         return s["out"]
     bf.moe_ffn({"q4_0": bf.Q4_0, "planes": bf.Q4_0_PLANES, "q4_k": bf.Q4_K}[c["fmt"]], s["ws"][0], s["ws"][1],
                s["ws"][2], s["x"], s["ids"], s["w"], s["y"], T=c["T"], K=c["K"], F=c["F"], N=c["K"], E=c["E"],
-               k=c["k"], otype=bf.OUT_F16 if c["out"] == "f16" else bf.OUT_F32)
+               k=c["k"], otype=bf.OUT_F16)
     return [s["y"]]
 
 
@@ -503,7 +504,7 @@ def work(case):
     if kind == "attn":
         rows = case["S"] * case["nq"] * case["Hq"] * case["D"]
         return {"bytes": sum(_reached(case)) * case["H"] * case["D"] * 9 // 8
-                + rows * (2 + (2 if case["out"] == "f16" else 4)),
+                + rows * 4,
                 "flops": 4 * case["D"] * case["Hq"] * sum(_seen(case))}
     if kind == "route":
         t, e = case["T"], case["E"]
@@ -511,7 +512,7 @@ def work(case):
     t, e, k = case["T"], case["E"], case["k"]
     used = e * (1 - (1 - k / e) ** t)              # experts that some row chose, on average
     weights = 3 * case["K"] * case["F"]
-    return {"bytes": int(used * weights * 9 / 16) + t * case["K"] * (2 + (2 if case["out"] == "f16" else 4)) + 8 * t * k,
+    return {"bytes": int(used * weights * 9 / 16) + t * case["K"] * 4 + 8 * t * k,
             "flops": 2 * t * k * weights}
 
 
