@@ -28,6 +28,10 @@ Q4_0, Q4_0_PLANES, Q4_K = 0, 1, 2
 OUT_F32, OUT_F16 = 0, 1
 # bf_ffn_form
 FFN_AUTO, FFN_ONE_LAUNCH, FFN_TWO_LAUNCHES, FFN_CALLS = 0, 1, 2, 3
+# bf_score
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+# bf_ltype
+LOGITS_F32, LOGITS_F16 = 0, 1
 # bf_algo
 ALGO_AUTO, ALGO_MFMA, ALGO_DOT2, ALGO_SIMPLE, ALGO_LDS, ALGO_SLAB, ALGO_SPLIT, ALGO_DENSE = 0, 1, 2, 3, 4, 5, 6, 7
 
@@ -38,6 +42,8 @@ EXPORTS = ("bf_busfill_q4", "bf_busfill_q4_ws", "bf_gemm", "bf_gemm_ex", "bf_gem
            "bf_gguf_open", "bf_gguf_close", "bf_gguf_tensor_count", "bf_gguf_tensor_at", "bf_gguf_find",
            "bf_gguf_get_u64", "bf_gguf_get_str", "bf_gguf_upload",
            "bf_ggml_mul_mat", "bf_ggml_mul_mat_workspace_bytes", "bf_ggml_mul_mat_ws",
+           "bf_kv4_bytes", "bf_kv4_store", "bf_kv4_load", "bf_kv4_attention", "bf_kv4_attention_workspace_bytes",
+           "bf_kv4_attention_ws", "bf_moe_route", "bf_moe_ffn", "bf_moe_ffn_workspace_bytes", "bf_moe_ffn_ws",
            "bf_status_str", "bf_last_error", "bf_version")
 
 
@@ -51,6 +57,37 @@ class GemmDesc(ctypes.Structure):
 class QWeights(ctypes.Structure):
     """bf_qweights: the weights of one linear (W, and the scale plane for planes)."""
     _fields_ = [("W", ctypes.c_void_p), ("W_aux", ctypes.c_void_p)]
+
+
+class Kv4Cache(ctypes.Structure):
+    """bf_kv4_cache: a 4-bit key/value cache in device memory (kv4_cache makes one)."""
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class Kv4AttentionArgs(ctypes.Structure):
+    """bf_kv4_attention_args."""
+    _fields_ = [("Q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("O", ctypes.c_void_p), ("ldo", ctypes.c_int64),
+                ("otype", ctypes.c_int), ("lse", ctypes.c_void_p), ("q_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("ldt", ctypes.c_int),
+                ("S", ctypes.c_int), ("T", ctypes.c_int), ("q_heads", ctypes.c_int), ("max_q", ctypes.c_int),
+                ("max_kv", ctypes.c_int), ("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_int)]
+
+
+class MoeRouteArgs(ctypes.Structure):
+    """bf_moe_route_args."""
+    _fields_ = [("logits", ctypes.c_void_p), ("ltype", ctypes.c_int), ("ldl", ctypes.c_int64), ("bias", ctypes.c_void_p),
+                ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("T", ctypes.c_int), ("E", ctypes.c_int),
+                ("k", ctypes.c_int), ("score", ctypes.c_int), ("groups", ctypes.c_int), ("top_groups", ctypes.c_int),
+                ("renorm", ctypes.c_int), ("factor", ctypes.c_float)]
+
+
+class MoeFfnArgs(ctypes.Structure):
+    """bf_moe_ffn_args."""
+    _fields_ = [("qtype", ctypes.c_int), ("gate", QWeights), ("up", QWeights), ("down", QWeights),
+                ("A", ctypes.c_void_p), ("lda", ctypes.c_int), ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+                ("C", ctypes.c_void_p), ("ldc", ctypes.c_int), ("otype", ctypes.c_int), ("T", ctypes.c_int),
+                ("K", ctypes.c_int), ("F", ctypes.c_int), ("N", ctypes.c_int), ("E", ctypes.c_int), ("k", ctypes.c_int)]
 
 
 class GgufTensor(ctypes.Structure):
@@ -165,6 +202,23 @@ def lib() -> ctypes.CDLL:
         L.bf_ggml_mul_mat_workspace_bytes.restype = sz
         L.bf_ggml_mul_mat_ws.argtypes = [gp, gp, gp, vp, sz, vp]
         L.bf_ggml_mul_mat_ws.restype = i
+        i64, cp, ap = ctypes.c_int64, ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AttentionArgs)
+        rp, mp = ctypes.POINTER(MoeRouteArgs), ctypes.POINTER(MoeFfnArgs)
+        L.bf_kv4_bytes.argtypes = [i, i, i, i]
+        L.bf_kv4_store.argtypes = [cp, vp, i64, vp, i64, vp, i, vp]
+        L.bf_kv4_load.argtypes = [cp, vp, vp, i64, vp, i64, i, vp]
+        L.bf_kv4_attention.argtypes = [cp, ap, vp]
+        L.bf_kv4_attention_workspace_bytes.argtypes = [cp, ap]
+        L.bf_kv4_attention_ws.argtypes = [cp, ap, vp, sz, vp]
+        L.bf_moe_route.argtypes = [rp, vp]
+        L.bf_moe_ffn.argtypes = [mp, vp]
+        L.bf_moe_ffn_workspace_bytes.argtypes = [mp]
+        L.bf_moe_ffn_ws.argtypes = [mp, vp, sz, vp]
+        for f in ("bf_kv4_store", "bf_kv4_load", "bf_kv4_attention", "bf_kv4_attention_ws", "bf_moe_route", "bf_moe_ffn",
+                  "bf_moe_ffn_ws"):
+            getattr(L, f).restype = i
+        for f in ("bf_kv4_bytes", "bf_kv4_attention_workspace_bytes", "bf_moe_ffn_workspace_bytes"):
+            getattr(L, f).restype = sz
         L.bf_status_str.argtypes = [i]
         L.bf_status_str.restype = ctypes.c_char_p
         L.bf_last_error.restype = ctypes.c_char_p
@@ -418,6 +472,101 @@ def ggml_mul_mat_ws(src0: GgmlTensor, src1: GgmlTensor, dst: GgmlTensor, workspa
                     stream=None) -> None:
     _check(lib().bf_ggml_mul_mat_ws(ctypes.byref(src0), ctypes.byref(src1), ctypes.byref(dst), _ptr(workspace),
                                     workspace_bytes, _stream(stream)), "bf_ggml_mul_mat_ws")
+
+
+def kv4_bytes(pages: int, page_size: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of a 4-bit key/value cache of this shape (0: not served)."""
+    return int(lib().bf_kv4_bytes(pages, page_size, kv_heads, head_dim))
+
+
+def kv4_cache(data, pages: int, page_size: int, kv_heads: int, head_dim: int) -> Kv4Cache:
+    """The cache in device memory `data` (a tensor or address of kv4_bytes bytes, 256-byte aligned), which
+    the caller keeps."""
+    return Kv4Cache(_ptr(data), pages, page_size, kv_heads, head_dim)
+
+
+def kv4_store(cache: Kv4Cache, K, V, slots, T: int, *, ldk: int | None = None, ldv: int | None = None,
+              stream=None) -> None:
+    """Quantizes T tokens' fp16 rows K and V into the cache's slots (int64; page * page_size + place; a slot
+    outside the cache skips its token)."""
+    width = cache.kv_heads * cache.head_dim
+    _check(lib().bf_kv4_store(ctypes.byref(cache), _ptr(K), width if ldk is None else ldk, _ptr(V),
+                              width if ldv is None else ldv, _ptr(slots), T, _stream(stream)), "bf_kv4_store")
+
+
+def kv4_load(cache: Kv4Cache, slots, K, V, T: int, *, ldk: int | None = None, ldv: int | None = None,
+             stream=None) -> None:
+    """The tokens of T slots back as fp16 rows (zeros for a slot outside the cache)."""
+    width = cache.kv_heads * cache.head_dim
+    _check(lib().bf_kv4_load(ctypes.byref(cache), _ptr(slots), _ptr(K), width if ldk is None else ldk, _ptr(V),
+                             width if ldv is None else ldv, T, _stream(stream)), "bf_kv4_load")
+
+
+def kv4_attention_args(cache: Kv4Cache, Q, O, q_start, kv_len, page_table, *, S: int, T: int, q_heads: int,
+                       max_q: int, max_kv: int, scale: float, ldq: int | None = None, ldo: int | None = None,
+                       ldt: int | None = None, causal: bool = True, window: int = 0, otype: int = OUT_F32,
+                       lse=None) -> Kv4AttentionArgs:
+    """A bf_kv4_attention_args; ldt defaults to page_table's second dimension."""
+    width = q_heads * cache.head_dim
+    return Kv4AttentionArgs(_ptr(Q), width if ldq is None else ldq, _ptr(O), width if ldo is None else ldo, otype,
+                            _ptr(lse), _ptr(q_start), _ptr(kv_len), _ptr(page_table),
+                            page_table.shape[-1] if ldt is None else ldt, S, T, q_heads, max_q, max_kv, scale,
+                            int(causal), window)
+
+
+def kv4_attention(cache: Kv4Cache, Q, O, q_start, kv_len, page_table, *, stream=None, **args) -> None:
+    """O = attention of S sequences' queries (rows q_start[s] .. q_start[s + 1] - 1 of Q, fp16) over their
+    kv_len[s] tokens of the 4-bit cache (page_table: int32 [S][ldt]); further arguments as kv4_attention_args."""
+    a = kv4_attention_args(cache, Q, O, q_start, kv_len, page_table, **args)
+    _check(lib().bf_kv4_attention(ctypes.byref(cache), ctypes.byref(a), _stream(stream)), "bf_kv4_attention")
+
+
+def kv4_attention_workspace_bytes(cache: Kv4Cache, args: Kv4AttentionArgs) -> int:
+    """Bytes of caller-owned workspace kv4_attention_ws needs (0: none)."""
+    return int(lib().bf_kv4_attention_workspace_bytes(ctypes.byref(cache), ctypes.byref(args)))
+
+
+def kv4_attention_ws(cache: Kv4Cache, args: Kv4AttentionArgs, workspace, workspace_bytes: int, stream=None) -> None:
+    """kv4_attention with a caller-owned workspace (as gemm_ws)."""
+    _check(lib().bf_kv4_attention_ws(ctypes.byref(cache), ctypes.byref(args), _ptr(workspace), workspace_bytes,
+                                     _stream(stream)), "bf_kv4_attention_ws")
+
+
+def moe_route(logits, ids, weights, T: int, E: int, k: int, *, bias=None, score: int = SCORE_SOFTMAX, groups: int = 1,
+              top_groups: int = 1, renorm: bool = True, factor: float = 1.0, ldl: int | None = None,
+              ltype: int | None = None, stream=None) -> None:
+    """ids[T][k] (int32) and weights[T][k] (fp32) of the k experts of largest score (+ bias) of each row of
+    logits [T][ldl] (fp32 or fp16: ltype, by default from the tensor's dtype)."""
+    if ltype is None:
+        import torch
+        ltype = {torch.float32: LOGITS_F32, torch.float16: LOGITS_F16}[logits.dtype]
+    a = MoeRouteArgs(_ptr(logits), ltype, E if ldl is None else ldl, _ptr(bias), _ptr(ids), _ptr(weights), T, E, k, score,
+                     groups, top_groups, int(renorm), factor)
+    _check(lib().bf_moe_route(ctypes.byref(a), _stream(stream)), "bf_moe_route")
+
+
+def moe_ffn_args(qtype: int, gate, up, down, A, ids, weights, C, *, T: int, K: int, F: int, N: int, E: int, k: int,
+                 lda: int | None = None, ldc: int | None = None, otype: int = OUT_F32) -> MoeFfnArgs:
+    """A bf_moe_ffn_args; gate, up and down are (W, W_aux) pairs as for ffn_swiglu, all experts' rows in one."""
+    qw = [QWeights(_ptr(w), _ptr(a)) for (w, a) in (gate, up, down)]
+    return MoeFfnArgs(qtype, qw[0], qw[1], qw[2], _ptr(A), K if lda is None else lda, _ptr(ids), _ptr(weights), _ptr(C),
+                      N if ldc is None else ldc, otype, T, K, F, N, E, k)
+
+
+def moe_ffn(qtype: int, gate, up, down, A, ids, weights, C, *, stream=None, **args) -> None:
+    """C[t] = sum_j weights[t][j] . the SwiGLU block of expert ids[t][j] on A[t]; further arguments as moe_ffn_args."""
+    a = moe_ffn_args(qtype, gate, up, down, A, ids, weights, C, **args)
+    _check(lib().bf_moe_ffn(ctypes.byref(a), _stream(stream)), "bf_moe_ffn")
+
+
+def moe_ffn_workspace_bytes(args: MoeFfnArgs) -> int:
+    """Bytes of caller-owned workspace moe_ffn_ws needs."""
+    return int(lib().bf_moe_ffn_workspace_bytes(ctypes.byref(args)))
+
+
+def moe_ffn_ws(args: MoeFfnArgs, workspace, workspace_bytes: int, stream=None) -> None:
+    """moe_ffn with a caller-owned workspace (as gemm_ws)."""
+    _check(lib().bf_moe_ffn_ws(ctypes.byref(args), _ptr(workspace), workspace_bytes, _stream(stream)), "bf_moe_ffn_ws")
 
 
 def version() -> int:

@@ -15,7 +15,9 @@
 #include <vector>
 
 #include "bf_device.h"
+#include "bf_kv4_launch.h"
 #include "bf_launch.h"
+#include "bf_moe_launch.h"
 
 namespace {
 
@@ -662,6 +664,200 @@ bf_status enqueue_ggml(const GgmlCall& c, const bf_ggml_tensor* s1, uint16_t* st
     }
     return launch_batched(bp, scratch, hs);
 }
+
+// ---------------------------------------------------------------- 4-bit cache and experts
+
+bf_status check_cache(const bf_kv4_cache* c) {
+    if (!c) return fail(BF_ERR_INVALID, "cache is NULL");
+    if (bf_kv4_bytes(c->pages, c->page_size, c->kv_heads, c->head_dim) == 0)
+        return fail(BF_ERR_INVALID, "cache of pages=%d page_size=%d kv_heads=%d head_dim=%d: page_size must be a multiple "
+                                    "of 32, head_dim 64, 96, 128 or 256, pages and kv_heads >= 1", c->pages,
+                    c->page_size, c->kv_heads, c->head_dim);
+    if (!c->data) return fail(BF_ERR_INVALID, "cache data is NULL");
+    if (!aligned(c->data, 256)) return fail(BF_ERR_INVALID, "cache data is not 256-byte aligned");
+    return BF_OK;
+}
+
+bf_status check_kv_rows(const bf_kv4_cache* c, const void* K, int64_t ldk, const void* V, int64_t ldv,
+                        const int64_t* slots, int T) {
+    bf_status st = check_cache(c);
+    if (st != BF_OK) return st;
+    if (!K || !V || !slots) return fail(BF_ERR_INVALID, "K, V or slots is NULL");
+    if (T < 1) return fail(BF_ERR_INVALID, "T=%d must be >= 1", T);
+    const int64_t width = (int64_t)c->kv_heads * c->head_dim;
+    if (ldk < width || ldv < width)
+        return fail(BF_ERR_INVALID, "ldk=%lld or ldv=%lld < kv_heads * head_dim = %lld", (long long)ldk, (long long)ldv,
+                    (long long)width);
+    if (!aligned(K, 16) || !aligned(V, 16) || ldk % 8 || ldv % 8)
+        return fail(BF_ERR_INVALID, "K and V rows must be 16-byte aligned (ldk, ldv %% 8 == 0)");
+    if (!aligned(slots, 8)) return fail(BF_ERR_INVALID, "slots is not 8-byte aligned");
+    if (c->kv_heads > 65535) return fail(BF_ERR_UNSUPPORTED, "kv_heads=%d: at most 65535", c->kv_heads);
+    return BF_OK;
+}
+
+bf::Kv4Shape shape_of(const bf_kv4_cache* c) { return bf::Kv4Shape{c->pages, c->page_size, c->kv_heads, c->head_dim}; }
+
+bf_status check_attention(const bf_kv4_cache* c, const bf_kv4_attention_args* a, bf::Kv4Args& o) {
+    bf_status st = check_cache(c);
+    if (st != BF_OK) return st;
+    if (!a) return fail(BF_ERR_INVALID, "args is NULL");
+    if (!a->Q || !a->O || !a->q_start || !a->kv_len || !a->page_table)
+        return fail(BF_ERR_INVALID, "Q, O, q_start, kv_len or page_table is NULL");
+    if (a->S < 1 || a->T < 1 || a->max_q < 1 || a->max_kv < 0 || a->ldt < 1)
+        return fail(BF_ERR_INVALID, "S=%d T=%d max_q=%d ldt=%d must be >= 1, max_kv=%d >= 0", a->S, a->T, a->max_q, a->ldt,
+                    a->max_kv);
+    if (a->q_heads < 1 || a->q_heads % c->kv_heads)
+        return fail(BF_ERR_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", a->q_heads, c->kv_heads);
+    const int64_t width = (int64_t)a->q_heads * c->head_dim;
+    if (a->ldq < width || a->ldo < width)
+        return fail(BF_ERR_INVALID, "ldq=%lld or ldo=%lld < q_heads * head_dim = %lld", (long long)a->ldq, (long long)a->ldo,
+                    (long long)width);
+    if (!aligned(a->Q, 16) || a->ldq % 8) return fail(BF_ERR_INVALID, "Q rows must be 16-byte aligned (ldq %% 8 == 0)");
+    if (a->otype != BF_OUT_F32 && a->otype != BF_OUT_F16) return fail(BF_ERR_INVALID, "unknown otype %d", (int)a->otype);
+    if (!aligned(a->O, a->otype == BF_OUT_F32 ? 4 : 2)) return fail(BF_ERR_INVALID, "O is not aligned to its element");
+    if (!aligned(a->lse, 4) || !aligned(a->q_start, 4) || !aligned(a->kv_len, 4) || !aligned(a->page_table, 4))
+        return fail(BF_ERR_INVALID, "lse, q_start, kv_len and page_table must be 4-byte aligned");
+    if (a->max_kv > (int64_t)a->ldt * c->page_size)
+        return fail(BF_ERR_INVALID, "max_kv=%d > ldt * page_size = %lld", a->max_kv, (long long)a->ldt * c->page_size);
+    if (a->max_kv > INT32_MAX - 64) return fail(BF_ERR_UNSUPPORTED, "max_kv=%d: at most 2^31 - 65", a->max_kv);
+    if (a->window < 0 || (a->window > 0 && !a->causal))
+        return fail(BF_ERR_INVALID, "window=%d: >= 0, and 0 without causal", a->window);
+    if (!(a->scale > -3e38f && a->scale < 3e38f)) return fail(BF_ERR_INVALID, "scale is not finite");
+    o.data = (uint8_t*)c->data;
+    o.c = shape_of(c);
+    o.Q = a->Q;
+    o.ldq = a->ldq;
+    o.O = a->O;
+    o.ldo = a->ldo;
+    o.out_f16 = a->otype == BF_OUT_F16;
+    o.lse = a->lse;
+    o.q_start = a->q_start;
+    o.kv_len = a->kv_len;
+    o.table = a->page_table;
+    o.ldt = a->ldt;
+    o.S = a->S;
+    o.T = a->T;
+    o.q_heads = a->q_heads;
+    o.max_q = a->max_q < a->T ? a->max_q : a->T;
+    o.max_kv = a->max_kv;
+    o.scale = a->scale;
+    o.causal = a->causal != 0;
+    o.window = a->window;
+    if (!bf::kv4_attention_fits(o))
+        return fail(BF_ERR_UNSUPPORTED, "attention over S=%d kv_heads=%d max_q=%d: more workgroups than a launch takes", a->S,
+                    c->kv_heads, a->max_q);
+    return BF_OK;
+}
+
+bf_status check_route(const bf_moe_route_args* a, bf::RouteArgs& o) {
+    if (!a) return fail(BF_ERR_INVALID, "args is NULL");
+    if (!a->logits || !a->ids || !a->weights) return fail(BF_ERR_INVALID, "logits, ids or weights is NULL");
+    if (a->ltype != BF_LOGITS_F32 && a->ltype != BF_LOGITS_F16) return fail(BF_ERR_INVALID, "unknown ltype %d", (int)a->ltype);
+    if (a->score != BF_SCORE_SOFTMAX && a->score != BF_SCORE_SIGMOID)
+        return fail(BF_ERR_INVALID, "unknown score %d", (int)a->score);
+    if (a->T < 1 || a->E < 1 || a->k < 1) return fail(BF_ERR_INVALID, "T=%d E=%d k=%d must be >= 1", a->T, a->E, a->k);
+    if (a->ldl < a->E) return fail(BF_ERR_INVALID, "ldl=%lld < E=%d", (long long)a->ldl, a->E);
+    if (a->groups < 1 || a->E % a->groups || a->top_groups < 1 || a->top_groups > a->groups)
+        return fail(BF_ERR_INVALID, "groups=%d must divide E=%d, top_groups=%d be in 1..groups", a->groups, a->E, a->top_groups);
+    if (a->k > a->top_groups * (a->E / a->groups))
+        return fail(BF_ERR_INVALID, "k=%d: only %d experts to choose from", a->k, a->top_groups * (a->E / a->groups));
+    if (!aligned(a->logits, a->ltype == BF_LOGITS_F32 ? 4 : 2) || !aligned(a->bias, 4) || !aligned(a->ids, 4) ||
+        !aligned(a->weights, 4))
+        return fail(BF_ERR_INVALID, "logits, bias, ids and weights must be aligned to their elements");
+    if (a->E > 1024 || a->k > 64 || a->groups > 64)
+        return fail(BF_ERR_UNSUPPORTED, "E=%d (at most 1024), k=%d (at most 64), groups=%d (at most 64)", a->E, a->k, a->groups);
+    o.logits = a->logits;
+    o.f16 = a->ltype == BF_LOGITS_F16;
+    o.ldl = a->ldl;
+    o.bias = a->bias;
+    o.ids = a->ids;
+    o.w = a->weights;
+    o.T = a->T;
+    o.E = a->E;
+    o.k = a->k;
+    o.sigmoid = a->score == BF_SCORE_SIGMOID;
+    o.groups = a->groups;
+    o.top_groups = a->top_groups;
+    o.renorm = a->renorm != 0;
+    o.factor = a->factor;
+    return BF_OK;
+}
+
+bf_status check_moe(const bf_moe_ffn_args* a, bf::MoeArgs& o) {
+    if (!a) return fail(BF_ERR_INVALID, "args is NULL");
+    if (a->T < 1 || a->E < 1 || a->k < 1) return fail(BF_ERR_INVALID, "T=%d E=%d k=%d must be >= 1", a->T, a->E, a->k);
+    bf_status st = check_gemm(a->qtype, a->gate.W, a->gate.W_aux, a->A, a->lda, a->C, a->ldc, a->otype, a->T, a->N, a->K);
+    if (st == BF_OK) st = check_weights(a->qtype, a->up.W, a->up.W_aux, a->F, a->K);
+    if (st == BF_OK) st = check_weights(a->qtype, a->down.W, a->down.W_aux, a->N, a->F);
+    if (st != BF_OK) return st;
+    if (!a->ids || !a->weights) return fail(BF_ERR_INVALID, "ids or weights is NULL");
+    if (!aligned(a->ids, 4) || !aligned(a->weights, 4)) return fail(BF_ERR_INVALID, "ids and weights must be 4-byte aligned");
+    if (a->E > 65535 || (int64_t)a->T * a->k > (1 << 24) || (int64_t)a->E * a->F > INT32_MAX || (int64_t)a->E * a->N > INT32_MAX ||
+        a->N > (1 << 24) || a->F > (1 << 24))
+        return fail(BF_ERR_UNSUPPORTED, "E=%d (at most 65535), T * k = %lld (2^24), N=%d and F=%d (2^24, over all experts 2^31 "
+                                        "- 1)", a->E, (long long)a->T * a->k, a->N, a->F);
+    o.qtype = (int)a->qtype;
+    o.gate = (const uint8_t*)a->gate.W;
+    o.gate_aux = (const uint8_t*)a->gate.W_aux;
+    o.up = (const uint8_t*)a->up.W;
+    o.up_aux = (const uint8_t*)a->up.W_aux;
+    o.down = (const uint8_t*)a->down.W;
+    o.down_aux = (const uint8_t*)a->down.W_aux;
+    o.A = a->A;
+    o.lda = a->lda;
+    o.ids = a->ids;
+    o.w = a->weights;
+    o.C = a->C;
+    o.ldc = a->ldc;
+    o.out_f16 = a->otype == BF_OUT_F16;
+    o.T = a->T;
+    o.K = a->K;
+    o.F = a->F;
+    o.N = a->N;
+    o.E = a->E;
+    o.k = a->k;
+    if (a->qtype == BF_Q4_K && !bf::moe_fast(o))
+        return fail(BF_ERR_UNSUPPORTED, "experts in Q4_K: 16-byte aligned A and W, lda %% 8 == 0 (lda=%d)", a->lda);
+    return BF_OK;
+}
+
+// `bytes` of the stream's workspace (the library's), or of the caller's.
+bf_status take_workspace(const char* who, size_t bytes, const bf::Scratch* scratch, hipStream_t hs, float** out) {
+    *out = nullptr;
+    if (scratch && bytes > scratch->bytes)
+        return fail(BF_ERR_INVALID, "%s: the call needs %zu bytes of workspace, %zu given", who, bytes, scratch->bytes);
+    if (!bytes) return BF_OK;
+    unsigned* counters = nullptr;
+    const hipError_t e = bf::split_workspace(scratch, hs, 0, bytes, &counters, out);
+    if (e == hipErrorStreamCaptureUnsupported)
+        return fail(BF_ERR_UNSUPPORTED, "%s: the workspace for this stream is allocated on first use, which cannot happen "
+                                        "during stream capture; make one uncaptured call of this size (or a larger one) on the "
+                                        "stream first", who);
+    return from_hip(e, who);
+}
+
+bf_status run_attention(const char* who, const bf_kv4_cache* c, const bf_kv4_attention_args* a, const bf::Scratch* scratch,
+                        void* stream) {
+    bf::Kv4Args o;
+    bf_status st = check_attention(c, a, o);
+    if (st != BF_OK) return st;
+    const auto held = stream_lock(stream);
+    float* ws = nullptr;
+    st = take_workspace(who, bf::kv4_attention_scratch_bytes(o), scratch, (hipStream_t)stream, &ws);
+    if (st != BF_OK) return st;
+    return from_hip(bf::kv4_attention(o, ws, (hipStream_t)stream), who);
+}
+
+bf_status run_moe(const char* who, const bf_moe_ffn_args* a, const bf::Scratch* scratch, void* stream) {
+    bf::MoeArgs o;
+    bf_status st = check_moe(a, o);
+    if (st != BF_OK) return st;
+    const auto held = stream_lock(stream);
+    float* ws = nullptr;
+    st = take_workspace(who, bf::moe_scratch_bytes(o), scratch, (hipStream_t)stream, &ws);
+    if (st != BF_OK) return st;
+    return from_hip(bf::moe_ffn(o, (uint8_t*)ws, (hipStream_t)stream), who);
+}
 }  // namespace
 
 extern "C" {
@@ -977,6 +1173,79 @@ bf_status bf_ggml_mul_mat_ws(const bf_ggml_tensor* src0, const bf_ggml_tensor* s
     const bf::Scratch sc{(uint8_t*)workspace, need};
     const auto held = stream_lock(stream);
     return enqueue_ggml(c, src1, staged, bp, need ? &sc : nullptr, (hipStream_t)stream);
+}
+
+size_t bf_kv4_bytes(int pages, int page_size, int kv_heads, int head_dim) {
+    if (pages < 1 || page_size < 32 || page_size % 32 || kv_heads < 1) return 0;
+    if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256) return 0;
+    const int64_t per = (int64_t)(page_size / 32) * kv_heads;                 // records of a page: pages * per < 2^31
+    if (per > INT32_MAX / pages) return 0;
+    return (size_t)pages * (size_t)per * (size_t)bf::kv4_record_bytes(head_dim);
+}
+
+bf_status bf_kv4_store(const bf_kv4_cache* cache, const uint16_t* K, int64_t ldk, const uint16_t* V, int64_t ldv,
+                       const int64_t* slots, int T, void* stream) {
+    g_last_error[0] = '\0';
+    const bf_status st = check_kv_rows(cache, K, ldk, V, ldv, slots, T);
+    if (st != BF_OK) return st;
+    return from_hip(bf::kv4_store((uint8_t*)cache->data, shape_of(cache), K, ldk, V, ldv, slots, T, (hipStream_t)stream),
+                    "kernel launch");
+}
+
+bf_status bf_kv4_load(const bf_kv4_cache* cache, const int64_t* slots, uint16_t* K, int64_t ldk, uint16_t* V, int64_t ldv,
+                      int T, void* stream) {
+    g_last_error[0] = '\0';
+    const bf_status st = check_kv_rows(cache, K, ldk, V, ldv, slots, T);
+    if (st != BF_OK) return st;
+    return from_hip(bf::kv4_load((const uint8_t*)cache->data, shape_of(cache), slots, K, ldk, V, ldv, T, (hipStream_t)stream),
+                    "kernel launch");
+}
+
+bf_status bf_kv4_attention(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* stream) {
+    g_last_error[0] = '\0';
+    return run_attention("bf_kv4_attention", cache, args, nullptr, stream);
+}
+
+size_t bf_kv4_attention_workspace_bytes(const bf_kv4_cache* cache, const bf_kv4_attention_args* args) {
+    g_last_error[0] = '\0';
+    bf::Kv4Args o;
+    return check_attention(cache, args, o) == BF_OK ? bf::kv4_attention_scratch_bytes(o) : 0;
+}
+
+bf_status bf_kv4_attention_ws(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+    g_last_error[0] = '\0';
+    const bf_status st = check_workspace(workspace, workspace_bytes);
+    if (st != BF_OK) return st;
+    const bf::Scratch sc{(uint8_t*)workspace, workspace_bytes};
+    return run_attention("bf_kv4_attention_ws", cache, args, &sc, stream);
+}
+
+bf_status bf_moe_route(const bf_moe_route_args* args, void* stream) {
+    g_last_error[0] = '\0';
+    bf::RouteArgs o;
+    const bf_status st = check_route(args, o);
+    if (st != BF_OK) return st;
+    return from_hip(bf::moe_route(o, (hipStream_t)stream), "kernel launch");
+}
+
+bf_status bf_moe_ffn(const bf_moe_ffn_args* args, void* stream) {
+    g_last_error[0] = '\0';
+    return run_moe("bf_moe_ffn", args, nullptr, stream);
+}
+
+size_t bf_moe_ffn_workspace_bytes(const bf_moe_ffn_args* args) {
+    g_last_error[0] = '\0';
+    bf::MoeArgs o;
+    return check_moe(args, o) == BF_OK ? bf::moe_scratch_bytes(o) : 0;
+}
+
+bf_status bf_moe_ffn_ws(const bf_moe_ffn_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    g_last_error[0] = '\0';
+    const bf_status st = check_workspace(workspace, workspace_bytes);
+    if (st != BF_OK) return st;
+    const bf::Scratch sc{(uint8_t*)workspace, workspace_bytes};
+    return run_moe("bf_moe_ffn_ws", args, &sc, stream);
 }
 
 const char* bf_status_str(bf_status s) {

@@ -1,0 +1,174 @@
+// Routing to experts: k_moe_route, one wave a token.
+//
+//   s = softmax(x) or sigmoid(x) over the E experts' logits;
+//   chosen: the k experts of largest s + bias (equal ones: the lowest index);
+//   with groups: E / groups consecutive experts each, a group's score the sum of
+//   its two largest s + bias, the experts of the top_groups best groups only;
+//   weights: s of the chosen (without the bias), over their sum if renorm, times
+//   factor.
+//
+// Without a bias the order of s is that of the logits, which are compared
+// themselves: nothing hangs on how exp rounds.  Lane l holds experts EPL l ..
+// EPL l + EPL - 1, so among equal values the lowest lane's first one has the
+// lowest index.  A NaN counts as the least of all values.
+#include <cfloat>
+
+#include "bf_device.h"
+#include "bf_grid.h"
+#include "bf_moe_launch.h"
+
+namespace bf {
+namespace {
+
+constexpr int kRtWaves = 4;
+
+// The value of lane 63 after a step-wise reduction over the wave's rows of 16,
+// then the rows; lanes without a source keep `none`.
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float v, float none, F f) {
+#define BF_DPP(ctrl, rows)                                                                                        \
+    v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none),                 \
+                                                                   __builtin_bit_cast(int, v), ctrl, rows, 0xF, false)))
+    BF_DPP(0x111, 0xF);        // row_shr:1, 2, 4, 8
+    BF_DPP(0x112, 0xF);
+    BF_DPP(0x114, 0xF);
+    BF_DPP(0x118, 0xF);
+    BF_DPP(0x142, 0xA);        // row_bcast:15 into rows 1 and 3
+    BF_DPP(0x143, 0xC);        // row_bcast:31 into rows 2 and 3
+#undef BF_DPP
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    return wave_reduce(v, -__builtin_inff(), [](float a, float b) { return __builtin_fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
+}
+
+__device__ __forceinline__ float lane_of(float v, int l) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+
+template <int EPL>
+__global__ __launch_bounds__(64 * kRtWaves) void k_moe_route(RouteArgs a) {
+    __shared__ float xs[kRtWaves][65 * EPL];       // selection scores, one pad word per 64
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = blockIdx.x * (int64_t)kRtWaves + wave;
+    const int e0 = lane * EPL;
+    const float ninf = -__builtin_inff();
+    float x[EPL], s[EPL], sel[EPL];
+    if (t < a.T) {
+        const int64_t at = t * a.ldl + e0;
+#pragma unroll
+        for (int i = 0; i < EPL; i++)
+            x[i] = e0 + i >= a.E ? ninf : a.f16 ? (float)((const _Float16*)a.logits)[at + i] : ((const float*)a.logits)[at + i];
+        if (a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) s[i] = 1.f / (1.f + expf(-x[i]));
+        } else {
+            float m = x[0];
+#pragma unroll
+            for (int i = 1; i < EPL; i++) m = __builtin_fmaxf(m, x[i]);
+            m = wave_max(m);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                s[i] = m == ninf && x[i] == ninf ? 0.f : expf(x[i] - m);   // a row of -inf: all zero
+                if (e0 + i < a.E) sum += s[i];
+            }
+            sum = wave_sum(sum);
+#pragma unroll
+            for (int i = 0; i < EPL; i++) s[i] = sum == 0.f ? 0.f : s[i] / sum;
+        }
+        // what is compared: -inf for experts that do not exist, -FLT_MAX at least for those that do
+#pragma unroll
+        for (int i = 0; i < EPL; i++) {
+            const float v = a.bias ? s[i] + (e0 + i < a.E ? a.bias[e0 + i] : 0.f) : a.groups > 1 ? s[i] : x[i];
+            sel[i] = e0 + i < a.E ? __builtin_fmaxf(v, -FLT_MAX) : ninf;
+        }
+    }
+    if (a.groups > 1) {
+        if (t < a.T) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) xs[wave][e0 + i + (e0 + i) / 64] = sel[i];
+        }
+        __syncthreads();
+        if (t < a.T) {
+            const int size = a.E / a.groups;
+            float best = ninf;
+            if (lane < a.groups) {
+                float b1 = ninf, b2 = ninf;
+                for (int i = 0; i < size; i++) {
+                    const int e = lane * size + i;
+                    const float v = xs[wave][e + e / 64];
+                    b2 = __builtin_fmaxf(b2, __builtin_fminf(b1, v));
+                    b1 = __builtin_fmaxf(b1, v);
+                }
+                best = size > 1 ? __builtin_fmaxf(b1 + b2, -FLT_MAX) : b1;
+            }
+            uint64_t keep = 0;
+            for (int i = 0; i < a.top_groups; i++) {
+                const float m = wave_max(best);
+                const int l = __builtin_ctzll(__ballot(best == m));
+                keep |= 1ull << l;
+                if (lane == l) best = ninf;
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const int g = (e0 + i) / size;
+                if (e0 + i < a.E) sel[i] = !((keep >> g) & 1) ? ninf : a.bias ? sel[i] : __builtin_fmaxf(x[i], -FLT_MAX);
+            }
+        }
+    }
+    if (t >= a.T) return;
+    int id = 0;
+    float w = 0.f;
+    for (int j = 0; j < a.k; j++) {
+        float b = sel[0];
+        int bi = 0;
+#pragma unroll
+        for (int i = 1; i < EPL; i++)
+            if (sel[i] > b) {
+                b = sel[i];
+                bi = i;
+            }
+        const float m = wave_max(b);
+        const int l = __builtin_ctzll(__ballot(b == m));
+        float sw = s[0];
+#pragma unroll
+        for (int i = 1; i < EPL; i++)
+            if (bi == i) sw = s[i];
+        const int e = l * EPL + __builtin_amdgcn_readlane(bi, l);
+        sw = lane_of(sw, l);
+        if (lane == j) {
+            id = e;
+            w = sw;
+        }
+        if (lane == l) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++)
+                if (bi == i) sel[i] = ninf;
+        }
+    }
+    if (a.renorm) {
+        const float sum = wave_sum(lane < a.k ? w : 0.f);
+        w = sum == 0.f ? 0.f : w / sum;
+    }
+    if (lane < a.k) {
+        a.ids[t * a.k + lane] = id;
+        a.w[t * a.k + lane] = w * a.factor;
+    }
+}
+
+}  // namespace
+
+hipError_t moe_route(const RouteArgs& a, hipStream_t st) {
+    const int epl = (a.E + 63) / 64;
+    auto k = epl <= 1 ? k_moe_route<1> : epl <= 2 ? k_moe_route<2> : epl <= 4 ? k_moe_route<4>
+             : epl <= 8 ? k_moe_route<8> : k_moe_route<16>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(((int64_t)a.T + kRtWaves - 1) / kRtWaves)), dim3(64 * kRtWaves), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace bf

@@ -420,6 +420,138 @@ size_t bf_ggml_mul_mat_workspace_bytes(const bf_ggml_tensor* src0, const bf_ggml
 bf_status bf_ggml_mul_mat_ws(const bf_ggml_tensor* src0, const bf_ggml_tensor* src1, const bf_ggml_tensor* dst,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit key/value cache
+ * A cache that holds keys and values as Q4_0 weights are held: per 32 values
+ * of a head an fp16 scale d and 4-bit codes q, value (q - 8) d, 4.5 bits a
+ * value.  The caller owns its memory: `pages` pages of `page_size` tokens (a
+ * multiple of 32), each page holding all heads, in the order that the
+ * attention kernels read (written by bf_kv4_store, read by bf_kv4_load and
+ * bf_kv4_attention).  A slot is page * page_size + place in the page.  No
+ * counterpart in the reference, which multiplies weights only
+ * (kernels/busfill_v1a.cu:41-104). */
+typedef struct {
+    void* data;              /* bf_kv4_bytes(...) bytes, 256-byte aligned */
+    int pages, page_size;
+    int kv_heads;
+    int head_dim;            /* 64, 96, 128 or 256 */
+} bf_kv4_cache;
+
+/* Bytes of a cache of this shape; 0 for one that is not served. */
+size_t bf_kv4_bytes(int pages, int page_size, int kv_heads, int head_dim);
+
+/* Quantizes T tokens' keys and values into their slots.  K and V are fp16,
+ * token t's head h at K + t ldk + h head_dim (rows 16-byte aligned, ldk and
+ * ldv multiples of 8); slots[t] is int64; a token whose slot is negative or
+ * past the cache is skipped.  The slots of one call must differ.  Per 32
+ * values: m = the one of largest magnitude (the first of equals), d =
+ * RN_fp16(m / -8), q = floor(x / d + 8.5) clamped to 0..15 (all 8 where d is
+ * 0); a block with an infinity or NaN reads back as NaN.  Whatever else the
+ * pages hold stays as it is. */
+bf_status bf_kv4_store(const bf_kv4_cache* cache, const uint16_t* K, int64_t ldk, const uint16_t* V, int64_t ldv,
+                       const int64_t* slots, int T, void* stream);
+
+/* The tokens of T slots back as fp16 rows, RN_fp16((q - 8) d); zeros for a
+ * slot that is negative or past the cache. */
+bf_status bf_kv4_load(const bf_kv4_cache* cache, const int64_t* slots, uint16_t* K, int64_t ldk, uint16_t* V,
+                      int64_t ldv, int T, void* stream);
+
+/* Attention of S sequences' queries over their cached tokens:
+ *   O[i][h] = sum_t softmax_t(scale Q[i][h] . K[t][g]) V[t][g],  g = h / (q_heads / kv_heads).
+ * Sequence s owns query rows q_start[s] .. q_start[s + 1] - 1 of Q and O and
+ * kv_len[s] cached tokens, token t in slot page_table[s ldt + t / page_size]
+ * page_size + t % page_size; its last query stands at token kv_len[s] - 1.
+ * causal: a query sees tokens up to its own.  window > 0 (causal only): the
+ * last `window` of those.  A page id that is negative or past the cache is a
+ * page that is not there: its tokens are seen by no one.  A query that sees no
+ * token gets a row of zeros (lse -inf).  max_q and max_kv are the caller's
+ * upper bounds of the queries of a sequence and of kv_len (larger ones are cut
+ * to them); max_kv <= ldt page_size.  Rows of no sequence are left alone.
+ * The arrays q_start, kv_len and page_table are device memory: nothing is read
+ * back, so a captured call serves every length up to max_kv. */
+typedef struct {
+    const uint16_t* Q;       /* [T][ldq] fp16, head h at column h head_dim; rows 16-byte aligned */
+    int64_t ldq;
+    void* O;                 /* [T][ldo] */
+    int64_t ldo;
+    bf_otype otype;
+    float* lse;              /* [T][q_heads] log of the softmax's sum (with the scores' maximum), or NULL */
+    const int32_t* q_start;  /* [S + 1] */
+    const int32_t* kv_len;   /* [S] */
+    const int32_t* page_table;
+    int ldt;                 /* entries of a sequence in page_table */
+    int S, T;
+    int q_heads;
+    int max_q, max_kv;
+    float scale;
+    int causal;
+    int window;
+} bf_kv4_attention_args;
+
+/* Partial sums of sequences that several workgroups share go to the library's
+ * workspace for the stream (as bf_gemm's), or to the caller's (_ws: 256-byte
+ * aligned, as bf_gemm_ws).  The result does not depend on which. */
+bf_status bf_kv4_attention(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* stream);
+size_t bf_kv4_attention_workspace_bytes(const bf_kv4_cache* cache, const bf_kv4_attention_args* args);
+bf_status bf_kv4_attention_ws(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- mixture of experts
+ * No counterpart in the reference, whose end-to-end runs drive a dense model
+ * (RESULTS.md:66-68). */
+typedef enum { BF_SCORE_SOFTMAX = 0, BF_SCORE_SIGMOID = 1 } bf_score;
+typedef enum { BF_LOGITS_F32 = 0, BF_LOGITS_F16 = 1 } bf_ltype;
+
+/* Routing: ids[t] = the k experts of largest s + bias, in falling order (equal
+ * ones: the lowest index first), s = softmax(logits[t]) or sigmoid(logits[t]);
+ * weights[t] = their s (without the bias), over their sum where renorm is set
+ * (all 0 where that is 0), times factor.  With groups > 1 the experts form
+ * that many runs of E / groups; a run's score is the sum of its two largest
+ * s + bias (of the one, in runs of one), and only the top_groups best runs'
+ * experts (equal ones: the lowest) are chosen from.  A NaN is the least of all
+ * when experts are chosen.  Without bias, experts are ordered by their logits. */
+typedef struct {
+    const void* logits;      /* [T][ldl] */
+    bf_ltype ltype;
+    int64_t ldl;
+    const float* bias;       /* [E] or NULL */
+    int32_t* ids;            /* [T][k] */
+    float* weights;          /* [T][k] */
+    int T, E, k;             /* E <= 1024, k <= 64 */
+    bf_score score;
+    int groups, top_groups;  /* 1, 1: no groups; groups <= 64 */
+    int renorm;
+    float factor;
+} bf_moe_route_args;
+bf_status bf_moe_route(const bf_moe_route_args* args, void* stream);
+
+/* The experts' SwiGLU feed-forward blocks:
+ *   C[t] = sum_j weights[t][j] down_e . (SiLU(gate_e . A[t]) * (up_e . A[t])),  e = ids[t][j],
+ * gate and up [E][F][K], down [E][N][F] in one format: expert e's rows follow
+ * expert e - 1's (W_aux likewise).  An id that is negative or not below E adds
+ * nothing (an expert that another GPU holds).  The intermediate is rounded to
+ * fp16 once, its weight already in it; the sums over experts run in fp32 in
+ * the order of j, so the result does not depend on the other rows' routing.
+ * Requirements as for bf_gemm; the matrix-core path takes K and F multiples of
+ * 256, 16-byte aligned A and W and lda % 8 == 0 (4-byte aligned W_aux); Q4_K
+ * needs it, other legal Q4_0 inputs run one thread per output. */
+typedef struct {
+    bf_qtype qtype;
+    bf_qweights gate, up, down;
+    const uint16_t* A;       /* [T][lda] fp16 */
+    int lda;
+    const int32_t* ids;      /* [T][k] */
+    const float* weights;    /* [T][k] */
+    void* C;                 /* [T][ldc] */
+    int ldc;
+    bf_otype otype;
+    int T, K, F, N, E, k;
+} bf_moe_ffn_args;
+/* The intermediates live in the library's workspace for the stream, or in the
+ * caller's (_ws, as bf_gemm_ws). */
+bf_status bf_moe_ffn(const bf_moe_ffn_args* args, void* stream);
+size_t bf_moe_ffn_workspace_bytes(const bf_moe_ffn_args* args);
+bf_status bf_moe_ffn_ws(const bf_moe_ffn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Static text for a status code. */
 const char* bf_status_str(bf_status status);
 

@@ -1,0 +1,282 @@
+"""Routing to experts and the experts' feed-forward block against 64-bit
+references (run on an MI355X).
+
+Tolerance of the block, per output, from the roundings it makes: the
+intermediate h = w SiLU(g) u to fp16 (2^-11 |h| + 2^-25), fp32 sums (2^-18 of the
+sum of magnitudes, generous), and for the Q4_0 formats each weight's fp16
+dequant (2^-11 of it), carried through |SiLU'| <= 1.1; fp16 outputs add 2^-11
+|c| + 2^-25.
+"""
+import numpy as np
+import pytest
+import torch
+
+import busfill as bf
+import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+QTS = [O.Q4_0_PLANES, O.Q4_0, O.Q4_K]
+SCALES = {O.Q4_K: (1e-4, 1e-3)}
+
+
+def to_dev(a):
+    a = np.ascontiguousarray(a)
+    return torch.from_numpy(a.view(np.int16) if a.dtype == np.uint16 else a).cuda()
+
+
+# ---------------------------------------------------------------- routing
+def route(x, k, bias=None, score=bf.SCORE_SOFTMAX, groups=1, top=1, renorm=True, factor=1.0, ldl=None):
+    T, E = x.shape if ldl is None else (x.shape[0], x.shape[1] - 3)
+    ids = torch.full((T, k), -7, dtype=torch.int32, device="cuda")
+    w = torch.full((T, k), 9.0, device="cuda")
+    bf.moe_route(x.cuda(), ids, w, T, E, k, bias=None if bias is None else bias.cuda(), score=score, groups=groups,
+                 top_groups=top, renorm=renorm, factor=factor, ldl=ldl)
+    return ids.cpu(), w.cpu().double()
+
+
+def ref_route(x, k, bias, score, groups, top, renorm, factor):
+    """Row by row: stable sorts, so equal scores go to the lowest index."""
+    x = x.numpy().astype(np.float64)
+    T, E = x.shape
+    ids, ws = np.zeros((T, k), np.int64), np.zeros((T, k))
+    for t in range(T):
+        if score == bf.SCORE_SOFTMAX:
+            m = x[t].max()
+            s = np.zeros(E) if m == -np.inf else np.exp(x[t] - m)
+            s = s / s.sum() if s.sum() else s
+        else:
+            s = 1 / (1 + np.exp(-x[t]))
+        sel = s + bias.numpy().astype(np.float64) if bias is not None else s
+        order = sel if bias is not None else x[t]
+        if groups > 1:
+            g = sel.reshape(groups, -1)
+            best = np.sort(g, 1)[:, ::-1][:, :2].sum(1)
+            keep = np.argsort(-best, kind="stable")[:top]
+            mask = np.zeros((groups, E // groups), bool)
+            mask[keep] = True
+            order = np.where(mask.reshape(-1), np.maximum(order, -1e300), -np.inf)
+        ids[t] = np.argsort(-np.maximum(order, -1e300) if groups == 1 else -order, kind="stable")[:k]
+        ws[t] = s[ids[t]]
+        if renorm:
+            ws[t] = ws[t] / ws[t].sum() if ws[t].sum() else 0
+    return torch.from_numpy(ids).int(), torch.from_numpy(ws * factor)
+
+
+def decided(x, k, bias, score, groups, top):
+    """Rows whose answer does not hang on fp32 rounding (differences under 1e-6 that are not exact ties)."""
+    a = ref_route(x, k, bias, score, groups, top, False, 1.0)[0]
+    ok = torch.ones(len(x), dtype=torch.bool)
+    for eps in (2e-6, -2e-6):
+        g = torch.Generator().manual_seed(int(eps > 0))
+        wobble = (torch.rand(x.shape[1], generator=g) * eps)
+        b = (bias if bias is not None else torch.zeros(x.shape[1])) + wobble
+        if bias is not None or groups > 1:
+            ok &= (ref_route(x, k, b, score, groups, top, False, 1.0)[0] == a).all(1)
+    return ok
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 8, 2), (5, 64, 8), (33, 60, 4), (17, 129, 8), (7, 256, 8), (3, 512, 12), (4, 1024, 64),
+                                   (2, 1, 1), (9, 16, 16)])
+@pytest.mark.parametrize("score", [bf.SCORE_SOFTMAX, bf.SCORE_SIGMOID])
+@pytest.mark.parametrize("f16", [False, True])
+def test_route(T, E, k, score, f16):
+    """fp16 logits: equal ones are common, and go to the lowest index."""
+    g = torch.Generator().manual_seed(T * E + k)
+    x = torch.randn(T, E, generator=g) * 2
+    x = x.half() if f16 else x
+    for renorm, factor in ((True, 1.0), (False, 2.5)):
+        ids, w = route(x, k, score=score, renorm=renorm, factor=factor)
+        ri, rw = ref_route(x.float(), k, None, score, 1, 1, renorm, factor)
+        assert torch.equal(ids, ri)
+        assert ((w - rw).abs() <= 1e-5 * rw + 1e-12).all()
+
+
+@pytest.mark.parametrize("E,groups,top,k", [(64, 8, 4, 8), (256, 8, 4, 8), (32, 32, 5, 3), (48, 4, 1, 12), (1024, 64, 64, 6),
+                                            (20, 4, 2, 10)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_groups(E, groups, top, k, biased):
+    g = torch.Generator().manual_seed(E + groups)
+    x = torch.randn(40, E, generator=g) * 1.5
+    bias = torch.randn(E, generator=g) * 0.1 if biased else None
+    for score in (bf.SCORE_SIGMOID, bf.SCORE_SOFTMAX):
+        ok = decided(x, k, bias, score, groups, top)
+        assert ok.float().mean() > 0.8
+        ids, w = route(x, k, bias=bias, score=score, groups=groups, top=top, factor=2.5)
+        ri, rw = ref_route(x, k, bias, score, groups, top, True, 2.5)
+        assert torch.equal(ids[ok], ri[ok])
+        assert ((w - rw).abs() <= 2e-5 * rw + 1e-12)[ok].all()
+
+
+@pytest.mark.parametrize("groups,top", [(1, 1), (4, 2)])
+def test_route_ties_and_infinities(groups, top):
+    """Rows of equal logits, of -inf, with one finite expert, and NaN (the last to be chosen)."""
+    E, k = 16, 5
+    x = torch.zeros(6, E)
+    x[1] = float("-inf")
+    x[2] = float("-inf")
+    x[2, 11] = 1.0
+    x[3, 5], x[3, 9] = 2.0, 2.0
+    x[4] = torch.arange(E).float().flip(0)
+    x[5, ::2] = float("-inf")
+    ids, w = route(x, k, groups=groups, top=top)
+    ri, rw = ref_route(x, k, None, bf.SCORE_SOFTMAX, groups, top, True, 1.0)
+    assert torch.equal(ids, ri) and ((w - rw).abs() <= 1e-6).all()
+    assert (w[1] == 0).all()                       # nothing to choose: no weight, not NaN
+    x = torch.randn(1, E)
+    x[0, 3] = float("nan")
+    assert 3 not in route(x, E - 1, score=bf.SCORE_SIGMOID)[0].tolist()[0]
+
+
+def test_route_row_stride():
+    x = torch.randn(9, 67)
+    ids, w = route(x, 6, ldl=67)
+    ri, rw = ref_route(x[:, :64], 6, None, bf.SCORE_SOFTMAX, 1, 1, True, 1.0)
+    assert torch.equal(ids, ri) and ((w - rw).abs() <= 1e-6).all()
+
+
+# ---------------------------------------------------------------- the experts' block
+class Experts:
+    def __init__(self, qt, E, K, F, N, seed=1):
+        self.qt, self.E, self.K, self.F, self.N = qt, E, K, F, N
+        shapes = [(E * F, K), (E * F, K), (E * N, F)]
+        ws = [O.gen_weights(qt, n, k, seed=seed + i, scale_range=SCALES.get(qt)) for i, (n, k) in enumerate(shapes)]
+        self.dev = [(to_dev(w.W), to_dev(w.W_aux) if w.W_aux is not None else None) for w in ws]
+        self.w64 = [torch.from_numpy(O.dequant_f32(w).astype(np.float64)).reshape(E, -1, k) for w, (_, k) in zip(ws, shapes)]
+
+    def run(self, x, ids, w, otype=bf.OUT_F32, lda=None, pad=0, workspace=False, stream=None):
+        T, k = ids.shape
+        c = torch.full((T, self.N + pad), 9.0, dtype=torch.float32 if otype == bf.OUT_F32 else torch.float16, device="cuda")
+        xd, idd, wd = x.cuda(), ids.int().cuda(), w.float().cuda()
+        kw = dict(T=T, K=self.K, F=self.F, N=self.N, E=self.E, k=k, otype=otype, lda=lda, ldc=self.N + pad)
+        torch.cuda.synchronize()
+        if workspace:
+            a = bf.moe_ffn_args(self.qt, *self.dev, xd, idd, wd, c, **kw)
+            n = bf.moe_ffn_workspace_bytes(a)
+            ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
+            torch.cuda.synchronize()
+            bf.moe_ffn_ws(a, ws, n, stream=stream)
+        else:
+            bf.moe_ffn(self.qt, *self.dev, xd, idd, wd, c, stream=stream, **kw)
+        torch.cuda.synchronize()
+        assert (c[:, self.N:] == 9.0).all()
+        return c[:, :self.N]
+
+    def check(self, T, k, seed=3, ids=None, otype=bf.OUT_F32, pad=0, **kw):
+        g = torch.Generator().manual_seed(seed)
+        wide = torch.randn(T, self.K + pad, generator=g).half()
+        if ids is None:
+            ids = torch.rand(T, self.E, generator=g).argsort(1)[:, :k]
+        w = torch.rand(ids.shape, generator=g) + 0.05
+        got = self.run(wide, ids, w, otype=otype, lda=self.K + pad, pad=pad, **kw).cpu().double()
+        x = wide[:, :self.K].double()
+        want, tol = torch.zeros(T, self.N).double(), torch.zeros(T, self.N).double()
+        rw = 0.0 if self.qt == O.Q4_K else 2.0 ** -11      # the weights' own rounding
+        acc = 2.0 ** -18
+        for e in range(self.E):
+            t, j = torch.nonzero(ids == e, as_tuple=True)
+            if len(t) == 0:
+                continue
+            wg, wu, wd = (m[e] for m in self.w64)
+            gt, ut, ww = x[t] @ wg.t(), x[t] @ wu.t(), w[t, j].double()[:, None]
+            dg, du = (x[t].abs() @ m.abs().t() * (rw + acc) for m in (wg, wu))
+            silu = gt * torch.sigmoid(gt)
+            h = ww * silu * ut
+            dh = ww * (1.1 * dg * (ut.abs() + du) + silu.abs() * du) + (2.0 ** -11 + 2.0 ** -20) * h.abs() + 2.0 ** -25
+            want.index_add_(0, t, h @ wd.t())
+            tol.index_add_(0, t, dh @ wd.abs().t() * (1 + rw + acc) + h.abs() @ wd.abs().t() * (rw + acc))
+        if otype == bf.OUT_F16:
+            tol = tol + 2.0 ** -11 * want.abs() + 2.0 ** -25
+        err = (got - want).abs()
+        assert (err <= tol + 1e-12).all(), float((err / tol).max())
+        return got
+
+
+@pytest.mark.parametrize("qt", QTS)
+@pytest.mark.parametrize("T,k,E", [(1, 2, 8), (1, 1, 1), (3, 4, 16), (16, 2, 4), (17, 2, 4), (33, 3, 5), (70, 1, 2), (100, 4, 6)])
+def test_experts(qt, T, k, E):
+    """From one token to more rows an expert than one pass takes; experts that no row chose."""
+    Experts(qt, E, 512, 256, 200).check(T, k)
+
+
+@pytest.mark.parametrize("qt", QTS)
+def test_experts_many_slots(qt):
+    """More slots than a workgroup looks through by itself: the sorted plan."""
+    Experts(qt, 12, 256, 512, 130).check(290, 4, otype=bf.OUT_F16)
+    Experts(qt, 3, 512, 256, 64).check(1100, 1)
+
+
+@pytest.mark.parametrize("T", [5, 600])
+def test_experts_all_to_one(T):
+    x = Experts(O.Q4_K, 6, 256, 256, 96)
+    x.check(T, 2, ids=torch.tensor([[4, 1]]).repeat(T, 1))
+    x.check(T, 2, ids=torch.tensor([[3, 3]]).repeat(T, 1))      # the same expert twice in a row
+
+
+@pytest.mark.parametrize("T", [4, 700])
+def test_experts_of_other_gpus(T):
+    """Ids outside 0 .. E - 1 add nothing; a row with none left is zero."""
+    x = Experts(O.Q4_0, 4, 256, 256, 64)
+    g = torch.Generator().manual_seed(8)
+    ids = torch.randint(-2, 6, (T, 3), generator=g)
+    ids[1] = torch.tensor([-1, 4, 2 ** 30])
+    got = x.check(T, 3, ids=ids)
+    assert (got[1] == 0).all()
+    x.check(T, 3, ids=torch.full((T, 3), -1))
+
+
+@pytest.mark.parametrize("qt", [O.Q4_0, O.Q4_0_PLANES])
+@pytest.mark.parametrize("K,F,N", [(32, 32, 1), (96, 288, 33), (256, 224, 40), (224, 256, 40)])
+def test_experts_odd_widths(qt, K, F, N):
+    """Widths that are not whole super-groups."""
+    Experts(qt, 5, K, F, N).check(7, 3)
+
+
+@pytest.mark.parametrize("qt", QTS)
+def test_experts_strides_workspace_stream(qt):
+    x = Experts(qt, 6, 512, 256, 256)
+    a = x.check(9, 2, pad=8)
+    b = x.check(9, 2, pad=8, workspace=True)
+    c = x.check(9, 2, pad=8, stream=torch.cuda.Stream())
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_experts_rows_do_not_depend_on_each_other():
+    """A row's bits are the same alone and among others, as long as both calls take the same kernels."""
+    x = Experts(O.Q4_K, 8, 512, 256, 128)
+    g = torch.Generator().manual_seed(2)
+    a = torch.randn(12, 512, generator=g).half()
+    ids, w = torch.rand(12, 8, generator=g).argsort(1)[:, :3], torch.rand(12, 3, generator=g)
+    all_ = x.run(a, ids, w)
+    for t in (0, 5, 11):
+        assert torch.equal(all_[t:t + 1], x.run(a[t:t + 1], ids[t:t + 1], w[t:t + 1]))
+
+
+def test_captured_block():
+    x = Experts(O.Q4_K, 8, 256, 256, 64)
+    st = torch.cuda.Stream()
+    a = torch.randn(6, 256).half().cuda()
+    logits = torch.randn(6, 8).cuda()
+    ids, w = torch.empty(6, 2, dtype=torch.int32, device="cuda"), torch.empty(6, 2, device="cuda")
+    c = torch.empty(6, 64, device="cuda")
+
+    def step(out):
+        bf.moe_route(logits, ids, w, 6, 8, 2)
+        bf.moe_ffn(x.qt, *x.dev, a, ids, w, out, T=6, K=256, F=256, N=64, E=8, k=2)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        step(c)
+    st.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        step(c)
+    for i in range(4):
+        logits.copy_(torch.randn(6, 8))
+        a.copy_(torch.randn(6, 256).half())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.empty_like(c)
+        step(want)
+        assert torch.equal(c, want)
