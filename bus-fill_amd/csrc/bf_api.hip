@@ -792,9 +792,9 @@ bf_status check_moe(const bf_moe_ffn_args* a, bf::MoeArgs& o) {
     if (st != BF_OK) return st;
     if (!a->ids || !a->weights) return fail(BF_ERR_INVALID, "ids or weights is NULL");
     if (!aligned(a->ids, 4) || !aligned(a->weights, 4)) return fail(BF_ERR_INVALID, "ids and weights must be 4-byte aligned");
-    if (a->E > 65535 || (int64_t)a->T * a->k > (1 << 24) || (int64_t)a->E * a->F > INT32_MAX || (int64_t)a->E * a->N > INT32_MAX ||
+    if (a->E > 4096 || (int64_t)a->T * a->k > (1 << 24) || (int64_t)a->E * a->F > INT32_MAX || (int64_t)a->E * a->N > INT32_MAX ||
         a->N > (1 << 24) || a->F > (1 << 24))
-        return fail(BF_ERR_UNSUPPORTED, "E=%d (at most 65535), T * k = %lld (2^24), N=%d and F=%d (2^24, over all experts 2^31 "
+        return fail(BF_ERR_UNSUPPORTED, "E=%d (at most 4096), T * k = %lld (2^24), N=%d and F=%d (2^24, over all experts 2^31 "
                                         "- 1)", a->E, (long long)a->T * a->k, a->N, a->F);
     o.qtype = (int)a->qtype;
     o.gate = (const uint8_t*)a->gate.W;

@@ -9,6 +9,7 @@
 //
 // Bound by the weights of the experts in use, each read once.
 #include <algorithm>
+#include <climits>
 
 #include "bf_formats.h"
 #include "bf_grid.h"
@@ -259,41 +260,63 @@ __global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW<QT, GU ? 2 :
     }
 }
 
-// Slots sorted by expert, in order within an expert: one workgroup an expert.
-// Every wave counts, then writes, its own run of slots.
+// Slots sorted by expert, in order within an expert, and the tiles they make:
+// one workgroup an expert.  Each counts all experts' slots (in LDS; integer
+// sums, so their order does not matter), then every wave writes its own run of
+// slots.
 constexpr int kPlanWaves = 16;
 __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __restrict__ ids, int slots, int E,
-                                                              int32_t* __restrict__ perm, int32_t* __restrict__ offs) {
-    __shared__ int less[kPlanWaves], same[kPlanWaves];
+                                                              int32_t* __restrict__ perm, int32_t* __restrict__ offs,
+                                                              int4* __restrict__ table, int* __restrict__ tiles) {
+    extern __shared__ int hist[];
+    __shared__ int same[kPlanWaves], sum[2][kPlanWaves];
     const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < E; i += 64 * kPlanWaves) hist[i] = 0;
+    __syncthreads();
     const int per = (slots + kPlanWaves - 1) / kPlanWaves, s0 = min(slots, wave * per), s1 = min(slots, s0 + per);
-    int nl = 0, ns = 0;
+    int ns = 0;
     for (int s = s0 + lane; s < s1; s += 64) {
         const int id = ids[s];
-        nl += id >= 0 && id < e;
+        if (id >= 0 && id < E) atomicAdd(&hist[id], 1);
         ns += id == e;
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) ns += __shfl_xor(ns, x);
+    if (lane == 0) same[wave] = ns;
+    __syncthreads();
+    // slots and tiles of the experts before e
+    int nl = 0, nt = 0;
+    for (int i = threadIdx.x; i < e; i += 64 * kPlanWaves) {
+        nl += hist[i];
+        nt += (hist[i] + kMoeTileRows - 1) / kMoeTileRows;
     }
 #pragma unroll
     for (int x = 32; x; x >>= 1) {
         nl += __shfl_xor(nl, x);
-        ns += __shfl_xor(ns, x);
+        nt += __shfl_xor(nt, x);
     }
     if (lane == 0) {
-        less[wave] = nl;
-        same[wave] = ns;
+        sum[0][wave] = nl;
+        sum[1][wave] = nt;
     }
     __syncthreads();
-    int base = 0, total = 0, at = 0;
+    int base = 0, tile = 0, at = 0;
 #pragma unroll
     for (int q = 0; q < kPlanWaves; q++) {
-        base += less[q];
+        base += sum[0][q];
+        tile += sum[1][q];
         if (q < wave) at += same[q];
-        total += same[q];
     }
+    const int total = hist[e], mine = (total + kMoeTileRows - 1) / kMoeTileRows;
     if (threadIdx.x == 0) {
         offs[e] = base;
-        if (e == E - 1) offs[E] = base + total;
+        if (e == E - 1) {
+            offs[E] = base + total;
+            *tiles = tile + mine;
+        }
     }
+    for (int i = threadIdx.x; i < mine; i += 64 * kPlanWaves)
+        table[tile + i] = int4{e, base + i * kMoeTileRows, min(kMoeTileRows, total - i * kMoeTileRows), 0};
     at += base;
     for (int s = s0; s < s1; s += 64) {
         const bool hit = s + lane < s1 && ids[s + lane] == e;
@@ -322,15 +345,29 @@ size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Workspace: h [slots][F] fp16, y [slots][N] fp32, the plan.
 struct MoeWs {
-    size_t y, perm, offs, end;
+    size_t y, perm, offs, table, tiles, end;
+    int64_t max_tiles;
     explicit MoeWs(const MoeArgs& a) {
         const size_t slots = (size_t)a.T * a.k;
         y = up256(slots * a.F * 2);
         perm = y + up256(slots * a.N * 4);
         offs = perm + up256(slots * 4);
-        end = offs + up256(((size_t)a.E + 1) * 4);
+        table = offs + up256(((size_t)a.E + 1) * 4);
+        max_tiles = (int64_t)std::min<size_t>(a.E, slots) + (int64_t)(slots / kMoeTileRows);
+        tiles = table + up256((size_t)max_tiles * 16);
+        end = tiles + 256;
     }
 };
+
+int64_t a_bytes(const MoeArgs& a) { return ((int64_t)(a.T - 1) * a.lda + a.K) * 2; }
+
+// The tile kernel: rows addressed with 32 bits from the buffer's start, and a
+// grid that fits a launch.
+bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
+    const int64_t slots = (int64_t)a.T * a.k, nt = std::max<int64_t>(a.F / 64, (a.N + 127) / 128);
+    return slots >= 16 * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
+           launch_fits(o.max_tiles * nt, 512) && o.max_tiles * nt < INT32_MAX;
+}
 
 bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -368,14 +405,45 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     Lists l{nullptr, nullptr};
     if (fast && slots > kScanSlots) {
         l = Lists{(const int32_t*)(ws + o.perm), (const int32_t*)(ws + o.offs)};
-        hipLaunchKernelGGL(k_moe_plan, dim3((unsigned)a.E), dim3(64 * kPlanWaves), 0, st, a.ids, (int)slots, a.E,
-                           (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs));
+        hipLaunchKernelGGL(k_moe_plan, dim3((unsigned)a.E), dim3(64 * kPlanWaves), a.E * 4, st, a.ids, (int)slots, a.E,
+                           (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs), (int4*)(ws + o.table), (int*)(ws + o.tiles));
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipError_t e = launch_rows<QT, true>(a, a.A, a.lda, ws, l, fast, st);
-    if (e != hipSuccess) return e;
-    e = launch_rows<QT, false>(a, (const uint16_t*)ws, a.F, ws + o.y, l, fast, st);
+    hipError_t e;
+    if (l.perm && tiles_serve(a, o)) {
+        MoeTileArgs t{};
+        t.perm = l.perm;
+        t.table = (const int4*)(ws + o.table);
+        t.tiles = (const int*)(ws + o.tiles);
+        t.W[0] = a.gate;
+        t.W[1] = a.up;
+        t.aux[0] = a.gate_aux;
+        t.aux[1] = a.up_aux;
+        t.A = a.A;
+        t.lda = a.lda;
+        t.a_bytes = (uint32_t)a_bytes(a);
+        t.out = ws;
+        t.R = a.F;
+        t.K = a.K;
+        t.nt = a.F / 64;
+        e = moe_tile(a, t, true, o.max_tiles, st);
+        if (e != hipSuccess) return e;
+        t.W[0] = a.down;
+        t.aux[0] = a.down_aux;
+        t.A = (const uint16_t*)ws;
+        t.lda = a.F;
+        t.a_bytes = (uint32_t)(slots * a.F * 2);
+        t.out = ws + o.y;
+        t.R = a.N;
+        t.K = a.F;
+        t.nt = (a.N + 127) / 128;
+        e = moe_tile(a, t, false, o.max_tiles, st);
+    } else {
+        e = launch_rows<QT, true>(a, a.A, a.lda, ws, l, fast, st);
+        if (e != hipSuccess) return e;
+        e = launch_rows<QT, false>(a, (const uint16_t*)ws, a.F, ws + o.y, l, fast, st);
+    }
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k_moe_sum, dim3((unsigned)(((int64_t)a.T * a.N + 255) / 256)), dim3(256), 0, st, a, (const float*)(ws + o.y));
     return hipGetLastError();

@@ -32,6 +32,21 @@ struct MoeArgs {
     int ldc, out_f16;
     int T, K, F, N, E, k;
 };
+// One of the two products over tiles of gathered rows (bf_moe_tile.hip).
+constexpr int kMoeTileRows = 256;
+struct MoeTileArgs {
+    const uint8_t *W[2], *aux[2];  // gate and up, or down
+    const uint16_t* A;         // rows of tokens, or of slots
+    uint32_t a_bytes;          // from A on: below 4 GB
+    int64_t lda;
+    void* out;                 // h fp16, or y fp32, by slot
+    int R, K, nt;              // weight rows of an expert, their length, column tiles
+    const int32_t* perm;       // slots by expert
+    const int4* table;         // tiles: expert, first place in perm, rows
+    const int* tiles;          // their number
+};
+hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, int64_t max_tiles, hipStream_t st);
+
 // The matrix-core kernels serve these widths and alignments.
 bool moe_fast(const MoeArgs& a);
 size_t moe_scratch_bytes(const MoeArgs& a);

@@ -1,0 +1,157 @@
+// The experts' products for prompts: k_moe_tile, the tile of the prefill GEMM
+// (bf_tile.h) over rows gathered by expert.
+//
+// An expert's slots are cut into runs of 256 rows (the last one shorter: a tile
+// takes 64, 128, 192 or 256 rows); a workgroup multiplies one run with 128
+// weight rows.  Activation rows are fetched through the slot list, row by row,
+// by the direct-to-LDS loads' own per-lane addresses, so nothing is gathered
+// beforehand.
+//
+// Gate and up: a tile's 128 weight rows are 32 gate rows, the same 32 up rows,
+// and the next 32 of both, which puts g and u of one output into the two column
+// tiles of one wave: h = w SiLU(g) u leaves the registers as the one fp16 row
+// that the down product reads.  Two k groups of waves hold half of each sum;
+// each hands the other half of the rows over and finishes the rest.
+#include <atomic>
+
+#include "bf_moe_launch.h"
+#include "bf_tile.h"
+
+namespace bf {
+namespace {
+
+// The outputs of a tile: run() of bf_tile.h, then the epilogue above.
+template <int QT, int TA, bool GU>
+__device__ __forceinline__ void moe_tile(uint8_t* lds, const MoeArgs& a, const MoeTileArgs& o, const int32_t* list, int rows,
+                                         int64_t e, int ni) {
+    using T = Tile<QT, TA, 1>;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    T t;
+    t.rsrc = u4{(uint32_t)(uintptr_t)o.A, (uint32_t)((uintptr_t)o.A >> 32) & 0xFFFFu, o.a_bytes, 0x00020000u};
+#pragma unroll
+    for (int q = 0; q < TA; q++) {
+        const int slot = list[min(8 * (wave + 8 * q) + (lane >> 3), rows - 1)];
+        t.voff[q] = (uint32_t)(GU ? slot / a.k : slot) * (uint32_t)o.lda * 2u +
+                    16u * (((uint32_t)lane & 7u) ^ (4u * (wave & 1) + (lane >> 4)));
+    }
+    t.lds0 = lds_addr(lds);
+    t.wave = wave;
+    t.j = threadIdx.x & 3;
+    const int wr = threadIdx.x >> 2;
+    // tile column -> weight row: GU 64 outputs of gate and up, 32 and 32 in turn
+    const int f = GU ? 64 * ni + 32 * (wr >> 6) + (wr & 31) : 128 * ni + wr;
+    const bool up = GU && (wr & 32);
+    const int64_t n = e * o.R + min(f, o.R - 1);
+    t.row = (up ? o.W[1] : o.W[0]) + n * row_bytes(QT, o.K);
+    t.aux = QT == QT_PLANES ? (up ? o.aux[1] : o.aux[0]) + n * (o.K >> 4) : nullptr;
+    t.wst = T::kAStage + wr * 128 + 16 * (tile_chunk<QT, 1>(t.j, 0) ^ ((wr >> 1) & 7));
+    const int kg = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
+    const uint32_t fr = (lane & 31) * 128 + 16 * ((4 * kg + (lane >> 5)) ^ ((lane >> 1) & 7));
+    t.fa = wm * (32 * TA * 128) + fr;
+    t.fw = T::kAStage + wn * (64 * 128) + fr;
+    t.mg = make_magic();
+#pragma unroll
+    for (int i = 0; i < TA; i++)
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) t.acc[i][b][x] = 0.f;
+    t.run(lds, 0, o.K >> 8);
+
+    // Group kg finishes accumulator registers 8 kg .. 8 kg + 7 of every tile.
+    uint8_t* const xch = lds + (threadIdx.x & 255) * 16;
+    constexpr int XB = TA * 4 * 4096;
+#pragma unroll
+    for (int i = 0; i < TA; i++)
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int x = 0; x < 8; x += 4) {
+                const f16x& v = t.acc[i][b];
+                *(f4*)(xch + kg * XB + ((i * 2 + b) * 2 + x / 4) * 4096) =
+                    kg ? f4{v[x], v[x + 1], v[x + 2], v[x + 3]} : f4{v[8 + x], v[9 + x], v[10 + x], v[11 + x]};
+            }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TA; i++)
+#pragma unroll
+        for (int x = 0; x < 8; x += 4) {
+            f4 y[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const f4 p = *(const f4*)(xch + (1 - kg) * XB + ((i * 2 + b) * 2 + x / 4) * 4096);
+                const f16x& v = t.acc[i][b];
+#pragma unroll
+                for (int c = 0; c < 4; c++) y[b][c] = kg ? p[c] + v[8 + x + c] : v[x + c] + p[c];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int r = 32 * TA * wm + 32 * i + 16 * kg + 2 * x + 4 * (lane >> 5) + c;
+                if (r >= rows) continue;
+                const int slot = list[r];
+                if constexpr (GU) {
+                    const float g = y[0][c];
+                    const float ex = __builtin_amdgcn_exp2f(g * -1.44269504088896341f);
+                    ((_Float16*)o.out)[(int64_t)slot * o.R + 64 * ni + 32 * wn + (lane & 31)] =
+                        (_Float16)(g * __builtin_amdgcn_rcpf(1.0f + ex) * y[1][c] * a.w[slot]);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const int n1 = 128 * ni + 64 * wn + 32 * b + (lane & 31);
+                        if (n1 < o.R) ((float*)o.out)[(int64_t)slot * o.R + n1] = y[b][c];
+                    }
+                }
+            }
+        }
+}
+
+template <int QT, bool GU>
+__global__ __launch_bounds__(kTlThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void k_moe_tile(MoeArgs a, MoeTileArgs o) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int units = *o.tiles * o.nt;
+    if ((int)blockIdx.x >= units) return;
+    const int v = xcd_unit((int)blockIdx.x, units), i = v / o.nt, ni = v - i * o.nt;
+    const int4 d = o.table[i];
+    const int e = __builtin_amdgcn_readfirstlane(d.x), rows = __builtin_amdgcn_readfirstlane(d.z);
+    const int32_t* list = o.perm + __builtin_amdgcn_readfirstlane(d.y);
+    if (rows > 192) moe_tile<QT, 4, GU>(lds, a, o, list, rows, e, ni);
+    else if (rows > 128) moe_tile<QT, 3, GU>(lds, a, o, list, rows, e, ni);
+    else if (rows > 64) moe_tile<QT, 2, GU>(lds, a, o, list, rows, e, ni);
+    else moe_tile<QT, 1, GU>(lds, a, o, list, rows, e, ni);
+}
+
+template <int QT, bool GU>
+hipError_t launch(const MoeArgs& a, const MoeTileArgs& o, int64_t max_tiles, hipStream_t st) {
+    using T = Tile<QT, 4, 1>;
+    auto k = k_moe_tile<QT, GU>;
+    constexpr int lds = T::NS * T::kStage;
+    static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)(max_tiles * o.nt)), dim3(kTlThreads), lds, st, a, o);
+    return hipGetLastError();
+}
+
+template <int QT>
+hipError_t dispatch(const MoeArgs& a, const MoeTileArgs& o, bool gu, int64_t max_tiles, hipStream_t st) {
+    return gu ? launch<QT, true>(a, o, max_tiles, st) : launch<QT, false>(a, o, max_tiles, st);
+}
+
+}  // namespace
+
+hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, int64_t max_tiles, hipStream_t st) {
+    if (a.qtype == QT_PLANES) return dispatch<QT_PLANES>(a, o, gu, max_tiles, st);
+    if (a.qtype == QT_Q4_0) return dispatch<QT_Q4_0>(a, o, gu, max_tiles, st);
+    return dispatch<QT_Q4_K>(a, o, gu, max_tiles, st);
+}
+
+}  // namespace bf
