@@ -80,23 +80,21 @@ __global__ __launch_bounds__(256) void k_kv4_store(uint8_t* __restrict__ data, K
     uint8_t q[32];
     const uint32_t d = quantize32(x, q);
     uint8_t* r = data + rec * kv4_record_bytes(c.dim);
-    const int g = tok >> 3;
     if (isv) {
-        uint8_t* p = r + kv4_v_at(c.dim) + 4 * c.dim * g + 8 * b + (tok & 7);
+        uint8_t* p = r + kv4_v_at(c.dim, tok, b, 0);
+        const int step = kv4_v_at(c.dim, tok, b, 1) - kv4_v_at(c.dim, tok, b, 0);
 #pragma unroll
-        for (int e = 0; e < 16; e++) p[nb * 8 * e] = (uint8_t)(q[e] | q[16 + e] << 4);
+        for (int e = 0; e < 16; e++) p[step * e] = (uint8_t)(q[e] | q[16 + e] << 4);
     } else {
-        uint8_t* p = r + c.dim / 2 * tok + 4 * b;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             uint32_t w = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) w |= (uint32_t)q[8 * k + e] << (4 * knib(e));
-            *(uint32_t*)(p + c.dim / 8 * k) = w;
+            *(uint32_t*)(r + kv4_k_at(c.dim, tok, b, k)) = w;
         }
     }
-    uint16_t* s = (uint16_t*)(r + (isv ? kv4_vs_at(c.dim) : kv4_ks_at(c.dim)) + c.dim / 2 * g);
-    s[8 * b + (tok & 7)] = (uint16_t)d;
+    *(uint16_t*)(r + (isv ? kv4_vs_at(c.dim, tok, b) : kv4_ks_at(c.dim, tok, b))) = (uint16_t)d;
 }
 
 // The same units back to fp16: RN16((q - 8) d), the product exact in fp32.
@@ -114,23 +112,21 @@ __global__ __launch_bounds__(256) void k_kv4_load(const uint8_t* __restrict__ da
     int tok;
     if (slot_at(c, slots[t], head, rec, tok)) {
         const uint8_t* r = data + rec * kv4_record_bytes(c.dim);
-        const int g = tok >> 3;
-        const float d = half_bits_to_float(((const uint16_t*)(r + (isv ? kv4_vs_at(c.dim) : kv4_ks_at(c.dim)) +
-                                                              c.dim / 2 * g))[8 * b + (tok & 7)]);
+        const float d = half_bits_to_float(*(const uint16_t*)(r + (isv ? kv4_vs_at(c.dim, tok, b) : kv4_ks_at(c.dim, tok, b))));
         uint8_t q[32];
         if (isv) {
-            const uint8_t* p = r + kv4_v_at(c.dim) + 4 * c.dim * g + 8 * b + (tok & 7);
+            const uint8_t* p = r + kv4_v_at(c.dim, tok, b, 0);
+            const int step = kv4_v_at(c.dim, tok, b, 1) - kv4_v_at(c.dim, tok, b, 0);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const uint32_t v = p[nb * 8 * e];
+                const uint32_t v = p[step * e];
                 q[e] = v & 15;
                 q[16 + e] = v >> 4;
             }
         } else {
-            const uint8_t* p = r + c.dim / 2 * tok + 4 * b;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const uint32_t w = *(const uint32_t*)(p + c.dim / 8 * k);
+                const uint32_t w = *(const uint32_t*)(r + kv4_k_at(c.dim, tok, b, k));
 #pragma unroll
                 for (int e = 0; e < 8; e++) q[8 * k + e] = (w >> (4 * knib(e))) & 15;
             }

@@ -26,20 +26,16 @@
 //   the accumulators are rarely rescaled.
 // * A workgroup's four waves take a chunk's records in turn; they meet in LDS.
 //   Sequences of several chunks are joined by a second launch.
-#include "bf_device.h"
+#include <atomic>
+
 #include "bf_grid.h"
 #include "bf_kv4_launch.h"
+#include "bf_lds.h"
 
 namespace bf {
 namespace {
 
-constexpr int kAtWaves = 4;
 constexpr float kLow = -1e30f;                     // a maximum below every score
-
-template <int BYTES, int ALIGN>
-__device__ __forceinline__ void ld_words(uint32_t* dst, const uint8_t* p) {
-    __builtin_memcpy(dst, __builtin_assume_aligned(p, ALIGN), BYTES);
-}
 
 // One record as a lane holds it.
 template <int NB> struct Kv4Rec {
@@ -47,16 +43,53 @@ template <int NB> struct Kv4Rec {
     uint32_t ks[4 * NB], vs[4 * NB];               // [block][8 tokens] halves
 };
 
-constexpr int align_of(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : 4; }
+// Records of a wave in LDS: one being multiplied, the others on their way.
+template <int NB> constexpr int kRecBytes = 1152 * NB;
+template <int NB, int WV> constexpr int kStages = 2;
+// Workgroups of four waves that a CU holds at once (registers and LDS).
+template <int NB> constexpr int kPerCu = NB <= 4 ? 4 : 2;
+
+// A record into LDS: 1 KB per load, the last one of the lanes that are left.
+template <int NB>
+__device__ __forceinline__ void fetch_rec(const uint8_t* rec, uint32_t lds, int lane) {
+    constexpr int full = kRecBytes<NB> / 1024, rest = kRecBytes<NB> % 1024 / 16;
+#pragma unroll
+    for (int i = 0; i < full; i++) dma16(rec + 1024 * i + 16 * lane, lds + 1024 * i);
+    if constexpr (rest > 0) {
+        if (lane < rest) dma16(rec + 1024 * full + 16 * lane, lds + 1024 * full);
+    }
+}
+template <int NB> constexpr int kRecLoads = (kRecBytes<NB> + 1023) / 1024;
+
+// w words (a constant wherever this is unrolled) from an address aligned to w or four of them.
+__device__ __forceinline__ void ld_words(uint32_t* dst, const uint8_t* p, int w) {
+    if (w == 4) {
+        const u4 v = *(const u4*)p;
+        dst[0] = v.x; dst[1] = v.y; dst[2] = v.z; dst[3] = v.w;
+    } else if (w == 2) {
+        const uint2 v = *(const uint2*)p;
+        dst[0] = v.x; dst[1] = v.y;
+    } else {
+        for (int i = 0; i < w; i++) dst[i] = ((const uint32_t*)p)[i];
+    }
+}
 
 template <int NB>
-__device__ __forceinline__ void load_rec(Kv4Rec<NB>& x, const uint8_t* rec, int r, int g) {
-    const uint8_t* kp = rec + 16 * NB * (8 * (r >> 2) + (r & 3)) + 4 * NB * g;
-    ld_words<4 * NB, align_of(4 * NB)>(x.k[0], kp);
-    ld_words<4 * NB, align_of(4 * NB)>(x.k[1], kp + 64 * NB);
-    ld_words<8 * NB, align_of(8 * NB)>(x.v, rec + kv4_v_at(32 * NB) + 128 * NB * g + 8 * NB * r);
-    ld_words<16 * NB, 16>(x.ks, rec + kv4_ks_at(32 * NB) + 16 * NB * g);
-    ld_words<16 * NB, 16>(x.vs, rec + kv4_vs_at(32 * NB) + 16 * NB * g);
+__device__ __forceinline__ void read_rec(Kv4Rec<NB>& x, const uint8_t* rec, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int b = 0; b < NB; b += 4)
+            ld_words(x.k[i] + b, rec + 512 * b + (i * 64 + lane) * 4 * (NB - b < 4 ? NB - b : 4), NB - b < 4 ? NB - b : 4);
+#pragma unroll
+    for (int b = 0; b < NB; b += 2)
+        ld_words(x.v + 2 * b, rec + 512 * NB + 512 * b + lane * 8 * (NB - b < 2 ? 1 : 2), NB - b < 2 ? 2 : 4);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        ld_words(x.ks + 4 * b, rec + 1024 * NB + 16 * NB * g + 16 * b, 4);
+        ld_words(x.vs + 4 * b, rec + 1088 * NB + 16 * NB * g + 16 * b, 4);
+    }
 }
 
 __device__ __forceinline__ float half_of(const uint32_t* w, int i) { return half_bits_to_float((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu); }
@@ -75,25 +108,24 @@ __device__ __forceinline__ h8 codes8(const Magic& mg, uint32_t x) {
     return __builtin_bit_cast(h8, u4{low2(mg, x), high2(mg, x), low2(mg, y), high2(mg, y)});
 }
 
-struct Row {                                       // of a row tile
-    int q0, nq, len, rows, row0, h, s;
-};
-
-// The row tile of unit u: ((s heads + h) row_tiles + rt); false where it has no rows.
-__device__ __forceinline__ bool row_tile_of(const Kv4Args& a, const Kv4Plan& p, int u, Row& o) {
-    const int rt = u % p.row_tiles;
-    u /= p.row_tiles;
-    o.h = u % a.c.heads;
-    o.s = u / a.c.heads;
-    o.q0 = min(max(a.q_start[o.s], 0), a.T);
-    const int q1 = min(max(a.q_start[o.s + 1], o.q0), a.T);
-    o.nq = min(q1 - o.q0, a.max_q);
-    o.len = min(max(a.kv_len[o.s], 0), a.max_kv);
-    o.row0 = rt * kKv4Rows;
-    const int64_t left = (int64_t)o.nq * p.group - o.row0;
-    o.rows = left < kKv4Rows ? (int)left : kKv4Rows;
-    return o.rows > 0;
+// {RN16(p d), RN16(q e)}: d and e the low or the high halves of two scale words.  (v_fma_mix forms
+// the product in fp32 and rounds it once.)
+__device__ __forceinline__ uint32_t scaled2(float p, float q, uint32_t d, uint32_t e, bool high) {
+    uint32_t o;
+    if (high) {
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(o) : "v"(p), "v"(d));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(o) : "v"(q), "v"(e));
+    } else {
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(o) : "v"(p), "v"(d));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(o) : "v"(q), "v"(e));
+    }
+    return o;
 }
+
+struct Row {                                       // a row tile of a sequence
+    int s, q0, nq, len, rows, row0;
+    int t0, t1;                                    // tiles of 32 cached tokens that it sees
+};
 
 // Cached tokens [lo, hi) that query i of the sequence sees.
 __device__ __forceinline__ int hi_of(const Kv4Args& a, const Row& o, int i) {
@@ -102,12 +134,26 @@ __device__ __forceinline__ int hi_of(const Kv4Args& a, const Row& o, int i) {
 __device__ __forceinline__ int lo_of(const Kv4Args& a, const Row& o, int i) {
     return a.window > 0 ? max(0, o.len - o.nq + i - a.window + 1) : 0;
 }
-// Tiles [t0, t1) that the row tile sees, and the chunks they make (at least one, perhaps empty).
-__device__ __forceinline__ int chunks_of(const Kv4Args& a, const Kv4Plan& p, const Row& o, int& t0, int& t1) {
-    t0 = lo_of(a, o, o.row0 / p.group) / kKv4Tile;
-    t1 = (hi_of(a, o, (o.row0 + o.rows - 1) / p.group) + kKv4Tile - 1) / kKv4Tile;
-    const int n = t1 - t0;
-    return n > p.chunk ? (n + p.chunk - 1) / p.chunk : 1;
+
+// Item i = s row_tiles + rt; false where it has no rows.
+__device__ __forceinline__ bool row_tile_of(const Kv4Args& a, const Kv4Plan& p, int i, Row& o) {
+    int rt = 0;
+    o.s = i;
+    if (p.row_tiles > 1) {
+        o.s = i / p.row_tiles;
+        rt = i - o.s * p.row_tiles;
+    }
+    const int qa = a.q_start[o.s], qb = a.q_start[o.s + 1], len = a.kv_len[o.s];
+    o.q0 = min(max(qa, 0), a.T);
+    o.nq = min(min(max(qb, o.q0), a.T) - o.q0, a.max_q);
+    o.len = min(max(len, 0), a.max_kv);
+    o.row0 = rt * kKv4Rows;
+    const int64_t left = (int64_t)o.nq * p.group - o.row0;
+    o.rows = left < kKv4Rows ? (int)left : kKv4Rows;
+    if (o.rows <= 0) return false;
+    o.t0 = lo_of(a, o, o.row0 / p.group) / kKv4Tile;
+    o.t1 = max(o.t0, (hi_of(a, o, (o.row0 + o.rows - 1) / p.group) + kKv4Tile - 1) / kKv4Tile);
+    return true;
 }
 
 __device__ __forceinline__ void store_out(const Kv4Args& a, int64_t at, float y) {
@@ -115,31 +161,32 @@ __device__ __forceinline__ void store_out(const Kv4Args& a, int64_t at, float y)
     else ((float*)a.O)[at] = y;
 }
 
-template <int NB>
-__global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p, float* __restrict__ ws) {
-    constexpr int D = 32 * NB, W = D < 128 ? D : 128;
-    __shared__ float xo[kAtWaves][kKv4Rows][W + 4];
-    __shared__ float xm[kAtWaves][kKv4Rows], xl[kAtWaves][kKv4Rows];
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sp = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-    Row o;
-    if (!row_tile_of(a, p, unit, o)) return;
-    int t0, t1;
-    const int chunks = chunks_of(a, p, o, t0, t1);
-    if (sp >= chunks) return;
-    const int c0 = t0 + sp * p.chunk, c1 = min(t1, c0 + p.chunk);
+// Tiles [c0, c1) of head h of a row tile: its rows of O where they are `all` of
+// it, else a slot of the workspace.
+template <int NB, int WV>
+__device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const Row& o, int h, int c0, int c1, bool all,
+                                       int64_t slot, float* __restrict__ ws, uint8_t* lds, float (*xm)[kKv4Rows],
+                                       float (*xl)[kKv4Rows]) {
+    constexpr int D = 32 * NB, W = D < 128 ? D : 128, ST = kStages<NB, WV>;
+    float (*const xo)[kKv4Rows][W + 4] = (float (*)[kKv4Rows][W + 4])lds;   // [WV], once the records are done with
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));                  // its multiples are formed here, not kept across units
+    const int lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ifirst = o.row0 / p.group, ilast = (o.row0 + o.rows - 1) / p.group;
     const int free0 = lo_of(a, o, ilast), free1 = hi_of(a, o, ifirst);   // tokens that every row sees
 
     // The lane's query row (rows past the last repeat it: computed, never stored)
     const int row = o.row0 + min(r, o.rows - 1), iq = row / p.group;
     const int lo = lo_of(a, o, iq), hi = hi_of(a, o, iq);
-    const uint16_t* qp = a.Q + (int64_t)(o.q0 + iq) * a.ldq + (o.h * p.group + row - iq * p.group) * D + 8 * g;
+    const uint16_t* qp = a.Q + (int64_t)(o.q0 + iq) * a.ldq + (h * p.group + row - iq * p.group) * D + 8 * g;
     h8 q[NB];
 #pragma unroll
-    for (int b = 0; b < NB; b++) q[b] = *(const h8*)(qp + 32 * b);
-    const float sc = a.scale * 1.44269504088896341f;
+    for (int b = 0; b < NB; b++) {
+        q[b] = *(const h8*)(qp + 32 * b);
+        if (a.scale < 0.f) q[b] = -q[b];               // so that a larger sum is a larger score
+    }
+    const float sc = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.44269504088896341f, 1e-30f);   // (above 0: -inf stays -inf)
     const Magic mg = make_magic();
 
     f4 olo[NB], ohi[NB];
@@ -152,30 +199,37 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
     // Lane n holds the record of the wave's n-th tile of the next 64 (-1: page absent)
     int recs = 0;
     auto look = [&](int n0) {
-        const int tile = c0 + wave + kAtWaves * (n0 + lane);
+        const int tile = c0 + wave + WV * (n0 + lane);
         recs = -1;
         if (tile < c1) {
             const int pg = tile / per_page, id = tab[pg];
-            if (id >= 0 && id < a.c.pages) recs = (id * a.c.heads + o.h) * per_page + (tile - pg * per_page);
+            if (id >= 0 && id < a.c.pages) recs = (id * a.c.heads + h) * per_page + (tile - pg * per_page);
         }
     };
-    const int mine = c1 - c0 > wave ? (c1 - c0 - wave + kAtWaves - 1) / kAtWaves : 0;
-    Kv4Rec<NB> x, y;
-    int rec = -1;
-    if (mine > 0) {
-        look(0);
-        rec = __builtin_amdgcn_readlane(recs, 0);
-        if (rec >= 0) load_rec<NB>(x, a.data + rec * kv4_record_bytes(D), r, g);
-    }
+    const int mine = c1 - c0 > wave ? (c1 - c0 - wave + WV - 1) / WV : 0;
+    const uint8_t* const ring = lds + wave * (ST * kRecBytes<NB>);
+    const uint32_t ring0 = lds_addr(ring);
+    // Record n into stage n % ST (where its page is absent: record 0, not used)
+    uint32_t here = 0;                             // bit n % 32: record n's page is there
+    auto fetch = [&](int n) {
+        if ((n & 63) == 0) look(n);
+        const int rec = __builtin_amdgcn_readlane(recs, n & 63);
+        here = (here & ~(1u << (n & 31))) | ((rec >= 0 ? 1u : 0u) << (n & 31));
+        fetch_rec<NB>(a.data + max(rec, 0) * kv4_record_bytes(D), ring0 + (n % ST) * kRecBytes<NB>, lane);
+    };
+    for (int n = 0; n < ST - 1 && n < mine; n++) fetch(n);
     for (int n = 0; n < mine; n++) {
-        int next = -1;
-        if (n + 1 < mine) {
-            if (((n + 1) & 63) == 0) look(n + 1);
-            next = __builtin_amdgcn_readlane(recs, (n + 1) & 63);
-            if (next >= 0) load_rec<NB>(y, a.data + next * kv4_record_bytes(D), r, g);
+        // the stage of record n - 1 is free: its values were in registers before they were used
+        if (n + ST - 1 < mine) {
+            fetch(n + ST - 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * kRecLoads<NB>) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        if (rec >= 0) {
-            const int tb = (c0 + wave + kAtWaves * n) * kKv4Tile;
+        if ((here >> (n & 31)) & 1) {
+            Kv4Rec<NB> x;
+            read_rec<NB>(x, ring + (n % ST) * kRecBytes<NB>, lane);
+            const int tb = (c0 + wave + WV * n) * kKv4Tile;
             const bool edge = tb < free0 || tb + kKv4Tile > free1;
             float s[8];
 #pragma unroll
@@ -188,7 +242,7 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
                     for (int e = 0; e < 4; e++) t[e] = __builtin_fmaf(half_of(x.ks + 4 * b, 4 * i + e), d[e], t[e]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * i + e] = t[e] * sc;
+                for (int e = 0; e < 4; e++) s[4 * i + e] = t[e];
             }
             if (edge) {
                 // hidden tokens: no score, and no scale either (a page's unwritten
@@ -206,6 +260,7 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
             float tm = s[0];
 #pragma unroll
             for (int e = 1; e < 8; e++) tm = __builtin_fmaxf(tm, s[e]);
+            tm *= sc;
             if (__any(tm > m + 3.f)) {
                 float mn = __builtin_fmaxf(m, tm);
                 mn = __builtin_fmaxf(mn, __shfl_xor(mn, 16));
@@ -225,17 +280,18 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] - m);
+                s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], sc, -m));
                 l += s[e];
             }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                h8 pd;                                 // tokens 0 2 1 3 4 6 5 7, as the masked bytes come
+                uint32_t pd4[4];                       // tokens 0 2, 1 3, 4 6, 5 7, as the masked bytes come
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int t = (e & 4) | ((e & 1) << 1) | ((e >> 1) & 1);
-                    pd[e] = (_Float16)(s[t] * half_of(x.vs + 4 * b, t));
+                for (int i = 0; i < 4; i++) {
+                    const int t = (i & 2) * 2 + (i & 1);
+                    pd4[i] = scaled2(s[t], s[t + 2], x.vs[4 * b + (t >> 1)], x.vs[4 * b + (t >> 1) + 1], i & 1);
                 }
+                const h8 pd = __builtin_bit_cast(h8, u4{pd4[0], pd4[1], pd4[2], pd4[3]});
                 const uint32_t v0 = x.v[2 * b], v1 = x.v[2 * b + 1], w0 = v0 >> 8, w1 = v1 >> 8;
                 const h8 vl = __builtin_bit_cast(h8, u4{low2(mg, v0), low2(mg, w0), low2(mg, v1), low2(mg, w1)});
                 const h8 vh = __builtin_bit_cast(h8, u4{high2(mg, v0), high2(mg, w0), high2(mg, v1), high2(mg, w1)});
@@ -243,8 +299,6 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
                 ohi[b] = mfma16x16x32(pd, vh, ohi[b]);
             }
         }
-        x = y;
-        rec = next;
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -254,10 +308,7 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
         xm[wave][r] = m;
         xl[wave][r] = l;
     }
-    float M = 0.f, L = 0.f, f[kAtWaves];
-    const int orow = threadIdx.x >> 4, oc = threadIdx.x & 15;
-    const int arow = o.row0 + orow, ai = arow / p.group, ah = o.h * p.group + arow - ai * p.group;
-    const int64_t part = (int64_t)unit * p.splits + sp;
+    __syncthreads();                               // every wave is done with its records
 #pragma unroll
     for (int cc = 0; cc < D; cc += W) {
         if (cc) __syncthreads();
@@ -269,64 +320,89 @@ __global__ __launch_bounds__(64 * kAtWaves) void k_kv4_attn(Kv4Args a, Kv4Plan p
                 xo[wave][4 * g + e][32 * b - cc + 16 + r] = ohi[b][e];
             }
         __syncthreads();
-        if (cc == 0) {
-            M = xm[0][orow];
+        constexpr int TPR = 64 * WV / kKv4Rows;
+        const int orow = tid / TPR, oc = tid % TPR;
+        if (orow >= o.rows) continue;
+        const int arow = o.row0 + orow, ai = arow / p.group, ah = h * p.group + arow - ai * p.group;
+        float M = xm[0][orow], L = 0.f, f[WV];
 #pragma unroll
-            for (int w = 1; w < kAtWaves; w++) M = __builtin_fmaxf(M, xm[w][orow]);
+        for (int w = 1; w < WV; w++) M = __builtin_fmaxf(M, xm[w][orow]);
 #pragma unroll
-            for (int w = 0; w < kAtWaves; w++) {
-                f[w] = __builtin_amdgcn_exp2f(xm[w][orow] - M);
-                L += xl[w][orow] * f[w];
-            }
+        for (int w = 0; w < WV; w++) {
+            f[w] = __builtin_amdgcn_exp2f(xm[w][orow] - M);
+            L += xl[w][orow] * f[w];
         }
-        if (orow < o.rows) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            for (int c = oc; c < W && cc + c < D; c += 16) {
-                float y = 0.f;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        for (int c = oc; c < W && cc + c < D; c += TPR) {
+            float y = 0.f;
 #pragma unroll
-                for (int w = 0; w < kAtWaves; w++) y += xo[w][orow][c] * f[w];
-                if (chunks > 1) ws[part * (kKv4Rows * D) + orow * D + cc + c] = y;
-                else store_out(a, (int64_t)(o.q0 + ai) * a.ldo + ah * D + cc + c, y * inv);
-            }
+            for (int w = 0; w < WV; w++) y += xo[w][orow][c] * f[w];
+            if (!all) ws[slot * (kKv4Rows * D) + orow * D + cc + c] = y;
+            else store_out(a, (int64_t)(o.q0 + ai) * a.ldo + ah * D + cc + c, y * inv);
         }
-    }
-    if (orow < o.rows && oc == 0) {
-        if (chunks > 1) {
-            float* ml = ws + p.parts * (kKv4Rows * D) + part * (2 * kKv4Rows) + 2 * orow;
-            ml[0] = M;
-            ml[1] = L;
-        } else if (a.lse) {
-            a.lse[(int64_t)(o.q0 + ai) * a.q_heads + ah] =
-                L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * 0.693147180559945309f;
+        if (cc == 0 && oc == 0) {
+            if (!all) {
+                float* ml = ws + p.slots * (kKv4Rows * D) + slot * (2 * kKv4Rows) + 2 * orow;
+                ml[0] = M;
+                ml[1] = L;
+            } else if (a.lse) {
+                a.lse[(int64_t)(o.q0 + ai) * a.q_heads + ah] =
+                    L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * 0.693147180559945309f;
+            }
         }
     }
 }
 
-// The chunks of a row, joined: one workgroup a row, its waves taking chunks in turn.
-template <int NB>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4Args a, Kv4Plan p, const float* __restrict__ ws) {
-    constexpr int D = 32 * NB, C = (D + 63) / 64;
-    __shared__ float xo[4][D];
-    __shared__ float xl[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int unit = blockIdx.x / kKv4Rows, row = blockIdx.x % kKv4Rows;
+// Item of a workgroup: grid y, and z in steps of kGridY.
+constexpr int kGridY = 32768;
+__device__ __forceinline__ int64_t grid_item() { return (int64_t)blockIdx.z * kGridY + blockIdx.y; }
+
+template <int NB, int WV>
+__global__ __launch_bounds__(64 * WV, kPerCu<NB>) void k_kv4_attn(Kv4Args a, Kv4Plan p, float* __restrict__ ws) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ float xm[WV][kKv4Rows], xl[WV][kKv4Rows];
+    const int64_t item = grid_item();
+    if (item >= p.items) return;
+    int sp = 0, h = blockIdx.x;
+    if (p.splits > 1) {
+        sp = blockIdx.x / a.c.heads;
+        h = blockIdx.x - sp * a.c.heads;
+    }
     Row o;
-    if (!row_tile_of(a, p, unit, o) || row >= o.rows) return;
-    int t0, t1;
-    const int chunks = chunks_of(a, p, o, t0, t1);
-    if (chunks == 1) return;
-    const int64_t part = (int64_t)unit * p.splits;
-    const float* ml = ws + p.parts * (kKv4Rows * D) + part * (2 * kKv4Rows) + 2 * row;
+    if (!row_tile_of(a, p, (int)item, o)) return;
+    const int c0 = o.t0 + sp * p.chunk;
+    if (sp > 0 && c0 >= o.t1) return;
+    attend<NB, WV>(a, p, o, h, c0, min(o.t1, c0 + p.chunk), o.t1 - o.t0 <= p.chunk, (item * a.c.heads + h) * p.splits + sp,
+                   ws, lds, xm, xl);
+}
+
+// The chunks of a row, joined: one workgroup a row, its waves taking chunks in turn.
+template <int NB, int WV>
+__global__ __launch_bounds__(64 * WV) void k_kv4_join(Kv4Args a, Kv4Plan p, int most, const float* __restrict__ ws) {
+    constexpr int D = 32 * NB, C = (D + 63) / 64;
+    __shared__ float xo[WV][D];
+    __shared__ float xl[WV];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t item = grid_item();
+    if (item >= p.items) return;
+    const int h = blockIdx.x / most, row = blockIdx.x - h * most;
+    Row o;
+    if (!row_tile_of(a, p, (int)item, o) || row >= o.rows) return;
+    const int parts = (o.t1 - o.t0 + p.chunk - 1) / p.chunk;
+    if (parts <= 1) return;
+    const int64_t slot = (item * a.c.heads + h) * p.splits;
+    const float* const mls = ws + p.slots * (kKv4Rows * D) + 2 * row;
     float M = kLow;
-    for (int s = lane; s < chunks; s += 64) M = __builtin_fmaxf(M, ml[s * (2 * kKv4Rows)]);
+    for (int i = lane; i < parts; i += 64) M = __builtin_fmaxf(M, mls[(slot + i) * (2 * kKv4Rows)]);
 #pragma unroll
     for (int x = 32; x; x >>= 1) M = __builtin_fmaxf(M, __shfl_xor(M, x));
     float y[C] = {}, L = 0.f;
 #pragma unroll 4
-    for (int s = wave; s < chunks; s += 4) {
-        const float f = __builtin_amdgcn_exp2f(ml[s * (2 * kKv4Rows)] - M);
-        L += f * ml[s * (2 * kKv4Rows) + 1];
-        const float* src = ws + (part + s) * (kKv4Rows * D) + row * D;
+    for (int i = wave; i < parts; i += WV) {
+        const int64_t s = slot + i;
+        const float f = __builtin_amdgcn_exp2f(mls[s * (2 * kKv4Rows)] - M);
+        L += f * mls[s * (2 * kKv4Rows) + 1];
+        const float* src = ws + s * (kKv4Rows * D) + row * D;
 #pragma unroll
         for (int c = 0; c < C; c++)
             if (lane + 64 * c < D) y[c] += f * src[lane + 64 * c];
@@ -336,24 +412,57 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Args a, Kv4Plan p, const fl
         if (lane + 64 * c < D) xo[wave][lane + 64 * c] = y[c];
     if (lane == 0) xl[wave] = L;
     __syncthreads();
-    const int arow = o.row0 + row, ai = arow / p.group, ah = o.h * p.group + arow - ai * p.group;
-    L = xl[0] + xl[1] + xl[2] + xl[3];
+    const int arow = o.row0 + row, ai = arow / p.group, ah = h * p.group + arow - ai * p.group;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < WV; w++) L += xl[w];
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    for (int c = threadIdx.x; c < D; c += 256)
-        store_out(a, (int64_t)(o.q0 + ai) * a.ldo + ah * D + c, (xo[0][c] + xo[1][c] + xo[2][c] + xo[3][c]) * inv);
+    for (int c = threadIdx.x; c < D; c += 64 * WV) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WV; w++) v += xo[w][c];
+        store_out(a, (int64_t)(o.q0 + ai) * a.ldo + ah * D + c, v * inv);
+    }
     if (a.lse && threadIdx.x == 0)
         a.lse[(int64_t)(o.q0 + ai) * a.q_heads + ah] =
             L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * 0.693147180559945309f;
 }
 
+int join_rows(const Kv4Args& a, const Kv4Plan& p) { return (int)std::min<int64_t>(kKv4Rows, (int64_t)a.max_q * p.group); }
+
+dim3 grid_of(const Kv4Plan& p, int64_t x) {
+    return dim3((unsigned)x, (unsigned)std::min<int64_t>(p.items, kGridY), (unsigned)((p.items + kGridY - 1) / kGridY));
+}
+
+template <int NB, int WV>
+hipError_t launch(const Kv4Args& a, const Kv4Plan& p, float* ws, hipStream_t st) {
+    constexpr int W = NB < 4 ? 32 * NB : 128, ring = WV * kStages<NB, WV> * kRecBytes<NB>, meet = WV * kKv4Rows * (W + 4) * 4;
+    constexpr int lds = ring > meet ? ring : meet;
+    auto k = k_kv4_attn<NB, WV>;
+    static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    hipLaunchKernelGGL(k, grid_of(p, (int64_t)p.splits * a.c.heads), dim3(64 * WV), lds, st, a, p, ws);
+    e = hipGetLastError();
+    if (e != hipSuccess || p.slots == 0) return e;
+    const int most = join_rows(a, p);
+    const dim3 grid = grid_of(p, (int64_t)a.c.heads * most);
+    // many chunks a row: more waves on each
+    if (p.splits > 32) hipLaunchKernelGGL((k_kv4_join<NB, 16>), grid, dim3(1024), 0, st, a, p, most, ws);
+    else hipLaunchKernelGGL((k_kv4_join<NB, 4>), grid, dim3(256), 0, st, a, p, most, ws);
+    return hipGetLastError();
+}
+
 template <int NB>
 hipError_t launch(const Kv4Args& a, const Kv4Plan& p, float* ws, hipStream_t st) {
-    const int64_t units = (int64_t)a.S * a.c.heads * p.row_tiles;
-    hipLaunchKernelGGL(k_kv4_attn<NB>, dim3((unsigned)(units * p.splits)), dim3(64 * kAtWaves), 0, st, a, p, ws);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL(k_kv4_join<NB>, dim3((unsigned)(units * kKv4Rows)), dim3(256), 0, st, a, p, ws);
-    return hipGetLastError();
+    return p.waves == 8 ? launch<NB, 8>(a, p, ws, st) : launch<NB, 4>(a, p, ws, st);
 }
 
 Kv4Plan plan_of(const Kv4Args& a) { return plan_kv4(a, device_cus() > 0 ? device_cus() : 256); }
@@ -362,8 +471,8 @@ Kv4Plan plan_of(const Kv4Args& a) { return plan_kv4(a, device_cus() > 0 ? device
 
 bool kv4_attention_fits(const Kv4Args& a) {
     const Kv4Plan p = plan_of(a);
-    const int64_t units = (int64_t)a.S * a.c.heads * p.row_tiles;
-    return launch_fits(units * p.splits, 64 * kAtWaves) && launch_fits(units * kKv4Rows, 256);
+    return launch_fits((int64_t)p.splits * a.c.heads, 64 * p.waves) && launch_fits((int64_t)a.c.heads * kKv4Rows, 1024) &&
+           p.items <= (int64_t)kGridY * 65535 && p.items * a.c.heads * p.splits * (64 * p.waves) < (int64_t(1) << 40);
 }
 
 size_t kv4_attention_scratch_bytes(const Kv4Args& a) { return plan_of(a).bytes; }

@@ -29,18 +29,31 @@ struct Kv4Args {
 };
 
 constexpr int kKv4Rows = 16;                       // query rows of a row tile (one matrix operand)
-constexpr int kKv4MaxSplits = 128;
 
-// Rows of one key/value head: query i and head j of the group, row i G + j.
-// Row tiles of 16; the tiles of 32 cached tokens that a row tile sees are cut
-// into chunks, one workgroup each.  A sequence's chunks are counted by the
-// kernel from its own length; `splits` is the most any of them can have.
+// Rows of one key/value head: query i and head j of the group, row i G + j, in
+// row tiles of 16.  An item is a row tile of a sequence; with a head it is a
+// unit.  The tiles of 32 cached tokens that a unit sees are cut into chunks, a
+// workgroup each; how many chunks a unit has the kernel finds from the lengths,
+// which live in device memory (`splits`: the most that any can have).  Units of
+// several chunks leave partial results, which a second launch joins.
 struct Kv4Plan {
-    int group, row_tiles, chunk, splits;
-    int64_t parts;                                 // partial results (0 where no sequence can have two chunks)
+    int group, row_tiles, waves, chunk, splits;
+    int64_t items;                                 // sequences x row tiles
+    int64_t slots;                                 // partial results (0: no unit can have two chunks)
     size_t bytes;                                  // their workspace
 };
 
+constexpr int kKv4Alone = 40;                      // tiles that one workgroup takes rather than share them
+constexpr int kKv4LeastChunk = 20;
+constexpr int kKv4PerCu = 4;                       // workgroups of four waves that a CU holds
+
+// Chunks: three times as many as the chip has places where that leaves each
+// kKv4LeastChunk tiles, so that sequences of different lengths even out
+// (measured at 32 sequences of 2000 to 8000 tokens, 8 heads of 128: chunks of
+// 12 / 20 / 40 / 64 tiles 60.6 / 58.6 / 58.7 / 64.0 us; one sequence of 131072,
+// 4 heads: 16 / 24 / 40 / 64 tiles 29.1 / 27.6 / 27.6 / 33.8 us).  Short
+// sequences are not cut (16 queries' heads over 1024 tokens of 64 values: 8.0
+// us alone, 11.3 us in chunks of 12).
 inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
     Kv4Plan p;
     p.group = a.q_heads / a.c.heads;
@@ -50,15 +63,14 @@ inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
         const int64_t span = std::min<int64_t>(a.max_q, (kKv4Rows + p.group - 2) / p.group + 1);
         seen = std::min<int64_t>(seen, (int64_t)a.window + span - 1);
     }
-    const int64_t most = (seen + 2 * kKv4Tile - 2) / kKv4Tile;   // the range may start inside a tile
-    const int64_t units = (int64_t)a.S * a.c.heads * p.row_tiles;
-    // About three workgroups of four waves per CU, at least a tile for each wave
-    const int64_t want = (units * most + 3 * cus - 1) / (3 * cus);
-    const int64_t least = (most + kKv4MaxSplits - 1) / kKv4MaxSplits;
-    p.chunk = (int)std::min(most, std::max({want, least, (int64_t)4}));
+    const int64_t most = std::max<int64_t>(1, (seen + 2 * kKv4Tile - 2) / kKv4Tile);   // the range may start inside a tile
+    p.items = (int64_t)a.S * p.row_tiles;
+    const int64_t units = p.items * a.c.heads, places = (int64_t)cus * (a.c.dim == 256 ? 2 : kKv4PerCu);
+    p.chunk = (int)(most <= kKv4Alone ? most : std::min(most, std::max<int64_t>(kKv4LeastChunk, (units * most + 3 * places - 1) / (3 * places))));
     p.splits = (int)((most + p.chunk - 1) / p.chunk);
-    p.parts = p.splits > 1 ? units * p.splits : 0;
-    p.bytes = (size_t)p.parts * kKv4Rows * (a.c.dim + 2) * sizeof(float);
+    p.waves = units * p.splits < cus ? 8 : 4;      // few workgroups: twice the waves on each
+    p.slots = p.splits > 1 ? units * p.splits : 0;
+    p.bytes = (size_t)p.slots * kKv4Rows * (a.c.dim + 2) * sizeof(float);
     return p;
 }
 

@@ -260,6 +260,11 @@ def test_query_magnitudes(qscale):
     Sequences([150], 2, 64).check([1], 4, qscale=qscale, scale=0.125 / qscale)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_scales_of_zero_and_below(scale):
+    Sequences([45, 130], 2, 64).check([3, 1], 2, scale=scale)
+
+
 def test_sharp_softmax():
     """Scores hundreds apart: the running maximum climbs from record to record.  (The score's fp32 error, 2^-22 of
     sums of |q k| near 3000, is part of p here: up to 2^-10, hence values of one sign and a bound on the whole.)"""
