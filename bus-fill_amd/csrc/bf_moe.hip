@@ -9,16 +9,21 @@
 //
 // Bound by the weights of the experts in use, each read once.
 #include <algorithm>
+#include <atomic>
 #include <climits>
+#include <cstdlib>
+#include <type_traits>
 
 #include "bf_formats.h"
 #include "bf_grid.h"
+#include "bf_lds.h"
 #include "bf_moe_launch.h"
 
 namespace bf {
 namespace {
 
-constexpr int kMoeWaves = 4;
+constexpr int kMoeWaves = 8;
+constexpr int kMoeStages = 2;                      // super-groups of a wave's weights in LDS
 constexpr int kScanSlots = 1024;                   // up to so many slots a workgroup finds its expert's by itself
 
 // Slots of one expert: in LDS (found by the workgroup), or in the plan's list.
@@ -27,164 +32,219 @@ struct Lists {
     const int32_t* offs;                           // [E + 1]
 };
 
-template <int QT, int NM> struct MoeW {
-    const uint8_t* W[NM];
-    const uint8_t* aux[NM];
+struct MoeW {                                      // gate and up, or down
+    const uint8_t *W[2], *aux[2];
 };
 
-// Sums of a lane's two 32-value sub-blocks as the operand that meets the mins:
-// {S / 32, S' / 32, 64 (S - hi), 64 (S' - hi')}, zero above.
-__device__ __forceinline__ h8 block_sums(const h8 a[8]) {
-    const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
-    h8 o;
-#pragma unroll
-    for (int e = 0; e < 8; e++) o[e] = (_Float16)0.f;
-#pragma unroll
-    for (int b = 0; b < 2; b++) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) s = __builtin_amdgcn_fdot2(h2{a[4 * b + i][e], a[4 * b + i][e + 1]}, one, s, false);
-        const _Float16 hi = (_Float16)(s * 0.03125f);
-        o[b] = hi;
-        o[2 + b] = (_Float16)((s - 32.f * (float)hi) * 64.f);
-    }
-    return o;
-}
-
-// One super-group: acc += a . w for NM matrices' 16 rows.  Q4_K weights enter as
-// the integers sc q, exact, and d and dmin multiply the super-group's sums; the
-// Q4_0 formats' as their fp16 dequant.
-template <int QT, int NM, int MT>
-__device__ __forceinline__ void multiply(const Magic& mg, const Raw<QT> raw[NM], const h8 a[MT][8], int kg, f4 acc[NM][MT]) {
+// One super-group of 16 weight rows: acc += a . w.  Q4_K weights enter as the
+// integers sc q and m, exact, and d and dmin multiply the super-group's sums: m
+// is one number for all of a lane's 32 weights of a sub-block, so sum_k a_k m_k
+// is a second product with that number as its operand (summing the activations
+// per sub-block first takes 44 more vector instructions of 200, and the matrix
+// unit has the time).  The Q4_0 formats' weights enter as their fp16 dequant.
+template <int QT, int MT>
+__device__ __forceinline__ void multiply(const Magic& mg, const Raw<QT>& raw, const h8 a[MT][8], int kg, f4 acc[MT]) {
     if constexpr (QT == QT_Q4_K) {
-        h8 as[MT];
+        const SclK sc = scales_int(raw, kg);
+        // {m, m'} of sub-blocks 2 kg, 2 kg + 1 (min_hi is 32 times them, exact)
+        const h2 mm = as_h2(sc.min_hi) * h2{(_Float16)0.03125f, (_Float16)0.03125f};
+        h8 mn[2];
 #pragma unroll
-        for (int t = 0; t < MT; t++) as[t] = block_sums(a[t]);
+        for (int e = 0; e < 8; e++) {
+            mn[0][e] = mm[0];
+            mn[1][e] = mm[1];
+        }
+        f4 s[MT], z[MT];
 #pragma unroll
-        for (int m = 0; m < NM; m++) {
-            const SclK sc = scales_int(raw[m], kg);
-            f4 s[MT], z[MT];
+        for (int t = 0; t < MT; t++) s[t] = z[t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < MT; t++) s[t] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const h8 w = weights_int(mg, raw[m], sc, i);
-#pragma unroll
-                for (int t = 0; t < MT; t++) s[t] = mfma16x16x32(a[t][i], w, s[t]);
-            }
-            const h8 mn = __builtin_bit_cast(h8, u4{sc.min_hi, sc.min_lo, 0u, 0u});
+        for (int i = 0; i < 8; i++) {
+            const h8 w = weights_int(mg, raw, sc, i);
 #pragma unroll
             for (int t = 0; t < MT; t++) {
-                z[t] = mfma16x16x32(as[t], mn, f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    acc[m][t][e] = __builtin_fmaf(sc.d, s[t][e], __builtin_fmaf(-sc.dmin, z[t][e], acc[m][t][e]));
+                s[t] = mfma16x16x32(a[t][i], w, s[t]);
+                z[t] = mfma16x16x32(a[t][i], mn[i >> 2], z[t]);
             }
         }
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[t][e] = __builtin_fmaf(sc.d, s[t][e], __builtin_fmaf(-sc.dmin, z[t][e], acc[t][e]));
     } else {
+        const Scl<QT> sc = scales(raw, kg);
 #pragma unroll
-        for (int m = 0; m < NM; m++) {
-            const Scl<QT> sc = scales(raw[m], kg);
+        for (int i = 0; i < 8; i++) {
+            const h8 w = weights(mg, raw, sc, i);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const h8 w = weights(mg, raw[m], sc, i);
-#pragma unroll
-                for (int t = 0; t < MT; t++) acc[m][t] = mfma16x16x32(a[t][i], w, acc[m][t]);
-            }
+            for (int t = 0; t < MT; t++) acc[t] = mfma16x16x32(a[t][i], w, acc[t]);
         }
     }
 }
 
-// Up to 16 MT slots of one expert against 16 weight rows of NM matrices: the
-// waves take super-groups in turn and meet in LDS.  GU: h of the slots; else y.
-template <int QT, int MT, bool GU>
-__device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW<QT, GU ? 2 : 1>& w, const uint16_t* A, int64_t lda,
-                                        void* out, int R, int K, int64_t n0, int f0, const int32_t* list, int cnt,
-                                        float* red) {
-    constexpr int NM = GU ? 2 : 1, RS = 20;        // LDS row stride: the four row groups of a wave on distinct banks
+// One super-group (144 bytes a row) of 16 weight rows into LDS, row after row:
+// pieces of 16 bytes, nine to a row.  Neighbouring lanes fetch neighbouring
+// pieces: as operand registers, where neighbouring lanes are different rows, the
+// same bytes took 192 accesses to the L1 cache and the activations 128 more
+// (86 % of its cycles at 32 rows, 64 experts; 228 us there, 138 from LDS).
+constexpr int kTileBytes = 16 * 144, kTileLoads = 3;
+template <int QT> struct TileFetch {
+    const uint8_t* src[kTileLoads];
+    uint32_t step[kTileLoads];                     // bytes from one super-group to the next
+    __device__ __forceinline__ void init(const uint8_t* W, const uint8_t* aux, int64_t n0, int rows, int K, int lane) {
+#pragma unroll
+        for (int q = 0; q < kTileLoads; q++) {
+            const int p = min(64 * q + lane, 143), row = p / 9, part = p - 9 * row;
+            src[q] = w_piece<QT>(W, aux, n0 + min(row, rows - 1), 0, part, K);
+            step[q] = QT != QT_PLANES ? 144 : part == 0 ? 16 : 128;
+        }
+    }
+    __device__ __forceinline__ void get(int s, uint32_t lds, int lane) const {
+#pragma unroll
+        for (int q = 0; q < kTileLoads; q++)
+            if (q < 2 || lane < 16) dma16(src[q] + (uint64_t)step[q] * s, lds + 1024 * q);
+    }
+};
+
+// The activations of a pass in LDS: slabs of CH super-groups of each row, two of
+// them (one being multiplied, one on its way), rows 16 bytes apart in banks.
+template <int CH> constexpr int kSlabRow = CH * 512 + 16;
+
+// Waits until at most n + BASE of the wave's loads are on their way (n <= 8; else BASE).
+template <int BASE>
+__device__ __forceinline__ void wait_loads(int n) {
+#define BF_WAIT(i) case i: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BASE + i) : "memory"); break;
+    switch (n) {
+        BF_WAIT(1) BF_WAIT(2) BF_WAIT(3) BF_WAIT(4) BF_WAIT(5) BF_WAIT(6) BF_WAIT(7) BF_WAIT(8)
+        default: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BASE) : "memory");
+    }
+#undef BF_WAIT
+}
+
+// Up to 16 MT slots of one expert against the weight rows of a workgroup: eight
+// waves, KS of them over the super-groups of one 16-row tile of one matrix (GU:
+// gate, up), each through a ring of its own, the activations shared; the waves
+// meet in LDS at the end.  GU: h of the slots; else y.
+template <int QT, int MT, bool GU, int KS>
+__device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out, int R,
+                                        int K, int64_t e, int tile0, const int32_t* list, int cnt, int cap, uint8_t* lds) {
+    constexpr int NM = GU ? 2 : 1, TW = kMoeWaves / (KS * NM), CH = KS < 2 ? 2 : KS, PER = CH / KS, ST = kMoeStages;
+    constexpr int RS = 20, TS = 16 * RS;           // stride of the sums' rows: the four row groups of a wave on distinct banks
     const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nsg = K >> 8;
-    const int64_t n = n0 + min(f0 + r, R - 1);
-    const uint16_t* ap[MT];
+    const int kp = wave % KS, mat = wave / KS % NM, tile = tile0 + wave / (KS * NM);
+    const int nsg = K >> 8, slabs = (nsg + CH - 1) / CH;
+    float* const red = (float*)lds;                // [wave][MT][16][RS], over everything else at the end
+    uint8_t* const ring = lds + wave * (ST * kTileBytes);
+    const uint32_t ring0 = lds_addr(ring);
+    uint8_t* const slab = lds + kMoeWaves * ST * kTileBytes;
+    const int slab_bytes = cap * kSlabRow<CH>;
+    const bool live = 16 * tile < R;
+    TileFetch<QT> wf;
+    wf.init(w.W[mat], w.aux[mat], e * R + (live ? 16 * tile : 0), live ? min(16, R - 16 * tile) : 1, K, lane);
+    // slab t: rows wave, wave + 8, ...; CH / 2 loads of 1 KB a row (past the row's end: its start, not used)
+    auto slab_get = [&](int t) {
+        const uint32_t to = lds_addr(slab) + (t & 1) * slab_bytes;
+        for (int i = wave; i < cnt; i += kMoeWaves) {
+            const int slot = list[i];
+            const uint16_t* row = A + (int64_t)(GU ? slot / a.k : slot) * lda;
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
-        const int i = 16 * t + r;
-        ap[t] = i < cnt ? A + (int64_t)(GU ? list[i] / a.k : list[i]) * lda + 64 * kg : nullptr;
-    }
-    const Magic mg = make_magic();
-    f4 acc[NM][MT];
-#pragma unroll
-    for (int m = 0; m < NM; m++)
-#pragma unroll
-        for (int t = 0; t < MT; t++) acc[m][t] = f4{0.f, 0.f, 0.f, 0.f};
-    Raw<QT> raw[NM], nxt[NM];
-    if (wave < nsg) {
-#pragma unroll
-        for (int m = 0; m < NM; m++) load_raw<QT>(raw[m], w.W[m], w.aux[m], n, wave, kg, K);
-    }
-    for (int s = wave; s < nsg; s += kMoeWaves) {
-        h8 x[MT][8];
-#pragma unroll
-        for (int t = 0; t < MT; t++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[t][i] = h8{};
-                if (ap[t]) x[t][i] = ld_act(ap[t] + 256 * s + 8 * i);
+            for (int q = 0; q < CH / 2; q++) {
+                const int c = 256 * CH * t + 512 * q + 8 * lane;
+                dma16(row + (c < K ? c : 0), to + i * kSlabRow<CH> + 1024 * q);
             }
-        if (s + kMoeWaves < nsg) {
-#pragma unroll
-            for (int m = 0; m < NM; m++) load_raw<QT>(nxt[m], w.W[m], w.aux[m], n, s + kMoeWaves, kg, K);
         }
-        multiply<QT, NM, MT>(mg, raw, x, kg, acc);
+    };
+    // the wave's n-th super-group
+    auto sg_at = [&](int n) { return n / PER * CH + kp + n % PER * KS; };
+    const Magic mg = make_magic();
+    f4 acc[MT];
 #pragma unroll
-        for (int m = 0; m < NM; m++) raw[m] = nxt[m];
+    for (int t = 0; t < MT; t++) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();                               // LDS is free
+    slab_get(0);
+    for (int n = 0; n < ST - 1; n++)
+        if (sg_at(n) < nsg) wf.get(sg_at(n), ring0 + n * kTileBytes, lane);
+    int at = 0;                                    // ring stage of the wave's next super-group
+    for (int t = 0; t < slabs; t++) {
+        // slab t is there, for every wave: the loads issued after it are at most the ring's
+        if (t == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        barrier_lds();
+        int newer = 0;                             // loads of the next slab
+        if (t + 1 < slabs) {
+            slab_get(t + 1);
+            newer = cnt > wave ? (cnt - wave + kMoeWaves - 1) / kMoeWaves * (CH / 2) : 0;
+        }
+        bool more = true;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int n = t * PER + j, s = sg_at(n), next = sg_at(n + ST - 1);
+            if (s >= nsg) break;
+            more = next < nsg;
+            if (more) {
+                const int to = at + ST - 1 < ST ? at + ST - 1 : at - 1;
+                wf.get(next, ring0 + to * kTileBytes, lane);
+                // (the wave's first ST - 1 super-groups of a slab were fetched before the next slab's activations)
+                wait_loads<(ST - 1) * kTileLoads>(j < ST - 1 ? newer : 0);
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            Raw<QT> raw;
+            lds_raw<QT>(raw, ring + at * kTileBytes + r * 144, kg);
+            h8 x[MT][8];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const uint8_t* row = slab + (t & 1) * slab_bytes + min(16 * m + r, cnt - 1) * kSlabRow<CH> + (s - CH * t) * 512 + 128 * kg;
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[m][i] = *(const h8*)(row + 16 * i);
+            }
+            multiply<QT, MT>(mg, raw, x, kg, acc);
+            at = at + 1 < ST ? at + 1 : 0;
+        }
+        // the next slab's loads are older than the ring's last one
+        if (t + 1 < slabs) {
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kTileLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
     }
-    __syncthreads();                               // the last use of red and of the list is over
+    __syncthreads();                               // everybody is done with ring and slabs
 #pragma unroll
-    for (int m = 0; m < NM; m++)
+    for (int t = 0; t < MT; t++)
 #pragma unroll
-        for (int t = 0; t < MT; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) red[((wave * NM + m) * MT + t) * (16 * RS) + (4 * kg + e) * RS + r] = acc[m][t][e];
+        for (int i = 0; i < 4; i++) red[(wave * MT + t) * TS + (4 * kg + i) * RS + r] = acc[t][i];
     __syncthreads();
-    const int row = threadIdx.x >> 4, col = threadIdx.x & 15;
-#pragma unroll
-    for (int t = 0; t < MT; t++) {
-        const int i = 16 * t + row;
-        if (i >= cnt || f0 + col >= R) continue;
+    for (int u = threadIdx.x; u < TW * MT * 256; u += 64 * kMoeWaves) {
+        const int tl = u / (MT * 256), t = u / 256 % MT, row = u / 16 % 16, col = u % 16;
+        const int i = 16 * t + row, f = 16 * (tile0 + tl) + col;
+        if (i >= cnt || f >= R) continue;
         float v[NM];
 #pragma unroll
         for (int m = 0; m < NM; m++) {
             v[m] = 0.f;
 #pragma unroll
-            for (int q = 0; q < kMoeWaves; q++) v[m] += red[((q * NM + m) * MT + t) * (16 * RS) + row * RS + col];
+            for (int q = 0; q < KS; q++) v[m] += red[(((tl * NM + m) * KS + q) * MT + t) * TS + row * RS + col];
         }
         const int slot = list[i];
         if constexpr (GU) {
-            const float e = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
-            ((_Float16*)out)[(int64_t)slot * R + f0 + col] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + e) * v[NM - 1] * a.w[slot]);
+            const float ex = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
+            ((_Float16*)out)[(int64_t)slot * R + f] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[NM - 1] * a.w[slot]);
         } else {
-            ((float*)out)[(int64_t)slot * R + f0 + col] = v[0];
+            ((float*)out)[(int64_t)slot * R + f] = v[0];
         }
     }
 }
 
-// grid x: tiles of 16 weight rows; y: experts, or slots where there are fewer
+// grid x: workgroups' weight rows; y: experts, or slots where there are fewer
 // of them (the first slot of an expert stands for it).
-template <int QT, int MT, bool GU>
-__global__ __launch_bounds__(64 * kMoeWaves) void k_moe_rows(MoeArgs a, MoeW<QT, GU ? 2 : 1> w, const uint16_t* A, int64_t lda,
-                                                             void* out, int R, int K, int by_slot, Lists l) {
-    constexpr int NM = GU ? 2 : 1;
-    __shared__ float red[kMoeWaves * NM * MT * 16 * 20];
+template <int QT, int MT, bool GU, int KS>
+__global__ __launch_bounds__(64 * kMoeWaves, MT == 1 ? 4 : 2)
+void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, int R, int K, int by_slot, int cap, Lists l) {
+    constexpr int TW = kMoeWaves / (KS * (GU ? 2 : 1));
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ int32_t found[kScanSlots];
     __shared__ int wave_cnt[kMoeWaves];
     const int slots = a.T * a.k;
     const int e = by_slot ? a.ids[blockIdx.y] : (int)blockIdx.y;
     if (e < 0 || e >= a.E) return;
-    const int f0 = 16 * blockIdx.x;
     const int32_t* list = found;
     int cnt = 0;
     if (l.perm) {
@@ -192,7 +252,6 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_rows(MoeArgs a, MoeW<QT,
         cnt = l.offs[e + 1] - l.offs[e];
     } else {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        bool first = true;                         // no earlier slot has this expert
         for (int s0 = 0; s0 < slots; s0 += 64 * kMoeWaves) {
             const int s = s0 + (int)threadIdx.x;
             const bool hit = s < slots && a.ids[s] == e;
@@ -209,15 +268,13 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_rows(MoeArgs a, MoeW<QT,
             if (hit) found[at + __builtin_popcountll(b & ((1ull << lane) - 1))] = s;
         }
         __syncthreads();
-        if (by_slot) first = found[0] == (int)blockIdx.y;
-        if (!first) return;
+        if (by_slot && found[0] != (int)blockIdx.y) return;
     }
-    const int64_t n0 = (int64_t)e * R;
-    for (int c = 0; c < cnt; c += 16 * MT) {
-        const int left = cnt - c;
-        if (MT > 2 && left > 32) rows_of<QT, MT, GU>(a, w, A, lda, out, R, K, n0, f0, list + c, left < 16 * MT ? left : 16 * MT, red);
-        else if (MT > 1 && left > 16) rows_of<QT, MT < 2 ? MT : 2, GU>(a, w, A, lda, out, R, K, n0, f0, list + c, left < 32 ? left : 32, red);
-        else rows_of<QT, 1, GU>(a, w, A, lda, out, R, K, n0, f0, list + c, left < 16 ? left : 16, red);
+    const int tile0 = TW * (int)blockIdx.x;
+    for (int c = 0; c < cnt; c += cap) {           // (cap <= 16 MT rows a pass)
+        const int n = min(cnt - c, cap);
+        if (MT > 1 && n > 16) rows_of<QT, MT, GU, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
+        else rows_of<QT, 1, GU, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
     }
 }
 
@@ -237,7 +294,7 @@ __device__ __forceinline__ float elem(const uint8_t* W, const uint8_t* aux, int6
 // The same two products, one thread an output: widths that are not whole
 // super-groups, unaligned operands (Q4_0 formats).
 template <int QT, bool GU>
-__global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW<QT, GU ? 2 : 1> w, const uint16_t* A, int64_t lda,
+__global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda,
                                                     void* out, int R, int K) {
     const int64_t slots = (int64_t)a.T * a.k;
     for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < slots * R; i += (int64_t)gridDim.x * 256) {
@@ -326,19 +383,34 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
     }
 }
 
-// c[t] = the sum of its slots' y, in slot order; slots without an expert add nothing.
+// c[t] = the sum of its slots' y, in slot order; slots without an expert add
+// nothing.  Four outputs a thread, a row's slots read together.
 __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const float* __restrict__ y) {
-    const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
-    if (i >= (int64_t)a.T * a.N) return;
-    const int64_t t = i / a.N;
-    const int n = (int)(i - t * a.N);
-    float v = 0.f;
-    for (int j = 0; j < a.k; j++) {
-        const int e = a.ids[t * a.k + j];
-        if (e >= 0 && e < a.E) v += y[(t * a.k + j) * a.N + n];
+    const int t = blockIdx.y, n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x);
+    if (n >= a.N) return;
+    const int32_t* ids = a.ids + (int64_t)t * a.k;
+    const float* row = y + (int64_t)t * a.k * a.N + n;
+    const bool whole = a.N % 4 == 0;
+    f4 v = f4{0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < a.k; j0 += 8) {
+        f4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = f4{0.f, 0.f, 0.f, 0.f};
+            if (j0 + j >= a.k || ids[j0 + j] < 0 || ids[j0 + j] >= a.E) continue;
+            const float* p = row + (int64_t)(j0 + j) * a.N;
+            if (whole) x[j] = *(const f4*)p;
+            else
+                for (int i = 0; i < 4 && n + i < a.N; i++) x[j][i] = p[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) v += x[j];
     }
-    if (a.out_f16) ((_Float16*)a.C)[t * a.ldc + n] = (_Float16)v;
-    else ((float*)a.C)[t * a.ldc + n] = v;
+    const int64_t at = (int64_t)t * a.ldc + n;
+    for (int i = 0; i < 4 && n + i < a.N; i++) {
+        if (a.out_f16) ((_Float16*)a.C)[at + i] = (_Float16)v[i];
+        else ((float*)a.C)[at + i] = v[i];
+    }
 }
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -365,21 +437,40 @@ int64_t a_bytes(const MoeArgs& a) { return ((int64_t)(a.T - 1) * a.lda + a.K) * 
 // grid that fits a launch.
 bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
     const int64_t slots = (int64_t)a.T * a.k, nt = std::max<int64_t>(a.F / 64, (a.N + 127) / 128);
-    return slots >= 16 * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
+    return slots >= (getenv("MOE_TILE") ? atoi(getenv("MOE_TILE")) : 16) * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
            launch_fits(o.max_tiles * nt, 512) && o.max_tiles * nt < INT32_MAX;
 }
 
 bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+template <int QT, bool GU, int MT, int KS>
+hipError_t launch_split(int64_t experts, hipStream_t st, const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out,
+                        int R, int K, int by_slot, const Lists& l) {
+    constexpr int TW = kMoeWaves / (KS * (GU ? 2 : 1)), CH = KS < 2 ? 2 : KS;
+    constexpr int ring = kMoeWaves * kMoeStages * kTileBytes, meet = kMoeWaves * MT * 16 * 20 * 4;
+    constexpr int most = std::max(ring + 2 * 16 * MT * kSlabRow<CH>, meet);
+    const int cap = (int)std::min<int64_t>(16 * MT, (int64_t)a.T * a.k);
+    const int lds = std::max(ring + 2 * cap * kSlabRow<CH>, meet);
+    const int tiles = (R + 15) / 16;
+    auto k = k_moe_rows<QT, MT, GU, KS>;
+    static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != hipSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)((tiles + TW - 1) / TW), (unsigned)experts), dim3(64 * kMoeWaves), lds, st, a, w, A, lda,
+                       out, R, K, by_slot, cap, l);
+    return hipGetLastError();
+}
+
 template <int QT, bool GU>
 hipError_t launch_rows(const MoeArgs& a, const uint16_t* A, int64_t lda, void* out, const Lists& l, bool fast, hipStream_t st) {
-    MoeW<QT, GU ? 2 : 1> w;
-    w.W[0] = GU ? a.gate : a.down;
-    w.aux[0] = GU ? a.gate_aux : a.down_aux;
-    if constexpr (GU) {
-        w.W[1] = a.up;
-        w.aux[1] = a.up_aux;
-    }
+    const MoeW w = GU ? MoeW{{a.gate, a.up}, {a.gate_aux, a.up_aux}} : MoeW{{a.down, nullptr}, {a.down_aux, nullptr}};
     const int R = GU ? a.F : a.N, K = GU ? a.K : a.F;
     const int64_t slots = (int64_t)a.T * a.k;
     if (!fast) {
@@ -391,10 +482,19 @@ hipError_t launch_rows(const MoeArgs& a, const uint16_t* A, int64_t lda, void* o
         }
     }
     const bool by_slot = !l.perm && slots < a.E;
-    const dim3 grid((unsigned)((R + 15) / 16), (unsigned)(by_slot ? slots : a.E));
-    auto k = a.T <= 16 ? k_moe_rows<QT, 1, GU> : a.T <= 32 ? k_moe_rows<QT, 2, GU> : k_moe_rows<QT, 4, GU>;
-    hipLaunchKernelGGL(k, grid, dim3(64 * kMoeWaves), 0, st, a, w, A, lda, out, R, K, (int)by_slot, l);
-    return hipGetLastError();
+    const int64_t experts = by_slot ? slots : a.E;
+    const int64_t waves = (int64_t)((R + 15) / 16) * (GU ? 2 : 1) * std::min<int64_t>(experts, slots);
+    // One wave a tile, but where that leaves the chip empty (K = 2048, F = 1024,
+    // gate and up / down in 4, 2, 1 parts: one row, 8 experts, 1024 waves 16.7,
+    // 18.1, 22.4 us; eight rows, 32 slots, 4096 waves 52.8, 33.7, 29.8).
+    const int ks = waves < 1536 ? 4 : waves < 3072 ? 2 : 1;
+    const auto go = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        return ks == 1 ? launch_split<QT, GU, MT, 1>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
+               : ks == 2 || MT == 2 ? launch_split<QT, GU, MT, 2>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
+                                    : launch_split<QT, GU, 1, 4>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l);
+    };
+    return slots <= 8 * (int64_t)a.E ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 2>());
 }
 
 template <int QT>
@@ -403,7 +503,7 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     const int64_t slots = (int64_t)a.T * a.k;
     const bool fast = moe_fast(a);
     Lists l{nullptr, nullptr};
-    if (fast && slots > kScanSlots) {
+    if (fast && (slots > kScanSlots || getenv("MOE_TILE"))) {
         l = Lists{(const int32_t*)(ws + o.perm), (const int32_t*)(ws + o.offs)};
         hipLaunchKernelGGL(k_moe_plan, dim3((unsigned)a.E), dim3(64 * kPlanWaves), a.E * 4, st, a.ids, (int)slots, a.E,
                            (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs), (int4*)(ws + o.table), (int*)(ws + o.tiles));
@@ -445,7 +545,7 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
         e = launch_rows<QT, false>(a, (const uint16_t*)ws, a.F, ws + o.y, l, fast, st);
     }
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_moe_sum, dim3((unsigned)(((int64_t)a.T * a.N + 255) / 256)), dim3(256), 0, st, a, (const float*)(ws + o.y));
+    hipLaunchKernelGGL(k_moe_sum, dim3((unsigned)((a.N + 1023) / 1024), (unsigned)a.T), dim3(256), 0, st, a, (const float*)(ws + o.y));
     return hipGetLastError();
 }
 
