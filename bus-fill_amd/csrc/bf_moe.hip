@@ -4,14 +4,16 @@
 //
 // over 4-bit weights in place.  A slot is one (t, j).  Three launches: h of
 // every slot (gate and up of the same 16 rows in one workgroup, SiLU(g) u w
-// rounded once to fp16), y = Wd h of every slot (fp32), and the sum of a row's
-// slots in their order.  The row's weight goes into h before its rounding.
+// rounded once to fp16), y = Wd h of every slot (in the output's type: for fp16
+// outputs each y is rounded as the output will be, which halves the bytes
+// between the last two launches, 262 MB of fp32 at 2000 rows of eight slots and
+// 4096 outputs), and the fp32 sum of a row's slots in their order.  The row's
+// weight goes into h before its rounding.
 //
 // Bound by the weights of the experts in use, each read once.
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cstdlib>
 #include <type_traits>
 
 #include "bf_formats.h"
@@ -24,6 +26,7 @@ namespace {
 
 constexpr int kMoeWaves = 8;
 constexpr int kMoeStages = 2;                      // super-groups of a wave's weights in LDS
+constexpr int kSumY = 32768;                       // rows of the sum along grid y
 constexpr int kScanSlots = 1024;                   // up to so many slots a workgroup finds its expert's by itself
 
 // Slots of one expert: in LDS (found by the workgroup), or in the plan's list.
@@ -79,6 +82,11 @@ __device__ __forceinline__ void multiply(const Magic& mg, const Raw<QT>& raw, co
             for (int t = 0; t < MT; t++) acc[t] = mfma16x16x32(a[t][i], w, acc[t]);
         }
     }
+}
+
+__device__ __forceinline__ void store_y(const MoeArgs& a, void* y, int64_t at, float v) {
+    if (a.out_f16) ((_Float16*)y)[at] = (_Float16)v;
+    else ((float*)y)[at] = v;
 }
 
 // One super-group (144 bytes a row) of 16 weight rows into LDS, row after row:
@@ -228,7 +236,7 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
             const float ex = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
             ((_Float16*)out)[(int64_t)slot * R + f] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[NM - 1] * a.w[slot]);
         } else {
-            ((float*)out)[(int64_t)slot * R + f] = v[0];
+            store_y(a, out, (int64_t)slot * R + f, v[0]);
         }
     }
 }
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW w, const uin
             const float ex = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
             ((_Float16*)out)[i] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[1] * a.w[slot]);
         } else {
-            ((float*)out)[i] = v[0];
+            store_y(a, out, i, v[0]);
         }
     }
 }
@@ -322,11 +330,20 @@ __global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW w, const uin
 // sums, so their order does not matter), then every wave writes its own run of
 // slots.
 constexpr int kPlanWaves = 16;
+// Of n slots: runs of 256, and the rest as one more of them from `least` rows on
+// (more than 256: no large tiles at all), else a small tile.
+__device__ __forceinline__ int large_tiles(int n, int least) {
+    return least > kMoeTileRows ? 0 : n / kMoeTileRows + (n % kMoeTileRows >= least);
+}
+__device__ __forceinline__ int small_tiles(int n, int least) {
+    return (n + kMoeTileRows - 1) / kMoeTileRows - large_tiles(n, least);
+}
 __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __restrict__ ids, int slots, int E,
                                                               int32_t* __restrict__ perm, int32_t* __restrict__ offs,
-                                                              int4* __restrict__ table, int* __restrict__ tiles) {
+                                                              int4* __restrict__ table, int* __restrict__ tiles, int max_tiles,
+                                                              int least) {
     extern __shared__ int hist[];
-    __shared__ int same[kPlanWaves], sum[2][kPlanWaves];
+    __shared__ int same[kPlanWaves], sum[3][kPlanWaves];
     const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < E; i += 64 * kPlanWaves) hist[i] = 0;
     __syncthreads();
@@ -341,39 +358,39 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
     for (int x = 32; x; x >>= 1) ns += __shfl_xor(ns, x);
     if (lane == 0) same[wave] = ns;
     __syncthreads();
-    // slots and tiles of the experts before e
-    int nl = 0, nt = 0;
+    // slots and tiles (large, small) of the experts before e
+    int n[3] = {0, 0, 0};
     for (int i = threadIdx.x; i < e; i += 64 * kPlanWaves) {
-        nl += hist[i];
-        nt += (hist[i] + kMoeTileRows - 1) / kMoeTileRows;
+        n[0] += hist[i];
+        n[1] += large_tiles(hist[i], least);
+        n[2] += small_tiles(hist[i], least);
     }
 #pragma unroll
-    for (int x = 32; x; x >>= 1) {
-        nl += __shfl_xor(nl, x);
-        nt += __shfl_xor(nt, x);
-    }
-    if (lane == 0) {
-        sum[0][wave] = nl;
-        sum[1][wave] = nt;
+    for (int c = 0; c < 3; c++) {
+#pragma unroll
+        for (int x = 32; x; x >>= 1) n[c] += __shfl_xor(n[c], x);
+        if (lane == 0) sum[c][wave] = n[c];
     }
     __syncthreads();
-    int base = 0, tile = 0, at = 0;
+    int before[3] = {0, 0, 0}, at = 0;
 #pragma unroll
     for (int q = 0; q < kPlanWaves; q++) {
-        base += sum[0][q];
-        tile += sum[1][q];
+#pragma unroll
+        for (int c = 0; c < 3; c++) before[c] += sum[c][q];
         if (q < wave) at += same[q];
     }
-    const int total = hist[e], mine = (total + kMoeTileRows - 1) / kMoeTileRows;
+    const int base = before[0], total = hist[e], large = large_tiles(total, least), small = small_tiles(total, least);
     if (threadIdx.x == 0) {
         offs[e] = base;
         if (e == E - 1) {
             offs[E] = base + total;
-            *tiles = tile + mine;
+            tiles[0] = before[1] + large;
+            tiles[1] = before[2] + small;
         }
     }
-    for (int i = threadIdx.x; i < mine; i += 64 * kPlanWaves)
-        table[tile + i] = int4{e, base + i * kMoeTileRows, min(kMoeTileRows, total - i * kMoeTileRows), 0};
+    for (int i = threadIdx.x; i < large + small; i += 64 * kPlanWaves)
+        table[i < large ? before[1] + i : max_tiles + before[2] + i - large] =
+            int4{e, base + i * kMoeTileRows, min(kMoeTileRows, total - i * kMoeTileRows), 0};
     at += base;
     for (int s = s0; s < s1; s += 64) {
         const bool hit = s + lane < s1 && ids[s + lane] == e;
@@ -385,28 +402,38 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
 
 // c[t] = the sum of its slots' y, in slot order; slots without an expert add
 // nothing.  Four outputs a thread, a row's slots read together.
-__global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const float* __restrict__ y) {
-    const int t = blockIdx.y, n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x);
-    if (n >= a.N) return;
-    const int32_t* ids = a.ids + (int64_t)t * a.k;
-    const float* row = y + (int64_t)t * a.k * a.N + n;
+template <typename Y>
+__global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const Y* __restrict__ y) {
+    typedef Y y4 __attribute__((ext_vector_type(4)));
+    const int64_t t = (int64_t)blockIdx.z * kSumY + blockIdx.y;
+    const int n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x);
+    if (t >= a.T || n >= a.N) return;
+    const int32_t* ids = a.ids + t * a.k;
+    const Y* row = y + t * a.k * a.N + n;
     const bool whole = a.N % 4 == 0;
     f4 v = f4{0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < a.k; j0 += 8) {
-        f4 x[8];
+        y4 x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            x[j] = f4{0.f, 0.f, 0.f, 0.f};
+            x[j] = y4{0, 0, 0, 0};
             if (j0 + j >= a.k || ids[j0 + j] < 0 || ids[j0 + j] >= a.E) continue;
-            const float* p = row + (int64_t)(j0 + j) * a.N;
-            if (whole) x[j] = *(const f4*)p;
+            const Y* p = row + (int64_t)(j0 + j) * a.N;
+            if (whole) x[j] = *(const y4*)p;
             else
                 for (int i = 0; i < 4 && n + i < a.N; i++) x[j][i] = p[i];
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) v += x[j];
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] += (float)x[j][i];
     }
-    const int64_t at = (int64_t)t * a.ldc + n;
+    const int64_t at = t * a.ldc + n;
+    if (a.out_f16 && whole && a.ldc % 4 == 0 && ((uintptr_t)a.C & 7) == 0) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        *(h4*)((_Float16*)a.C + at) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        return;
+    }
     for (int i = 0; i < 4 && n + i < a.N; i++) {
         if (a.out_f16) ((_Float16*)a.C)[at + i] = (_Float16)v[i];
         else ((float*)a.C)[at + i] = v[i];
@@ -415,29 +442,38 @@ __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const float* __restr
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Workspace: h [slots][F] fp16, y [slots][N] fp32, the plan.
+// Workspace: h [slots][F] fp16, y [slots][N] in the output's type, the plan.
 struct MoeWs {
     size_t y, perm, offs, table, tiles, end;
     int64_t max_tiles;
     explicit MoeWs(const MoeArgs& a) {
         const size_t slots = (size_t)a.T * a.k;
         y = up256(slots * a.F * 2);
-        perm = y + up256(slots * a.N * 4);
+        perm = y + up256(slots * a.N * (a.out_f16 ? 2 : 4));
         offs = perm + up256(slots * 4);
         table = offs + up256(((size_t)a.E + 1) * 4);
         max_tiles = (int64_t)std::min<size_t>(a.E, slots) + (int64_t)(slots / kMoeTileRows);
-        tiles = table + up256((size_t)max_tiles * 16);
+        tiles = table + up256((size_t)max_tiles * 32);
         end = tiles + 256;
     }
 };
 
 int64_t a_bytes(const MoeArgs& a) { return ((int64_t)(a.T - 1) * a.lda + a.K) * 2; }
 
-// The tile kernel: rows addressed with 32 bits from the buffer's start, and a
-// grid that fits a launch.
+// Rows from which a run of slots takes a large tile: 193 where the whole block
+// has twice as many of them as the chip has CUs, else none does.
+int large_least(const MoeArgs& a) {
+    const int64_t slots = (int64_t)a.T * a.k, cus = device_cus() > 0 ? device_cus() : 256;
+    return slots / kMoeTileRows * (std::min(2 * a.F, a.N) / 256) >= 2 * cus ? 193 : kMoeTileRows + 1;
+}
+
+// The tile kernel: from 24 rows an expert on average (64 experts of 2048 x 1024,
+// eight a row: at 130 rows 106 us in rows, 133 in tiles; at 250 rows 164 and
+// 140), rows addressed with 32 bits from the buffer's start, and a grid that
+// fits a launch.
 bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
     const int64_t slots = (int64_t)a.T * a.k, nt = std::max<int64_t>(a.F / 64, (a.N + 127) / 128);
-    return slots >= (getenv("MOE_TILE") ? atoi(getenv("MOE_TILE")) : 16) * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
+    return slots >= 24 * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
            launch_fits(o.max_tiles * nt, 512) && o.max_tiles * nt < INT32_MAX;
 }
 
@@ -503,10 +539,10 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     const int64_t slots = (int64_t)a.T * a.k;
     const bool fast = moe_fast(a);
     Lists l{nullptr, nullptr};
-    if (fast && (slots > kScanSlots || getenv("MOE_TILE"))) {
+    if (fast && (slots > kScanSlots || tiles_serve(a, o))) {
         l = Lists{(const int32_t*)(ws + o.perm), (const int32_t*)(ws + o.offs)};
         hipLaunchKernelGGL(k_moe_plan, dim3((unsigned)a.E), dim3(64 * kPlanWaves), a.E * 4, st, a.ids, (int)slots, a.E,
-                           (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs), (int4*)(ws + o.table), (int*)(ws + o.tiles));
+                           (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs), (int4*)(ws + o.table), (int*)(ws + o.tiles), (int)o.max_tiles, large_least(a));
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -526,8 +562,10 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
         t.out = ws;
         t.R = a.F;
         t.K = a.K;
-        t.nt = a.F / 64;
-        e = moe_tile(a, t, true, o.max_tiles, st);
+        t.nt[0] = a.F / 128;
+        t.nt[1] = a.F / 64;
+        t.max_tiles = (int)o.max_tiles;
+        e = moe_tile(a, t, true, st);
         if (e != hipSuccess) return e;
         t.W[0] = a.down;
         t.aux[0] = a.down_aux;
@@ -537,15 +575,18 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
         t.out = ws + o.y;
         t.R = a.N;
         t.K = a.F;
-        t.nt = (a.N + 127) / 128;
-        e = moe_tile(a, t, false, o.max_tiles, st);
+        t.nt[0] = (a.N + 255) / 256;
+        t.nt[1] = (a.N + 127) / 128;
+        e = moe_tile(a, t, false, st);
     } else {
         e = launch_rows<QT, true>(a, a.A, a.lda, ws, l, fast, st);
         if (e != hipSuccess) return e;
         e = launch_rows<QT, false>(a, (const uint16_t*)ws, a.F, ws + o.y, l, fast, st);
     }
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_moe_sum, dim3((unsigned)((a.N + 1023) / 1024), (unsigned)a.T), dim3(256), 0, st, a, (const float*)(ws + o.y));
+    const dim3 grid((unsigned)((a.N + 1023) / 1024), (unsigned)std::min(a.T, kSumY), (unsigned)((a.T + kSumY - 1) / kSumY));
+    if (a.out_f16) hipLaunchKernelGGL(k_moe_sum<_Float16>, grid, dim3(256), 0, st, a, (const _Float16*)(ws + o.y));
+    else hipLaunchKernelGGL(k_moe_sum<float>, grid, dim3(256), 0, st, a, (const float*)(ws + o.y));
     return hipGetLastError();
 }
 

@@ -39,13 +39,15 @@ struct MoeTileArgs {
     const uint16_t* A;         // rows of tokens, or of slots
     uint32_t a_bytes;          // from A on: below 4 GB
     int64_t lda;
-    void* out;                 // h fp16, or y fp32, by slot
-    int R, K, nt;              // weight rows of an expert, their length, column tiles
+    void* out;                 // h fp16, or y in the output's type, by slot
+    int R, K;                  // weight rows of an expert, their length
+    int nt[2];                 // column tiles of a large and of a small tile's rows
     const int32_t* perm;       // slots by expert
-    const int4* table;         // tiles: expert, first place in perm, rows
-    const int* tiles;          // their number
+    const int4* table;         // max_tiles large tiles, then the small ones: expert, first place in perm, rows
+    const int* tiles;          // how many of either
+    int max_tiles;             // of both together
 };
-hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, int64_t max_tiles, hipStream_t st);
+hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, hipStream_t st);
 
 // The matrix-core kernels serve these widths and alignments.
 bool moe_fast(const MoeArgs& a);

@@ -1,17 +1,18 @@
 // The experts' products for prompts: k_moe_tile, the tile of the prefill GEMM
 // (bf_tile.h) over rows gathered by expert.
 //
-// An expert's slots are cut into runs of 256 rows (the last one shorter: a tile
-// takes 64, 128, 192 or 256 rows); a workgroup multiplies one run with 128
-// weight rows.  Activation rows are fetched through the slot list, row by row,
-// by the direct-to-LDS loads' own per-lane addresses, so nothing is gathered
-// beforehand.
+// An expert's slots are cut into runs of 256.  Whole runs, and a rest of more
+// than 192, take a large tile, 256 rows x 256 weight rows (NB = 2 of bf_tile.h);
+// a shorter rest a small one, 64, 128 or 192 rows x 128 weight rows.  Activation
+// rows are fetched through the slot list, row by row, by the direct-to-LDS
+// loads' own per-lane addresses, so nothing is gathered beforehand.
 //
-// Gate and up: a tile's 128 weight rows are 32 gate rows, the same 32 up rows,
-// and the next 32 of both, which puts g and u of one output into the two column
+// Gate and up: a tile's weight rows are 32 gate rows, the same 32 up rows, and
+// the next 32 of both, which puts g and u of one output into the two column
 // tiles of one wave: h = w SiLU(g) u leaves the registers as the one fp16 row
-// that the down product reads.  Two k groups of waves hold half of each sum;
-// each hands the other half of the rows over and finishes the rest.
+// that the down product reads.  (Small tiles: two k groups of waves hold half of
+// each sum; each hands the other half of the rows over and finishes the rest.)
+#include <algorithm>
 #include <atomic>
 
 #include "bf_moe_launch.h"
@@ -20,11 +21,30 @@
 namespace bf {
 namespace {
 
+// One output pair of a lane: columns c (tile 0) and c + 32 (tile 1) of the wave's 64.
+template <bool GU>
+__device__ __forceinline__ void put(const MoeArgs& a, const MoeTileArgs& o, int slot, int c64, int lane, float y0, float y1) {
+    if constexpr (GU) {
+        const float ex = __builtin_amdgcn_exp2f(y0 * -1.44269504088896341f);
+        ((_Float16*)o.out)[(int64_t)slot * o.R + c64 / 2 + (lane & 31)] =
+            (_Float16)(y0 * __builtin_amdgcn_rcpf(1.0f + ex) * y1 * a.w[slot]);
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int n = c64 + 32 * b + (lane & 31);
+            const int64_t at = (int64_t)slot * o.R + n;
+            if (n >= o.R) continue;
+            if (a.out_f16) ((_Float16*)o.out)[at] = (_Float16)(b ? y1 : y0);
+            else ((float*)o.out)[at] = b ? y1 : y0;
+        }
+    }
+}
+
 // The outputs of a tile: run() of bf_tile.h, then the epilogue above.
-template <int QT, int TA, bool GU>
+template <int QT, int TA, int NB, bool GU>
 __device__ __forceinline__ void moe_tile(uint8_t* lds, const MoeArgs& a, const MoeTileArgs& o, const int32_t* list, int rows,
                                          int64_t e, int ni) {
-    using T = Tile<QT, TA, 1>;
+    using T = Tile<QT, TA, NB>;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     T t;
@@ -37,16 +57,17 @@ __device__ __forceinline__ void moe_tile(uint8_t* lds, const MoeArgs& a, const M
     }
     t.lds0 = lds_addr(lds);
     t.wave = wave;
-    t.j = threadIdx.x & 3;
-    const int wr = threadIdx.x >> 2;
+    constexpr int TPR = 4 / NB;                    // threads of a weight row
+    t.j = threadIdx.x % TPR;
+    const int wr = threadIdx.x / TPR;
     // tile column -> weight row: GU 64 outputs of gate and up, 32 and 32 in turn
-    const int f = GU ? 64 * ni + 32 * (wr >> 6) + (wr & 31) : 128 * ni + wr;
+    const int f = GU ? T::BN / 2 * ni + 32 * (wr >> 6) + (wr & 31) : T::BN * ni + wr;
     const bool up = GU && (wr & 32);
     const int64_t n = e * o.R + min(f, o.R - 1);
     t.row = (up ? o.W[1] : o.W[0]) + n * row_bytes(QT, o.K);
     t.aux = QT == QT_PLANES ? (up ? o.aux[1] : o.aux[0]) + n * (o.K >> 4) : nullptr;
-    t.wst = T::kAStage + wr * 128 + 16 * (tile_chunk<QT, 1>(t.j, 0) ^ ((wr >> 1) & 7));
-    const int kg = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
+    t.wst = T::kAStage + wr * 128 + 16 * (tile_chunk<QT, NB>(t.j, 0) ^ ((wr >> 1) & 7));
+    const int kg = NB == 1 ? wave >> 2 : 0, wm = NB == 1 ? (wave >> 1) & 1 : wave >> 2, wn = wave & (2 * NB - 1);
     const uint32_t fr = (lane & 31) * 128 + 16 * ((4 * kg + (lane >> 5)) ^ ((lane >> 1) & 7));
     t.fa = wm * (32 * TA * 128) + fr;
     t.fw = T::kAStage + wn * (64 * 128) + fr;
@@ -58,6 +79,18 @@ __device__ __forceinline__ void moe_tile(uint8_t* lds, const MoeArgs& a, const M
 #pragma unroll
             for (int x = 0; x < 16; x++) t.acc[i][b][x] = 0.f;
     t.run(lds, 0, o.K >> 8);
+
+    const int c64 = T::BN * ni + 64 * wn;
+    if constexpr (NB == 2) {
+#pragma unroll
+        for (int i = 0; i < TA; i++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) {
+                const int r = 32 * TA * wm + 32 * i + 8 * (x / 4) + 4 * (lane >> 5) + x % 4;
+                if (r < rows) put<GU>(a, o, list[r], c64, lane, t.acc[i][0][x], t.acc[i][1][x]);
+            }
+        return;
+    }
 
     // Group kg finishes accumulator registers 8 kg .. 8 kg + 7 of every tile.
     uint8_t* const xch = lds + (threadIdx.x & 255) * 16;
@@ -88,20 +121,7 @@ __device__ __forceinline__ void moe_tile(uint8_t* lds, const MoeArgs& a, const M
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int r = 32 * TA * wm + 32 * i + 16 * kg + 2 * x + 4 * (lane >> 5) + c;
-                if (r >= rows) continue;
-                const int slot = list[r];
-                if constexpr (GU) {
-                    const float g = y[0][c];
-                    const float ex = __builtin_amdgcn_exp2f(g * -1.44269504088896341f);
-                    ((_Float16*)o.out)[(int64_t)slot * o.R + 64 * ni + 32 * wn + (lane & 31)] =
-                        (_Float16)(g * __builtin_amdgcn_rcpf(1.0f + ex) * y[1][c] * a.w[slot]);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const int n1 = 128 * ni + 64 * wn + 32 * b + (lane & 31);
-                        if (n1 < o.R) ((float*)o.out)[(int64_t)slot * o.R + n1] = y[b][c];
-                    }
-                }
+                if (r < rows) put<GU>(a, o, list[r], c64, lane, y[0][c], y[1][c]);
             }
         }
 }
@@ -110,23 +130,26 @@ template <int QT, bool GU>
 __global__ __launch_bounds__(kTlThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_moe_tile(MoeArgs a, MoeTileArgs o) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    const int units = *o.tiles * o.nt;
+    // large tiles first, so that the small ones fill the last round
+    const int large = o.tiles[0] * o.nt[0], units = large + o.tiles[1] * o.nt[1];
     if ((int)blockIdx.x >= units) return;
-    const int v = xcd_unit((int)blockIdx.x, units), i = v / o.nt, ni = v - i * o.nt;
-    const int4 d = o.table[i];
+    const bool big = (int)blockIdx.x < large;
+    const int v = big ? xcd_unit((int)blockIdx.x, large) : xcd_unit((int)blockIdx.x - large, units - large);
+    const int nt = big ? o.nt[0] : o.nt[1], i = v / nt, ni = v - i * nt;
+    const int4 d = o.table[(big ? 0 : o.max_tiles) + i];
     const int e = __builtin_amdgcn_readfirstlane(d.x), rows = __builtin_amdgcn_readfirstlane(d.z);
     const int32_t* list = o.perm + __builtin_amdgcn_readfirstlane(d.y);
-    if (rows > 192) moe_tile<QT, 4, GU>(lds, a, o, list, rows, e, ni);
-    else if (rows > 128) moe_tile<QT, 3, GU>(lds, a, o, list, rows, e, ni);
-    else if (rows > 64) moe_tile<QT, 2, GU>(lds, a, o, list, rows, e, ni);
-    else moe_tile<QT, 1, GU>(lds, a, o, list, rows, e, ni);
+    if (big) moe_tile<QT, 4, 2, GU>(lds, a, o, list, rows, e, ni);
+    else if (rows > 192) moe_tile<QT, 4, 1, GU>(lds, a, o, list, rows, e, ni);
+    else if (rows > 128) moe_tile<QT, 3, 1, GU>(lds, a, o, list, rows, e, ni);
+    else if (rows > 64) moe_tile<QT, 2, 1, GU>(lds, a, o, list, rows, e, ni);
+    else moe_tile<QT, 1, 1, GU>(lds, a, o, list, rows, e, ni);
 }
 
 template <int QT, bool GU>
-hipError_t launch(const MoeArgs& a, const MoeTileArgs& o, int64_t max_tiles, hipStream_t st) {
-    using T = Tile<QT, 4, 1>;
+hipError_t launch(const MoeArgs& a, const MoeTileArgs& o, hipStream_t st) {
     auto k = k_moe_tile<QT, GU>;
-    constexpr int lds = T::NS * T::kStage;
+    constexpr int lds = std::max(Tile<QT, 4, 1>::NS * Tile<QT, 4, 1>::kStage, Tile<QT, 4, 2>::NS * Tile<QT, 4, 2>::kStage);
     static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -137,21 +160,21 @@ hipError_t launch(const MoeArgs& a, const MoeTileArgs& o, int64_t max_tiles, hip
         if (e != hipSuccess) return e;
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
-    hipLaunchKernelGGL(k, dim3((unsigned)(max_tiles * o.nt)), dim3(kTlThreads), lds, st, a, o);
+    hipLaunchKernelGGL(k, dim3((unsigned)((int64_t)o.max_tiles * o.nt[1])), dim3(kTlThreads), lds, st, a, o);
     return hipGetLastError();
 }
 
 template <int QT>
-hipError_t dispatch(const MoeArgs& a, const MoeTileArgs& o, bool gu, int64_t max_tiles, hipStream_t st) {
-    return gu ? launch<QT, true>(a, o, max_tiles, st) : launch<QT, false>(a, o, max_tiles, st);
+hipError_t dispatch(const MoeArgs& a, const MoeTileArgs& o, bool gu, hipStream_t st) {
+    return gu ? launch<QT, true>(a, o, st) : launch<QT, false>(a, o, st);
 }
 
 }  // namespace
 
-hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, int64_t max_tiles, hipStream_t st) {
-    if (a.qtype == QT_PLANES) return dispatch<QT_PLANES>(a, o, gu, max_tiles, st);
-    if (a.qtype == QT_Q4_0) return dispatch<QT_Q4_0>(a, o, gu, max_tiles, st);
-    return dispatch<QT_Q4_K>(a, o, gu, max_tiles, st);
+hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, hipStream_t st) {
+    if (a.qtype == QT_PLANES) return dispatch<QT_PLANES>(a, o, gu, st);
+    if (a.qtype == QT_Q4_0) return dispatch<QT_Q4_0>(a, o, gu, st);
+    return dispatch<QT_Q4_K>(a, o, gu, st);
 }
 
 }  // namespace bf

@@ -162,13 +162,16 @@ class Experts:
         assert (c[:, self.N:] == 9.0).all()
         return c[:, :self.N]
 
-    def check(self, T, k, seed=3, ids=None, otype=bf.OUT_F32, pad=0, **kw):
+    def check(self, T, k, seed=3, ids=None, otype=bf.OUT_F32, pad=0, rows=None, **kw):
+        """rows: the rows that are compared (all of them by default)."""
         g = torch.Generator().manual_seed(seed)
         wide = torch.randn(T, self.K + pad, generator=g).half()
         if ids is None:
             ids = torch.rand(T, self.E, generator=g).argsort(1)[:, :k]
         w = torch.rand(ids.shape, generator=g) + 0.05
         got = self.run(wide, ids, w, otype=otype, lda=self.K + pad, pad=pad, **kw).cpu().double()
+        if rows is not None:
+            got, wide, ids, w, T = got[rows], wide[rows], ids[rows], w[rows], len(rows)
         x = wide[:, :self.K].double()
         want, tol = torch.zeros(T, self.N).double(), torch.zeros(T, self.N).double()
         rw = 0.0 if self.qt == O.Q4_K else 2.0 ** -11      # the weights' own rounding
@@ -204,6 +207,20 @@ def test_experts_many_slots(qt):
     """More slots than a workgroup looks through by itself: the sorted plan."""
     Experts(qt, 12, 256, 512, 130).check(290, 4, otype=bf.OUT_F16)
     Experts(qt, 3, 512, 256, 64).check(1100, 1)
+
+
+@pytest.mark.parametrize("qt", QTS)
+@pytest.mark.parametrize("otype", [bf.OUT_F32, bf.OUT_F16])
+def test_experts_large_tiles(qt, otype):
+    """Enough rows for tiles of 256 x 256, beside small ones: 16800 slots over 30 experts, one of them with 193 rows and
+    one with 1000, compared at 70 rows and at every row of those two experts' last tiles."""
+    T, k, E = 4200, 4, 30
+    g = torch.Generator().manual_seed(5)
+    ids = 2 + torch.rand(T, E - 2, generator=g).argsort(1)[:, :k]
+    ids[:193, 0] = 0
+    ids[3000:4000, 3] = 1
+    rows = torch.cat([torch.arange(0, 4200, 61), torch.arange(150, 193), torch.arange(3980, 4000)])
+    Experts(qt, E, 256, 1024, 2048).check(T, k, ids=ids, otype=otype, rows=rows)
 
 
 @pytest.mark.parametrize("T", [5, 600])
