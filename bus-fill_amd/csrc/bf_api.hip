@@ -719,6 +719,8 @@ bf_status check_attention(const bf_kv4_cache* c, const bf_kv4_attention_args* a,
         return fail(BF_ERR_INVALID, "lse, q_start, kv_len and page_table must be 4-byte aligned");
     if (a->max_kv > (int64_t)a->ldt * c->page_size)
         return fail(BF_ERR_INVALID, "max_kv=%d > ldt * page_size = %lld", a->max_kv, (long long)a->ldt * c->page_size);
+    if ((int64_t)a->max_q * (a->q_heads / c->kv_heads) > (1 << 30))
+        return fail(BF_ERR_UNSUPPORTED, "max_q=%d: at most 2^30 rows a key/value head", a->max_q);
     if (a->max_kv > INT32_MAX - 64) return fail(BF_ERR_UNSUPPORTED, "max_kv=%d: at most 2^31 - 65", a->max_kv);
     if (a->window < 0 || (a->window > 0 && !a->causal))
         return fail(BF_ERR_INVALID, "window=%d: >= 0, and 0 without causal", a->window);

@@ -29,13 +29,13 @@
 #include <atomic>
 
 #include "bf_grid.h"
+#include "bf_kv4_dev.h"
 #include "bf_kv4_launch.h"
 #include "bf_lds.h"
 
 namespace bf {
 namespace {
 
-constexpr float kLow = -1e30f;                     // a maximum below every score
 
 // One record as a lane holds it.
 template <int NB> struct Kv4Rec {
@@ -90,75 +90,6 @@ __device__ __forceinline__ void read_rec(Kv4Rec<NB>& x, const uint8_t* rec, int 
         ld_words(x.ks + 4 * b, rec + 1024 * NB + 16 * NB * g + 16 * b, 4);
         ld_words(x.vs + 4 * b, rec + 1088 * NB + 16 * NB * g + 16 * b, 4);
     }
-}
-
-__device__ __forceinline__ float half_of(const uint32_t* w, int i) { return half_bits_to_float((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu); }
-
-// Codes of two tokens or values per half: the nibbles at bits 0-3 / 4-7 of each half of x, minus 8.
-__device__ __forceinline__ uint32_t low2(const Magic& mg, uint32_t x) {
-    return as_u32(as_h2(and_or(x, mg.lo_mask, mg.lo_bits)) + h2{(_Float16)-1032.0f, (_Float16)-1032.0f});
-}
-__device__ __forceinline__ uint32_t high2(const Magic& mg, uint32_t x) {
-    return as_u32(as_h2(and_or(x, mg.hi_mask, mg.hi_bits)) + h2{(_Float16)-72.0f, (_Float16)-72.0f});
-}
-
-// Eight K codes of one word, in order.
-__device__ __forceinline__ h8 codes8(const Magic& mg, uint32_t x) {
-    const uint32_t y = x >> 8;
-    return __builtin_bit_cast(h8, u4{low2(mg, x), high2(mg, x), low2(mg, y), high2(mg, y)});
-}
-
-// {RN16(p d), RN16(q e)}: d and e the low or the high halves of two scale words.  (v_fma_mix forms
-// the product in fp32 and rounds it once.)
-__device__ __forceinline__ uint32_t scaled2(float p, float q, uint32_t d, uint32_t e, bool high) {
-    uint32_t o;
-    if (high) {
-        asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(o) : "v"(p), "v"(d));
-        asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(o) : "v"(q), "v"(e));
-    } else {
-        asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(o) : "v"(p), "v"(d));
-        asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(o) : "v"(q), "v"(e));
-    }
-    return o;
-}
-
-struct Row {                                       // a row tile of a sequence
-    int s, q0, nq, len, rows, row0;
-    int t0, t1;                                    // tiles of 32 cached tokens that it sees
-};
-
-// Cached tokens [lo, hi) that query i of the sequence sees.
-__device__ __forceinline__ int hi_of(const Kv4Args& a, const Row& o, int i) {
-    return a.causal ? max(0, o.len - o.nq + i + 1) : o.len;
-}
-__device__ __forceinline__ int lo_of(const Kv4Args& a, const Row& o, int i) {
-    return a.window > 0 ? max(0, o.len - o.nq + i - a.window + 1) : 0;
-}
-
-// Item i = s row_tiles + rt; false where it has no rows.
-__device__ __forceinline__ bool row_tile_of(const Kv4Args& a, const Kv4Plan& p, int i, Row& o) {
-    int rt = 0;
-    o.s = i;
-    if (p.row_tiles > 1) {
-        o.s = i / p.row_tiles;
-        rt = i - o.s * p.row_tiles;
-    }
-    const int qa = a.q_start[o.s], qb = a.q_start[o.s + 1], len = a.kv_len[o.s];
-    o.q0 = min(max(qa, 0), a.T);
-    o.nq = min(min(max(qb, o.q0), a.T) - o.q0, a.max_q);
-    o.len = min(max(len, 0), a.max_kv);
-    o.row0 = rt * kKv4Rows;
-    const int64_t left = (int64_t)o.nq * p.group - o.row0;
-    o.rows = left < kKv4Rows ? (int)left : kKv4Rows;
-    if (o.rows <= 0) return false;
-    o.t0 = lo_of(a, o, o.row0 / p.group) / kKv4Tile;
-    o.t1 = max(o.t0, (hi_of(a, o, (o.row0 + o.rows - 1) / p.group) + kKv4Tile - 1) / kKv4Tile);
-    return true;
-}
-
-__device__ __forceinline__ void store_out(const Kv4Args& a, int64_t at, float y) {
-    if (a.out_f16) ((_Float16*)a.O)[at] = (_Float16)y;
-    else ((float*)a.O)[at] = y;
 }
 
 // Tiles [c0, c1) of head h of a row tile: its rows of O where they are `all` of
@@ -471,6 +402,7 @@ Kv4Plan plan_of(const Kv4Args& a) { return plan_kv4(a, device_cus() > 0 ? device
 
 bool kv4_attention_fits(const Kv4Args& a) {
     const Kv4Plan p = plan_of(a);
+    if (p.prompt) return launch_fits(p.items * a.c.heads, 256);
     return launch_fits((int64_t)p.splits * a.c.heads, 64 * p.waves) && launch_fits((int64_t)a.c.heads * kKv4Rows, 1024) &&
            p.items <= (int64_t)kGridY * 65535 && p.items * a.c.heads * p.splits * (64 * p.waves) < (int64_t(1) << 40);
 }
@@ -479,6 +411,7 @@ size_t kv4_attention_scratch_bytes(const Kv4Args& a) { return plan_of(a).bytes; 
 
 hipError_t kv4_attention(const Kv4Args& a, float* ws, hipStream_t st) {
     const Kv4Plan p = plan_of(a);
+    if (p.prompt) return kv4_prompt(a, p, device_cus() > 0 ? device_cus() : 256, st);
     switch (a.c.dim) {
         case 64: return launch<2>(a, p, ws, st);
         case 96: return launch<3>(a, p, ws, st);

@@ -20,4 +20,7 @@ size_t kv4_attention_scratch_bytes(const Kv4Args& a);
 // ws: kv4_attention_scratch_bytes(a) bytes (NULL when 0)
 hipError_t kv4_attention(const Kv4Args& a, float* ws, hipStream_t st);
 
+// The prompt kernel (a plan with p.prompt set).
+hipError_t kv4_prompt(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st);
+
 }  // namespace bf

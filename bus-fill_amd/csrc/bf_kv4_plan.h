@@ -29,6 +29,7 @@ struct Kv4Args {
 };
 
 constexpr int kKv4Rows = 16;                       // query rows of a row tile (one matrix operand)
+constexpr int kKv4PromptRows = 128;                // ... of the prompt kernel's (four waves of 32)
 
 // Rows of one key/value head: query i and head j of the group, row i G + j, in
 // row tiles of 16.  An item is a row tile of a sequence; with a head it is a
@@ -37,7 +38,8 @@ constexpr int kKv4Rows = 16;                       // query rows of a row tile (
 // which live in device memory (`splits`: the most that any can have).  Units of
 // several chunks leave partial results, which a second launch joins.
 struct Kv4Plan {
-    int group, row_tiles, waves, chunk, splits;
+    int group, tile_rows, row_tiles, waves, chunk, splits;
+    int prompt;                                    // the prompt kernel: no chunks
     int64_t items;                                 // sequences x row tiles
     int64_t slots;                                 // partial results (0: no unit can have two chunks)
     size_t bytes;                                  // their workspace
@@ -57,16 +59,21 @@ constexpr int kKv4PerCu = 4;                       // workgroups of four waves t
 inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
     Kv4Plan p;
     p.group = a.q_heads / a.c.heads;
-    p.row_tiles = (int)(((int64_t)a.max_q * p.group + kKv4Rows - 1) / kKv4Rows);
+    // The prompt kernel from 64 rows a sequence and head on, where its row tiles
+    // fill half the chip.
+    const int64_t rows = (int64_t)a.max_q * p.group, blocks = (rows + kKv4PromptRows - 1) / kKv4PromptRows;
+    p.prompt = rows >= 64 && (int64_t)a.S * a.c.heads * blocks >= cus / 2;
+    p.tile_rows = p.prompt ? kKv4PromptRows : kKv4Rows;
+    p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t seen = a.max_kv;                       // cached tokens a row tile can see
     if (a.window > 0) {
-        const int64_t span = std::min<int64_t>(a.max_q, (kKv4Rows + p.group - 2) / p.group + 1);
+        const int64_t span = std::min<int64_t>(a.max_q, (p.tile_rows + p.group - 2) / p.group + 1);
         seen = std::min<int64_t>(seen, (int64_t)a.window + span - 1);
     }
     const int64_t most = std::max<int64_t>(1, (seen + 2 * kKv4Tile - 2) / kKv4Tile);   // the range may start inside a tile
     p.items = (int64_t)a.S * p.row_tiles;
     const int64_t units = p.items * a.c.heads, places = (int64_t)cus * (a.c.dim == 256 ? 2 : kKv4PerCu);
-    p.chunk = (int)(most <= kKv4Alone ? most : std::min(most, std::max<int64_t>(kKv4LeastChunk, (units * most + 3 * places - 1) / (3 * places))));
+    p.chunk = (int)(p.prompt || most <= kKv4Alone ? most : std::min(most, std::max<int64_t>(kKv4LeastChunk, (units * most + 3 * places - 1) / (3 * places))));
     p.splits = (int)((most + p.chunk - 1) / p.chunk);
     p.waves = units * p.splits < cus ? 8 : 4;      // few workgroups: twice the waves on each
     p.slots = p.splits > 1 ? units * p.splits : 0;

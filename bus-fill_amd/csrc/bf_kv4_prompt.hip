@@ -1,0 +1,278 @@
+// Attention of many queries a sequence over the 4-bit cache: k_kv4_prompt (the
+// formula: bf_kv4_attn.hip, whose kernel keeps 16 rows a wave in registers and
+// decodes every record for each of them).
+//
+// A workgroup of four waves takes 128 rows (queries x heads of a group) of one
+// key/value head and walks over the records that they see.  A record is decoded
+// once for all of them: its codes as the fp16 integers q - 8 and its scales go
+// to LDS, keys by token, values by column, two records by turns.  Each wave
+// multiplies with its 32 rows:
+//
+// * S^T = K Q^T, a 32 x 32 tile of v_mfma_f32_32x32x16_f16 per block of 32
+//   values, whose sums the keys' scales multiply in fp32.  A lane then holds 16
+//   of the 32 tokens of its query; as the A operand of P V it needs eight tokens
+//   per instruction in the same lane, so the values' columns are stored with
+//   their tokens in that order and nothing moves between lanes.
+// * P d in fp16 for each block of 32 columns (one rounding), times q - 8.
+//   Scores and probabilities are as exact as the single-token kernel's; keys and
+//   values scaled to fp16 in LDS would take 128 of the loop's 250 vector
+//   instructions away and add two roundings of 2^-12.
+// * Bound by the vector instructions of softmax and scales: per 32 x 32 tile of
+//   128 columns about 1000 cycles of a SIMD beside 512 of MFMA.
+//
+// Causal rows see ever more tokens: units go out longest first, every other
+// round of one per CU in reverse, so that the units that meet on a CU add up to
+// about the same.
+#include <atomic>
+
+#include "bf_grid.h"
+#include "bf_kv4_dev.h"
+#include "bf_kv4_launch.h"
+
+namespace bf {
+namespace {
+
+constexpr int kPrWaves = 4, kPrThreads = 64 * kPrWaves;
+static_assert(kKv4PromptRows == 32 * kPrWaves);
+
+// LDS rows: 16 bytes past a multiple of 128 (keys, by token) or at 80 bytes
+// (values, by column): the eight rows of a 16-byte read on distinct banks.
+template <int NB> struct PrLds {
+    static constexpr int D = 32 * NB, KRow = 2 * D + 16, VRow = 80;
+    static constexpr int V = kKv4Tile * KRow, S = V + D * VRow, Bytes = S + 128 * NB;
+};
+
+// A thread's share of a record on its way to LDS.
+template <int NB> struct PrRaw {
+    static constexpr int KW = (128 * NB + kPrThreads - 1) / kPrThreads, VW = (64 * NB + kPrThreads - 1) / kPrThreads;
+    uint32_t k[KW];
+    uint2 v[VW];
+    uint32_t ks, vs;
+};
+
+template <int NB>
+__device__ __forceinline__ void load(PrRaw<NB>& x, const uint8_t* rec, int tid) {
+#pragma unroll
+    for (int i = 0; i < PrRaw<NB>::KW; i++) x.k[i] = *(const uint32_t*)(rec + 4 * min(tid + kPrThreads * i, 128 * NB - 1));
+#pragma unroll
+    for (int i = 0; i < PrRaw<NB>::VW; i++) x.v[i] = *(const uint2*)(rec + 512 * NB + 8 * min(tid + kPrThreads * i, 64 * NB - 1));
+    x.ks = *(const uint32_t*)(rec + 1024 * NB + 4 * min(tid, 16 * NB - 1));
+    x.vs = *(const uint32_t*)(rec + 1088 * NB + 4 * min(tid, 16 * NB - 1));
+}
+
+// Values of column d, tokens 8 g + 4 h + c, at place 16 (g / 2) + 8 h + 4 (g % 2) + c
+// of the column; scales of block b at 32 b + 16 h + 4 g + c (keys', then values').
+template <int NB>
+__device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint8_t* lds, int tid) {
+    using L = PrLds<NB>;
+#pragma unroll
+    for (int i = 0; i < PrRaw<NB>::KW; i++) {
+        const int u = tid + kPrThreads * i;
+        if (128 * NB % kPrThreads && u >= 128 * NB) break;
+        const int p = u / 512, w = NB - 4 * p < 4 ? NB - 4 * p : 4, at = u - 512 * p, idx = at / w, b = 4 * p + at - idx * w;
+        const int r = idx & 15, t = 8 * (r >> 2) + 4 * (idx >> 6) + (r & 3), g = (idx >> 4) & 3;
+        *(h8*)(lds + t * L::KRow + 64 * b + 16 * g) = codes8(mg, x.k[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PrRaw<NB>::VW; i++) {
+        const int u = tid + kPrThreads * i;
+        if (64 * NB % kPrThreads && u >= 64 * NB) break;
+        const int p = u / 128, w = NB - 2 * p < 2 ? 1 : 2, at = u - 128 * p, idx = at / w, b = 2 * p + at - idx * w;
+        const int g = idx >> 4, c = idx & 15;
+        uint8_t* col = lds + L::V + (32 * b + c) * L::VRow + 32 * (g >> 1) + 8 * (g & 1);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            // tokens 0 2 and 1 3 of four, as masks leave them, into 0 1 and 2 3
+            const uint32_t v = h ? x.v[i].y : x.v[i].x, w8 = v >> 8;
+            const uint32_t a0 = low2(mg, v), a1 = low2(mg, w8), b0 = high2(mg, v), b1 = high2(mg, w8);
+            *(uint2*)(col + 16 * h) = uint2{perm_b32(a1, a0, 0x05040100u), perm_b32(a1, a0, 0x07060302u)};
+            *(uint2*)(col + 16 * L::VRow + 16 * h) = uint2{perm_b32(b1, b0, 0x05040100u), perm_b32(b1, b0, 0x07060302u)};
+        }
+    }
+    if (tid < 16 * NB) {
+        // A values' scale that is no number becomes 0, and the keys' scale of that
+        // token and block NaN instead: rows that do not see the token multiply its
+        // values by 0, which must give 0 whatever an unwritten page holds.
+        uint32_t bad = 0;
+        if ((x.vs & 0x7C00u) == 0x7C00u) bad |= 0x0000FFFFu;
+        if ((x.vs & 0x7C000000u) == 0x7C000000u) bad |= 0xFFFF0000u;
+        const int g = tid / (4 * NB), b = tid / 4 % NB, e = tid % 4;
+        uint8_t* to = lds + L::S + 2 * (32 * b + 16 * (e >> 1) + 4 * g + 2 * (e & 1));
+        *(uint32_t*)to = x.ks | bad;
+        *(uint32_t*)(to + 64 * NB) = x.vs & ~bad;
+    }
+}
+
+template <int NB>
+__global__ __launch_bounds__(kPrThreads, NB < 4 ? 3 : NB == 4 ? 2 : 1) void k_kv4_prompt(Kv4Args a, Kv4Plan p, int cus) {
+    using L = PrLds<NB>;
+    constexpr int D = 32 * NB;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h2 = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // longest units first, every other round of `cus` in reverse
+    const int units = (int)(p.items * a.c.heads), round = blockIdx.x / cus, in = blockIdx.x - round * cus;
+    const int rank = round & 1 ? min((round + 1) * cus, units) - 1 - in : (int)blockIdx.x;
+    const int h = rank % a.c.heads, rest = rank / a.c.heads, s = rest % a.S, rt = p.row_tiles - 1 - rest / a.S;
+    Row o;
+    if (!row_tile_of(a, p, s * p.row_tiles + rt, o)) return;
+
+    // the lane's query row; rows past the last repeat it
+    const int row = o.row0 + min(32 * wave + col, o.rows - 1), iq = row / p.group;
+    const int lo = lo_of(a, o, iq), hi = hi_of(a, o, iq);
+    const int w0 = o.row0 + min(32 * wave, o.rows - 1), w1 = o.row0 + min(32 * wave + 31, o.rows - 1);
+    const int wlo = lo_of(a, o, w0 / p.group), whi = hi_of(a, o, w1 / p.group);     // tokens that some row of the wave sees
+    const int free0 = lo_of(a, o, w1 / p.group), free1 = hi_of(a, o, w0 / p.group); // ... that all do
+    const int head = h * p.group + row - iq * p.group;
+    const uint16_t* qp = a.Q + (int64_t)(o.q0 + iq) * a.ldq + head * D + 8 * h2;
+    h8 q[2 * NB];
+#pragma unroll
+    for (int c = 0; c < 2 * NB; c++) {
+        q[c] = *(const h8*)(qp + 16 * c);
+        if (a.scale < 0.f) q[c] = -q[c];               // so that a larger sum is a larger score
+    }
+    const float sc = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.44269504088896341f, 1e-30f);   // (above 0: -inf stays -inf)
+    const Magic mg = make_magic();
+    f16x acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[b][e] = 0.f;
+    float m = kLow, l = 0.f;
+
+    const int per_page = a.c.page_size / kKv4Tile;
+    const int32_t* const tab = a.table + (int64_t)o.s * a.ldt;
+    auto record = [&](int tile) {                  // -1: its page is absent
+        const int pg = tile / per_page, id = __builtin_amdgcn_readfirstlane(tab[pg]);
+        return id >= 0 && id < a.c.pages ? (id * a.c.heads + h) * per_page + (tile - pg * per_page) : -1;
+    };
+    // One record, of tokens tb ...
+    auto tile_of = [&](const uint8_t* buf, int tb) {
+        float x[16];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            f16x d = {};
+            const uint8_t* kr = buf + col * L::KRow + 64 * b + 16 * h2;
+            d = mfma32x32x16(*(const h8*)kr, q[2 * b], d);
+            d = mfma32x32x16(*(const h8*)(kr + 32), q[2 * b + 1], d);
+            const h8 k0 = *(const h8*)(buf + L::S + 64 * b + 32 * h2), k1 = *(const h8*)(buf + L::S + 64 * b + 32 * h2 + 16);
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                x[e] = b == 0 ? (float)(e < 8 ? k0[e & 7] : k1[e & 7]) * d[e]
+                              : __builtin_fmaf((float)(e < 8 ? k0[e & 7] : k1[e & 7]), d[e], x[e]);
+        }
+        // the lane's tokens: register 4 a + c is token 8 a + 4 h2 + c
+        if (tb < free0 || tb + kKv4Tile > free1) {     // hidden from some row of the wave
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int t = tb + 8 * (e >> 2) + 4 * h2 + (e & 3);
+                x[e] = t >= lo && t < hi ? x[e] : -__builtin_inff();
+            }
+        }
+        float tm = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) tm = __builtin_fmaxf(tm, x[e]);
+        tm *= sc;
+        if (__any(tm > m + 3.f)) {
+            float mn = __builtin_fmaxf(m, tm);
+            mn = __builtin_fmaxf(mn, __shfl_xor(mn, 32));
+            const float al = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float f = __shfl(al, 8 * (e >> 2) + 4 * h2 + (e & 3));
+#pragma unroll
+                for (int b = 0; b < NB; b++) acc[b][e] *= f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], sc, -m));
+            l += x[e];
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const uint8_t* vr = buf + L::V + (32 * b + col) * L::VRow + 16 * h2;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const u4 vs = *(const u4*)(buf + L::S + 64 * NB + 64 * b + 32 * h2 + 16 * i);
+                u4 pd;
+#pragma unroll
+                for (int e = 0; e < 4; e++) pd[e] = scaled_pair(x[8 * i + 2 * e], x[8 * i + 2 * e + 1], vs[e]);
+                acc[b] = mfma32x32x16(__builtin_bit_cast(h8, pd), *(const h8*)(vr + 32 * i), acc[b]);
+            }
+        }
+    };
+    PrRaw<NB> raw;
+    int rec = -1, next = -1;
+    if (o.t0 < o.t1) {
+        rec = record(o.t0);
+        load<NB>(raw, a.data + max(rec, 0) * kv4_record_bytes(D), tid);
+        decode<NB>(mg, raw, lds, tid);
+        if (o.t0 + 1 < o.t1) {
+            next = record(o.t0 + 1);
+            load<NB>(raw, a.data + max(next, 0) * kv4_record_bytes(D), tid);
+        }
+        __syncthreads();
+    }
+    for (int tile = o.t0; tile < o.t1; tile++) {
+        const uint8_t* const buf = lds + ((tile - o.t0) & 1) * L::Bytes;
+        if (tile + 1 < o.t1) decode<NB>(mg, raw, lds + ((tile + 1 - o.t0) & 1) * L::Bytes, tid);
+        const int after = tile + 2 < o.t1 ? record(tile + 2) : -1;
+        if (tile + 2 < o.t1) load<NB>(raw, a.data + max(after, 0) * kv4_record_bytes(D), tid);
+        const int tb = tile * kKv4Tile;
+        if (rec >= 0 && tb < whi && tb + kKv4Tile > wlo) {
+            tile_of(buf, tb);
+        }
+        rec = next;
+        next = after;
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t at = (int64_t)(o.q0 + iq) * a.ldo + head * D;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const int r = 8 * (e >> 2) + 4 * h2 + (e & 3);             // the row of the lane's sums, held by lane r as a query
+        const float f = __shfl(inv, r);
+        const int64_t to = (int64_t)__shfl((long long)at, r);
+        if (32 * wave + r >= o.rows) continue;
+#pragma unroll
+        for (int b = 0; b < NB; b++) store_out(a, to + 32 * b + col, acc[b][e] * f);
+    }
+    if (a.lse && h2 == 0 && 32 * wave + col < o.rows)
+        a.lse[(int64_t)(o.q0 + iq) * a.q_heads + head] =
+            l == 0.f ? -__builtin_inff() : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+}
+
+template <int NB>
+hipError_t launch(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st) {
+    auto k = k_kv4_prompt<NB>;
+    constexpr int lds = 2 * PrLds<NB>::Bytes;
+    static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)(p.items * a.c.heads)), dim3(kPrThreads), lds, st, a, p, cus);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t kv4_prompt(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st) {
+    switch (a.c.dim) {
+        case 64: return launch<2>(a, p, cus, st);
+        case 96: return launch<3>(a, p, cus, st);
+        case 128: return launch<4>(a, p, cus, st);
+        default: return launch<8>(a, p, cus, st);
+    }
+}
+
+}  // namespace bf

@@ -349,10 +349,19 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
     __syncthreads();
     const int per = (slots + kPlanWaves - 1) / kPlanWaves, s0 = min(slots, wave * per), s1 = min(slots, s0 + per);
     int ns = 0;
-    for (int s = s0 + lane; s < s1; s += 64) {
-        const int id = ids[s];
-        if (id >= 0 && id < E) atomicAdd(&hist[id], 1);
-        ns += id == e;
+    // (eight loads at a time: one by one the two passes over 16000 slots take 14 us)
+    auto load8 = [&](int s, int id[8]) {
+#pragma unroll
+        for (int q = 0; q < 8; q++) id[q] = s + 64 * q + lane < s1 ? ids[s + 64 * q + lane] : -1;
+    };
+    for (int s = s0; s < s1; s += 512) {
+        int id[8];
+        load8(s, id);
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            if (id[q] >= 0 && id[q] < E) atomicAdd(&hist[id[q]], 1);
+            ns += id[q] == e;
+        }
     }
 #pragma unroll
     for (int x = 32; x; x >>= 1) ns += __shfl_xor(ns, x);
@@ -392,11 +401,15 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
         table[i < large ? before[1] + i : max_tiles + before[2] + i - large] =
             int4{e, base + i * kMoeTileRows, min(kMoeTileRows, total - i * kMoeTileRows), 0};
     at += base;
-    for (int s = s0; s < s1; s += 64) {
-        const bool hit = s + lane < s1 && ids[s + lane] == e;
-        const uint64_t b = __ballot(hit);
-        if (hit) perm[at + __builtin_popcountll(b & ((1ull << lane) - 1))] = s + lane;
-        at += __builtin_popcountll(b);
+    for (int s = s0; s < s1; s += 512) {
+        int id[8];
+        load8(s, id);
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            const uint64_t b = __ballot(id[q] == e);
+            if (id[q] == e) perm[at + __builtin_popcountll(b & ((1ull << lane) - 1))] = s + 64 * q + lane;
+            at += __builtin_popcountll(b);
+        }
     }
 }
 

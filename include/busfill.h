@@ -445,7 +445,8 @@ size_t bf_kv4_bytes(int pages, int page_size, int kv_heads, int head_dim);
  * past the cache is skipped.  The slots of one call must differ.  Per 32
  * values: m = the one of largest magnitude (the first of equals), d =
  * RN_fp16(m / -8), q = floor(x / d + 8.5) clamped to 0..15 (all 8 where d is
- * 0); a block with an infinity or NaN reads back as NaN.  Whatever else the
+ * 0); a block with an infinity or NaN reads back as NaN (and rows that attend
+ * to its token are NaN, in that block's columns at least).  Whatever else the
  * pages hold stays as it is. */
 bf_status bf_kv4_store(const bf_kv4_cache* cache, const uint16_t* K, int64_t ldk, const uint16_t* V, int64_t ldv,
                        const int64_t* slots, int T, void* stream);
