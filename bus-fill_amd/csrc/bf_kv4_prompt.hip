@@ -14,11 +14,13 @@
 //   per instruction in the same lane, so the values' columns are stored with
 //   their tokens in that order and nothing moves between lanes.
 // * P d in fp16 for each block of 32 columns (one rounding), times q - 8.
-//   Scores and probabilities are as exact as the single-token kernel's; keys and
-//   values scaled to fp16 in LDS would take 128 of the loop's 250 vector
-//   instructions away and add two roundings of 2^-12.
-// * Bound by the vector instructions of softmax and scales: per 32 x 32 tile of
-//   128 columns about 1000 cycles of a SIMD beside 512 of MFMA.
+//   Scores and probabilities are as exact as the single-token kernel's.  (Keys
+//   and values as exact fp16 pairs in LDS instead, hi and lo of (q - 8) d, need
+//   no scales here and twice the matrix products: 114 us where this takes 95.)
+// * 2000 causal tokens, 40 heads over 8 of 128: 94 us, 430 TFLOP/s of the visible
+//   pairs; the vector instructions of softmax and scales take half of the SIMDs'
+//   cycles, the matrix products 16 %.  Of the rest, decoding costs 19 us (timed
+//   without it), and the longest units (63 records) outlast the others.
 //
 // Causal rows see ever more tokens: units go out longest first, every other
 // round of one per CU in reverse, so that the units that meet on a CU add up to
@@ -104,7 +106,7 @@ __device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint
 }
 
 template <int NB>
-__global__ __launch_bounds__(kPrThreads, NB < 4 ? 3 : NB == 4 ? 2 : 1) void k_kv4_prompt(Kv4Args a, Kv4Plan p, int cus) {
+__global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4Args a, Kv4Plan p, int cus) {
     using L = PrLds<NB>;
     constexpr int D = 32 * NB;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -142,25 +144,58 @@ __global__ __launch_bounds__(kPrThreads, NB < 4 ? 3 : NB == 4 ? 2 : 1) void k_kv
 
     const int per_page = a.c.page_size / kKv4Tile;
     const int32_t* const tab = a.table + (int64_t)o.s * a.ldt;
-    auto record = [&](int tile) {                  // -1: its page is absent
-        const int pg = tile / per_page, id = __builtin_amdgcn_readfirstlane(tab[pg]);
-        return id >= 0 && id < a.c.pages ? (id * a.c.heads + h) * per_page + (tile - pg * per_page) : -1;
+    // Lane n holds the record of the n-th tile of the next 64 (-1: page absent, or no such tile)
+    int recs = -1;
+    auto look = [&](int n0) {
+        const int tile = o.t0 + n0 + lane;
+        recs = -1;
+        if (tile < o.t1) {
+            const int pg = tile / per_page, id = tab[pg];
+            if (id >= 0 && id < a.c.pages) recs = (id * a.c.heads + h) * per_page + (tile - pg * per_page);
+        }
     };
     // One record, of tokens tb ...
     auto tile_of = [&](const uint8_t* buf, int tb) {
+        // LDS reads run a phase ahead: the keys of up to four blocks before their
+        // products, the values before the exponentials (left to the compiler each
+        // stood right before its use, 27 waits a record).
+        constexpr int HB = NB < 4 ? NB : 4;
         float x[16];
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            f16x d = {};
-            const uint8_t* kr = buf + col * L::KRow + 64 * b + 16 * h2;
-            d = mfma32x32x16(*(const h8*)kr, q[2 * b], d);
-            d = mfma32x32x16(*(const h8*)(kr + 32), q[2 * b + 1], d);
-            const h8 k0 = *(const h8*)(buf + L::S + 64 * b + 32 * h2), k1 = *(const h8*)(buf + L::S + 64 * b + 32 * h2 + 16);
+        for (int b0 = 0; b0 < NB; b0 += HB) {
+            h8 kf[HB][2], ks[HB][2];
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                x[e] = b == 0 ? (float)(e < 8 ? k0[e & 7] : k1[e & 7]) * d[e]
-                              : __builtin_fmaf((float)(e < 8 ? k0[e & 7] : k1[e & 7]), d[e], x[e]);
+            for (int b = 0; b < HB; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) kf[b][i] = *(const h8*)(buf + col * L::KRow + 64 * (b0 + b) + 16 * h2 + 32 * i);
+#pragma unroll
+            for (int b = 0; b < HB; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) ks[b][i] = *(const h8*)(buf + L::S + 64 * (b0 + b) + 32 * h2 + 16 * i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int b = 0; b < HB; b++) {
+                const f16x zero = {};
+                const f16x d = mfma32x32x16(kf[b][1], q[2 * (b0 + b) + 1], mfma32x32x16(kf[b][0], q[2 * (b0 + b)], zero));
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    x[e] = b0 + b == 0 ? (float)ks[b][e >> 3][e & 7] * d[e] : __builtin_fmaf((float)ks[b][e >> 3][e & 7], d[e], x[e]);
+            }
         }
+        h8 vf[HB][2];
+        u4 vs[HB][2];
+        auto values = [&](int b0) {
+#pragma unroll
+            for (int b = 0; b < HB; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    vs[b][i] = *(const u4*)(buf + L::S + 64 * NB + 64 * (b0 + b) + 32 * h2 + 16 * i);
+                    vf[b][i] = *(const h8*)(buf + L::V + (32 * (b0 + b) + col) * L::VRow + 16 * h2 + 32 * i);
+                }
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        values(0);
+        __builtin_amdgcn_sched_barrier(0);
         // the lane's tokens: register 4 a + c is token 8 a + 4 h2 + c
         if (tb < free0 || tb + kKv4Tile > free1) {     // hidden from some row of the wave
 #pragma unroll
@@ -186,45 +221,48 @@ __global__ __launch_bounds__(kPrThreads, NB < 4 ? 3 : NB == 4 ? 2 : 1) void k_kv
                 for (int b = 0; b < NB; b++) acc[b][e] *= f;
             }
         }
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], sc, -m));
-            l += x[e];
+            part[e & 3] += x[e];
         }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const uint8_t* vr = buf + L::V + (32 * b + col) * L::VRow + 16 * h2;
+        for (int b0 = 0; b0 < NB; b0 += HB) {
+            if (b0) values(b0);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const u4 vs = *(const u4*)(buf + L::S + 64 * NB + 64 * b + 32 * h2 + 16 * i);
-                u4 pd;
+            for (int b = 0; b < HB; b++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) pd[e] = scaled_pair(x[8 * i + 2 * e], x[8 * i + 2 * e + 1], vs[e]);
-                acc[b] = mfma32x32x16(__builtin_bit_cast(h8, pd), *(const h8*)(vr + 32 * i), acc[b]);
-            }
+                for (int i = 0; i < 2; i++) {
+                    u4 pd;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) pd[e] = scaled_pair(x[8 * i + 2 * e], x[8 * i + 2 * e + 1], vs[b][i][e]);
+                    acc[b0 + b] = mfma32x32x16(__builtin_bit_cast(h8, pd), vf[b][i], acc[b0 + b]);
+                }
         }
     };
+    // Tile t0 + n's record (-1: record 0 is read and not used).
     PrRaw<NB> raw;
-    int rec = -1, next = -1;
-    if (o.t0 < o.t1) {
-        rec = record(o.t0);
+    auto fetch = [&](int n) {
+        if ((n & 63) == 0) look(n);
+        const int rec = __builtin_amdgcn_readlane(recs, n & 63);
         load<NB>(raw, a.data + max(rec, 0) * kv4_record_bytes(D), tid);
+        return rec;
+    };
+    const int walk = o.t1 - o.t0;
+    int rec = -1, next = -1;
+    if (walk > 0) {
+        rec = fetch(0);
         decode<NB>(mg, raw, lds, tid);
-        if (o.t0 + 1 < o.t1) {
-            next = record(o.t0 + 1);
-            load<NB>(raw, a.data + max(next, 0) * kv4_record_bytes(D), tid);
-        }
+        next = fetch(1);
         __syncthreads();
     }
-    for (int tile = o.t0; tile < o.t1; tile++) {
-        const uint8_t* const buf = lds + ((tile - o.t0) & 1) * L::Bytes;
-        if (tile + 1 < o.t1) decode<NB>(mg, raw, lds + ((tile + 1 - o.t0) & 1) * L::Bytes, tid);
-        const int after = tile + 2 < o.t1 ? record(tile + 2) : -1;
-        if (tile + 2 < o.t1) load<NB>(raw, a.data + max(after, 0) * kv4_record_bytes(D), tid);
-        const int tb = tile * kKv4Tile;
-        if (rec >= 0 && tb < whi && tb + kKv4Tile > wlo) {
-            tile_of(buf, tb);
-        }
+    for (int n = 0; n < walk; n++) {
+        if (n + 1 < walk) decode<NB>(mg, raw, lds + ((n + 1) & 1) * L::Bytes, tid);
+        const int after = n + 2 < walk ? fetch(n + 2) : -1;
+        const int tb = (o.t0 + n) * kKv4Tile;
+        if (rec >= 0 && tb < whi && tb + kKv4Tile > wlo) tile_of(lds + (n & 1) * L::Bytes, tb);
         rec = next;
         next = after;
         __syncthreads();
@@ -235,11 +273,11 @@ __global__ __launch_bounds__(kPrThreads, NB < 4 ? 3 : NB == 4 ? 2 : 1) void k_kv
 #pragma unroll
     for (int e = 0; e < 16; e++) {
         const int r = 8 * (e >> 2) + 4 * h2 + (e & 3);             // the row of the lane's sums, held by lane r as a query
-        const float f = __shfl(inv, r);
+        const float g0 = __shfl(inv, r);
         const int64_t to = (int64_t)__shfl((long long)at, r);
         if (32 * wave + r >= o.rows) continue;
 #pragma unroll
-        for (int b = 0; b < NB; b++) store_out(a, to + 32 * b + col, acc[b][e] * f);
+        for (int b = 0; b < NB; b++) store_out(a, to + 32 * b + col, acc[b][e] * g0);
     }
     if (a.lse && h2 == 0 && 32 * wave + col < o.rows)
         a.lse[(int64_t)(o.q0 + iq) * a.q_heads + head] =
@@ -250,6 +288,7 @@ template <int NB>
 hipError_t launch(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st) {
     auto k = k_kv4_prompt<NB>;
     constexpr int lds = 2 * PrLds<NB>::Bytes;
+
     static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
