@@ -3,10 +3,11 @@
 // Store, per 32 values x of a head: m = the value of largest magnitude (the
 // first of equals), d = RN16(m / -8), q = clamp(floor(x / d + 8.5), 0, 15), so
 // m itself is code 0 and x is at most d / 2 from (q - 8) d inside the range (d
-// on the far side, where +m would be code 16).  x and d are fp16, so x / d is
-// either exactly half way between two integers or at least 2^-12 from it,
-// while the fp32 quotient and sum are off by at most 2^-20: the codes are those
-// of the exact formula.  d = 0: all codes 8.  A block with an infinity or a NaN
+// on the far side, where +m would be code 16).  x and d are fp16, 11-bit
+// integers times powers of two, so x / d is either exactly half way between two
+// integers or at least 2^-13 from it: floor(x rcp(d) + 8.5 + 2^-14), off by less
+// than 2^-18 in fp32, gives the codes of the exact formula without a division.
+// d = 0: all codes 8.  A block with an infinity or a NaN
 // gets d = NaN, codes 8: it reads as NaN, not as a finite guess.
 #include "bf_device.h"
 #include "bf_kv4_launch.h"
@@ -25,28 +26,30 @@ __device__ __forceinline__ float half_at(const u4 x[4], int e) {
 
 // One block's scale bits and codes.
 __device__ __forceinline__ uint32_t quantize32(const u4 x[4], uint8_t q[32]) {
-    float m = 0.f, am = 0.f;
-    bool finite = true;
+    float hi = half_at(x, 0), lo = hi, bad = 0.f;
+    const h2 none = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
     for (int e = 0; e < 32; e++) {
-        const float v = half_at(x, e), a = __builtin_fabsf(v);
-        finite &= a <= 65504.f;                        // false for NaN
-        if (a > am) {
-            am = a;
-            m = v;
-        }
+        hi = __builtin_fmaxf(hi, half_at(x, e));
+        lo = __builtin_fminf(lo, half_at(x, e));
+        if ((e & 1) == 0) bad = __builtin_amdgcn_fdot2(as_h2(x[e >> 3][(e >> 1) & 3]), none, bad, false);   // NaN from an infinity or NaN
     }
+    float m = hi > -lo ? hi : lo;
+    if (hi == -lo)                                     // both magnitudes: the first of them
+#pragma unroll
+        for (int e = 31; e >= 0; e--)
+            if (__builtin_fabsf(half_at(x, e)) == hi) m = half_at(x, e);
     const _Float16 d16 = (_Float16)(m * -0.125f);
-    const float d = (float)d16;
+    const float r = __builtin_amdgcn_rcpf((float)d16);
 #pragma unroll
     for (int e = 0; e < 32; e++) {
-        const float t = __builtin_floorf(half_at(x, e) / d + 8.5f);
+        const float t = __builtin_floorf(__builtin_fmaf(half_at(x, e), r, 8.5f + 0x1p-14f));
         q[e] = (uint8_t)(int)__builtin_fminf(__builtin_fmaxf(t, 0.f), 15.f);
     }
-    if (finite && d != 0.f) return __builtin_bit_cast(uint16_t, d16);
+    if (bad == 0.f && d16 != (_Float16)0.f) return __builtin_bit_cast(uint16_t, d16);
 #pragma unroll
     for (int e = 0; e < 32; e++) q[e] = 8;
-    return finite ? 0u : kNan16;
+    return bad == 0.f ? 0u : kNan16;
 }
 
 // The record and token of a slot; false for a slot outside the cache.
@@ -60,23 +63,24 @@ __device__ __forceinline__ bool slot_at(const Kv4Shape& c, int64_t slot, int hea
     return true;
 }
 
-// One block (32 values) per thread: token, K or V, block; heads along grid y.
+// One block (32 values) per thread: token, block; heads along grid y, keys and
+// values along z (a wave of both would take both ways through the codes' places).
 __global__ __launch_bounds__(256) void k_kv4_store(uint8_t* __restrict__ data, Kv4Shape c, const uint16_t* __restrict__ K,
                                                    int64_t ldk, const uint16_t* __restrict__ V, int64_t ldv,
                                                    const int64_t* __restrict__ slots, int T) {
     const int nb = c.dim / 32, head = blockIdx.y;
     const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
-    const int64_t t = i / (2 * nb);
+    const int64_t t = i / nb;
     if (t >= T) return;
-    const int u = (int)(i - t * (2 * nb)), b = u >> 1;
-    const bool isv = u & 1;
-    int64_t rec;
-    int tok;
-    if (!slot_at(c, slots[t], head, rec, tok)) return;
+    const int b = (int)(i - t * nb);
+    const bool isv = blockIdx.z;
     const uint16_t* src = (isv ? V + t * ldv : K + t * ldk) + head * c.dim + 32 * b;
     u4 x[4];
 #pragma unroll
     for (int w = 0; w < 4; w++) x[w] = *(const u4*)(src + 8 * w);
+    int64_t rec;
+    int tok;
+    if (!slot_at(c, slots[t], head, rec, tok)) return;
     uint8_t q[32];
     const uint32_t d = quantize32(x, q);
     uint8_t* r = data + rec * kv4_record_bytes(c.dim);
@@ -103,10 +107,10 @@ __global__ __launch_bounds__(256) void k_kv4_load(const uint8_t* __restrict__ da
                                                   int64_t ldk, uint16_t* __restrict__ V, int64_t ldv, int T) {
     const int nb = c.dim / 32, head = blockIdx.y;
     const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
-    const int64_t t = i / (2 * nb);
+    const int64_t t = i / nb;
     if (t >= T) return;
-    const int u = (int)(i - t * (2 * nb)), b = u >> 1;
-    const bool isv = u & 1;
+    const int b = (int)(i - t * nb);
+    const bool isv = blockIdx.z;
     u4 out[4] = {};
     int64_t rec;
     int tok;
@@ -142,7 +146,7 @@ __global__ __launch_bounds__(256) void k_kv4_load(const uint8_t* __restrict__ da
 }
 
 dim3 units_grid(const Kv4Shape& c, int T) {
-    return dim3((unsigned)(((int64_t)T * 2 * (c.dim / 32) + 255) / 256), (unsigned)c.heads);
+    return dim3((unsigned)(((int64_t)T * (c.dim / 32) + 255) / 256), (unsigned)c.heads, 2);
 }
 
 }  // namespace

@@ -45,85 +45,85 @@ __device__ __forceinline__ float wave_sum(float v) {
     return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
 }
 
-__device__ __forceinline__ float lane_of(float v, int l) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+// The two largest of two pairs of largest ones.
+__device__ __forceinline__ void top2(float& b1, float& b2, float o1, float o2) {
+    b2 = __builtin_fmaxf(__builtin_fminf(b1, o1), __builtin_fmaxf(b2, o2));
+    b1 = __builtin_fmaxf(b1, o1);
 }
 
 template <int EPL>
 __global__ __launch_bounds__(64 * kRtWaves) void k_moe_route(RouteArgs a) {
-    __shared__ float xs[kRtWaves][65 * EPL];       // selection scores, one pad word per 64
+    __shared__ float xs[kRtWaves][65 * EPL];       // of one wave each: a value per expert, one pad word per 64
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t t = blockIdx.x * (int64_t)kRtWaves + wave;
+    if (t >= a.T) return;
     const int e0 = lane * EPL;
     const float ninf = -__builtin_inff();
     float x[EPL], s[EPL], sel[EPL];
-    if (t < a.T) {
-        const int64_t at = t * a.ldl + e0;
+    const int64_t at = t * a.ldl + e0;
 #pragma unroll
-        for (int i = 0; i < EPL; i++)
-            x[i] = e0 + i >= a.E ? ninf : a.f16 ? (float)((const _Float16*)a.logits)[at + i] : ((const float*)a.logits)[at + i];
-        if (a.sigmoid) {
+    for (int i = 0; i < EPL; i++)
+        x[i] = e0 + i >= a.E ? ninf : a.f16 ? (float)((const _Float16*)a.logits)[at + i] : ((const float*)a.logits)[at + i];
+    if (a.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++) s[i] = 1.f / (1.f + expf(-x[i]));
-        } else {
-            float m = x[0];
+        for (int i = 0; i < EPL; i++) s[i] = __builtin_amdgcn_rcpf(1.f + expf(-x[i]));
+    } else {
+        float m = x[0];
 #pragma unroll
-            for (int i = 1; i < EPL; i++) m = __builtin_fmaxf(m, x[i]);
-            m = wave_max(m);
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                s[i] = m == ninf && x[i] == ninf ? 0.f : expf(x[i] - m);   // a row of -inf: all zero
-                if (e0 + i < a.E) sum += s[i];
-            }
-            sum = wave_sum(sum);
-#pragma unroll
-            for (int i = 0; i < EPL; i++) s[i] = sum == 0.f ? 0.f : s[i] / sum;
-        }
-        // what is compared: -inf for experts that do not exist, -FLT_MAX at least for those that do
+        for (int i = 1; i < EPL; i++) m = __builtin_fmaxf(m, x[i]);
+        m = wave_max(m);
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
-            const float v = a.bias ? s[i] + (e0 + i < a.E ? a.bias[e0 + i] : 0.f) : a.groups > 1 ? s[i] : x[i];
-            sel[i] = e0 + i < a.E ? __builtin_fmaxf(v, -FLT_MAX) : ninf;
+            s[i] = m == ninf && x[i] == ninf ? 0.f : expf(x[i] - m);   // a row of -inf: all zero
+            if (e0 + i < a.E) sum += s[i];
         }
+        sum = wave_sum(sum);
+#pragma unroll
+        for (int i = 0; i < EPL; i++) s[i] = sum == 0.f ? 0.f : s[i] * __builtin_amdgcn_rcpf(sum);
+    }
+    // what is compared: -inf for experts that do not exist, -FLT_MAX at least for those that do
+#pragma unroll
+    for (int i = 0; i < EPL; i++) {
+        const float v = a.bias ? s[i] + (e0 + i < a.E ? a.bias[e0 + i] : 0.f) : a.groups > 1 ? s[i] : x[i];
+        sel[i] = e0 + i < a.E ? __builtin_fmaxf(v, -FLT_MAX) : ninf;
     }
     if (a.groups > 1) {
-        if (t < a.T) {
+        const int size = a.E / a.groups, lanes = size / EPL;
+        float b1 = ninf, b2 = ninf;
+        if (lanes * EPL == size && (lanes & (lanes - 1)) == 0) {       // a power of two of lanes holds a group: they meet
+#pragma unroll
+            for (int i = 0; i < EPL; i++) top2(b1, b2, sel[i], ninf);
+            for (int d = 1; d < lanes; d *= 2) top2(b1, b2, __shfl_xor(b1, d), __shfl_xor(b2, d));
+            const int from = min(lane * lanes, 63);
+            b1 = __shfl(b1, from);
+            b2 = __shfl(b2, from);
+        } else {                                                       // lane g walks through group g
 #pragma unroll
             for (int i = 0; i < EPL; i++) xs[wave][e0 + i + (e0 + i) / 64] = sel[i];
+            for (int i = 0; lane < a.groups && i < size; i++) {
+                const int e = lane * size + i;
+                top2(b1, b2, xs[wave][e + e / 64], ninf);
+            }
         }
-        __syncthreads();
-        if (t < a.T) {
-            const int size = a.E / a.groups;
-            float best = ninf;
-            if (lane < a.groups) {
-                float b1 = ninf, b2 = ninf;
-                for (int i = 0; i < size; i++) {
-                    const int e = lane * size + i;
-                    const float v = xs[wave][e + e / 64];
-                    b2 = __builtin_fmaxf(b2, __builtin_fminf(b1, v));
-                    b1 = __builtin_fmaxf(b1, v);
-                }
-                best = size > 1 ? __builtin_fmaxf(b1 + b2, -FLT_MAX) : b1;
-            }
-            uint64_t keep = 0;
-            for (int i = 0; i < a.top_groups; i++) {
-                const float m = wave_max(best);
-                const int l = __builtin_ctzll(__ballot(best == m));
-                keep |= 1ull << l;
-                if (lane == l) best = ninf;
-            }
+        float best = lane >= a.groups ? ninf : size > 1 ? __builtin_fmaxf(b1 + b2, -FLT_MAX) : b1;
+        uint64_t keep = 0;
+        for (int i = 0; i < a.top_groups; i++) {
+            const float m = wave_max(best);
+            const int l = __builtin_ctzll(__ballot(best == m));
+            keep |= 1ull << l;
+            if (lane == l) best = ninf;
+        }
 #pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                const int g = (e0 + i) / size;
-                if (e0 + i < a.E) sel[i] = !((keep >> g) & 1) ? ninf : a.bias ? sel[i] : __builtin_fmaxf(x[i], -FLT_MAX);
-            }
+        for (int i = 0; i < EPL; i++) {
+            const int g = (e0 + i) / size;
+            if (e0 + i < a.E) sel[i] = !((keep >> g) & 1) ? ninf : a.bias ? sel[i] : __builtin_fmaxf(x[i], -FLT_MAX);
         }
     }
-    if (t >= a.T) return;
+#pragma unroll
+    for (int i = 0; i < EPL; i++) xs[wave][e0 + i + (e0 + i) / 64] = s[i];
     int id = 0;
-    float w = 0.f;
     for (int j = 0; j < a.k; j++) {
         float b = sel[0];
         int bi = 0;
@@ -135,22 +135,13 @@ __global__ __launch_bounds__(64 * kRtWaves) void k_moe_route(RouteArgs a) {
             }
         const float m = wave_max(b);
         const int l = __builtin_ctzll(__ballot(b == m));
-        float sw = s[0];
-#pragma unroll
-        for (int i = 1; i < EPL; i++)
-            if (bi == i) sw = s[i];
         const int e = l * EPL + __builtin_amdgcn_readlane(bi, l);
-        sw = lane_of(sw, l);
-        if (lane == j) {
-            id = e;
-            w = sw;
-        }
-        if (lane == l) {
+        if (lane == j) id = e;
 #pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (bi == i) sel[i] = ninf;
-        }
+        for (int i = 0; i < EPL; i++)
+            if (e0 + i == e) sel[i] = ninf;
     }
+    float w = xs[wave][id + id / 64];
     if (a.renorm) {
         const float sum = wave_sum(lane < a.k ? w : 0.f);
         w = sum == 0.f ? 0.f : w / sum;
