@@ -89,6 +89,10 @@ __device__ __forceinline__ void store_y(const MoeArgs& a, void* y, int64_t at, f
     else ((float*)y)[at] = v;
 }
 
+// What a launch of k_moe_rows computes: h (gate and up), y (down, by slot), or
+// the outputs of a single row (down over its slots' experts as one long sum).
+enum : int { kMoeH = 0, kMoeY = 1, kMoeRow = 2 };
+
 // One super-group (144 bytes a row) of 16 weight rows into LDS, row after row:
 // pieces of 16 bytes, nine to a row.  Neighbouring lanes fetch neighbouring
 // pieces: as operand registers, where neighbouring lanes are different rows, the
@@ -98,6 +102,7 @@ constexpr int kTileBytes = 16 * 144, kTileLoads = 3;
 template <int QT> struct TileFetch {
     const uint8_t* src[kTileLoads];
     uint32_t step[kTileLoads];                     // bytes from one super-group to the next
+    int64_t expert;                                // ... from one expert to the next (planes: of scales, eight times that of codes)
     __device__ __forceinline__ void init(const uint8_t* W, const uint8_t* aux, int64_t n0, int rows, int K, int lane) {
 #pragma unroll
         for (int q = 0; q < kTileLoads; q++) {
@@ -106,10 +111,12 @@ template <int QT> struct TileFetch {
             step[q] = QT != QT_PLANES ? 144 : part == 0 ? 16 : 128;
         }
     }
-    __device__ __forceinline__ void get(int s, uint32_t lds, int lane) const {
+    __device__ __forceinline__ void get(int s, int e, uint32_t lds, int lane) const {
 #pragma unroll
-        for (int q = 0; q < kTileLoads; q++)
-            if (q < 2 || lane < 16) dma16(src[q] + (uint64_t)step[q] * s, lds + 1024 * q);
+        for (int q = 0; q < kTileLoads; q++) {
+            const int64_t at = expert * e * (QT == QT_PLANES && step[q] == 128 ? 8 : 1) + (uint64_t)step[q] * s;
+            if (q < 2 || lane < 16) dma16(src[q] + at, lds + 1024 * q);
+        }
     }
 };
 
@@ -132,15 +139,17 @@ __device__ __forceinline__ void wait_loads(int n) {
 // waves, KS of them over the super-groups of one 16-row tile of one matrix (GU:
 // gate, up), each through a ring of its own, the activations shared; the waves
 // meet in LDS at the end.  GU: h of the slots; else y.
-template <int QT, int MT, bool GU, int KS>
+template <int QT, int MT, int MODE, int KS>
 __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out, int R,
                                         int K, int64_t e, int tile0, const int32_t* list, int cnt, int cap, uint8_t* lds) {
+    constexpr bool GU = MODE == kMoeH, ONE = MODE == kMoeRow;
     constexpr int NM = GU ? 2 : 1, TW = kMoeWaves / (KS * NM), CH = KS < 2 ? 2 : KS, PER = CH / KS, ST = kMoeStages;
     constexpr int RS = 20, TS = 16 * RS;           // stride of the sums' rows: the four row groups of a wave on distinct banks
     const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kp = wave % KS, mat = wave / KS % NM, tile = tile0 + wave / (KS * NM);
-    const int nsg = K >> 8, slabs = (nsg + CH - 1) / CH;
+    // ONE: the row's slots one after the other, `list` their experts (K and the activations run through them all)
+    const int per = K >> 8, nsg = ONE ? a.k * per : per, slabs = (nsg + CH - 1) / CH, width = ONE ? a.k * K : K;
     float* const red = (float*)lds;                // [wave][MT][16][RS], over everything else at the end
     uint8_t* const ring = lds + wave * (ST * kTileBytes);
     const uint32_t ring0 = lds_addr(ring);
@@ -149,16 +158,25 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
     const bool live = 16 * tile < R;
     TileFetch<QT> wf;
     wf.init(w.W[mat], w.aux[mat], e * R + (live ? 16 * tile : 0), live ? min(16, R - 16 * tile) : 1, K, lane);
+    wf.expert = QT == QT_PLANES ? (int64_t)R * (K >> 4) : (int64_t)R * per * 144;
+    auto weights_get = [&](int s, uint32_t to) {
+        if constexpr (ONE) {
+            const int j = s / per;
+            wf.get(s - j * per, max(list[j], 0), to, lane);
+        } else {
+            wf.get(s, 0, to, lane);
+        }
+    };
     // slab t: rows wave, wave + 8, ...; CH / 2 loads of 1 KB a row (past the row's end: its start, not used)
     auto slab_get = [&](int t) {
         const uint32_t to = lds_addr(slab) + (t & 1) * slab_bytes;
         for (int i = wave; i < cnt; i += kMoeWaves) {
-            const int slot = list[i];
+            const int slot = ONE ? 0 : list[i];
             const uint16_t* row = A + (int64_t)(GU ? slot / a.k : slot) * lda;
 #pragma unroll
             for (int q = 0; q < CH / 2; q++) {
                 const int c = 256 * CH * t + 512 * q + 8 * lane;
-                dma16(row + (c < K ? c : 0), to + i * kSlabRow<CH> + 1024 * q);
+                dma16(row + (c < width ? c : 0), to + i * kSlabRow<CH> + 1024 * q);
             }
         }
     };
@@ -171,7 +189,7 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
     __syncthreads();                               // LDS is free
     slab_get(0);
     for (int n = 0; n < ST - 1; n++)
-        if (sg_at(n) < nsg) wf.get(sg_at(n), ring0 + n * kTileBytes, lane);
+        if (sg_at(n) < nsg) weights_get(sg_at(n), ring0 + n * kTileBytes);
     int at = 0;                                    // ring stage of the wave's next super-group
     for (int t = 0; t < slabs; t++) {
         // slab t is there, for every wave: the loads issued after it are at most the ring's
@@ -190,7 +208,7 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
             more = next < nsg;
             if (more) {
                 const int to = at + ST - 1 < ST ? at + ST - 1 : at - 1;
-                wf.get(next, ring0 + to * kTileBytes, lane);
+                weights_get(next, ring0 + to * kTileBytes);
                 // (the wave's first ST - 1 super-groups of a slab were fetched before the next slab's activations)
                 wait_loads<(ST - 1) * kTileLoads>(j < ST - 1 ? newer : 0);
             } else {
@@ -205,7 +223,7 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[m][i] = *(const h8*)(row + 16 * i);
             }
-            multiply<QT, MT>(mg, raw, x, kg, acc);
+            if (!ONE || list[s / per] >= 0) multiply<QT, MT>(mg, raw, x, kg, acc);   // (a slot without an expert: h is not there)
             at = at + 1 < ST ? at + 1 : 0;
         }
         // the next slab's loads are older than the ring's last one
@@ -231,6 +249,11 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
 #pragma unroll
             for (int q = 0; q < KS; q++) v[m] += red[(((tl * NM + m) * KS + q) * MT + t) * TS + row * RS + col];
         }
+        if constexpr (ONE) {
+            if (a.out_f16) ((_Float16*)a.C)[f] = (_Float16)v[0];
+            else ((float*)a.C)[f] = v[0];
+            continue;
+        }
         const int slot = list[i];
         if constexpr (GU) {
             const float ex = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
@@ -243,14 +266,20 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
 
 // grid x: workgroups' weight rows; y: experts, or slots where there are fewer
 // of them (the first slot of an expert stands for it).
-template <int QT, int MT, bool GU, int KS>
+template <int QT, int MT, int MODE, int KS>
 __global__ __launch_bounds__(64 * kMoeWaves, MT == 1 ? 4 : 2)
 void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, int R, int K, int by_slot, int cap, Lists l) {
-    constexpr int TW = kMoeWaves / (KS * (GU ? 2 : 1));
+    constexpr int TW = kMoeWaves / (KS * (MODE == kMoeH ? 2 : 1));
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ int32_t found[kScanSlots];
     __shared__ int wave_cnt[kMoeWaves];
     const int slots = a.T * a.k;
+    if constexpr (MODE == kMoeRow) {
+        for (int j = threadIdx.x; j < a.k; j += 64 * kMoeWaves) found[j] = a.ids[j] < a.E ? a.ids[j] : -1;
+        __syncthreads();
+        rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, 0, TW * (int)blockIdx.x, found, 1, 1, lds);
+        return;
+    }
     const int e = by_slot ? a.ids[blockIdx.y] : (int)blockIdx.y;
     if (e < 0 || e >= a.E) return;
     const int32_t* list = found;
@@ -281,8 +310,8 @@ void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, in
     const int tile0 = TW * (int)blockIdx.x;
     for (int c = 0; c < cnt; c += cap) {           // (cap <= 16 MT rows a pass)
         const int n = min(cnt - c, cap);
-        if (MT > 1 && n > 16) rows_of<QT, MT, GU, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
-        else rows_of<QT, 1, GU, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
+        if (MT > 1 && n > 16) rows_of<QT, MT, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
+        else rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
     }
 }
 
@@ -492,16 +521,16 @@ bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
 
 bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int QT, bool GU, int MT, int KS>
+template <int QT, int MODE, int MT, int KS>
 hipError_t launch_split(int64_t experts, hipStream_t st, const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out,
                         int R, int K, int by_slot, const Lists& l) {
-    constexpr int TW = kMoeWaves / (KS * (GU ? 2 : 1)), CH = KS < 2 ? 2 : KS;
+    constexpr int TW = kMoeWaves / (KS * (MODE == kMoeH ? 2 : 1)), CH = KS < 2 ? 2 : KS;
     constexpr int ring = kMoeWaves * kMoeStages * kTileBytes, meet = kMoeWaves * MT * 16 * 20 * 4;
-    constexpr int most = std::max(ring + 2 * 16 * MT * kSlabRow<CH>, meet);
-    const int cap = (int)std::min<int64_t>(16 * MT, (int64_t)a.T * a.k);
+    constexpr int rows = MODE == kMoeRow ? 1 : 16 * MT, most = std::max(ring + 2 * rows * kSlabRow<CH>, meet);
+    const int cap = (int)std::min<int64_t>(rows, (int64_t)a.T * a.k);
     const int lds = std::max(ring + 2 * cap * kSlabRow<CH>, meet);
     const int tiles = (R + 15) / 16;
-    auto k = k_moe_rows<QT, MT, GU, KS>;
+    auto k = k_moe_rows<QT, MT, MODE, KS>;
     static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -539,9 +568,10 @@ hipError_t launch_rows(const MoeArgs& a, const uint16_t* A, int64_t lda, void* o
     const int ks = waves < 1536 ? 4 : waves < 3072 ? 2 : 1;
     const auto go = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
-        return ks == 1 ? launch_split<QT, GU, MT, 1>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
-               : ks == 2 || MT == 2 ? launch_split<QT, GU, MT, 2>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
-                                    : launch_split<QT, GU, 1, 4>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l);
+        constexpr int MODE = GU ? kMoeH : kMoeY;
+        return ks == 1 ? launch_split<QT, MODE, MT, 1>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
+               : ks == 2 || MT == 2 ? launch_split<QT, MODE, MT, 2>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
+                                    : launch_split<QT, MODE, 1, 4>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l);
     };
     return slots <= 8 * (int64_t)a.E ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 2>());
 }
@@ -594,6 +624,12 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     } else {
         e = launch_rows<QT, true>(a, a.A, a.lda, ws, l, fast, st);
         if (e != hipSuccess) return e;
+        // One row: its slots' h lie one after the other, and the down products of
+        // its experts are one sum (8 experts of 2048 x 1024: 16.7 us with y and its
+        // sum, 14.2 without).
+        if (fast && a.T == 1 && !l.perm && slots * a.F < (1 << 30))
+            return launch_split<QT, kMoeRow, 1, 8>(1, st, a, MoeW{{a.down, nullptr}, {a.down_aux, nullptr}}, (const uint16_t*)ws, a.F,
+                                                   nullptr, a.N, a.F, 0, l);
         e = launch_rows<QT, false>(a, (const uint16_t*)ws, a.F, ws + o.y, l, fast, st);
     }
     if (e != hipSuccess) return e;

@@ -531,7 +531,8 @@ bf_status bf_moe_route(const bf_moe_route_args* args, void* stream);
  * expert e - 1's (W_aux likewise).  An id that is negative or not below E adds
  * nothing (an expert that another GPU holds).  The intermediate is rounded to
  * fp16 once, its weight already in it; the sums over experts run in fp32 in
- * the order of j, so the result does not depend on the other rows' routing.
+ * the order of j, so a row's result does not depend on the other rows' routing
+ * (for a given number of rows: a single row's sum over experts is one sum).
  * Requirements as for bf_gemm; the matrix-core path takes K and F multiples of
  * 256, 16-byte aligned A and W and lda % 8 == 0 (4-byte aligned W_aux); Q4_K
  * needs it, other legal Q4_0 inputs run one thread per output. */
