@@ -22,8 +22,11 @@
  *       * bf_gemm_ws / bf_gemm_batched_ws / bf_busfill_q4_ws: the caller owns
  *         it (size from bf_gemm_workspace_bytes / bf_gemm_batched_workspace_bytes);
  *         the library allocates nothing and keeps no state between calls.
+ *         bf_kv4_attention_ws and bf_moe_ffn_ws do the same for their partial
+ *         results and intermediates.
  *       * bf_gemm_noalloc: a fixed array in device memory per GPU.
- *       * bf_gemm, bf_gemm_batched, bf_busfill_q4, bf_ffn_swiglu: the
+ *       * bf_gemm, bf_gemm_batched, bf_busfill_q4, bf_ffn_swiglu,
+ *         bf_kv4_attention, bf_moe_ffn: the
  *         library's workspace for the (device, stream) -- per host thread for
  *         hipStreamPerThread -- allocated by the first call on the stream that
  *         needs it and grown by a later call that needs more (each region that
@@ -531,8 +534,9 @@ bf_status bf_moe_route(const bf_moe_route_args* args, void* stream);
  * expert e - 1's (W_aux likewise).  An id that is negative or not below E adds
  * nothing (an expert that another GPU holds).  The intermediate is rounded to
  * fp16 once, its weight already in it; the sums over experts run in fp32 in
- * the order of j, so a row's result does not depend on the other rows' routing
- * (for a given number of rows: a single row's sum over experts is one sum).
+ * the order of j (a single row's as one long sum).  Equal calls give equal
+ * bits; how many rows there are, and with many of them how many an expert has,
+ * selects the kernels, and with them the order of the sums over K and F.
  * Requirements as for bf_gemm; the matrix-core path takes K and F multiples of
  * 256, 16-byte aligned A and W and lda % 8 == 0 (4-byte aligned W_aux); Q4_K
  * needs it, other legal Q4_0 inputs run one thread per output. */
