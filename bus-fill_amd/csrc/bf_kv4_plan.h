@@ -45,17 +45,28 @@ struct Kv4Plan {
     size_t bytes;                                  // their workspace
 };
 
-constexpr int kKv4Alone = 40;                      // tiles that one workgroup takes rather than share them
-constexpr int kKv4LeastChunk = 20;
 constexpr int kKv4PerCu = 4;                       // workgroups of four waves that a CU holds
+constexpr int kKv4Alone = 40;                      // tiles that one workgroup takes rather than share them
+constexpr int kKv4AloneMany = 256;                 // ... where there are workgroups enough without
+constexpr int kKv4LeastFill = 8;                   // tiles of a chunk (a wave each)
+constexpr int kKv4LeastChunk = 20;                 // ... where sequences differ in length
 
-// Chunks: three times as many as the chip has places where that leaves each
-// kKv4LeastChunk tiles, so that sequences of different lengths even out
-// (measured at 32 sequences of 2000 to 8000 tokens, 8 heads of 128: chunks of
-// 12 / 20 / 40 / 64 tiles 60.6 / 58.6 / 58.7 / 64.0 us; one sequence of 131072,
-// 4 heads: 16 / 24 / 40 / 64 tiles 29.1 / 27.6 / 27.6 / 33.8 us).  Short
-// sequences are not cut (16 queries' heads over 1024 tokens of 64 values: 8.0
-// us alone, 11.3 us in chunks of 12).
+// Chunks.  A joining launch costs 4 to 6 us and an unevenly filled last round of
+// workgroups as much, lengths are in device memory (max_kv is all the host
+// knows), and a chip of 256 CUs reads at full rate with eight waves on each.
+// Measured in us, 8 key/value heads of 128 unless said, one query a sequence:
+// * Up to 40 tiles, alone (1030 tokens: 10.8, in chunks of 8 tiles 10.5; 16
+//   sequences of up to 1100: 11.6 and 14.0).
+// * From 3/4 as many units as CUs and up to 256 tiles, alone, eight waves (64
+//   sequences of up to 2048: 25.3, chunks of 20 tiles and four waves 38.7; 24 of
+//   up to 3000: 21.8 and 23.9; 32 of up to 8000: 49.7 and 53.3).  Past that a
+//   sequence much longer than the others would keep one workgroup too long.
+// * One sequence, or chunks of up to 32 tiles: as many chunks as fill the CUs
+//   once, eight waves (131072 tokens, 4 heads: 65 tiles 22.7, 33 tiles 25.4, 20
+//   tiles and four waves 30.0; 32768: 17.0 and 19.2; 2048: 10.7 and 12.5).
+// * Else three times as many as the chip has places of four waves, so that
+//   sequences of different lengths even out (20 of up to 8000: 37.8, filling
+//   once 42.8 to 47).
 inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
     Kv4Plan p;
     p.group = a.q_heads / a.c.heads;
@@ -73,9 +84,14 @@ inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
     const int64_t most = std::max<int64_t>(1, (seen + 2 * kKv4Tile - 2) / kKv4Tile);   // the range may start inside a tile
     p.items = (int64_t)a.S * p.row_tiles;
     const int64_t units = p.items * a.c.heads, places = (int64_t)cus * (a.c.dim == 256 ? 2 : kKv4PerCu);
-    p.chunk = (int)(p.prompt || most <= kKv4Alone ? most : std::min(most, std::max<int64_t>(kKv4LeastChunk, (units * most + 3 * places - 1) / (3 * places))));
+    const int64_t share = std::max<int64_t>(1, cus / units), fill = (most + share - 1) / share;
+    if (p.prompt || most <= kKv4Alone || (4 * units >= 3 * (int64_t)cus && most <= kKv4AloneMany)) p.chunk = (int)most;
+    else if (share > 1 && (a.S == 1 || fill <= 32)) p.chunk = (int)std::max<int64_t>(kKv4LeastFill, fill);
+    else p.chunk = (int)std::min(most, std::max<int64_t>(kKv4LeastChunk, (units * most + 3 * places - 1) / (3 * places)));
     p.splits = (int)((most + p.chunk - 1) / p.chunk);
-    p.waves = units * p.splits < cus ? 8 : 4;      // few workgroups: twice the waves on each
+    // Eight waves where there are no more workgroups than CUs, or long walks of whole sequences (64 of up to 500
+    // tokens: 12.1 with eight, 11.8 with four; 24 of up to 3000: 21.6 and 26.0)
+    p.waves = units * p.splits <= cus || (p.splits == 1 && most > kKv4Alone) ? 8 : 4;
     p.slots = p.splits > 1 ? units * p.splits : 0;
     p.bytes = (size_t)p.slots * kKv4Rows * (a.c.dim + 2) * sizeof(float);
     return p;

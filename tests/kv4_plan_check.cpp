@@ -81,7 +81,7 @@ void check_plans() {
                                     // a range of `seen` tokens may start at any token of a tile
                                     const int64_t tiles = seen == 0 ? 0 : (seen + kKv4Tile - 1 + kKv4Tile - 1) / kKv4Tile;
                                     expect((int64_t)p.chunk * p.splits >= tiles, "chunks cover the tiles", tiles, p.chunk, p.splits);
-                                    expect(p.splits == 1 || (p.chunk >= kKv4LeastChunk && !p.prompt), "chunks of a size", p.chunk, p.splits, p.prompt);
+                                    expect(p.splits == 1 || (p.chunk >= kKv4LeastFill && !p.prompt), "chunks of a size", p.chunk, p.splits, p.prompt);
                                     expect(p.slots == (p.splits > 1 ? p.items * heads * p.splits : 0), "slots", p.slots);
                                     expect(p.bytes == (size_t)p.slots * 16 * (dim + 2) * 4, "bytes", p.slots, (int64_t)p.bytes);
                                     expect(p.waves == 4 || p.waves == 8, "waves", p.waves);
