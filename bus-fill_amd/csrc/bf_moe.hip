@@ -10,7 +10,11 @@
 // 4096 outputs), and the fp32 sum of a row's slots in their order.  The row's
 // weight goes into h before its rounding.
 //
-// Bound by the weights of the experts in use, each read once.
+// Bound by the weights of the experts in use, each read once.  Up to about 24
+// slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
+// row of 2048 x 1024 14.2 us for 28 MB; 32 rows, 64 experts of 5120 x 1280, 161 us
+// for 697 MB, 4.3 TB/s), above that k_moe_tile (2000 rows, 64 experts of 4096 x
+// 1792, Q4_0: 957 us for 705 GFLOP).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -89,15 +93,17 @@ __device__ __forceinline__ void store_y(const MoeArgs& a, void* y, int64_t at, f
     else ((float*)y)[at] = v;
 }
 
-// What a launch of k_moe_rows computes: h (gate and up), y (down, by slot), or
-// the outputs of a single row (down over its slots' experts as one long sum).
-enum : int { kMoeH = 0, kMoeY = 1, kMoeRow = 2 };
+// What a launch of k_moe_rows computes: h (gate and up), y (down, by slot; or with
+// all the activations of a pass in LDS), or the outputs of a single row (down over
+// its slots' experts as one long sum).
+enum : int { kMoeH = 0, kMoeY = 1, kMoeRow = 2, kMoeWhole = 3 };
 
 // One super-group (144 bytes a row) of 16 weight rows into LDS, row after row:
 // pieces of 16 bytes, nine to a row.  Neighbouring lanes fetch neighbouring
 // pieces: as operand registers, where neighbouring lanes are different rows, the
 // same bytes took 192 accesses to the L1 cache and the activations 128 more
-// (86 % of its cycles at 32 rows, 64 experts; 228 us there, 138 from LDS).
+// (86 % of its cycles; the whole block at 32 rows of 64 experts of 5120 x 1280,
+// eight a row: 220 us so, 171 through LDS).
 constexpr int kTileBytes = 16 * 144, kTileLoads = 3;
 template <int QT> struct TileFetch {
     const uint8_t* src[kTileLoads];
@@ -264,14 +270,74 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
     }
 }
 
+// y of up to 16 slots of one expert against `many` tiles of 16 weight rows a
+// wave, where all of the slots' activations fit in LDS: one barrier, then every
+// wave streams its own tiles (32 rows, 64 experts, eight a row: 5120 x 1280 166.7
+// us with rows_of, 160.9 so; 2048 x 1024 64.7 and 61.2; 100 rows, 128 experts of
+// 4096 x 256, four a row: 74.2 and 60.1).
+template <int QT>
+__device__ __forceinline__ void rows_whole(const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out, int R,
+                                           int K, int64_t e, int tile0, int many, const int32_t* list, int cnt, uint8_t* lds) {
+    constexpr int ST = kMoeStages;
+    const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per = K >> 8, tiles = R >> 4, first = tile0 + wave, mine = first < tiles ? min(many, (tiles - first + kMoeWaves - 1) / kMoeWaves) : 0;
+    uint8_t* const ring = lds + wave * (ST * kTileBytes);
+    const uint32_t ring0 = lds_addr(ring);
+    uint8_t* const x0 = lds + kMoeWaves * ST * kTileBytes;
+    const int stride = 2 * K + 16;
+    TileFetch<QT> wf;
+    wf.init(w.W[0], w.aux[0], e * R + (mine ? 16 * first : 0), 16, K, lane);
+    wf.expert = 16 * kMoeWaves * (QT == QT_PLANES ? (int64_t)(K >> 4) : (int64_t)per * 144);   // (from one tile of the wave to the next)
+    __syncthreads();                               // LDS is free
+    int fs = 0, ft = 0;                            // the next super-group to fetch
+    auto fetch = [&](int n) {
+        wf.get(fs, ft, ring0 + (n % ST) * kTileBytes, lane);
+        if (++fs == per) fs = 0, ft++;
+    };
+    const int total = mine * per;
+    for (int i = wave; i < cnt; i += kMoeWaves) {
+        const uint16_t* row = A + (int64_t)list[i] * lda;
+        for (int c = 0; c < K; c += 512)
+            if (c + 8 * lane < K) dma16(row + c + 8 * lane, lds_addr(x0) + i * stride + 2 * c);
+    }
+    if (total) fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    barrier_lds();
+    const Magic mg = make_magic();
+    const uint8_t* const row = x0 + min(r, cnt - 1) * stride + 128 * kg;
+    int n = 0;
+    for (int t = 0; t < mine; t++) {
+        f4 acc[1] = {f4{0.f, 0.f, 0.f, 0.f}};
+        for (int s = 0; s < per; s++, n++) {
+            if (n + 1 < total) {
+                fetch(n + 1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kTileLoads) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            Raw<QT> raw;
+            lds_raw<QT>(raw, ring + (n % ST) * kTileBytes + r * 144, kg);
+            h8 x[1][8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[0][i] = *(const h8*)(row + 512 * s + 16 * i);
+            multiply<QT, 1>(mg, raw, x, kg, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (4 * kg + i < cnt) store_y(a, out, (int64_t)list[4 * kg + i] * R + 16 * (first + kMoeWaves * t) + r, acc[0][i]);
+    }
+}
+
 // grid x: workgroups' weight rows; y: experts, or slots where there are fewer
 // of them (the first slot of an expert stands for it).
 template <int QT, int MT, int MODE, int KS>
 __global__ __launch_bounds__(64 * kMoeWaves, MT == 1 ? 4 : 2)
-void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, int R, int K, int by_slot, int cap, Lists l) {
+void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, int R, int K, int by_slot, int cap, int many, Lists l) {
     constexpr int TW = kMoeWaves / (KS * (MODE == kMoeH ? 2 : 1));
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ int32_t found[kScanSlots];
+    __shared__ int32_t own[MODE == kMoeWhole ? 1 : kScanSlots];
+    int32_t* const found = MODE == kMoeWhole ? (int32_t*)(lds + kMoeWaves * kMoeStages * kTileBytes + cap * (2 * K + 16)) : own;
     __shared__ int wave_cnt[kMoeWaves];
     const int slots = a.T * a.k;
     if constexpr (MODE == kMoeRow) {
@@ -310,6 +376,10 @@ void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, in
     const int tile0 = TW * (int)blockIdx.x;
     for (int c = 0; c < cnt; c += cap) {           // (cap <= 16 MT rows a pass)
         const int n = min(cnt - c, cap);
+        if constexpr (MODE == kMoeWhole) {
+            rows_whole<QT>(a, w, A, lda, out, R, K, e, TW * many * (int)blockIdx.x, many, list + c, n, lds);
+            continue;
+        }
         if (MT > 1 && n > 16) rows_of<QT, MT, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
         else rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
     }
@@ -521,6 +591,14 @@ bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
 
 bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+constexpr int kWholeMost = 81920 - 512;            // two workgroups a CU
+// LDS of k_moe_rows in its kMoeWhole form: the waves' rings, the activations, the list of slots
+int64_t whole_bytes(const MoeArgs& a, int K) {
+    const int64_t slots = (int64_t)a.T * a.k;
+    return kMoeWaves * kMoeStages * kTileBytes + std::min<int64_t>(16, slots) * (2 * (int64_t)K + 16) +
+           4 * std::min<int64_t>(slots, kScanSlots);
+}
+
 template <int QT, int MODE, int MT, int KS>
 hipError_t launch_split(int64_t experts, hipStream_t st, const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out,
                         int R, int K, int by_slot, const Lists& l) {
@@ -542,7 +620,29 @@ hipError_t launch_split(int64_t experts, hipStream_t st, const MoeArgs& a, const
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     hipLaunchKernelGGL(k, dim3((unsigned)((tiles + TW - 1) / TW), (unsigned)experts), dim3(64 * kMoeWaves), lds, st, a, w, A, lda,
-                       out, R, K, by_slot, cap, l);
+                       out, R, K, by_slot, cap, 1, l);
+    return hipGetLastError();
+}
+
+template <int QT>
+hipError_t launch_whole(int64_t experts, int many, hipStream_t st, const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda,
+                        void* out, int R, int K, int by_slot, const Lists& l) {
+    const int cap = (int)std::min<int64_t>(16, (int64_t)a.T * a.k);
+    const int lds = (int)whole_bytes(a, K);
+    auto k = k_moe_rows<QT, 1, kMoeWhole, 1>;
+    static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kWholeMost);
+        if (e != hipSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const int per = kMoeWaves * many, tiles = R / 16;
+    hipLaunchKernelGGL(k, dim3((unsigned)((tiles + per - 1) / per), (unsigned)experts), dim3(64 * kMoeWaves), lds, st, a, w, A, lda,
+                       out, R, K, by_slot, cap, many, l);
     return hipGetLastError();
 }
 
@@ -566,6 +666,15 @@ hipError_t launch_rows(const MoeArgs& a, const uint16_t* A, int64_t lda, void* o
     // gate and up / down in 4, 2, 1 parts: one row, 8 experts, 1024 waves 16.7,
     // 18.1, 22.4 us; eight rows, 32 slots, 4096 waves 52.8, 33.7, 29.8).
     const int ks = waves < 1536 ? 4 : waves < 3072 ? 2 : 1;
+    if constexpr (!GU) {
+        // As many tiles a wave as leave one round of two workgroups a CU (32 rows, 64
+        // experts of 5120 x 1280: 5 tiles, 512 workgroups 160.9 us; 4 and 8 tiles 168.6
+        // and 177.0; 2048 x 1024: 2 tiles 61.2, 1 and 3 tiles 63.8 and 65.7).
+        const int64_t groups = (R / 16 + kMoeWaves - 1) / kMoeWaves, cus = device_cus() > 0 ? device_cus() : 256;
+        const int many = (int)std::clamp<int64_t>((groups * std::min<int64_t>(experts, slots) + 2 * cus - 1) / (2 * cus), 1, 8);
+        if (ks == 1 && slots <= 8 * (int64_t)a.E && R % 16 == 0 && whole_bytes(a, K) <= kWholeMost)
+            return launch_whole<QT>(experts, many, st, a, w, A, lda, out, R, K, (int)by_slot, l);
+    }
     const auto go = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         constexpr int MODE = GU ? kMoeH : kMoeY;

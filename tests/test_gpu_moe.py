@@ -235,6 +235,15 @@ def test_experts_large_tiles(qt, otype):
     Experts(qt, E, 256, 1024, 2048).check(T, k, ids=ids, otype=otype, rows=rows)
 
 
+@pytest.mark.parametrize("qt", QTS)
+def test_experts_several_tiles_a_wave(qt):
+    """Enough experts and outputs that a wave of the down products takes several tiles, the last ones short; evenly
+    spread slots, and all to two experts (several passes of 16)."""
+    x = Experts(qt, 40, 512, 512, 1808)
+    x.check(30, 5)
+    x.check(60, 2, ids=torch.tensor([[3, 39]]).repeat(60, 1), otype=bf.OUT_F16, pad=8)
+
+
 @pytest.mark.parametrize("T", [5, 600])
 def test_experts_all_to_one(T):
     x = Experts(O.Q4_K, 6, 256, 256, 96)
