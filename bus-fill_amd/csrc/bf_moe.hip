@@ -4,11 +4,11 @@
 //
 // over 4-bit weights in place.  A slot is one (t, j).  Three launches: h of
 // every slot (gate and up of the same 16 rows in one workgroup, SiLU(g) u w
-// rounded once to fp16), y = Wd h of every slot (in the output's type: for fp16
-// outputs each y is rounded as the output will be, which halves the bytes
-// between the last two launches, 262 MB of fp32 at 2000 rows of eight slots and
-// 4096 outputs), and the fp32 sum of a row's slots in their order.  The row's
-// weight goes into h before its rounding.
+// rounded once to fp16), y = Wd h of every slot, and the fp32 sum of a row's slots
+// in their order.  The row's weight goes into h before its rounding.  y is fp32,
+// but for fp16 outputs of many rows, where each y is rounded as the output will
+// be, which halves the bytes between the last two launches (262 MB of fp32 at
+// 2000 rows of eight slots and 4096 outputs).
 //
 // Bound by the weights of the experts in use, each read once.  Up to about 24
 // slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
@@ -31,6 +31,7 @@ namespace {
 constexpr int kMoeWaves = 8;
 constexpr int kMoeStages = 2;                      // super-groups of a wave's weights in LDS
 constexpr int kSumY = 32768;                       // rows of the sum along grid y
+constexpr int kMoeTileSlots = 24;                  // slots an expert, on average, from which tiles take the products
 constexpr int kScanSlots = 1024;                   // up to so many slots a workgroup finds its expert's by itself
 
 // Slots of one expert: in LDS (found by the workgroup), or in the plan's list.
@@ -88,8 +89,13 @@ __device__ __forceinline__ void multiply(const Magic& mg, const Raw<QT>& raw, co
     }
 }
 
+// y in fp16: for fp16 outputs of many rows.
+__host__ __device__ __forceinline__ bool y_f16(const MoeArgs& a) {
+    return a.out_f16 && (int64_t)a.T * a.k >= kMoeTileSlots * (int64_t)a.E;
+}
+
 __device__ __forceinline__ void store_y(const MoeArgs& a, void* y, int64_t at, float v) {
-    if (a.out_f16) ((_Float16*)y)[at] = (_Float16)v;
+    if (y_f16(a)) ((_Float16*)y)[at] = (_Float16)v;
     else ((float*)y)[at] = v;
 }
 
@@ -554,14 +560,14 @@ __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const Y* __restrict_
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Workspace: h [slots][F] fp16, y [slots][N] in the output's type, the plan.
+// Workspace: h [slots][F] fp16, y [slots][N] fp32 or fp16, the plan.
 struct MoeWs {
     size_t y, perm, offs, table, tiles, end;
     int64_t max_tiles;
     explicit MoeWs(const MoeArgs& a) {
         const size_t slots = (size_t)a.T * a.k;
         y = up256(slots * a.F * 2);
-        perm = y + up256(slots * a.N * (a.out_f16 ? 2 : 4));
+        perm = y + up256(slots * a.N * (y_f16(a) ? 2 : 4));
         offs = perm + up256(slots * 4);
         table = offs + up256(((size_t)a.E + 1) * 4);
         max_tiles = (int64_t)std::min<size_t>(a.E, slots) + (int64_t)(slots / kMoeTileRows);
@@ -585,7 +591,7 @@ int large_least(const MoeArgs& a) {
 // fits a launch.
 bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
     const int64_t slots = (int64_t)a.T * a.k, nt = std::max<int64_t>(a.F / 64, (a.N + 127) / 128);
-    return slots >= 24 * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
+    return slots >= kMoeTileSlots * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
            launch_fits(o.max_tiles * nt, 512) && o.max_tiles * nt < INT32_MAX;
 }
 
@@ -743,7 +749,7 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     }
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)((a.N + 1023) / 1024), (unsigned)std::min(a.T, kSumY), (unsigned)((a.T + kSumY - 1) / kSumY));
-    if (a.out_f16) hipLaunchKernelGGL(k_moe_sum<_Float16>, grid, dim3(256), 0, st, a, (const _Float16*)(ws + o.y));
+    if (y_f16(a)) hipLaunchKernelGGL(k_moe_sum<_Float16>, grid, dim3(256), 0, st, a, (const _Float16*)(ws + o.y));
     else hipLaunchKernelGGL(k_moe_sum<float>, grid, dim3(256), 0, st, a, (const float*)(ws + o.y));
     return hipGetLastError();
 }

@@ -39,7 +39,7 @@ struct MoeTileArgs {
     const uint16_t* A;         // rows of tokens, or of slots
     uint32_t a_bytes;          // from A on: below 4 GB
     int64_t lda;
-    void* out;                 // h fp16, or y in the output's type, by slot
+    void* out;                 // h fp16, or y (fp16 for fp16 outputs), by slot
     int R, K;                  // weight rows of an expert, their length
     int nt[2];                 // column tiles of a large and of a small tile's rows
     const int32_t* perm;       // slots by expert

@@ -200,7 +200,9 @@ def test_experts_workspace(qtype):
     L, a = bf.lib(), experts(qtype)
     need = bf.moe_ffn_workspace_bytes(a)
     assert need >= 8 * (256 * 2 + 128 * 4)                     # h and y of every slot
-    assert bf.moe_ffn_workspace_bytes(experts(qtype, otype=bf.OUT_F16)) < need
+    assert bf.moe_ffn_workspace_bytes(experts(qtype, otype=bf.OUT_F16)) == need
+    many = [bf.moe_ffn_workspace_bytes(experts(qtype, T=400, otype=o)) for o in (bf.OUT_F32, bf.OUT_F16)]
+    assert many[1] < many[0]                                   # (y in fp16)
     assert bf.moe_ffn_workspace_bytes(experts(qtype, T=4000)) >= 8000 * (256 * 2 + 128 * 4)
     ws = lambda p, n: lambda: L.bf_moe_ffn_ws(ctypes.byref(a), p, n, None)
     refused(ws(FAKE, need - 1), f"needs {need} bytes")
