@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
                 const f16x d = mfma32x32x16(kf[b][1], q[2 * (b0 + b) + 1], mfma32x32x16(kf[b][0], q[2 * (b0 + b)], zero));
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    x[e] = b0 + b == 0 ? (float)ks[b][e >> 3][e & 7] * d[e] : __builtin_fmaf((float)ks[b][e >> 3][e & 7], d[e], x[e]);
+                    x[e] = __builtin_fmaf((float)ks[b][e >> 3][e & 7], d[e], b0 + b ? x[e] : 0.f);   // (one v_fma_mix_f32 each)
             }
         }
         h8 vf[HB][2];
