@@ -45,6 +45,29 @@ struct Kv4Plan {
     size_t bytes;                                  // their workspace
 };
 
+// The prompt kernel takes 128 rows through a record in 1.2 to 1.4 us (heads of 128),
+// and as long where a workgroup has a CU to itself; k_kv4_attn takes 16 rows
+// through one in 0.19 us of a CU.  So the first where there is work for several
+// rounds of the CUs (row tiles of 16, times the share of the longest row's tokens
+// that the average one sees, at least seven a CU) and its blocks of 128 rows are
+// at least 3/4 full.  Prompt kernel and k_kv4_attn in us, 40 heads over 8 of 128:
+// prompts of 1000 tokens 52 and 41, 1500 73 and 87, 2000 93 and 134, 16 of 256 45 and
+// 72; 512 queries over 2000 91 and 56; 32 times 20 queries over 2000 93 and 81, 48
+// queries 132 and 169.  16 heads over 8 of 64: 2000 tokens 59 and 38, 4000 113 and
+// 112, 8 prompts of 1000 49 and 67; 16 over 4 of 256: 3000 tokens 280 and 267.
+inline bool prompt_serves(const Kv4Args& a, int group, int cus) {
+    const int64_t rows = (int64_t)a.max_q * group, tiles = (rows + kKv4Rows - 1) / kKv4Rows;
+    if (tiles < 6 * ((rows + kKv4PromptRows - 1) / kKv4PromptRows)) return false;
+    const int64_t all = std::min(a.S * tiles, (int64_t)a.T * group / kKv4Rows + a.S) * a.c.heads;
+    double share = 1.0;                            // causal rows: the first ones see less
+    if (a.causal && a.max_kv > 0) {
+        const double reach = a.window > 0 ? std::min(a.window, a.max_kv) : a.max_kv;
+        const double ramp = std::min<double>(a.max_q, std::max(0.0, reach - (a.max_kv - std::min(a.max_q, a.max_kv))));
+        share -= ramp * ramp / (2.0 * a.max_q * reach);
+    }
+    return (double)all * share >= 7.0 * cus;
+}
+
 constexpr int kKv4PerCu = 4;                       // workgroups of four waves that a CU holds
 constexpr int kKv4Alone = 40;                      // tiles that one workgroup takes rather than share them
 constexpr int kKv4AloneMany = 256;                 // ... where there are workgroups enough without
@@ -70,10 +93,8 @@ constexpr int kKv4LeastChunk = 20;                 // ... where sequences differ
 inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
     Kv4Plan p;
     p.group = a.q_heads / a.c.heads;
-    // The prompt kernel from 64 rows a sequence and head on, where its row tiles
-    // fill half the chip.
-    const int64_t rows = (int64_t)a.max_q * p.group, blocks = (rows + kKv4PromptRows - 1) / kKv4PromptRows;
-    p.prompt = rows >= 64 && (int64_t)a.S * a.c.heads * blocks >= cus / 2;
+    const int64_t rows = (int64_t)a.max_q * p.group;
+    p.prompt = prompt_serves(a, p.group, cus);
     p.tile_rows = p.prompt ? kKv4PromptRows : kKv4Rows;
     p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t seen = a.max_kv;                       // cached tokens a row tile can see

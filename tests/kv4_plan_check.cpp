@@ -1,8 +1,10 @@
 // CPU check of the 4-bit cache's layout and of the attention's launch plans
 // (bus-fill_amd/csrc/bf_kv4.h, bf_kv4_plan.h).  Prints what it expected on
-// failure; exit status 0 when all holds.
+// failure; exit status 0 when all holds.  `kv4_plan_check plan S T heads group
+// max_q max_kv causal window` prints a plan on 256 CUs, heads of 128 (prompt kernel, chunk, splits, waves).
 #include <cstdint>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <vector>
 
@@ -92,6 +94,23 @@ void check_plans() {
 }  // namespace
 
 int main(int argc, char** argv) {
+    if (argc == 10 && !std::strcmp(argv[1], "plan")) {
+        Kv4Args a;
+        std::memset(&a, 0, sizeof a);
+        int v[8];
+        for (int i = 0; i < 8; i++) v[i] = std::atoi(argv[2 + i]);
+        a.c = Kv4Shape{1, 64, v[2], 128};
+        a.S = v[0];
+        a.T = v[1];
+        a.q_heads = v[2] * v[3];
+        a.max_q = v[4];
+        a.max_kv = v[5];
+        a.causal = v[6];
+        a.window = v[7];
+        const Kv4Plan p = plan_kv4(a, 256);
+        std::printf("%d %d %d %d\n", p.prompt, p.chunk, p.splits, p.waves);
+        return 0;
+    }
     if (argc < 2 || !std::strcmp(argv[1], "layout")) check_layout();
     if (argc < 2 || !std::strcmp(argv[1], "plans")) check_plans();
     std::printf("%d failures\n", failures);

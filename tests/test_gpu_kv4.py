@@ -221,34 +221,34 @@ def test_several_queries(nqs, lens, group):
 def test_prompts(dim):
     """Enough rows for the kernel of many queries a sequence: whole and partial row tiles, queries behind cached tokens,
     sequences without queries and without tokens, a page that ends inside a record."""
-    s = Sequences([40, 65, 33, 150, 0, 96, 7, 31], 16, dim, page=32)
+    s = Sequences([40, 65, 33, 150, 0, 96, 7, 31], 40, dim, page=32)
     s.check([40, 33, 33, 50, 5, 0, 9, 31], 4, otype=bf.OUT_F16, pad=8)
 
 
-@pytest.mark.parametrize("causal,window,group,absent", [(False, 0, 4, ()), (True, 40, 3, ()), (True, 0, 16, ((1, 1), (2, 0))),
-                                                        (True, 1, 5, ()), (True, 0, 7, ())])
-def test_prompts_masks(causal, window, group, absent):
-    s = Sequences([100, 130, 64, 77], 32, 64)
+@pytest.mark.parametrize("heads,causal,window,group,absent", [
+    (40, False, 0, 4, ()), (64, True, 40, 3, ()), (32, True, 0, 16, ((1, 1), (2, 0))), (48, True, 1, 5, ()), (32, True, 0, 7, ())])
+def test_prompts_masks(heads, causal, window, group, absent):
+    s = Sequences([100, 130, 64, 77], heads, 64)
     s.check([70, 22, 64, 40], group, causal=causal, window=window, absent=absent)
     s.check([70, 22, 64, 40], group, causal=causal, window=window, absent=absent, scale=-0.1)
 
 
 def test_prompt_longer():
     """Several rounds of units on the chip, rows that see up to 20 records."""
-    Sequences([600], 4, 128).check([600], 8, otype=bf.OUT_F16)
+    Sequences([600], 16, 128).check([600], 8, otype=bf.OUT_F16)
 
 
 def test_prompt_nan_tokens_reach_only_those_who_see_them():
-    s = Sequences([80], 128, 64)
+    s = Sequences([120], 128, 64)
     k = torch.full((1, 128, 64), float("nan")).half().cuda()
     slot = (s.table[0, 0].long() * 64 + 40).reshape(1).cuda()
     for nan_keys in (True, False):
         bf.kv4_store(s.cache.c, k if nan_keys else torch.zeros_like(k), k, slot, 1)
-        q = torch.randn(80, 128 * 64).half().cuda()
-        o = torch.empty(80, 128 * 64, device="cuda")
+        q = torch.randn(120, 512 * 64).half().cuda()
+        o = torch.empty(120, 512 * 64, device="cuda")
         dev = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
-        bf.kv4_attention(s.cache.c, q, o, dev([0, 80]), dev([80]), s.table.cuda(), S=1, T=80, q_heads=128, max_q=80,
-                         max_kv=80, scale=0.1)
+        bf.kv4_attention(s.cache.c, q, o, dev([0, 120]), dev([120]), s.table.cuda(), S=1, T=120, q_heads=512, max_q=120,
+                         max_kv=120, scale=0.1)
         assert not o[:40].isnan().any() and o[40:].isnan().all()
 
 
