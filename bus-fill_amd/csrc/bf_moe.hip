@@ -10,7 +10,7 @@
 // be, which halves the bytes between the last two launches (262 MB of fp32 at
 // 2000 rows of eight slots and 4096 outputs).
 //
-// Bound by the weights of the experts in use, each read once.  Up to about 24
+// Bound by the weights of the experts in use, each read once.  Up to 28
 // slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
 // row of 2048 x 1024 14.2 us for 28 MB; 32 rows, 64 experts of 5120 x 1280, 161 us
 // for 697 MB, 4.3 TB/s), above that k_moe_tile (2000 rows, 64 experts of 4096 x
@@ -31,7 +31,7 @@ namespace {
 constexpr int kMoeWaves = 8;
 constexpr int kMoeStages = 2;                      // super-groups of a wave's weights in LDS
 constexpr int kSumY = 32768;                       // rows of the sum along grid y
-constexpr int kMoeTileSlots = 24;                  // slots an expert, on average, from which tiles take the products
+constexpr int kMoeTileSlots = 28;                  // slots an expert, on average, from which tiles take the products
 constexpr int kScanSlots = 1024;                   // up to so many slots a workgroup finds its expert's by itself
 
 // Slots of one expert: in LDS (found by the workgroup), or in the plan's list.
@@ -578,17 +578,22 @@ struct MoeWs {
 
 int64_t a_bytes(const MoeArgs& a) { return ((int64_t)(a.T - 1) * a.lda + a.K) * 2; }
 
-// Rows from which a run of slots takes a large tile: 193 where the whole block
-// has twice as many of them as the chip has CUs, else none does.
+// Rows from which a run of slots takes a large tile: 193 where whole runs alone
+// make large tiles for 3/8 of the CUs, else none does (large and small only, us:
+// 2000 rows of eight, 64 experts of 4096 x 1792, 868 tiles 934 and 1067; 500 rows of
+// four, 8 experts, 98 tiles 181 and 203; 1000 rows of four, 16 experts of 2048 x
+// 512, 60 tiles 102 and 83; 500 rows of two, 4 experts of 4096 x 1792, 42 tiles 163
+// and 102).
 int large_least(const MoeArgs& a) {
     const int64_t slots = (int64_t)a.T * a.k, cus = device_cus() > 0 ? device_cus() : 256;
-    return slots / kMoeTileRows * (std::min(2 * a.F, a.N) / 256) >= 2 * cus ? 193 : kMoeTileRows + 1;
+    return 8 * (slots / kMoeTileRows) * (std::min(2 * a.F, a.N) / 256) >= 3 * cus ? 193 : kMoeTileRows + 1;
 }
 
-// The tile kernel: from 24 rows an expert on average (64 experts of 2048 x 1024,
-// eight a row: at 130 rows 106 us in rows, 133 in tiles; at 250 rows 164 and
-// 140), rows addressed with 32 bits from the buffer's start, and a grid that
-// fits a launch.
+// The tile kernel: from 28 slots an expert on average (rows and tiles in us, 64
+// experts, eight a row, of 2048 x 1024: 200 rows 137 and 132, 225 rows 146 and 136;
+// of 4096 x 1792: 200 rows 329 and 399, 225 rows 374 and 401, 260 rows 444 and 397),
+// rows addressed with 32 bits from the buffer's start, and a grid that fits a
+// launch.
 bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
     const int64_t slots = (int64_t)a.T * a.k, nt = std::max<int64_t>(a.F / 64, (a.N + 127) / 128);
     return slots >= kMoeTileSlots * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
@@ -678,7 +683,7 @@ hipError_t launch_rows(const MoeArgs& a, const uint16_t* A, int64_t lda, void* o
         // and 177.0; 2048 x 1024: 2 tiles 61.2, 1 and 3 tiles 63.8 and 65.7).
         const int64_t groups = (R / 16 + kMoeWaves - 1) / kMoeWaves, cus = device_cus() > 0 ? device_cus() : 256;
         const int many = (int)std::clamp<int64_t>((groups * std::min<int64_t>(experts, slots) + 2 * cus - 1) / (2 * cus), 1, 8);
-        if (ks == 1 && slots <= 8 * (int64_t)a.E && R % 16 == 0 && whole_bytes(a, K) <= kWholeMost)
+        if (ks == 1 && slots <= 16 * (int64_t)a.E && R % 16 == 0 && whole_bytes(a, K) <= kWholeMost)
             return launch_whole<QT>(experts, many, st, a, w, A, lda, out, R, K, (int)by_slot, l);
     }
     const auto go = [&](auto mt) {
@@ -688,7 +693,10 @@ hipError_t launch_rows(const MoeArgs& a, const uint16_t* A, int64_t lda, void* o
                : ks == 2 || MT == 2 ? launch_split<QT, MODE, MT, 2>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l)
                                     : launch_split<QT, MODE, 1, 4>(experts, st, a, w, A, lda, out, R, K, (int)by_slot, l);
     };
-    return slots <= 8 * (int64_t)a.E ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 2>());
+    // Two row tiles a pass where most experts have more than one (one and two in us, 64
+    // experts of 2048 x 1024, eight a row: 100 rows 89.5 and 93.1, 130 rows 107.8 and
+    // 103.8; 8 experts of 4096 x 1792, two a row: 40 rows 35.3 and 43.9).
+    return slots <= 16 * (int64_t)a.E ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 2>());
 }
 
 template <int QT>
