@@ -7,8 +7,14 @@
 // integers times powers of two, so x / d is either exactly half way between two
 // integers or at least 2^-13 from it: floor(x rcp(d) + 8.5 + 2^-14), off by less
 // than 2^-18 in fp32, gives the codes of the exact formula without a division.
-// d = 0: all codes 8.  A block with an infinity or a NaN
-// gets d = NaN, codes 8: it reads as NaN, not as a finite guess.
+// d = 0: all codes 8.  A block with an infinity or a NaN gets d = NaN, codes 8: it
+// reads as NaN, not as a finite guess.
+//
+// Bytes: 2 read and 9/16 written per value (the read-back the other way).  2000
+// tokens of 8 heads of 128: 5.7 us to store and 6.0 to load 10.5 MB (a copy's rate
+// would be 2.2), 131072 tokens of 4 heads 88 us, 3.9 TB/s; 32 tokens 4.1 and 3.7 us,
+// a launch and its first loads.  A block per thread, so that its scale needs no
+// other lane; the price is values' codes stored byte by byte, 32 tokens apart.
 #include "bf_device.h"
 #include "bf_kv4_launch.h"
 

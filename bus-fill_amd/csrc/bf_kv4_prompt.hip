@@ -17,10 +17,10 @@
 //   Scores and probabilities are as exact as the single-token kernel's.  (Keys
 //   and values as exact fp16 pairs in LDS instead, hi and lo of (q - 8) d, need
 //   no scales here and twice the matrix products: 114 us where this takes 95.)
-// * 2000 causal tokens, 40 heads over 8 of 128: 94 us, 430 TFLOP/s of the visible
-//   pairs; the vector instructions of softmax and scales take half of the SIMDs'
-//   cycles, the matrix products 16 %.  Of the rest, decoding costs 19 us (timed
-//   without it), and the longest units (63 records) outlast the others.
+// * 2000 causal tokens, 40 heads over 8 of 128: 93 us, 440 TFLOP/s of the visible
+//   pairs; vector instructions issue in 65 % of the SIMDs' cycles, matrix products
+//   in 21 %.  A record takes 1.2 us of a CU that holds two workgroups or more, 1.4
+//   where one is alone; decoding is 19 us of the 93 (timed without it).
 //
 // Causal rows see ever more tokens: units go out longest first, every other
 // round of one per CU in reverse, so that the units that meet on a CU add up to

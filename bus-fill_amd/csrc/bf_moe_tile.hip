@@ -12,6 +12,12 @@
 // tiles of one wave: h = w SiLU(g) u leaves the registers as the one fp16 row
 // that the down product reads.  (Small tiles: two k groups of waves hold half of
 // each sum; each hands the other half of the rows over and finishes the rest.)
+//
+// 2000 rows of eight, 64 experts of 4096 x 1792 (Q4_0): gate and up 575 us, 820
+// TFLOP/s, down 317, 740; the prefill GEMM with whole tiles only reaches 950.  A third
+// of the experts have a few rows more than 256, whose small tiles decode as many
+// weights as a full one, and the last round of large tiles is half empty.  Matrix
+// units 42 to 47 % busy, vector instructions 27 %.
 #include <algorithm>
 #include <atomic>
 
