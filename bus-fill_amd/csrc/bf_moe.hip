@@ -10,7 +10,7 @@
 // be, which halves the bytes between the last two launches (262 MB of fp32 at
 // 2000 rows of eight slots and 4096 outputs).
 //
-// Bound by the weights of the experts in use, each read once.  Up to 28
+// Bound by the weights of the experts in use, each read once.  Up to 24
 // slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
 // row of 2048 x 1024 14.2 us for 28 MB; 32 rows, 64 experts of 5120 x 1280, 161 us
 // for 697 MB, 4.3 TB/s), above that k_moe_tile (2000 rows, 64 experts of 4096 x
@@ -31,7 +31,7 @@ namespace {
 constexpr int kMoeWaves = 8;
 constexpr int kMoeStages = 2;                      // super-groups of a wave's weights in LDS
 constexpr int kSumY = 32768;                       // rows of the sum along grid y
-constexpr int kMoeTileSlots = 28;                  // slots an expert, on average, from which tiles take the products
+constexpr int kMoeTileSlots = 24;                  // slots an expert, on average, from which tiles take the products
 constexpr int kScanSlots = 1024;                   // up to so many slots a workgroup finds its expert's by itself
 
 // Slots of one expert: in LDS (found by the workgroup), or in the plan's list.
@@ -49,7 +49,8 @@ struct MoeW {                                      // gate and up, or down
 // is one number for all of a lane's 32 weights of a sub-block, so sum_k a_k m_k
 // is a second product with that number as its operand (summing the activations
 // per sub-block first takes 44 more vector instructions of 200, and the matrix
-// unit has the time).  The Q4_0 formats' weights enter as their fp16 dequant.
+// unit has the time).  The Q4_0 formats' weights enter as their fp16 dequant, as in bf_gemm (one rounding
+// of 2^-11 of a weight: their blocks' scales change within an instruction's k).
 template <int QT, int MT>
 __device__ __forceinline__ void multiply(const Magic& mg, const Raw<QT>& raw, const h8 a[MT][8], int kg, f4 acc[MT]) {
     if constexpr (QT == QT_Q4_K) {
@@ -435,18 +436,16 @@ __global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW w, const uin
 // sums, so their order does not matter), then every wave writes its own run of
 // slots.
 constexpr int kPlanWaves = 16;
-// Of n slots: runs of 256, and the rest as one more of them from `least` rows on
-// (more than 256: no large tiles at all), else a small tile.
+// Of n slots: runs of `run`.  Runs of 256 are large tiles, and so is a rest from
+// `least` rows on (more than 256: no large tiles at all); all others small tiles.
 __device__ __forceinline__ int large_tiles(int n, int least) {
     return least > kMoeTileRows ? 0 : n / kMoeTileRows + (n % kMoeTileRows >= least);
 }
-__device__ __forceinline__ int small_tiles(int n, int least) {
-    return (n + kMoeTileRows - 1) / kMoeTileRows - large_tiles(n, least);
-}
+__device__ __forceinline__ int small_tiles(int n, int least, int run) { return (n + run - 1) / run - large_tiles(n, least); }
 __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __restrict__ ids, int slots, int E,
                                                               int32_t* __restrict__ perm, int32_t* __restrict__ offs,
                                                               int4* __restrict__ table, int* __restrict__ tiles, int max_tiles,
-                                                              int least) {
+                                                              int least, int run) {
     extern __shared__ int hist[];
     __shared__ int same[kPlanWaves], sum[3][kPlanWaves];
     const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -477,7 +476,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
     for (int i = threadIdx.x; i < e; i += 64 * kPlanWaves) {
         n[0] += hist[i];
         n[1] += large_tiles(hist[i], least);
-        n[2] += small_tiles(hist[i], least);
+        n[2] += small_tiles(hist[i], least, run);
     }
 #pragma unroll
     for (int c = 0; c < 3; c++) {
@@ -493,7 +492,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
         for (int c = 0; c < 3; c++) before[c] += sum[c][q];
         if (q < wave) at += same[q];
     }
-    const int base = before[0], total = hist[e], large = large_tiles(total, least), small = small_tiles(total, least);
+    const int base = before[0], total = hist[e], large = large_tiles(total, least), small = small_tiles(total, least, run);
     if (threadIdx.x == 0) {
         offs[e] = base;
         if (e == E - 1) {
@@ -504,7 +503,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
     }
     for (int i = threadIdx.x; i < large + small; i += 64 * kPlanWaves)
         table[i < large ? before[1] + i : max_tiles + before[2] + i - large] =
-            int4{e, base + i * kMoeTileRows, min(kMoeTileRows, total - i * kMoeTileRows), 0};
+            int4{e, base + i * run, min(run, total - i * run), 0};
     at += base;
     for (int s = s0; s < s1; s += 512) {
         int id[8];
@@ -560,6 +559,12 @@ __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const Y* __restrict_
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// Slots of a run: 64, in a kernel of two workgroups a CU, up to 48 slots an expert
+// on average, else 256 (64 and 256 in us, 64 experts, eight a row, of 4096 x 1792:
+// 230 rows 360 and 393, 400 rows 416 and 422, 500 rows 516 and 469; of 2048 x 1024:
+// 230 rows 116 and 136, 400 rows 127 and 148, 600 rows 191 and 195).
+int run_rows(const MoeArgs& a) { return (int64_t)a.T * a.k < 48 * (int64_t)a.E ? 64 : kMoeTileRows; }
+
 // Workspace: h [slots][F] fp16, y [slots][N] fp32 or fp16, the plan.
 struct MoeWs {
     size_t y, perm, offs, table, tiles, end;
@@ -570,7 +575,7 @@ struct MoeWs {
         perm = y + up256(slots * a.N * (y_f16(a) ? 2 : 4));
         offs = perm + up256(slots * 4);
         table = offs + up256(((size_t)a.E + 1) * 4);
-        max_tiles = (int64_t)std::min<size_t>(a.E, slots) + (int64_t)(slots / kMoeTileRows);
+        max_tiles = (int64_t)std::min<size_t>(a.E, slots) + (int64_t)(slots / run_rows(a));
         tiles = table + up256((size_t)max_tiles * 32);
         end = tiles + 256;
     }
@@ -586,14 +591,13 @@ int64_t a_bytes(const MoeArgs& a) { return ((int64_t)(a.T - 1) * a.lda + a.K) * 
 // and 102).
 int large_least(const MoeArgs& a) {
     const int64_t slots = (int64_t)a.T * a.k, cus = device_cus() > 0 ? device_cus() : 256;
-    return 8 * (slots / kMoeTileRows) * (std::min(2 * a.F, a.N) / 256) >= 3 * cus ? 193 : kMoeTileRows + 1;
+    return run_rows(a) == kMoeTileRows && 8 * (slots / kMoeTileRows) * (std::min(2 * a.F, a.N) / 256) >= 3 * cus ? 193 : kMoeTileRows + 1;
 }
 
-// The tile kernel: from 28 slots an expert on average (rows and tiles in us, 64
-// experts, eight a row, of 2048 x 1024: 200 rows 137 and 132, 225 rows 146 and 136;
-// of 4096 x 1792: 200 rows 329 and 399, 225 rows 374 and 401, 260 rows 444 and 397),
-// rows addressed with 32 bits from the buffer's start, and a grid that fits a
-// launch.
+// The tile kernels: from 24 slots an expert on average (rows and tiles in us, 64
+// experts, eight a row, of 2048 x 1024: 160 rows 118 and 116, 200 rows 137 and 116; of
+// 4096 x 1792: 200 rows 329 and 357, 225 rows 374 and 360), rows addressed with 32
+// bits from the buffer's start, and a grid that fits a launch.
 bool tiles_serve(const MoeArgs& a, const MoeWs& o) {
     const int64_t slots = (int64_t)a.T * a.k, nt = std::max<int64_t>(a.F / 64, (a.N + 127) / 128);
     return slots >= kMoeTileSlots * (int64_t)a.E && a_bytes(a) < (int64_t(1) << 32) && slots * a.F * 2 < (int64_t(1) << 32) &&
@@ -708,7 +712,7 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     if (fast && (slots > kScanSlots || tiles_serve(a, o))) {
         l = Lists{(const int32_t*)(ws + o.perm), (const int32_t*)(ws + o.offs)};
         hipLaunchKernelGGL(k_moe_plan, dim3((unsigned)a.E), dim3(64 * kPlanWaves), a.E * 4, st, a.ids, (int)slots, a.E,
-                           (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs), (int4*)(ws + o.table), (int*)(ws + o.tiles), (int)o.max_tiles, large_least(a));
+                           (int32_t*)(ws + o.perm), (int32_t*)(ws + o.offs), (int4*)(ws + o.table), (int*)(ws + o.tiles), (int)o.max_tiles, large_least(a), run_rows(a));
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -731,6 +735,7 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
         t.nt[0] = a.F / 128;
         t.nt[1] = a.F / 64;
         t.max_tiles = (int)o.max_tiles;
+        t.run = run_rows(a);
         e = moe_tile(a, t, true, st);
         if (e != hipSuccess) return e;
         t.W[0] = a.down;

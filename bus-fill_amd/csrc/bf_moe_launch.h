@@ -46,6 +46,7 @@ struct MoeTileArgs {
     const int4* table;         // max_tiles large tiles, then the small ones: expert, first place in perm, rows
     const int* tiles;          // how many of either
     int max_tiles;             // of both together
+    int run;                   // rows of a run: 64 (small tiles only) or kMoeTileRows
 };
 hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, hipStream_t st);
 

@@ -1,7 +1,8 @@
 // The experts' products for prompts: k_moe_tile, the tile of the prefill GEMM
 // (bf_tile.h) over rows gathered by expert.
 //
-// An expert's slots are cut into runs of 256.  Whole runs, and a rest of more
+// An expert's slots are cut into runs of 256 (of 64 where experts have few: the
+// caller's rule, k_moe_tile64).  Whole runs, and a rest of more
 // than 192, take a large tile, 256 rows x 256 weight rows (NB = 2 of bf_tile.h);
 // a shorter rest a small one, 64, 128 or 192 rows x 128 weight rows.  Activation
 // rows are fetched through the slot list, row by row, by the direct-to-LDS
@@ -152,10 +153,26 @@ void k_moe_tile(MoeArgs a, MoeTileArgs o) {
     else moe_tile<QT, 1, 1, GU>(lds, a, o, list, rows, e, ni);
 }
 
+// Runs of 64 rows only, with the registers and LDS of two workgroups a CU: their
+// weights are decoded once a run as well, which a CU alone with eight waves waits for.
 template <int QT, bool GU>
+__global__ __launch_bounds__(kTlThreads) __attribute__((amdgpu_waves_per_eu(4, 4)))
+void k_moe_tile64(MoeArgs a, MoeTileArgs o) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int units = o.tiles[1] * o.nt[1];
+    if ((int)blockIdx.x >= units) return;
+    const int v = xcd_unit((int)blockIdx.x, units), i = v / o.nt[1];
+    const int4 d = o.table[o.max_tiles + i];
+    moe_tile<QT, 1, 1, GU>(lds, a, o, o.perm + __builtin_amdgcn_readfirstlane(d.y), __builtin_amdgcn_readfirstlane(d.z),
+                           __builtin_amdgcn_readfirstlane(d.x), v - i * o.nt[1]);
+}
+
+template <int QT, bool GU, bool SMALL>
 hipError_t launch(const MoeArgs& a, const MoeTileArgs& o, hipStream_t st) {
-    auto k = k_moe_tile<QT, GU>;
-    constexpr int lds = std::max(Tile<QT, 4, 1>::NS * Tile<QT, 4, 1>::kStage, Tile<QT, 4, 2>::NS * Tile<QT, 4, 2>::kStage);
+    using T1 = Tile<QT, 1, 1>;
+    auto k = SMALL ? k_moe_tile64<QT, GU> : k_moe_tile<QT, GU>;
+    constexpr int lds = SMALL ? T1::NS * T1::kStage
+                              : std::max(Tile<QT, 4, 1>::NS * Tile<QT, 4, 1>::kStage, Tile<QT, 4, 2>::NS * Tile<QT, 4, 2>::kStage);
     static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -172,7 +189,8 @@ hipError_t launch(const MoeArgs& a, const MoeTileArgs& o, hipStream_t st) {
 
 template <int QT>
 hipError_t dispatch(const MoeArgs& a, const MoeTileArgs& o, bool gu, hipStream_t st) {
-    return gu ? launch<QT, true>(a, o, st) : launch<QT, false>(a, o, st);
+    if (o.run != kMoeTileRows) return gu ? launch<QT, true, true>(a, o, st) : launch<QT, false, true>(a, o, st);
+    return gu ? launch<QT, true, false>(a, o, st) : launch<QT, false, false>(a, o, st);
 }
 
 }  // namespace

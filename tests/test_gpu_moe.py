@@ -244,6 +244,16 @@ def test_experts_several_tiles_a_wave(qt):
     x.check(60, 2, ids=torch.tensor([[3, 39]]).repeat(60, 1), otype=bf.OUT_F16, pad=8)
 
 
+@pytest.mark.parametrize("qt", QTS)
+def test_experts_runs_of_64(qt):
+    """24 to 48 slots an expert on average: most with one run of 64, some with several, one with none."""
+    x = Experts(qt, 10, 512, 256, 144)
+    x.check(75, 4)
+    ids = torch.full((200, 2), 7)
+    ids[:, 1] = torch.arange(200) % 3
+    x.check(200, 2, ids=ids, otype=bf.OUT_F16, pad=8)
+
+
 @pytest.mark.parametrize("T", [5, 600])
 def test_experts_all_to_one(T):
     x = Experts(O.Q4_K, 6, 256, 256, 96)
