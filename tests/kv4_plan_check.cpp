@@ -80,8 +80,8 @@ void check_plans() {
                                         }
                                         if (window + span - 1 < seen) seen = window + span - 1;
                                     }
-                                    // a range of `seen` tokens may start at any token of a tile
-                                    const int64_t tiles = seen == 0 ? 0 : (seen + kKv4Tile - 1 + kKv4Tile - 1) / kKv4Tile;
+                                    // a window's range may start at any token of a tile, others start at token 0
+                                    const int64_t off = window ? kKv4Tile - 1 : 0, tiles = seen == 0 ? 0 : (off + seen + kKv4Tile - 1) / kKv4Tile;
                                     expect((int64_t)p.chunk * p.splits >= tiles, "chunks cover the tiles", tiles, p.chunk, p.splits);
                                     expect(p.splits == 1 || (p.chunk >= kKv4LeastFill && !p.prompt), "chunks of a size", p.chunk, p.splits, p.prompt);
                                     expect(p.slots == (p.splits > 1 ? p.items * heads * p.splits : 0), "slots", p.slots);

@@ -44,6 +44,7 @@ def test_prompts_take_the_prompt_kernel(checker, S, T, heads, group, max_q, max_
 def test_other_queries_do_not(checker):
     assert plan(checker, 1, 1000, 8, 5, 1000, 1000, 1, 0)[0] == 0
     assert plan(checker, 1, 512, 8, 5, 512, 8000, 1, 0)[0] == 0
-    assert plan(checker, 32, 32, 8, 5, 1, 8000, 1, 0) == (0, 251, 1, 8)          # whole sequences
-    assert plan(checker, 1, 1, 4, 8, 1, 131072, 1, 0) == (0, 65, 64, 8)          # as many chunks as CUs
+    assert plan(checker, 32, 32, 8, 5, 1, 8000, 1, 0) == (0, 250, 1, 8)          # whole sequences
+    assert plan(checker, 32, 32, 8, 4, 1, 8192, 1, 0) == (0, 256, 1, 8)
+    assert plan(checker, 1, 1, 4, 8, 1, 131072, 1, 0) == (0, 64, 64, 8)          # as many chunks as CUs
     assert plan(checker, 20, 20, 8, 5, 1, 8000, 1, 0)[2:] == (13, 4)             # chunks that even out
