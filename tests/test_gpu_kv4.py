@@ -345,6 +345,36 @@ def test_same_bits_again():
         assert torch.equal(a, s.check([1], 8))
 
 
+@pytest.mark.parametrize("nq", [1, 300])
+def test_cache_of_more_than_4_gb(nq):
+    """Pages on both sides of 2^32 bytes: single tokens and, with 300 queries, the kernel of many queries."""
+    s = Sequences([330, 300], 8, 256, page=256)
+    pages = 8000
+    big = Cache.__new__(Cache)
+    big.page, big.heads, big.dim, big.pages = 256, 8, 256, pages
+    big.data = torch.empty(bf.kv4_bytes(pages, 256, 8, 256), dtype=torch.uint8, device="cuda")
+    assert big.data.numel() > 1 << 32
+    big.c = bf.kv4_cache(big.data, pages, 256, 8, 256)
+    k = torch.empty(630, 8, 256, dtype=torch.float16, device="cuda")
+    v, table, at = torch.empty_like(k), torch.tensor([[pages - 1, 3], [0, pages - 2]], dtype=torch.int32), 0
+    for i, n in enumerate(s.lens):                             # the same values, at other places
+        t = torch.arange(n)
+        old, new = (p[i].long()[t // 256] * 256 + t % 256 for p in (s.table, table))
+        bf.kv4_load(s.cache.c, old.cuda(), k[at:], v[at:], n)
+        bf.kv4_store(big.c, k[at:], v[at:], new.cuda(), n)
+        k2, v2 = torch.empty_like(k[:n]), torch.empty_like(v[:n])
+        bf.kv4_load(big.c, new.cuda(), k2, v2, n)
+        s.k[i], s.v[i] = k2.cpu().double(), v2.cpu().double()
+        for got, kept in ((s.k[i], k[at:at + n]), (s.v[i], v[at:at + n])):
+            want = R.quantize(kept.cpu())
+            assert torch.equal(got, want.half().double())
+            got.copy_(want)
+        torch.cuda.synchronize()
+        at += n
+    s.cache, s.table, s.ldt = big, table, 2
+    s.check([nq, nq], 16)
+
+
 def test_captured_decode_step():
     """Store and attention in a graph, replayed as the sequences grow: the lengths live in device memory."""
     heads, dim, page, most = 2, 64, 64, 512

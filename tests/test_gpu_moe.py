@@ -301,6 +301,29 @@ def test_experts_rows_do_not_depend_on_each_other():
         assert torch.equal(all_[t:t + 2], x.run(a[t:t + 2], ids[t:t + 2], w[t:t + 2]))
 
 
+def test_experts_of_more_than_4_gb():
+    """The last expert's matrices begin behind 2^32 bytes; all but the first's and the last's weights are zero."""
+    E, K, F, N = 4096, 1024, 2048, 2048
+    x = Experts(O.Q4_K, 2, K, F, N)
+    small = [w for w, _ in x.dev]
+    dev = []
+    for w in small:
+        half = w.numel() // 2
+        b = torch.zeros(half * E, dtype=torch.uint8, device="cuda")
+        assert b.numel() > 1 << 32
+        b[:half], b[-half:] = w.reshape(-1)[:half], w.reshape(-1)[half:]
+        dev.append((b, None))
+    x.dev, x.E = dev, E
+    two, x.w64 = x.w64, None
+
+    class Far(list):
+        def __getitem__(self, e):
+            return super().__getitem__(0 if e == 0 else 1)
+
+    x.w64 = [Far([m[0], m[1]]) for m in two]
+    x.check(6, 2, ids=torch.tensor([[0, E - 1], [E - 1, 0], [E - 1, -1], [0, -1], [E - 1, E], [0, E - 1]]))
+
+
 def test_captured_block():
     x = Experts(O.Q4_K, 8, 256, 256, 64)
     st = torch.cuda.Stream()

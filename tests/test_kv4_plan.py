@@ -35,7 +35,8 @@ def plan(checker, *shape):
 @pytest.mark.parametrize("S,T,heads,group,max_q,max_kv,causal,window", [
     (8, 201, 40, 4, 50, 150, 1, 0), (4, 196, 40, 4, 70, 130, 0, 0), (4, 196, 64, 3, 70, 130, 1, 40),
     (4, 196, 32, 16, 70, 130, 1, 0), (4, 196, 48, 5, 70, 130, 1, 1), (4, 196, 32, 7, 70, 130, 1, 0),
-    (1, 600, 16, 8, 600, 600, 1, 0), (1, 120, 128, 4, 120, 120, 1, 0), (1, 2000, 8, 5, 2000, 2000, 1, 0)])
+    (1, 600, 16, 8, 600, 600, 1, 0), (2, 600, 8, 16, 300, 330, 1, 0), (1, 120, 128, 4, 120, 120, 1, 0),
+    (1, 2000, 8, 5, 2000, 2000, 1, 0)])
 def test_prompts_take_the_prompt_kernel(checker, S, T, heads, group, max_q, max_kv, causal, window):
     """The prompts of the GPU tests (and one of 2000 tokens, 40 heads over 8) take the kernel that they are there for."""
     assert plan(checker, S, T, heads, group, max_q, max_kv, causal, window)[0] == 1
