@@ -20,10 +20,11 @@
 //   two key operands) is the layout of the next product's A operand: no value
 //   moves between lanes.
 // * Values: P d_t in fp16 (one rounding; d differs from block to block, so
-//   each block of 32 columns has its operand), times q - 8.
+//   each block of 32 columns has its operand), times q - 8.  P is kept in the
+//   range that the largest scale so far leaves (Range in bf_kv4_dev.h).
 // * Running maximum and sum in fp32; the maximum is raised only when a score
-//   exceeds it by more than 2^3, so P <= 8 and P d_t <= 65504 always holds, and
-//   the accumulators are rarely rescaled.
+//   exceeds it by a factor of more than 2^3, so the accumulators are rarely
+//   rescaled.
 // * A workgroup's four waves take a chunk's records in turn; they meet in LDS.
 //   Sequences of several chunks are joined by a second launch.
 // * A wave's records come to LDS by direct loads, the next one while one is
@@ -126,13 +127,15 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
         q[b] = *(const h8*)(qp + 32 * b);
         if (a.scale < 0.f) q[b] = -q[b];               // so that a larger sum is a larger score
     }
-    const float sc = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.44269504088896341f, 1e-30f);   // (above 0: -inf stays -inf)
+    const float sc = log2_scale(a.scale);
+    const int seen0 = lo_of(a, o, ifirst), seen1 = hi_of(a, o, ilast);     // tokens that some row sees
     const Magic mg = make_magic();
 
     f4 olo[NB], ohi[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) olo[b] = ohi[b] = f4{0.f, 0.f, 0.f, 0.f};
-    float m = kLow, l = 0.f;
+    Range rg;
+    float l = 0.f;
 
     const int per_page = a.c.page_size / kKv4Tile;
     const int32_t* const tab = a.table + (int64_t)o.s * a.ldt;
@@ -168,7 +171,16 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
         }
         if ((here >> (n & 31)) & 1) {
             Kv4Rec<NB> x;
-            read_rec<NB>(x, ring + (n % ST) * kRecBytes<NB>, lane);
+            const uint8_t* const rec = ring + (n % ST) * kRecBytes<NB>;
+            // the values' scales, a word (block b, tokens 8 g + 2 j, + 1: word 4 NB g + 4 b + j) a lane
+            constexpr int SW = 16 * NB, SL = (SW + 63) / 64;
+            uint32_t vw[SL], d = 0;
+#pragma unroll
+            for (int i = 0; i < SL; i++) {
+                vw[i] = *(const uint32_t*)(rec + 1088 * NB + 4 * min(64 * i + lane, SW - 1));
+                d = max(d, larger_half(vw[i]));
+            }
+            read_rec<NB>(x, rec, lane);
             const int tb = (c0 + wave + WV * n) * kKv4Tile;
             const bool edge = tb < free0 || tb + kKv4Tile > free1;
             float s[8];
@@ -200,13 +212,16 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
             float tm = s[0];
 #pragma unroll
             for (int e = 1; e < 8; e++) tm = __builtin_fmaxf(tm, s[e]);
-            tm *= sc;
-            if (__any(tm > m + 3.f)) {
-                float mn = __builtin_fmaxf(m, tm);
-                mn = __builtin_fmaxf(mn, __shfl_xor(mn, 16));
-                mn = __builtin_fmaxf(mn, __shfl_xor(mn, 32));
-                const float al = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
+            if (__any(rg.over(tm, sc) || d > rg.top)) {
+                tm = __builtin_fmaxf(tm, __shfl_xor(tm, 16));
+                tm = __builtin_fmaxf(tm, __shfl_xor(tm, 32));
+                d = 0;
+#pragma unroll
+                for (int i = 0; i < SL; i++) {
+                    const int w = min(64 * i + lane, SW - 1);
+                    d = max(d, larger_seen(vw[i], tb + 8 * (w / (4 * NB)) + 2 * (w % 4), seen0, seen1));
+                }
+                const float al = rg.raise(tm, top_of(rg.top, d), sc);
                 l *= al;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -220,7 +235,7 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], sc, -m));
+                s[e] = rg.p(s[e], sc);
                 l += s[e];
             }
 #pragma unroll
@@ -245,7 +260,7 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
 
     // The waves' results meet, 128 columns at a time.
     if (g == 0) {
-        xm[wave][r] = m;
+        xm[wave][r] = rg.log2_unit(sc);
         xl[wave][r] = l;
     }
     __syncthreads();                               // every wave is done with its records

@@ -41,7 +41,7 @@ static_assert(kKv4PromptRows == 32 * kPrWaves);
 // (values, by column): the eight rows of a 16-byte read on distinct banks.
 template <int NB> struct PrLds {
     static constexpr int D = 32 * NB, KRow = 2 * D + 16, VRow = 80;
-    static constexpr int V = kKv4Tile * KRow, S = V + D * VRow, Bytes = S + 128 * NB;
+    static constexpr int V = kKv4Tile * KRow, S = V + D * VRow, Top = S + 128 * NB, Bytes = Top + 16;
 };
 
 // A thread's share of a record on its way to LDS.
@@ -64,8 +64,11 @@ __device__ __forceinline__ void load(PrRaw<NB>& x, const uint8_t* rec, int tid) 
 
 // Values of column d, tokens 8 g + 4 h + c, at place 16 (g / 2) + 8 h + 4 (g % 2) + c
 // of the column; scales of block b at 32 b + 16 h + 4 g + c (keys', then values').
+// top: the range of the values' scales so far (Range), of tokens tb ... in
+// [lo, hi); each wave that holds scales leaves its own beside the record.
 template <int NB>
-__device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint8_t* lds, int tid) {
+__device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint8_t* lds, int tid, uint32_t& top, int tb, int lo,
+                                       int hi) {
     using L = PrLds<NB>;
 #pragma unroll
     for (int i = 0; i < PrRaw<NB>::KW; i++) {
@@ -102,6 +105,8 @@ __device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint
         uint8_t* to = lds + L::S + 2 * (32 * b + 16 * (e >> 1) + 4 * g + 2 * (e & 1));
         *(uint32_t*)to = x.ks | bad;
         *(uint32_t*)(to + 64 * NB) = x.vs & ~bad;
+        if (__any(larger_half(x.vs & ~bad) > top)) top = top_of(top, larger_seen(x.vs, tb + 8 * g + 2 * e, lo, hi));
+        if ((tid & 63) == 0) *(uint32_t*)(lds + L::Top + (tid >> 4)) = top;
     }
 }
 
@@ -133,14 +138,15 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
         q[c] = *(const h8*)(qp + 16 * c);
         if (a.scale < 0.f) q[c] = -q[c];               // so that a larger sum is a larger score
     }
-    const float sc = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.44269504088896341f, 1e-30f);   // (above 0: -inf stays -inf)
+    const float sc = log2_scale(a.scale);
     const Magic mg = make_magic();
     f16x acc[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[b][e] = 0.f;
-    float m = kLow, l = 0.f;
+    Range rg;
+    float l = 0.f;
 
     const int per_page = a.c.page_size / kKv4Tile;
     const int32_t* const tab = a.table + (int64_t)o.s * a.ldt;
@@ -161,6 +167,8 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
         // stood right before its use, 27 waits a record).
         constexpr int HB = NB < 4 ? NB : 4;
         float x[16];
+        uint32_t top = *(const uint32_t*)(buf + L::Top);
+        if constexpr (NB > 4) top = max(top, *(const uint32_t*)(buf + L::Top + 4));
 #pragma unroll
         for (int b0 = 0; b0 < NB; b0 += HB) {
             h8 kf[HB][2], ks[HB][2];
@@ -207,12 +215,9 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
         float tm = x[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) tm = __builtin_fmaxf(tm, x[e]);
-        tm *= sc;
-        if (__any(tm > m + 3.f)) {
-            float mn = __builtin_fmaxf(m, tm);
-            mn = __builtin_fmaxf(mn, __shfl_xor(mn, 32));
-            const float al = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+        if (__any(rg.over(tm, sc) || top > rg.top)) {
+            tm = __builtin_fmaxf(tm, __shfl_xor(tm, 32));
+            const float al = rg.raise(tm, max(rg.top, (uint32_t)__builtin_amdgcn_readfirstlane((int)top)), sc);
             l *= al;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], sc, -m));
+            x[e] = rg.p(x[e], sc);
             part[e & 3] += x[e];
         }
         l += (part[0] + part[1]) + (part[2] + part[3]);
@@ -251,15 +256,17 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
         return rec;
     };
     const int walk = o.t1 - o.t0;
+    const int seen0 = lo_of(a, o, o.row0 / p.group), seen1 = hi_of(a, o, (o.row0 + o.rows - 1) / p.group);   // by some row
+    uint32_t seen_top = rg.top;
     int rec = -1, next = -1;
     if (walk > 0) {
         rec = fetch(0);
-        decode<NB>(mg, raw, lds, tid);
+        decode<NB>(mg, raw, lds, tid, seen_top, o.t0 * kKv4Tile, seen0, rec >= 0 ? seen1 : 0);
         next = fetch(1);
         __syncthreads();
     }
     for (int n = 0; n < walk; n++) {
-        if (n + 1 < walk) decode<NB>(mg, raw, lds + ((n + 1) & 1) * L::Bytes, tid);
+        if (n + 1 < walk) decode<NB>(mg, raw, lds + ((n + 1) & 1) * L::Bytes, tid, seen_top, (o.t0 + n + 1) * kKv4Tile, seen0, next >= 0 ? seen1 : 0);
         const int after = n + 2 < walk ? fetch(n + 2) : -1;
         const int tb = (o.t0 + n) * kKv4Tile;
         if (rec >= 0 && tb < whi && tb + kKv4Tile > wlo) tile_of(lds + (n & 1) * L::Bytes, tb);
@@ -281,7 +288,7 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
     }
     if (a.lse && h2 == 0 && 32 * wave + col < o.rows)
         a.lse[(int64_t)(o.q0 + iq) * a.q_heads + head] =
-            l == 0.f ? -__builtin_inff() : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+            l == 0.f ? -__builtin_inff() : (rg.log2_unit(sc) + __builtin_log2f(l)) * 0.693147180559945309f;
 }
 
 template <int NB>
