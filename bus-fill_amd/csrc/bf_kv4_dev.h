@@ -117,7 +117,7 @@ __device__ __forceinline__ int hi_of(const Kv4Args& a, const Row& o, int i) {
     return a.causal ? max(0, o.len - o.nq + i + 1) : o.len;
 }
 __device__ __forceinline__ int lo_of(const Kv4Args& a, const Row& o, int i) {
-    return a.window > 0 ? max(0, o.len - o.nq + i - a.window + 1) : 0;
+    return a.window > 0 ? max(0, max(0, o.len - o.nq + i + 1) - a.window) : 0;   // (positions down to -2^30, windows up to 2^31 - 1)
 }
 
 // Item i = s row_tiles + rt; false where it has no rows.
