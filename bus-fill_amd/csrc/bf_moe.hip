@@ -5,10 +5,7 @@
 // over 4-bit weights in place.  A slot is one (t, j).  Three launches: h of
 // every slot (gate and up of the same 16 rows in one workgroup, SiLU(g) u w
 // rounded once to fp16), y = Wd h of every slot, and the fp32 sum of a row's slots
-// in their order.  The row's weight goes into h before its rounding.  y is fp32,
-// but for fp16 outputs of many rows, where each y is rounded as the output will
-// be, which halves the bytes between the last two launches (262 MB of fp32 at
-// 2000 rows of eight slots and 4096 outputs).
+// in their order.  The row's weight goes into h before its rounding.
 //
 // Bound by the weights of the experts in use, each read once.  Up to 24
 // slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
@@ -23,7 +20,7 @@
 #include "bf_formats.h"
 #include "bf_grid.h"
 #include "bf_lds.h"
-#include "bf_moe_launch.h"
+#include "bf_moe_dev.h"
 
 namespace bf {
 namespace {
@@ -31,7 +28,6 @@ namespace {
 constexpr int kMoeWaves = 8;
 constexpr int kMoeStages = 2;                      // super-groups of a wave's weights in LDS
 constexpr int kSumY = 32768;                       // rows of the sum along grid y
-constexpr int kMoeTileSlots = 24;                  // slots an expert, on average, from which tiles take the products
 constexpr int kScanSlots = 1024;                   // up to so many slots a workgroup finds its expert's by itself
 
 // Slots of one expert: in LDS (found by the workgroup), or in the plan's list.
@@ -88,16 +84,6 @@ __device__ __forceinline__ void multiply(const Magic& mg, const Raw<QT>& raw, co
             for (int t = 0; t < MT; t++) acc[t] = mfma16x16x32(a[t][i], w, acc[t]);
         }
     }
-}
-
-// y in fp16: for fp16 outputs of many rows.
-__host__ __device__ __forceinline__ bool y_f16(const MoeArgs& a) {
-    return a.out_f16 && (int64_t)a.T * a.k >= kMoeTileSlots * (int64_t)a.E;
-}
-
-__device__ __forceinline__ void store_y(const MoeArgs& a, void* y, int64_t at, float v) {
-    if (y_f16(a)) ((_Float16*)y)[at] = (_Float16)v;
-    else ((float*)y)[at] = v;
 }
 
 // What a launch of k_moe_rows computes: h (gate and up), y (down, by slot; or with
@@ -519,31 +505,25 @@ __global__ __launch_bounds__(64 * kPlanWaves) void k_moe_plan(const int32_t* __r
 
 // c[t] = the sum of its slots' y, in slot order; slots without an expert add
 // nothing.  Four outputs a thread, a row's slots read together.
-template <typename Y>
-__global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const Y* __restrict__ y) {
-    typedef Y y4 __attribute__((ext_vector_type(4)));
+template <bool Y24>
+__global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const void* __restrict__ y) {
     const int64_t t = (int64_t)blockIdx.z * kSumY + blockIdx.y;
     const int n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x);
     if (t >= a.T || n >= a.N) return;
     const int32_t* ids = a.ids + t * a.k;
-    const Y* row = y + t * a.k * a.N + n;
+    const int64_t row = t * a.k * a.N + n;
     const bool whole = a.N % 4 == 0;
     f4 v = f4{0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < a.k; j0 += 8) {
-        y4 x[8];
+        f4 x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            x[j] = y4{0, 0, 0, 0};
+            x[j] = f4{0.f, 0.f, 0.f, 0.f};
             if (j0 + j >= a.k || ids[j0 + j] < 0 || ids[j0 + j] >= a.E) continue;
-            const Y* p = row + (int64_t)(j0 + j) * a.N;
-            if (whole) x[j] = *(const y4*)p;
-            else
-                for (int i = 0; i < 4 && n + i < a.N; i++) x[j][i] = p[i];
+            x[j] = load_y4<Y24>(a, y, row + (int64_t)(j0 + j) * a.N, whole, a.N - n);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] += (float)x[j][i];
+        for (int j = 0; j < 8; j++) v += x[j];
     }
     const int64_t at = t * a.ldc + n;
     if (a.out_f16 && whole && a.ldc % 4 == 0 && ((uintptr_t)a.C & 7) == 0) {
@@ -565,14 +545,14 @@ size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 // 230 rows 116 and 136, 400 rows 127 and 148, 600 rows 191 and 195).
 int run_rows(const MoeArgs& a) { return (int64_t)a.T * a.k < 48 * (int64_t)a.E ? 64 : kMoeTileRows; }
 
-// Workspace: h [slots][F] fp16, y [slots][N] fp32 or fp16, the plan.
+// Workspace: h [slots][F] fp16, y [slots][N] in 32 or 24 bits, the plan.
 struct MoeWs {
     size_t y, perm, offs, table, tiles, end;
     int64_t max_tiles;
     explicit MoeWs(const MoeArgs& a) {
         const size_t slots = (size_t)a.T * a.k;
         y = up256(slots * a.F * 2);
-        perm = y + up256(slots * a.N * (y_f16(a) ? 2 : 4));
+        perm = y + (y_24(a) ? (size_t)y_24_high(a) + up256(slots * a.N) : up256(slots * a.N * 4));
         offs = perm + up256(slots * 4);
         table = offs + up256(((size_t)a.E + 1) * 4);
         max_tiles = (int64_t)std::min<size_t>(a.E, slots) + (int64_t)(slots / run_rows(a));
@@ -762,8 +742,8 @@ hipError_t run(const MoeArgs& a, uint8_t* ws, hipStream_t st) {
     }
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)((a.N + 1023) / 1024), (unsigned)std::min(a.T, kSumY), (unsigned)((a.T + kSumY - 1) / kSumY));
-    if (y_f16(a)) hipLaunchKernelGGL(k_moe_sum<_Float16>, grid, dim3(256), 0, st, a, (const _Float16*)(ws + o.y));
-    else hipLaunchKernelGGL(k_moe_sum<float>, grid, dim3(256), 0, st, a, (const float*)(ws + o.y));
+    if (y_24(a)) hipLaunchKernelGGL(k_moe_sum<true>, grid, dim3(256), 0, st, a, ws + o.y);
+    else hipLaunchKernelGGL(k_moe_sum<false>, grid, dim3(256), 0, st, a, ws + o.y);
     return hipGetLastError();
 }
 

@@ -32,6 +32,7 @@ struct MoeArgs {
     int ldc, out_f16;
     int T, K, F, N, E, k;
 };
+
 // One of the two products over tiles of gathered rows (bf_moe_tile.hip).
 constexpr int kMoeTileRows = 256;
 struct MoeTileArgs {
@@ -39,7 +40,7 @@ struct MoeTileArgs {
     const uint16_t* A;         // rows of tokens, or of slots
     uint32_t a_bytes;          // from A on: below 4 GB
     int64_t lda;
-    void* out;                 // h fp16, or y (fp16 for fp16 outputs), by slot
+    void* out;                 // h (fp16) or y (bf_moe_dev.h), by slot
     int R, K;                  // weight rows of an expert, their length
     int nt[2];                 // column tiles of a large and of a small tile's rows
     const int32_t* perm;       // slots by expert
@@ -48,6 +49,15 @@ struct MoeTileArgs {
     int max_tiles;             // of both together
     int run;                   // rows of a run: 64 (small tiles only) or kMoeTileRows
 };
+
+// y in 24 bits, else in 32 (bf_moe_dev.h).
+constexpr int kMoeTileSlots = 24;                  // slots an expert, on average, from which tiles take the products
+__host__ __device__ inline bool y_24(const MoeArgs& a) {
+    return a.out_f16 && (int64_t)a.T * a.k >= kMoeTileSlots * (int64_t)a.E;
+}
+// Bytes of the plane of its upper 16 bits.
+__host__ __device__ inline int64_t y_24_high(const MoeArgs& a) { return ((int64_t)a.T * a.k * a.N * 2 + 255) & ~(int64_t)255; }
+
 hipError_t moe_tile(const MoeArgs& a, const MoeTileArgs& o, bool gu, hipStream_t st);
 
 // The matrix-core kernels serve these widths and alignments.

@@ -534,7 +534,8 @@ bf_status bf_moe_route(const bf_moe_route_args* args, void* stream);
  * expert e - 1's (W_aux likewise).  An id that is negative or not below E adds
  * nothing (an expert that another GPU holds).  The intermediate is rounded to
  * fp16 once, its weight already in it; the sums over experts run in fp32 in
- * the order of j (a single row's as one long sum).  Equal calls give equal
+ * the order of j (a single row's as one long sum), over terms held in fp32, or,
+ * for fp16 outputs and T k >= 24 E, in an fp32's upper 24 bits (2^-16 of each).  Equal calls give equal
  * bits; how many rows there are, and with many of them how many an expert has,
  * selects the kernels, and with them the order of the sums over K and F.
  * Requirements as for bf_gemm; the matrix-core path takes K and F multiples of
