@@ -3,9 +3,9 @@
 //   c[t] = sum_j w[t][j] Wd_e . (SiLU(Wg_e . a_t) * (Wu_e . a_t)),   e = ids[t][j]
 //
 // over 4-bit weights in place.  A slot is one (t, j).  Three launches: h of
-// every slot (gate and up of the same 16 rows in one workgroup, SiLU(g) u w
-// rounded once to fp16), y = Wd h of every slot, and the fp32 sum of a row's slots
-// in their order.  The row's weight goes into h before its rounding.
+// every slot (gate and up of the same 16 rows in one workgroup, SiLU(g) u times
+// the weight's first part rounded once to fp16), y = Wd h of every slot, and the
+// fp32 sum of a row's slots in their order, times the second part (bf_moe_dev.h).
 //
 // Bound by the weights of the experts in use, each read once.  Up to 24
 // slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
@@ -140,14 +140,16 @@ __device__ __forceinline__ void wait_loads(int n) {
 // meet in LDS at the end.  GU: h of the slots; else y.
 template <int QT, int MT, int MODE, int KS>
 __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const uint16_t* A, int64_t lda, void* out, int R,
-                                        int K, int64_t e, int tile0, const int32_t* list, int cnt, int cap, uint8_t* lds) {
+                                        int K, int64_t e, int tile0, const int32_t* list, const float* rest, int cnt, int cap,
+                                        uint8_t* lds) {
     constexpr bool GU = MODE == kMoeH, ONE = MODE == kMoeRow;
     constexpr int NM = GU ? 2 : 1, TW = kMoeWaves / (KS * NM), CH = KS < 2 ? 2 : KS, PER = CH / KS, ST = kMoeStages;
     constexpr int RS = 20, TS = 16 * RS;           // stride of the sums' rows: the four row groups of a wave on distinct banks
     const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kp = wave % KS, mat = wave / KS % NM, tile = tile0 + wave / (KS * NM);
-    // ONE: the row's slots one after the other, `list` their experts (K and the activations run through them all)
+    // ONE: the row's slots one after the other, `list` their experts, `rest` what multiplies their products (K and
+    // the activations run through them all)
     const int per = K >> 8, nsg = ONE ? a.k * per : per, slabs = (nsg + CH - 1) / CH, width = ONE ? a.k * K : K;
     float* const red = (float*)lds;                // [wave][MT][16][RS], over everything else at the end
     uint8_t* const ring = lds + wave * (ST * kTileBytes);
@@ -222,7 +224,15 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[m][i] = *(const h8*)(row + 16 * i);
             }
-            if (!ONE || list[s / per] >= 0) multiply<QT, MT>(mg, raw, x, kg, acc);   // (a slot without an expert: h is not there)
+            if constexpr (ONE) {
+                if (list[s / per] >= 0) {              // (a slot without an expert: h is not there)
+                    f4 y[MT] = {f4{0.f, 0.f, 0.f, 0.f}};
+                    multiply<QT, MT>(mg, raw, x, kg, y);
+                    acc[0] += rest[s / per] * y[0];
+                }
+            } else {
+                multiply<QT, MT>(mg, raw, x, kg, acc);
+            }
             at = at + 1 < ST ? at + 1 : 0;
         }
         // the next slab's loads are older than the ring's last one
@@ -256,7 +266,7 @@ __device__ __forceinline__ void rows_of(const MoeArgs& a, const MoeW& w, const u
         const int slot = list[i];
         if constexpr (GU) {
             const float ex = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
-            ((_Float16*)out)[(int64_t)slot * R + f] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[NM - 1] * a.w[slot]);
+            ((_Float16*)out)[(int64_t)slot * R + f] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[NM - 1] * weight_in_h(a.w[slot]));
         } else {
             store_y(a, out, (int64_t)slot * R + f, v[0]);
         }
@@ -334,9 +344,13 @@ void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, in
     __shared__ int wave_cnt[kMoeWaves];
     const int slots = a.T * a.k;
     if constexpr (MODE == kMoeRow) {
-        for (int j = threadIdx.x; j < a.k; j += 64 * kMoeWaves) found[j] = a.ids[j] < a.E ? a.ids[j] : -1;
+        __shared__ float rest[kScanSlots];
+        for (int j = threadIdx.x; j < a.k; j += 64 * kMoeWaves) {
+            found[j] = a.ids[j] < a.E ? a.ids[j] : -1;
+            rest[j] = weight_of_y(a.w[j]);
+        }
         __syncthreads();
-        rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, 0, TW * (int)blockIdx.x, found, 1, 1, lds);
+        rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, 0, TW * (int)blockIdx.x, found, rest, 1, 1, lds);
         return;
     }
     const int e = by_slot ? a.ids[blockIdx.y] : (int)blockIdx.y;
@@ -373,8 +387,8 @@ void k_moe_rows(MoeArgs a, MoeW w, const uint16_t* A, int64_t lda, void* out, in
             rows_whole<QT>(a, w, A, lda, out, R, K, e, TW * many * (int)blockIdx.x, many, list + c, n, lds);
             continue;
         }
-        if (MT > 1 && n > 16) rows_of<QT, MT, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
-        else rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, n, cap, lds);
+        if (MT > 1 && n > 16) rows_of<QT, MT, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, nullptr, n, cap, lds);
+        else rows_of<QT, 1, MODE, KS>(a, w, A, lda, out, R, K, e, tile0, list + c, nullptr, n, cap, lds);
     }
 }
 
@@ -410,7 +424,7 @@ __global__ __launch_bounds__(256) void k_moe_simple(MoeArgs a, MoeW w, const uin
         }
         if constexpr (GU) {
             const float ex = __builtin_amdgcn_exp2f(v[0] * -1.44269504088896341f);
-            ((_Float16*)out)[i] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[1] * a.w[slot]);
+            ((_Float16*)out)[i] = (_Float16)(v[0] * __builtin_amdgcn_rcpf(1.0f + ex) * v[1] * weight_in_h(a.w[slot]));
         } else {
             store_y(a, out, i, v[0]);
         }
@@ -516,14 +530,17 @@ __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const void* __restri
     f4 v = f4{0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < a.k; j0 += 8) {
         f4 x[8];
+        float wt[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             x[j] = f4{0.f, 0.f, 0.f, 0.f};
+            wt[j] = 0.f;
             if (j0 + j >= a.k || ids[j0 + j] < 0 || ids[j0 + j] >= a.E) continue;
+            wt[j] = weight_of_y(a.w[t * a.k + j0 + j]);
             x[j] = load_y4<Y24>(a, y, row + (int64_t)(j0 + j) * a.N, whole, a.N - n);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) v += x[j];
+        for (int j = 0; j < 8; j++) v += wt[j] * x[j];
     }
     const int64_t at = t * a.ldc + n;
     if (a.out_f16 && whole && a.ldc % 4 == 0 && ((uintptr_t)a.C & 7) == 0) {

@@ -1,7 +1,13 @@
-// Device-side parts shared by the experts' kernels: y, the down product of every
-// slot, between the launch that makes it and the one that sums a row's slots.
+// Device-side parts shared by the experts' kernels: the routing weight's two parts,
+// and y, the down product of every slot, between the launch that makes it and the
+// one that sums a row's slots.
 //
-// fp32; for fp16 outputs from kMoeTileSlots slots an expert on, where its bytes count
+// The weight: its power of two, from 1/8 to 1, goes into h before h is rounded to
+// fp16, the rest multiplies y in the fp32 sum.  All of it in h makes h subnormal
+// where weights are small (1e-4 over h of 0.05: up to 6e-3 of it lost); none of it makes h
+// infinite from 65504 on, where eight weights of 1/8 reach 5e5.
+//
+// y is fp32; for fp16 outputs from kMoeTileSlots slots an expert on, where its bytes count
 // (2000 rows of eight slots and 4096 outputs: 262 MB), the upper 24 bits of the fp32, to
 // nearest: fp32's range, so terms that cancel may be of any size, and 2^-16 of a
 // term's own size, 32 times finer than the output's rounding.  Two planes: the
@@ -14,6 +20,12 @@
 
 namespace bf {
 namespace {
+
+__device__ __forceinline__ uint32_t weight_exponent(float w) {   // 124 (1/8) to 127 (1)
+    return min(max((__builtin_bit_cast(uint32_t, w) >> 23) & 0xFFu, 124u), 127u);
+}
+__device__ __forceinline__ float weight_in_h(float w) { return __builtin_bit_cast(float, weight_exponent(w) << 23); }
+__device__ __forceinline__ float weight_of_y(float w) { return w * __builtin_bit_cast(float, (254u - weight_exponent(w)) << 23); }   // (exact)
 
 // The bits of v, its upper 24 to nearest (ties away from 0; to even, and NaNs apart,
 // took 5 us more of the down products' 316).  Infinities stay, and so do NaNs: they

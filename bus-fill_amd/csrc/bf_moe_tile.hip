@@ -10,7 +10,7 @@
 //
 // Gate and up: a tile's weight rows are 32 gate rows, the same 32 up rows, and
 // the next 32 of both, which puts g and u of one output into the two column
-// tiles of one wave: h = w SiLU(g) u leaves the registers as the one fp16 row
+// tiles of one wave: h = SiLU(g) u leaves the registers as the one fp16 row
 // that the down product reads.  (Small tiles: two k groups of waves hold half of
 // each sum; each hands the other half of the rows over and finishes the rest.)
 //
@@ -34,7 +34,7 @@ __device__ __forceinline__ void put(const MoeArgs& a, const MoeTileArgs& o, int 
     if constexpr (GU) {
         const float ex = __builtin_amdgcn_exp2f(y0 * -1.44269504088896341f);
         ((_Float16*)o.out)[(int64_t)slot * o.R + c64 / 2 + (lane & 31)] =
-            (_Float16)(y0 * __builtin_amdgcn_rcpf(1.0f + ex) * y1 * a.w[slot]);
+            (_Float16)(y0 * __builtin_amdgcn_rcpf(1.0f + ex) * y1 * weight_in_h(a.w[slot]));
     } else {
 #pragma unroll
         for (int b = 0; b < 2; b++) {

@@ -533,7 +533,8 @@ bf_status bf_moe_route(const bf_moe_route_args* args, void* stream);
  * gate and up [E][F][K], down [E][N][F] in one format: expert e's rows follow
  * expert e - 1's (W_aux likewise).  An id that is negative or not below E adds
  * nothing (an expert that another GPU holds).  The intermediate is rounded to
- * fp16 once, its weight already in it; the sums over experts run in fp32 in
+ * fp16 once, with its weight's power of two (1/8 to 1) in it; the rest of the
+ * weight multiplies in the sums over experts, which run in fp32 in
  * the order of j (a single row's as one long sum), over terms held in fp32, or,
  * for fp16 outputs and T k >= 24 E, in an fp32's upper 24 bits (2^-16 of each).  Equal calls give equal
  * bits; how many rows there are, and with many of them how many an expert has,

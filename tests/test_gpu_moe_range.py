@@ -67,3 +67,59 @@ def test_experts_outputs_beyond_fp16_that_cancel(qt, T):
         assert torch.isfinite(got).all()
         t = tol + (2.0 ** -11 * want.abs() + 2.0 ** -25 if otype == bf.OUT_F16 else 0.0)
         assert ((got - want).abs() <= t).all(), float(((got - want).abs() / t).max())
+
+
+def weighted(x, a, ids, w):
+    """terms(), with the intermediate rounded before the part of the weight outside 1/8 .. 1 is multiplied: 2^-11 of it,
+    or 2^-25 times the larger of that part and 1."""
+    want, _, top_h, top_y = terms(x, a, ids, w)
+    tol, (rw, acc) = torch.zeros_like(want), ((0.0 if x.qt == O.Q4_K else 2.0 ** -11), 2.0 ** -18)
+    for j in range(ids.shape[1]):
+        for t in range(ids.shape[0]):
+            wg, wu, wd = (m[int(ids[t, j])] for m in x.w64)
+            r, ww = a[t].double(), abs(float(w[t, j]))
+            gt, ut = wg @ r, wu @ r
+            dg, du = ((rw + acc) * (m.abs() @ r.abs()) for m in (wg, wu))
+            silu = gt * torch.sigmoid(gt)
+            h = (ww * silu * ut).abs()
+            rest = 8 * ww if ww < 0.125 else max(2.0, ww)
+            dh = ww * (1.1 * dg * (ut.abs() + du) + silu.abs() * du) + (2.0 ** -11 + 2.0 ** -20) * h + 2.0 ** -25 * rest
+            tol[t] += wd.abs() @ dh * (1 + rw + acc) + wd.abs() @ h * (rw + acc)
+    return want, tol, top_h, top_y
+
+
+@pytest.mark.parametrize("qt", QTS)
+@pytest.mark.parametrize("T,E,F", [(1, 8, 256), (1, 8, 1024), (6, 8, 256), (40, 3, 256), (70, 3, 512)])
+@pytest.mark.parametrize("size", [1e-6, 3e-4, 0.02])
+def test_small_weights_keep_the_intermediates_accuracy(qt, T, E, F, size):
+    """Weights that nothing has normalised, intermediates about 0.05."""
+    x = Experts(qt, E, 256, F, 136, seed=4)
+    g = torch.Generator().manual_seed(T + F)
+    a = torch.randn(T, 256, generator=g)
+    ids = torch.rand(T, E, generator=g).argsort(1)[:, :2]
+    w = size * (0.5 + torch.rand(T, 2, generator=g))
+    _, _, h, _ = terms(x, a.half(), ids, torch.ones_like(w))
+    a = (a * (0.2 / h) ** 0.5).half()
+    want, tol, _, _ = weighted(x, a, ids, w)
+    got = x.run(a, ids, w).cpu().double()
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("qt", QTS)
+@pytest.mark.parametrize("T,E", [(1, 8), (6, 8), (40, 3), (70, 3)])
+def test_weights_bring_large_intermediates_into_range(qt, T, E):
+    """Intermediates up to 3e5, beyond fp16, whose weights are about 1/8; weights above 1 and below 0 beside them."""
+    x = Experts(qt, E, 256, 256, 136, seed=6)
+    g = torch.Generator().manual_seed(T)
+    a = torch.randn(T, 256, generator=g)
+    ids = torch.rand(T, E, generator=g).argsort(1)[:, :2]
+    w = 0.126 + 0.02 * torch.rand(T, 2, generator=g)
+    _, _, h, _ = terms(x, a.half(), ids, torch.ones_like(w))
+    big = (a * (3e5 / h) ** 0.5).half()
+    want, tol, _, _ = weighted(x, big, ids, w)
+    got = x.run(big, ids, w).cpu().double()
+    assert torch.isfinite(got).all() and ((got - want).abs() <= tol).all()
+    w = torch.stack([2.5 + torch.rand(T, generator=g), -torch.rand(T, generator=g)], 1)
+    a = a.half()
+    want, tol, _, _ = weighted(x, a, ids, w)
+    assert ((x.run(a, ids, w).cpu().double() - want).abs() <= tol).all()
