@@ -512,7 +512,10 @@ typedef enum { BF_LOGITS_F32 = 0, BF_LOGITS_F16 = 1 } bf_ltype;
  * that many runs of E / groups; a run's score is the sum of its two largest
  * s + bias (of the one, in runs of one), and only the top_groups best runs'
  * experts (equal ones: the lowest) are chosen from.  A NaN is the least of all
- * when experts are chosen.  Without bias, experts are ordered by their logits. */
+ * when experts are chosen, -inf the least but for it (in a run's score both are
+ * -inf).  Without bias, experts are ordered by their logits.  A NaN logit's s is
+ * NaN, and the other experts' softmax is taken without it; logits of +inf share
+ * the softmax; a row of nothing above -inf has s = 0. */
 typedef struct {
     const void* logits;      /* [T][ldl] */
     bf_ltype ltype;
