@@ -678,6 +678,8 @@ bf_status check_cache(const bf_kv4_cache* c) {
     return BF_OK;
 }
 
+bf::Kv4Shape shape_of(const bf_kv4_cache* c) { return bf::Kv4Shape{c->pages, c->page_size, c->kv_heads, c->head_dim}; }
+
 bf_status check_kv_rows(const bf_kv4_cache* c, const void* K, int64_t ldk, const void* V, int64_t ldv,
                         const int64_t* slots, int T) {
     bf_status st = check_cache(c);
@@ -692,10 +694,9 @@ bf_status check_kv_rows(const bf_kv4_cache* c, const void* K, int64_t ldk, const
         return fail(BF_ERR_INVALID, "K and V rows must be 16-byte aligned (ldk, ldv %% 8 == 0)");
     if (!aligned(slots, 8)) return fail(BF_ERR_INVALID, "slots is not 8-byte aligned");
     if (c->kv_heads > 65535) return fail(BF_ERR_UNSUPPORTED, "kv_heads=%d: at most 65535", c->kv_heads);
+    if (!bf::kv4_rows_fit(shape_of(c), T)) return fail(BF_ERR_UNSUPPORTED, "T=%d: more workgroups than a launch takes", T);
     return BF_OK;
 }
-
-bf::Kv4Shape shape_of(const bf_kv4_cache* c) { return bf::Kv4Shape{c->pages, c->page_size, c->kv_heads, c->head_dim}; }
 
 bf_status check_attention(const bf_kv4_cache* c, const bf_kv4_attention_args* a, bf::Kv4Args& o) {
     bf_status st = check_cache(c);
@@ -768,6 +769,7 @@ bf_status check_route(const bf_moe_route_args* a, bf::RouteArgs& o) {
         return fail(BF_ERR_INVALID, "logits, bias, ids and weights must be aligned to their elements");
     if (a->E > 1024 || a->k > 64 || a->groups > 64)
         return fail(BF_ERR_UNSUPPORTED, "E=%d (at most 1024), k=%d (at most 64), groups=%d (at most 64)", a->E, a->k, a->groups);
+    if (!bf::moe_route_fits(a->T)) return fail(BF_ERR_UNSUPPORTED, "T=%d: more workgroups than a launch takes", a->T);
     o.logits = a->logits;
     o.f16 = a->ltype == BF_LOGITS_F16;
     o.ldl = a->ldl;

@@ -16,6 +16,7 @@
 // a launch and its first loads.  A block per thread, so that its scale needs no
 // other lane; the price is values' codes stored byte by byte, 32 tokens apart.
 #include "bf_device.h"
+#include "bf_grid.h"
 #include "bf_kv4_launch.h"
 
 namespace bf {
@@ -151,11 +152,12 @@ __global__ __launch_bounds__(256) void k_kv4_load(const uint8_t* __restrict__ da
     for (int w = 0; w < 4; w++) *(u4*)(dst + 8 * w) = out[w];
 }
 
-dim3 units_grid(const Kv4Shape& c, int T) {
-    return dim3((unsigned)(((int64_t)T * (c.dim / 32) + 255) / 256), (unsigned)c.heads, 2);
-}
+int64_t units_groups(const Kv4Shape& c, int T) { return ((int64_t)T * (c.dim / 32) + 255) / 256; }
+dim3 units_grid(const Kv4Shape& c, int T) { return dim3((unsigned)units_groups(c, T), (unsigned)c.heads, 2); }
 
 }  // namespace
+
+bool kv4_rows_fit(const Kv4Shape& c, int T) { return launch_fits(units_groups(c, T), 256); }
 
 hipError_t kv4_store(uint8_t* data, const Kv4Shape& c, const uint16_t* K, int64_t ldk, const uint16_t* V, int64_t ldv,
                      const int64_t* slots, int T, hipStream_t st) {

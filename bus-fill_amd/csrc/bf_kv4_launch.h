@@ -9,6 +9,8 @@
 
 namespace bf {
 
+// The grid of T tokens' store or load fits a launch.
+bool kv4_rows_fit(const Kv4Shape& c, int T);
 hipError_t kv4_store(uint8_t* data, const Kv4Shape& c, const uint16_t* K, int64_t ldk, const uint16_t* V, int64_t ldv,
                      const int64_t* slots, int T, hipStream_t st);
 hipError_t kv4_load(const uint8_t* data, const Kv4Shape& c, const int64_t* slots, uint16_t* K, int64_t ldk, uint16_t* V,

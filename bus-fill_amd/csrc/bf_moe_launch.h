@@ -19,6 +19,7 @@ struct RouteArgs {
     int sigmoid, groups, top_groups, renorm;
     float factor;
 };
+bool moe_route_fits(int T);    // its grid fits a launch
 hipError_t moe_route(const RouteArgs& a, hipStream_t st);
 
 struct MoeArgs {

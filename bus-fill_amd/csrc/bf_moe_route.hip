@@ -174,13 +174,16 @@ __global__ __launch_bounds__(64 * kRtWaves) void k_moe_route(RouteArgs a) {
     }
 }
 
+int64_t groups_of(int T) { return ((int64_t)T + kRtWaves - 1) / kRtWaves; }
 }  // namespace
+
+bool moe_route_fits(int T) { return launch_fits(groups_of(T), 64 * kRtWaves); }
 
 hipError_t moe_route(const RouteArgs& a, hipStream_t st) {
     const int epl = (a.E + 63) / 64;
     auto k = epl <= 1 ? k_moe_route<1> : epl <= 2 ? k_moe_route<2> : epl <= 4 ? k_moe_route<4>
              : epl <= 8 ? k_moe_route<8> : k_moe_route<16>;
-    hipLaunchKernelGGL(k, dim3((unsigned)(((int64_t)a.T + kRtWaves - 1) / kRtWaves)), dim3(64 * kRtWaves), 0, st, a);
+    hipLaunchKernelGGL(k, dim3((unsigned)groups_of(a.T)), dim3(64 * kRtWaves), 0, st, a);
     return hipGetLastError();
 }
 
