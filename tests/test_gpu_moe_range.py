@@ -123,3 +123,11 @@ def test_weights_bring_large_intermediates_into_range(qt, T, E):
     a = a.half()
     want, tol, _, _ = weighted(x, a, ids, w)
     assert ((x.run(a, ids, w).cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("qt", [O.Q4_0, O.Q4_0_PLANES])
+@pytest.mark.parametrize("K,F,N", [(96, 288, 33), (224, 32, 40), (32, 96, 1)])
+@pytest.mark.parametrize("T", [20, 70])
+def test_widths_off_256_with_many_rows(qt, K, F, N, T):
+    """fp16 outputs of the kernel of one thread an output, on both sides of 24 slots an expert."""
+    Experts(qt, 5, K, F, N).check(T, 3, otype=bf.OUT_F16)
