@@ -532,15 +532,15 @@ __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs a, const void* __restri
         f4 x[8];
         float wt[8];
 #pragma unroll
+        for (int j = 0; j < 8; j++) wt[j] = a.w[t * a.k + min(j0 + j, a.k - 1)];
+#pragma unroll
         for (int j = 0; j < 8; j++) {
             x[j] = f4{0.f, 0.f, 0.f, 0.f};
-            wt[j] = 0.f;
-            if (j0 + j >= a.k || ids[j0 + j] < 0 || ids[j0 + j] >= a.E) continue;
-            wt[j] = weight_of_y(a.w[t * a.k + j0 + j]);
-            x[j] = load_y4<Y24>(a, y, row + (int64_t)(j0 + j) * a.N, whole, a.N - n);
+            if (j0 + j >= a.k || ids[j0 + j] < 0 || ids[j0 + j] >= a.E) wt[j] = 0.f;
+            else x[j] = load_y4<Y24>(a, y, row + (int64_t)(j0 + j) * a.N, whole, a.N - n);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) v += wt[j] * x[j];
+        for (int j = 0; j < 8; j++) v += weight_of_y(wt[j]) * x[j];
     }
     const int64_t at = t * a.ldc + n;
     if (a.out_f16 && whole && a.ldc % 4 == 0 && ((uintptr_t)a.C & 7) == 0) {
