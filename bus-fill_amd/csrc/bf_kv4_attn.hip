@@ -31,11 +31,11 @@
 //   multiplied (from registers instead, 80 us where this took 54).
 //
 // Measured, one query a sequence, heads of 128: 32 sequences of 2000 to 8000 tokens,
-// 40 heads over 8, 50 us for 184 MB (3.7 TB/s; the longest sequence's workgroup
+// 40 heads over 8, 51 us for 184 MB (3.6 TB/s; the longest sequence's workgroup
 // lasts until the end); one of 131072 tokens, 32 over 4, 23 us for 75 MB with the
-// join's 4.5; one of 519 tokens 8 us, which are the chain of lengths, page ids, first
-// record, three records a wave and the waves' meeting.  VALU 56 % busy, matrix units
-// 10 %.
+// join's 4.5; one of 519 tokens 8.4 us, which are the chain of lengths, page ids, first
+// record, three records a wave and the waves' meeting.  VALU 51 % busy, matrix units
+// 9 %.
 #include <atomic>
 
 #include "bf_grid.h"

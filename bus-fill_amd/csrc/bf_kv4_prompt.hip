@@ -13,12 +13,13 @@
 //   of the 32 tokens of its query; as the A operand of P V it needs eight tokens
 //   per instruction in the same lane, so the values' columns are stored with
 //   their tokens in that order and nothing moves between lanes.
-// * P d in fp16 for each block of 32 columns (one rounding), times q - 8.
-//   Scores and probabilities are as exact as the single-token kernel's.  (Keys
+// * P d in fp16 for each block of 32 columns (one rounding; P in the range that
+//   the scales leave, Range in bf_kv4_dev.h: the waves that decode a record leave the
+//   largest scale so far beside it), times q - 8.  Scores and probabilities are as exact as the single-token kernel's.  (Keys
 //   and values as exact fp16 pairs in LDS instead, hi and lo of (q - 8) d, need
-//   no scales here and twice the matrix products: 114 us where this takes 95.)
-// * 2000 causal tokens, 40 heads over 8 of 128: 93 us, 440 TFLOP/s of the visible
-//   pairs; vector instructions issue in 65 % of the SIMDs' cycles, matrix products
+//   no scales here and twice the matrix products: 114 us where this took 95.)
+// * 2000 causal tokens, 40 heads over 8 of 128: 94 us, 436 TFLOP/s of the visible
+//   pairs; vector instructions issue in 67 % of the SIMDs' cycles, matrix products
 //   in 21 %.  A record takes 1.2 us of a CU that holds two workgroups or more, 1.4
 //   where one is alone; decoding is 19 us of the 93 (timed without it).
 //

@@ -11,7 +11,7 @@
 // slots an expert k_moe_rows takes the products (Q4_K, eight experts a row: one
 // row of 2048 x 1024 14.2 us for 28 MB; 32 rows, 64 experts of 5120 x 1280, 161 us
 // for 697 MB, 4.3 TB/s), above that k_moe_tile (2000 rows, 64 experts of 4096 x
-// 1792, Q4_0: 916 to 955 us for 705 GFLOP).
+// 1792, Q4_0: 942 to 966 us for 705 GFLOP).
 #include <algorithm>
 #include <atomic>
 #include <climits>

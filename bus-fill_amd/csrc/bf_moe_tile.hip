@@ -15,7 +15,7 @@
 // each sum; each hands the other half of the rows over and finishes the rest.)
 //
 // 2000 rows of eight, 64 experts of 4096 x 1792 (Q4_0): gate and up 575 us, 820
-// TFLOP/s, down 317, 740; the prefill GEMM with whole tiles only reaches 950.  A third
+// TFLOP/s, down 312, 750; the prefill GEMM with whole tiles only reaches 950.  A third
 // of the experts have a few rows more than 256, whose small tiles decode as many
 // weights as a full one, and the last round of large tiles is half empty.  Matrix
 // units 42 to 47 % busy, vector instructions 27 %.

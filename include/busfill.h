@@ -537,11 +537,14 @@ bf_status bf_moe_route(const bf_moe_route_args* args, void* stream);
  * expert e - 1's (W_aux likewise).  An id that is negative or not below E adds
  * nothing (an expert that another GPU holds).  The intermediate is rounded to
  * fp16 once, with its weight's power of two (1/8 to 1) in it; the rest of the
- * weight multiplies in the sums over experts, which run in fp32 in
- * the order of j (a single row's as one long sum), over terms held in fp32, or,
- * for fp16 outputs and T k >= 24 E, in an fp32's upper 24 bits (2^-16 of each).  Equal calls give equal
- * bits; how many rows there are, and with many of them how many an expert has,
- * selects the kernels, and with them the order of the sums over K and F.
+ * weight multiplies in the sums over experts, which run in fp32 in the order of j
+ * (a single row's as one long sum), over terms held in fp32, or, for fp16 outputs
+ * and T k >= 24 E, in an fp32's upper 24 bits (2^-16 of each).  On the
+ * matrix-core path the Q4_0 formats' weights enter as RN_fp16((q - 8) d), as in
+ * bf_gemm, and Q4_K's are rounded to fp16 from T k >= 24 E on; weights are not
+ * rounded otherwise.  Equal calls give equal bits; how many rows there are, and
+ * with many of them how many an expert has, selects the kernels, and with them
+ * the order of the sums over K and F.
  * Requirements as for bf_gemm; the matrix-core path takes K and F multiples of
  * 256, 16-byte aligned A and W and lda % 8 == 0 (4-byte aligned W_aux); Q4_K
  * needs it, other legal Q4_0 inputs run one thread per output. */
