@@ -16,7 +16,7 @@ def form(E, R, gu, T, k):
     assert slots < 24 * E
     experts = min(E, slots)
     waves = (R + 15) // 16 * (2 if gu else 1) * experts
-    ks = 4 if waves < 1536 else 2 if waves < 3072 else 1
+    ks = 4 if waves < 1536 else 2 if waves < 2 * 1536 else 1
     mt = 1 if slots <= 16 * E else 2
     return (2 if mt == 2 and ks == 4 else ks), mt, slots <= 1024
 
