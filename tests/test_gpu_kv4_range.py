@@ -93,7 +93,6 @@ FORMS = {"whole": (1, 1100, 2, 5, 1), "eight waves": (24, 1500, 8, 1, 1), "chunk
          "queries": (2, 1280, 1, 4, 9), "prompt": (1, 1500, 8, 8, 1500)}
 
 
-
 def sink(form, dim, down, size, equal):
     """Keys, values, queries: token 0 has no value and `down` powers of two more weight than the others; their values
     are about `size`, of one sign (so that rounding errors cannot cancel), all equal or random."""
