@@ -32,6 +32,10 @@ FFN_AUTO, FFN_ONE_LAUNCH, FFN_TWO_LAUNCHES, FFN_CALLS = 0, 1, 2, 3
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 # bf_ltype
 LOGITS_F32, LOGITS_F16 = 0, 1
+# bf_rope
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+# bf_dtype
+F32, F16 = 0, 1
 # bf_algo
 ALGO_AUTO, ALGO_MFMA, ALGO_DOT2, ALGO_SIMPLE, ALGO_LDS, ALGO_SLAB, ALGO_SPLIT, ALGO_DENSE = 0, 1, 2, 3, 4, 5, 6, 7
 
@@ -43,7 +47,9 @@ EXPORTS = ("bf_busfill_q4", "bf_busfill_q4_ws", "bf_gemm", "bf_gemm_ex", "bf_gem
            "bf_gguf_get_u64", "bf_gguf_get_str", "bf_gguf_upload",
            "bf_ggml_mul_mat", "bf_ggml_mul_mat_workspace_bytes", "bf_ggml_mul_mat_ws",
            "bf_kv4_bytes", "bf_kv4_store", "bf_kv4_load", "bf_kv4_attention", "bf_kv4_attention_workspace_bytes",
-           "bf_kv4_attention_ws", "bf_moe_route", "bf_moe_ffn", "bf_moe_ffn_workspace_bytes", "bf_moe_ffn_ws",
+           "bf_kv4_attention_ws", "bf_kv4_attention_sinks", "bf_kv4_attention_sinks_workspace_bytes",
+           "bf_kv4_attention_sinks_ws", "bf_kv4_append", "bf_rms_norm", "bf_lora", "bf_lora_workspace_bytes", "bf_lora_ws",
+           "bf_moe_route", "bf_moe_ffn", "bf_moe_ffn_workspace_bytes", "bf_moe_ffn_ws",
            "bf_status_str", "bf_last_error", "bf_version")
 
 
@@ -72,6 +78,37 @@ class Kv4AttentionArgs(ctypes.Structure):
                 ("kv_len", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("ldt", ctypes.c_int),
                 ("S", ctypes.c_int), ("T", ctypes.c_int), ("q_heads", ctypes.c_int), ("max_q", ctypes.c_int),
                 ("max_kv", ctypes.c_int), ("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_int)]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    """bf_kv4_append_args."""
+    _fields_ = [("Q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("Q_out", ctypes.c_void_p), ("ldqo", ctypes.c_int64),
+                ("K", ctypes.c_void_p), ("ldk", ctypes.c_int64), ("K_out", ctypes.c_void_p), ("ldko", ctypes.c_int64),
+                ("V", ctypes.c_void_p), ("ldv", ctypes.c_int64), ("slots", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("freq", ctypes.c_void_p), ("q_heads", ctypes.c_int), ("rot", ctypes.c_int), ("style", ctypes.c_int),
+                ("factor", ctypes.c_float), ("T", ctypes.c_int)]
+
+
+class RmsNormArgs(ctypes.Structure):
+    """bf_rms_norm_args."""
+    _fields_ = [("X", ctypes.c_void_p), ("xtype", ctypes.c_int), ("ldx", ctypes.c_int64), ("delta", ctypes.c_void_p),
+                ("dtype", ctypes.c_int), ("ldd", ctypes.c_int64), ("R", ctypes.c_void_p), ("ldr", ctypes.c_int64),
+                ("weight", ctypes.c_void_p), ("wtype", ctypes.c_int), ("offset", ctypes.c_float), ("eps", ctypes.c_float),
+                ("H", ctypes.c_void_p), ("ldh", ctypes.c_int64), ("Aq", ctypes.c_void_p), ("T", ctypes.c_int),
+                ("K", ctypes.c_int)]
+
+
+class LoraPart(ctypes.Structure):
+    """bf_lora_part: the A and B of all adapters for one slice of a projection's columns."""
+    _fields_ = [("A", ctypes.c_void_p), ("B", ctypes.c_void_p), ("N", ctypes.c_int), ("at", ctypes.c_int)]
+
+
+class LoraArgs(ctypes.Structure):
+    """bf_lora_args."""
+    _fields_ = [("X", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("ids", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("ranks", ctypes.c_void_p), ("adapters", ctypes.c_int), ("rank", ctypes.c_int), ("parts", ctypes.c_int),
+                ("part", ctypes.POINTER(LoraPart)), ("C", ctypes.c_void_p), ("ldc", ctypes.c_int64), ("Y", ctypes.c_void_p),
+                ("ldy", ctypes.c_int64), ("otype", ctypes.c_int), ("T", ctypes.c_int), ("K", ctypes.c_int)]
 
 
 class MoeRouteArgs(ctypes.Structure):
@@ -210,14 +247,25 @@ def lib() -> ctypes.CDLL:
         L.bf_kv4_attention.argtypes = [cp, ap, vp]
         L.bf_kv4_attention_workspace_bytes.argtypes = [cp, ap]
         L.bf_kv4_attention_ws.argtypes = [cp, ap, vp, sz, vp]
+        L.bf_kv4_attention_sinks.argtypes = [cp, ap, i, vp]
+        L.bf_kv4_attention_sinks_workspace_bytes.argtypes = [cp, ap, i]
+        L.bf_kv4_attention_sinks_ws.argtypes = [cp, ap, i, vp, sz, vp]
+        lp = ctypes.POINTER(LoraArgs)
+        L.bf_kv4_append.argtypes = [cp, ctypes.POINTER(Kv4AppendArgs), vp]
+        L.bf_rms_norm.argtypes = [ctypes.POINTER(RmsNormArgs), vp]
+        L.bf_lora.argtypes = [lp, vp]
+        L.bf_lora_workspace_bytes.argtypes = [lp]
+        L.bf_lora_ws.argtypes = [lp, vp, sz, vp]
         L.bf_moe_route.argtypes = [rp, vp]
         L.bf_moe_ffn.argtypes = [mp, vp]
         L.bf_moe_ffn_workspace_bytes.argtypes = [mp]
         L.bf_moe_ffn_ws.argtypes = [mp, vp, sz, vp]
         for f in ("bf_kv4_store", "bf_kv4_load", "bf_kv4_attention", "bf_kv4_attention_ws", "bf_moe_route", "bf_moe_ffn",
-                  "bf_moe_ffn_ws"):
+                  "bf_moe_ffn_ws", "bf_kv4_attention_sinks", "bf_kv4_attention_sinks_ws", "bf_kv4_append", "bf_rms_norm",
+                  "bf_lora", "bf_lora_ws"):
             getattr(L, f).restype = i
-        for f in ("bf_kv4_bytes", "bf_kv4_attention_workspace_bytes", "bf_moe_ffn_workspace_bytes"):
+        for f in ("bf_kv4_bytes", "bf_kv4_attention_workspace_bytes", "bf_moe_ffn_workspace_bytes",
+                  "bf_kv4_attention_sinks_workspace_bytes", "bf_lora_workspace_bytes"):
             getattr(L, f).restype = sz
         L.bf_status_str.argtypes = [i]
         L.bf_status_str.restype = ctypes.c_char_p
@@ -530,6 +578,89 @@ def kv4_attention_ws(cache: Kv4Cache, args: Kv4AttentionArgs, workspace, workspa
     """kv4_attention with a caller-owned workspace (as gemm_ws)."""
     _check(lib().bf_kv4_attention_ws(ctypes.byref(cache), ctypes.byref(args), _ptr(workspace), workspace_bytes,
                                      _stream(stream)), "bf_kv4_attention_ws")
+
+
+def kv4_attention_sinks(cache: Kv4Cache, Q, O, q_start, kv_len, page_table, *, sinks: int, stream=None, **args) -> None:
+    """kv4_attention whose window leaves the first `sinks` tokens in sight."""
+    a = kv4_attention_args(cache, Q, O, q_start, kv_len, page_table, **args)
+    _check(lib().bf_kv4_attention_sinks(ctypes.byref(cache), ctypes.byref(a), sinks, _stream(stream)), "bf_kv4_attention_sinks")
+
+
+def kv4_attention_sinks_workspace_bytes(cache: Kv4Cache, args: Kv4AttentionArgs, sinks: int) -> int:
+    """Bytes of caller-owned workspace kv4_attention_sinks_ws needs (0: none)."""
+    return int(lib().bf_kv4_attention_sinks_workspace_bytes(ctypes.byref(cache), ctypes.byref(args), sinks))
+
+
+def kv4_attention_sinks_ws(cache: Kv4Cache, args: Kv4AttentionArgs, sinks: int, workspace, workspace_bytes: int,
+                           stream=None) -> None:
+    """kv4_attention_sinks with a caller-owned workspace (as gemm_ws)."""
+    _check(lib().bf_kv4_attention_sinks_ws(ctypes.byref(cache), ctypes.byref(args), sinks, _ptr(workspace), workspace_bytes,
+                                           _stream(stream)), "bf_kv4_attention_sinks_ws")
+
+
+def kv4_append(cache: Kv4Cache, K, V, slots, positions, freq, T: int, *, Q=None, Q_out=None, q_heads: int = 0, K_out=None,
+               rot: int | None = None, style: int = ROPE_HALVES, factor: float = 1.0, ldq: int | None = None,
+               ldqo: int | None = None, ldk: int | None = None, ldko: int | None = None, ldv: int | None = None,
+               stream=None) -> None:
+    """T tokens' queries and keys (fp16 rows) rotated by their positions (int64; freq: fp32 [rot / 2], radians a position;
+    rot: the whole head by default), queries to Q_out, keys and values into the cache's slots as by kv4_store, rotated keys
+    to K_out too where given."""
+    kv, q = cache.kv_heads * cache.head_dim, q_heads * cache.head_dim
+    a = Kv4AppendArgs(_ptr(Q), q if ldq is None else ldq, _ptr(Q_out), q if ldqo is None else ldqo, _ptr(K),
+                      kv if ldk is None else ldk, _ptr(K_out), kv if ldko is None else ldko, _ptr(V), kv if ldv is None else ldv,
+                      _ptr(slots), _ptr(positions), _ptr(freq), q_heads, cache.head_dim if rot is None else rot, style, factor, T)
+    _check(lib().bf_kv4_append(ctypes.byref(cache), ctypes.byref(a), _stream(stream)), "bf_kv4_append")
+
+
+def _dtype(t) -> int:
+    import torch
+    return F32 if t is None else {torch.float32: F32, torch.float16: F16}[t.dtype]
+
+
+def rms_norm(X, T: int, K: int, *, H=None, Aq=None, delta=None, R=None, weight=None, offset: float = 0.0, eps: float = 1e-6,
+             ldx: int | None = None, ldd: int | None = None, ldr: int | None = None, ldh: int | None = None,
+             xtype: int | None = None, dtype: int | None = None, wtype: int | None = None, stream=None) -> None:
+    """r = X + delta; H (fp16 rows) and, or, Aq (q8_bytes(T, K) bytes, gemm_q8's activations) = r / sqrt(mean(r^2) + eps)
+    (weight + offset); R = r where given.  X, delta and weight are fp32 or fp16 (xtype, dtype, wtype: by default from the
+    tensors' dtypes)."""
+    a = RmsNormArgs(_ptr(X), _dtype(X) if xtype is None else xtype, K if ldx is None else ldx, _ptr(delta),
+                    _dtype(delta) if dtype is None else dtype, K if ldd is None else ldd, _ptr(R), K if ldr is None else ldr,
+                    _ptr(weight), _dtype(weight) if wtype is None else wtype, offset, eps, _ptr(H), K if ldh is None else ldh,
+                    _ptr(Aq), T, K)
+    _check(lib().bf_rms_norm(ctypes.byref(a), _stream(stream)), "bf_rms_norm")
+
+
+def lora_parts(parts):
+    """Parts of a lora call from (A, B, N, at): A fp16 [adapters][rank][K], B fp16 [adapters][N][rank] (device tensors or
+    addresses, which the caller keeps), columns at .. at + N - 1."""
+    out = (LoraPart * max(1, len(parts)))()
+    for o, (A, B, N, at) in zip(out, parts):
+        o.A, o.B, o.N, o.at = _ptr(A), _ptr(B), N, at
+    return out
+
+
+def lora_args(X, ids, parts, C, Y, *, T: int, K: int, adapters: int, rank: int, scales=None, ranks=None,
+              ldx: int | None = None, ldc: int | None = None, ldy: int | None = None, otype: int = OUT_F32) -> LoraArgs:
+    """A bf_lora_args; parts from lora_parts.  ldc and ldy default to the parts' last column."""
+    width = max(p.at + p.N for p in parts)
+    return LoraArgs(_ptr(X), K if ldx is None else ldx, _ptr(ids), _ptr(scales), _ptr(ranks), adapters, rank, len(parts), parts,
+                    _ptr(C), width if ldc is None else ldc, _ptr(Y), width if ldy is None else ldy, otype, T, K)
+
+
+def lora(X, ids, parts, C, Y, *, stream=None, **args) -> None:
+    """Y = C + each row's low-rank adapter ids[t] (int32; negative: none) of X; further arguments as lora_args."""
+    a = lora_args(X, ids, parts, C, Y, **args)
+    _check(lib().bf_lora(ctypes.byref(a), _stream(stream)), "bf_lora")
+
+
+def lora_workspace_bytes(args: LoraArgs) -> int:
+    """Bytes of caller-owned workspace lora_ws needs."""
+    return int(lib().bf_lora_workspace_bytes(ctypes.byref(args)))
+
+
+def lora_ws(args: LoraArgs, workspace, workspace_bytes: int, stream=None) -> None:
+    """lora with a caller-owned workspace (as gemm_ws)."""
+    _check(lib().bf_lora_ws(ctypes.byref(args), _ptr(workspace), workspace_bytes, _stream(stream)), "bf_lora_ws")
 
 
 def moe_route(logits, ids, weights, T: int, E: int, k: int, *, bias=None, score: int = SCORE_SOFTMAX, groups: int = 1,

@@ -17,6 +17,7 @@
 #include "bf_device.h"
 #include "bf_kv4_launch.h"
 #include "bf_launch.h"
+#include "bf_lora_launch.h"
 #include "bf_moe_launch.h"
 
 namespace {
@@ -698,7 +699,7 @@ bf_status check_kv_rows(const bf_kv4_cache* c, const void* K, int64_t ldk, const
     return BF_OK;
 }
 
-bf_status check_attention(const bf_kv4_cache* c, const bf_kv4_attention_args* a, bf::Kv4Args& o) {
+bf_status check_attention(const bf_kv4_cache* c, const bf_kv4_attention_args* a, int sinks, bf::Kv4Args& o) {
     bf_status st = check_cache(c);
     if (st != BF_OK) return st;
     if (!a) return fail(BF_ERR_INVALID, "args is NULL");
@@ -746,9 +747,132 @@ bf_status check_attention(const bf_kv4_cache* c, const bf_kv4_attention_args* a,
     o.scale = a->scale;
     o.causal = a->causal != 0;
     o.window = a->window;
+    if (sinks < 0) return fail(BF_ERR_INVALID, "sinks=%d must be >= 0", sinks);
+    o.sinks = a->window > 0 ? sinks : 0;
     if (!bf::kv4_attention_fits(o))
         return fail(BF_ERR_UNSUPPORTED, "attention over S=%d kv_heads=%d max_q=%d: more workgroups than a launch takes", a->S,
                     c->kv_heads, a->max_q);
+    return BF_OK;
+}
+
+// A row pointer of fp16 rows in 16-byte pieces, `width` wide.
+bf_status check_f16_rows(const char* name, const void* p, int64_t ld, int64_t width) {
+    if (ld < width) return fail(BF_ERR_INVALID, "ld=%lld of %s < %lld", (long long)ld, name, (long long)width);
+    if (!aligned(p, 16) || ld % 8) return fail(BF_ERR_INVALID, "%s rows must be 16-byte aligned (ld=%lld %% 8 == 0)", name, (long long)ld);
+    return BF_OK;
+}
+
+bf_status check_append(const bf_kv4_cache* c, const bf_kv4_append_args* a, bf::Kv4AppendArgs& o) {
+    bf_status st = check_cache(c);
+    if (st != BF_OK) return st;
+    if (!a) return fail(BF_ERR_INVALID, "args is NULL");
+    st = check_kv_rows(c, a->K, a->ldk, a->V, a->ldv, a->slots, a->T);
+    if (st != BF_OK) return st;
+    if (!a->positions || !a->freq) return fail(BF_ERR_INVALID, "positions or freq is NULL");
+    if (!aligned(a->positions, 8)) return fail(BF_ERR_INVALID, "positions is not 8-byte aligned");
+    if (!aligned(a->freq, 4)) return fail(BF_ERR_INVALID, "freq is not 4-byte aligned");
+    if (a->rot < 16 || a->rot > c->head_dim || a->rot % 16)
+        return fail(BF_ERR_INVALID, "rot=%d must be a multiple of 16 from 16 to head_dim=%d", a->rot, c->head_dim);
+    if (a->style != BF_ROPE_HALVES && a->style != BF_ROPE_PAIRS) return fail(BF_ERR_INVALID, "unknown style %d", (int)a->style);
+    if (!a->Q != !a->Q_out || !a->Q != (a->q_heads == 0) || a->q_heads < 0)
+        return fail(BF_ERR_INVALID, "q_heads=%d: Q and Q_out go with q_heads >= 1, and are NULL with 0", a->q_heads);
+    const int64_t width = (int64_t)c->kv_heads * c->head_dim, qwidth = (int64_t)a->q_heads * c->head_dim;
+    if (a->Q) {
+        st = check_f16_rows("Q", a->Q, a->ldq, qwidth);
+        if (st == BF_OK) st = check_f16_rows("Q_out", a->Q_out, a->ldqo, qwidth);
+    }
+    if (st == BF_OK && a->K_out) st = check_f16_rows("K_out", a->K_out, a->ldko, width);
+    if (st != BF_OK) return st;
+    if (a->Q_out == a->Q && a->Q && a->ldqo != a->ldq) return fail(BF_ERR_INVALID, "Q_out is Q: ldqo must be ldq");
+    if (a->K_out == a->K && a->ldko != a->ldk) return fail(BF_ERR_INVALID, "K_out is K: ldko must be ldk");
+    if (a->q_heads > (1 << 20)) return fail(BF_ERR_UNSUPPORTED, "q_heads=%d: at most 2^20", a->q_heads);
+    if (!bf::kv4_append_fits(a->T)) return fail(BF_ERR_UNSUPPORTED, "T=%d: more workgroups than a launch takes", a->T);
+    o = bf::Kv4AppendArgs{(uint8_t*)c->data, shape_of(c), a->Q, a->ldq, a->Q_out, a->ldqo, a->K, a->ldk, a->K_out, a->ldko,
+                          a->V, a->ldv, a->slots, a->positions, a->freq, a->q_heads, a->rot, a->style == BF_ROPE_PAIRS, a->T,
+                          a->factor};
+    return BF_OK;
+}
+
+bool known(bf_dtype t) { return t == BF_F32 || t == BF_F16; }
+
+bf_status check_norm(const bf_rms_norm_args* a, bf::NormArgs& o) {
+    if (!a) return fail(BF_ERR_INVALID, "args is NULL");
+    if (!a->X) return fail(BF_ERR_INVALID, "X is NULL");
+    if (!a->H && !a->Aq) return fail(BF_ERR_INVALID, "H and Aq are both NULL");
+    if (a->T < 1 || a->K < 1) return fail(BF_ERR_INVALID, "T=%d K=%d must be >= 1", a->T, a->K);
+    if (!known(a->xtype)) return fail(BF_ERR_INVALID, "unknown xtype %d", (int)a->xtype);
+    if (a->delta && !known(a->dtype)) return fail(BF_ERR_INVALID, "unknown dtype %d", (int)a->dtype);
+    if (a->weight && !known(a->wtype)) return fail(BF_ERR_INVALID, "unknown wtype %d", (int)a->wtype);
+    if (a->ldx < a->K || (a->delta && a->ldd < a->K) || (a->R && a->ldr < a->K) || (a->H && a->ldh < a->K))
+        return fail(BF_ERR_INVALID, "ldx=%lld, ldd=%lld, ldr=%lld or ldh=%lld < K=%d", (long long)a->ldx, (long long)a->ldd,
+                    (long long)a->ldr, (long long)a->ldh, a->K);
+    const int xs = a->xtype == BF_F16 ? 2 : 4;
+    if (!aligned(a->X, xs) || !aligned(a->R, xs) || !aligned(a->H, 2) || (a->delta && !aligned(a->delta, a->dtype == BF_F16 ? 2 : 4)) ||
+        (a->weight && !aligned(a->weight, a->wtype == BF_F16 ? 2 : 4)))
+        return fail(BF_ERR_INVALID, "X, delta, R, weight or H is not aligned to its element");
+    if (a->R == a->X && a->ldr != a->ldx) return fail(BF_ERR_INVALID, "R is X: ldr must be ldx");
+    if (a->H && (const void*)a->H == a->delta && (a->dtype != BF_F16 || a->ldh != a->ldd))
+        return fail(BF_ERR_INVALID, "H is delta: delta must be fp16 and ldh be ldd");
+    if (a->Aq && a->K % 32) return fail(BF_ERR_INVALID, "K=%d is not a multiple of 32 (Aq)", a->K);
+    if (!aligned(a->Aq, 16)) return fail(BF_ERR_INVALID, "Aq is not 16-byte aligned");
+    if (!(a->eps >= 0.f && a->eps < 3e38f)) return fail(BF_ERR_INVALID, "eps must be finite and >= 0");
+    if (!bf::rms_norm_fits(a->T, a->K))
+        return fail(BF_ERR_UNSUPPORTED, "T=%d K=%d: K is at most 32768, T 2^22 - 1", a->T, a->K);
+    o = bf::NormArgs{a->X, a->ldx, a->xtype == BF_F16, a->delta, a->ldd, a->dtype == BF_F16, a->R, a->ldr, a->weight,
+                     a->wtype == BF_F16, a->offset, a->eps, a->H, a->ldh, a->Aq, a->T, a->K};
+    return BF_OK;
+}
+
+bf_status check_lora(const bf_lora_args* a, bf::LoraArgs& o) {
+    if (!a) return fail(BF_ERR_INVALID, "args is NULL");
+    if (!a->X || !a->ids || !a->part || !a->C || !a->Y) return fail(BF_ERR_INVALID, "X, ids, part, C or Y is NULL");
+    if (a->T < 1 || a->adapters < 1) return fail(BF_ERR_INVALID, "T=%d adapters=%d must be >= 1", a->T, a->adapters);
+    if (a->K < 8 || a->K % 8) return fail(BF_ERR_INVALID, "K=%d is not a multiple of 8", a->K);
+    if (a->rank < 8 || a->rank % 8) return fail(BF_ERR_INVALID, "rank=%d is not a multiple of 8", a->rank);
+    if (a->parts < 1 || a->parts > bf::kLoraParts) return fail(BF_ERR_INVALID, "parts=%d: 1 to %d", a->parts, bf::kLoraParts);
+    if (a->otype != BF_OUT_F32 && a->otype != BF_OUT_F16) return fail(BF_ERR_INVALID, "unknown otype %d", (int)a->otype);
+    const bf_status st = check_f16_rows("X", a->X, a->ldx, a->K);
+    if (st != BF_OK) return st;
+    const int f16 = a->otype == BF_OUT_F16, es = f16 ? 2 : 4, piece = 16 / es;
+    if (!aligned(a->C, es) || !aligned(a->Y, es)) return fail(BF_ERR_INVALID, "C or Y is not aligned to its element");
+    if (!aligned(a->ids, 4) || !aligned(a->scales, 4) || !aligned(a->ranks, 4))
+        return fail(BF_ERR_INVALID, "ids, scales and ranks must be 4-byte aligned");
+    if (a->C == a->Y && a->ldc != a->ldy) return fail(BF_ERR_INVALID, "Y is C: ldy must be ldc");
+    o.wide = aligned(a->C, 16) && aligned(a->Y, 16) && a->ldc % piece == 0 && a->ldy % piece == 0;
+    for (int i = 0; i < a->parts; i++) {
+        const bf_lora_part& p = a->part[i];
+        if (!p.A || !p.B) return fail(BF_ERR_INVALID, "part %d: A or B is NULL", i);
+        if (!aligned(p.A, 16) || !aligned(p.B, 16)) return fail(BF_ERR_INVALID, "part %d: A or B is not 16-byte aligned", i);
+        if (p.N < 1 || p.at < 0) return fail(BF_ERR_INVALID, "part %d: N=%d must be >= 1, at=%d >= 0", i, p.N, p.at);
+        if ((int64_t)p.at + p.N > a->ldc || (int64_t)p.at + p.N > a->ldy)
+            return fail(BF_ERR_INVALID, "part %d: columns %d to %lld, ldc=%lld, ldy=%lld", i, p.at, (long long)p.at + p.N - 1,
+                        (long long)a->ldc, (long long)a->ldy);
+        for (int j = 0; j < i; j++)
+            if (p.at < (int64_t)a->part[j].at + a->part[j].N && a->part[j].at < (int64_t)p.at + p.N)
+                return fail(BF_ERR_INVALID, "parts %d and %d overlap", j, i);
+        o.wide = o.wide && p.at % piece == 0;
+        o.part[i] = bf::LoraPart{p.A, p.B, p.N, p.at};
+    }
+    for (int i = a->parts; i < bf::kLoraParts; i++) o.part[i] = bf::LoraPart{nullptr, nullptr, 0, 0};
+    o.X = a->X;
+    o.ldx = a->ldx;
+    o.ids = a->ids;
+    o.scales = a->scales;
+    o.ranks = a->ranks;
+    o.adapters = a->adapters;
+    o.rank = a->rank;
+    o.parts = a->parts;
+    o.C = a->C;
+    o.ldc = a->ldc;
+    o.Y = a->Y;
+    o.ldy = a->ldy;
+    o.out_f16 = f16;
+    o.T = a->T;
+    o.K = a->K;
+    if (a->rank > 4096 || a->K > (1 << 24)) return fail(BF_ERR_UNSUPPORTED, "rank=%d K=%d: at most 4096 and 2^24", a->rank, a->K);
+    for (int i = 0; i < a->parts; i++)
+        if (a->part[i].N > (1 << 24)) return fail(BF_ERR_UNSUPPORTED, "part %d: N=%d: at most 2^24", i, a->part[i].N);
+    if (!bf::lora_fits(o)) return fail(BF_ERR_UNSUPPORTED, "T=%d rank=%d: more workgroups than a launch takes", a->T, a->rank);
     return BF_OK;
 }
 
@@ -840,16 +964,27 @@ bf_status take_workspace(const char* who, size_t bytes, const bf::Scratch* scrat
     return from_hip(e, who);
 }
 
-bf_status run_attention(const char* who, const bf_kv4_cache* c, const bf_kv4_attention_args* a, const bf::Scratch* scratch,
-                        void* stream) {
+bf_status run_attention(const char* who, const bf_kv4_cache* c, const bf_kv4_attention_args* a, int sinks,
+                        const bf::Scratch* scratch, void* stream) {
     bf::Kv4Args o;
-    bf_status st = check_attention(c, a, o);
+    bf_status st = check_attention(c, a, sinks, o);
     if (st != BF_OK) return st;
     const auto held = stream_lock(stream);
     float* ws = nullptr;
     st = take_workspace(who, bf::kv4_attention_scratch_bytes(o), scratch, (hipStream_t)stream, &ws);
     if (st != BF_OK) return st;
     return from_hip(bf::kv4_attention(o, ws, (hipStream_t)stream), who);
+}
+
+bf_status run_lora(const char* who, const bf_lora_args* a, const bf::Scratch* scratch, void* stream) {
+    bf::LoraArgs o;
+    bf_status st = check_lora(a, o);
+    if (st != BF_OK) return st;
+    const auto held = stream_lock(stream);
+    float* ws = nullptr;
+    st = take_workspace(who, bf::lora_scratch_bytes(o), scratch, (hipStream_t)stream, &ws);
+    if (st != BF_OK) return st;
+    return from_hip(bf::lora(o, ws, (hipStream_t)stream), who);
 }
 
 bf_status run_moe(const char* who, const bf_moe_ffn_args* a, const bf::Scratch* scratch, void* stream) {
@@ -1207,13 +1342,13 @@ bf_status bf_kv4_load(const bf_kv4_cache* cache, const int64_t* slots, uint16_t*
 
 bf_status bf_kv4_attention(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* stream) {
     g_last_error[0] = '\0';
-    return run_attention("bf_kv4_attention", cache, args, nullptr, stream);
+    return run_attention("bf_kv4_attention", cache, args, 0, nullptr, stream);
 }
 
 size_t bf_kv4_attention_workspace_bytes(const bf_kv4_cache* cache, const bf_kv4_attention_args* args) {
     g_last_error[0] = '\0';
     bf::Kv4Args o;
-    return check_attention(cache, args, o) == BF_OK ? bf::kv4_attention_scratch_bytes(o) : 0;
+    return check_attention(cache, args, 0, o) == BF_OK ? bf::kv4_attention_scratch_bytes(o) : 0;
 }
 
 bf_status bf_kv4_attention_ws(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* workspace,
@@ -1222,7 +1357,62 @@ bf_status bf_kv4_attention_ws(const bf_kv4_cache* cache, const bf_kv4_attention_
     const bf_status st = check_workspace(workspace, workspace_bytes);
     if (st != BF_OK) return st;
     const bf::Scratch sc{(uint8_t*)workspace, workspace_bytes};
-    return run_attention("bf_kv4_attention_ws", cache, args, &sc, stream);
+    return run_attention("bf_kv4_attention_ws", cache, args, 0, &sc, stream);
+}
+
+bf_status bf_kv4_attention_sinks(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, int sinks, void* stream) {
+    g_last_error[0] = '\0';
+    return run_attention("bf_kv4_attention_sinks", cache, args, sinks, nullptr, stream);
+}
+
+size_t bf_kv4_attention_sinks_workspace_bytes(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, int sinks) {
+    g_last_error[0] = '\0';
+    bf::Kv4Args o;
+    return check_attention(cache, args, sinks, o) == BF_OK ? bf::kv4_attention_scratch_bytes(o) : 0;
+}
+
+bf_status bf_kv4_attention_sinks_ws(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, int sinks, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    g_last_error[0] = '\0';
+    const bf_status st = check_workspace(workspace, workspace_bytes);
+    if (st != BF_OK) return st;
+    const bf::Scratch sc{(uint8_t*)workspace, workspace_bytes};
+    return run_attention("bf_kv4_attention_sinks_ws", cache, args, sinks, &sc, stream);
+}
+
+bf_status bf_kv4_append(const bf_kv4_cache* cache, const bf_kv4_append_args* args, void* stream) {
+    g_last_error[0] = '\0';
+    bf::Kv4AppendArgs o;
+    const bf_status st = check_append(cache, args, o);
+    if (st != BF_OK) return st;
+    return from_hip(bf::kv4_append(o, (hipStream_t)stream), "kernel launch");
+}
+
+bf_status bf_rms_norm(const bf_rms_norm_args* args, void* stream) {
+    g_last_error[0] = '\0';
+    bf::NormArgs o;
+    const bf_status st = check_norm(args, o);
+    if (st != BF_OK) return st;
+    return from_hip(bf::rms_norm(o, (hipStream_t)stream), "kernel launch");
+}
+
+bf_status bf_lora(const bf_lora_args* args, void* stream) {
+    g_last_error[0] = '\0';
+    return run_lora("bf_lora", args, nullptr, stream);
+}
+
+size_t bf_lora_workspace_bytes(const bf_lora_args* args) {
+    g_last_error[0] = '\0';
+    bf::LoraArgs o;
+    return check_lora(args, o) == BF_OK ? bf::lora_scratch_bytes(o) : 0;
+}
+
+bf_status bf_lora_ws(const bf_lora_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    g_last_error[0] = '\0';
+    const bf_status st = check_workspace(workspace, workspace_bytes);
+    if (st != BF_OK) return st;
+    const bf::Scratch sc{(uint8_t*)workspace, workspace_bytes};
+    return run_lora("bf_lora_ws", args, &sc, stream);
 }
 
 bf_status bf_moe_route(const bf_moe_route_args* args, void* stream) {

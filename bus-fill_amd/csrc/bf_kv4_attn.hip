@@ -2,7 +2,7 @@
 //
 //   o_i = sum_t p_it v_t / sum_t p_it,  p_it = exp(scale q_i . k_t - max),
 //   over the tokens t that query i sees: t <= position (causal), t > position -
-//   window, and t's page present.  No token seen: o = 0.
+//   window or t < sinks, and t's page present.  No token seen: o = 0.
 //
 // Bound by the cache's bytes (4.5 bits a value) for single tokens.  One wave
 // multiplies a record (32 tokens) at a time with 16 query rows (the heads of a
@@ -104,7 +104,7 @@ __device__ __forceinline__ void read_rec(Kv4Rec<NB>& x, const uint8_t* rec, int 
 
 // Tiles [c0, c1) of head h of a row tile: its rows of O where they are `all` of
 // it, else a slot of the workspace.
-template <int NB, int WV>
+template <int NB, int WV, bool SINK>
 __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const Row& o, int h, int c0, int c1, bool all,
                                        int64_t slot, float* __restrict__ ws, uint8_t* lds, float (*xm)[kKv4Rows],
                                        float (*xl)[kKv4Rows]) {
@@ -142,9 +142,9 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
     // Lane n holds the record of the wave's n-th tile of the next 64 (-1: page absent)
     int recs = 0;
     auto look = [&](int n0) {
-        const int tile = c0 + wave + WV * (n0 + lane);
+        const int at = c0 + wave + WV * (n0 + lane), tile = o.tile<SINK>(at);
         recs = -1;
-        if (tile < c1) {
+        if (at < c1) {
             const int pg = tile / per_page, id = tab[pg];
             if (id >= 0 && id < a.c.pages) recs = (id * a.c.heads + h) * per_page + (tile - pg * per_page);
         }
@@ -181,8 +181,8 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
                 d = max(d, larger_half(vw[i]));
             }
             read_rec<NB>(x, rec, lane);
-            const int tb = (c0 + wave + WV * n) * kKv4Tile;
-            const bool edge = tb < free0 || tb + kKv4Tile > free1;
+            const int tb = o.tile<SINK>(c0 + wave + WV * n) * kKv4Tile;
+            const bool edge = (tb < free0 && !(SINK && tb + kKv4Tile <= a.sinks)) || tb + kKv4Tile > free1;
             float s[8];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -202,7 +202,7 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int t = tb + 8 * g + e;
-                    const bool see = t >= lo && t < hi;
+                    const bool see = sees<SINK>(t, lo, hi, a.sinks);
                     s[e] = see ? s[e] : -__builtin_inff();
 #pragma unroll
                     for (int b = 0; b < NB; b++)
@@ -219,7 +219,7 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
 #pragma unroll
                 for (int i = 0; i < SL; i++) {
                     const int w = min(64 * i + lane, SW - 1);
-                    d = max(d, larger_seen(vw[i], tb + 8 * (w / (4 * NB)) + 2 * (w % 4), seen0, seen1));
+                    d = max(d, larger_seen<SINK>(vw[i], tb + 8 * (w / (4 * NB)) + 2 * (w % 4), seen0, seen1, a.sinks));
                 }
                 const float al = rg.raise(tm, top_of(rg.top, d), sc);
                 l *= al;
@@ -312,7 +312,7 @@ __device__ __forceinline__ void attend(const Kv4Args& a, const Kv4Plan& p, const
 constexpr int kGridY = 32768;
 __device__ __forceinline__ int64_t grid_item() { return (int64_t)blockIdx.z * kGridY + blockIdx.y; }
 
-template <int NB, int WV>
+template <int NB, int WV, bool SINK>
 __global__ __launch_bounds__(64 * WV, kPerCu<NB>) void k_kv4_attn(Kv4Args a, Kv4Plan p, float* __restrict__ ws) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float xm[WV][kKv4Rows], xl[WV][kKv4Rows];
@@ -324,15 +324,15 @@ __global__ __launch_bounds__(64 * WV, kPerCu<NB>) void k_kv4_attn(Kv4Args a, Kv4
         h = blockIdx.x - sp * a.c.heads;
     }
     Row o;
-    if (!row_tile_of(a, p, (int)item, o)) return;
+    if (!row_tile_of<SINK>(a, p, (int)item, o)) return;
     const int c0 = o.t0 + sp * p.chunk;
     if (sp > 0 && c0 >= o.t1) return;
-    attend<NB, WV>(a, p, o, h, c0, min(o.t1, c0 + p.chunk), o.t1 - o.t0 <= p.chunk, (item * a.c.heads + h) * p.splits + sp,
+    attend<NB, WV, SINK>(a, p, o, h, c0, min(o.t1, c0 + p.chunk), o.t1 - o.t0 <= p.chunk, (item * a.c.heads + h) * p.splits + sp,
                    ws, lds, xm, xl);
 }
 
 // The chunks of a row, joined: one workgroup a row, its waves taking chunks in turn.
-template <int NB, int WV>
+template <int NB, int WV, bool SINK>
 __global__ __launch_bounds__(64 * WV) void k_kv4_join(Kv4Args a, Kv4Plan p, int most, const float* __restrict__ ws) {
     constexpr int D = 32 * NB, C = (D + 63) / 64;
     __shared__ float xo[WV][D];
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(64 * WV) void k_kv4_join(Kv4Args a, Kv4Plan p, int 
     if (item >= p.items) return;
     const int h = blockIdx.x / most, row = blockIdx.x - h * most;
     Row o;
-    if (!row_tile_of(a, p, (int)item, o) || row >= o.rows) return;
+    if (!row_tile_of<SINK>(a, p, (int)item, o) || row >= o.rows) return;
     const int parts = (o.t1 - o.t0 + p.chunk - 1) / p.chunk;
     if (parts <= 1) return;
     const int64_t slot = (item * a.c.heads + h) * p.splits;
@@ -389,11 +389,11 @@ dim3 grid_of(const Kv4Plan& p, int64_t x) {
     return dim3((unsigned)x, (unsigned)std::min<int64_t>(p.items, kGridY), (unsigned)((p.items + kGridY - 1) / kGridY));
 }
 
-template <int NB, int WV>
+template <int NB, int WV, bool SINK>
 hipError_t launch(const Kv4Args& a, const Kv4Plan& p, float* ws, hipStream_t st) {
     constexpr int W = NB < 4 ? 32 * NB : 128, ring = WV * kStages<NB, WV> * kRecBytes<NB>, meet = WV * kKv4Rows * (W + 4) * 4;
     constexpr int lds = ring > meet ? ring : meet;
-    auto k = k_kv4_attn<NB, WV>;
+    auto k = k_kv4_attn<NB, WV, SINK>;
     static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -410,14 +410,15 @@ hipError_t launch(const Kv4Args& a, const Kv4Plan& p, float* ws, hipStream_t st)
     const int most = join_rows(a, p);
     const dim3 grid = grid_of(p, (int64_t)a.c.heads * most);
     // many chunks a row: more waves on each
-    if (p.splits > 32) hipLaunchKernelGGL((k_kv4_join<NB, 16>), grid, dim3(1024), 0, st, a, p, most, ws);
-    else hipLaunchKernelGGL((k_kv4_join<NB, 4>), grid, dim3(256), 0, st, a, p, most, ws);
+    if (p.splits > 32) hipLaunchKernelGGL((k_kv4_join<NB, 16, SINK>), grid, dim3(1024), 0, st, a, p, most, ws);
+    else hipLaunchKernelGGL((k_kv4_join<NB, 4, SINK>), grid, dim3(256), 0, st, a, p, most, ws);
     return hipGetLastError();
 }
 
 template <int NB>
 hipError_t launch(const Kv4Args& a, const Kv4Plan& p, float* ws, hipStream_t st) {
-    return p.waves == 8 ? launch<NB, 8>(a, p, ws, st) : launch<NB, 4>(a, p, ws, st);
+    if (a.sinks > 0) return p.waves == 8 ? launch<NB, 8, true>(a, p, ws, st) : launch<NB, 4, true>(a, p, ws, st);
+    return p.waves == 8 ? launch<NB, 8, false>(a, p, ws, st) : launch<NB, 4, false>(a, p, ws, st);
 }
 
 Kv4Plan plan_of(const Kv4Args& a) { return plan_kv4(a, device_cus() > 0 ? device_cus() : 256); }

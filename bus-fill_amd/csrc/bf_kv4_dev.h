@@ -55,10 +55,15 @@ __device__ __forceinline__ float log2_scale(float scale) {
 
 // The larger magnitude of a word's two halves, as bits.
 __device__ __forceinline__ uint32_t larger_half(uint32_t w) { return max(w & 0x7FFFu, (w >> 16) & 0x7FFFu); }
-// ... of those that are finite and whose tokens t, t + 1 are in [lo, hi)
-__device__ __forceinline__ uint32_t larger_seen(uint32_t w, int t, int lo, int hi) {
+// Token t is in [lo, hi) or one of the first `sinks` below hi.
+template <bool SINK> __device__ __forceinline__ bool sees(int t, int lo, int hi, int sinks) {
+    return (t >= lo || (SINK && t < sinks)) && t < hi;
+}
+// ... of those that are finite and whose tokens t, t + 1 are seen
+template <bool SINK>
+__device__ __forceinline__ uint32_t larger_seen(uint32_t w, int t, int lo, int hi, int sinks) {
     const uint32_t a = w & 0x7FFFu, b = (w >> 16) & 0x7FFFu;
-    return max(t >= lo && t < hi && a < 0x7C00u ? a : 0u, t + 1 >= lo && t + 1 < hi && b < 0x7C00u ? b : 0u);
+    return max(sees<SINK>(t, lo, hi, sinks) && a < 0x7C00u ? a : 0u, sees<SINK>(t + 1, lo, hi, sinks) && b < 0x7C00u ? b : 0u);
 }
 // top, or the largest value of the exponent field of the wave's largest d, if that is larger
 __device__ __forceinline__ uint32_t top_of(uint32_t top, uint32_t d) {
@@ -109,7 +114,10 @@ __device__ __forceinline__ uint32_t scaled_pair(float p, float q, uint32_t de) {
 
 struct Row {                                       // a row tile of a sequence
     int s, q0, nq, len, rows, row0;
-    int t0, t1;                                    // tiles of 32 cached tokens that it sees
+    // Tiles of 32 cached tokens that it sees: t0 .. t1 - 1.  With first tokens in sight (sinks) whose tiles lie before
+    // the window's: those below w0 stand for tiles 0 .. w0 - t0 - 1, the window's begin at w0.
+    int t0, t1, w0;
+    template <bool SINK> __device__ __forceinline__ int tile(int i) const { return SINK && i < w0 ? i - t0 : i; }
 };
 
 // Cached tokens [lo, hi) that query i of the sequence sees.
@@ -121,6 +129,7 @@ __device__ __forceinline__ int lo_of(const Kv4Args& a, const Row& o, int i) {
 }
 
 // Item i = s row_tiles + rt; false where it has no rows.
+template <bool SINK>
 __device__ __forceinline__ bool row_tile_of(const Kv4Args& a, const Kv4Plan& p, int i, Row& o) {
     int rt = 0;
     o.s = i;
@@ -136,8 +145,14 @@ __device__ __forceinline__ bool row_tile_of(const Kv4Args& a, const Kv4Plan& p, 
     const int64_t left = (int64_t)o.nq * p.group - o.row0;
     o.rows = left < p.tile_rows ? (int)left : p.tile_rows;
     if (o.rows <= 0) return false;
-    o.t0 = lo_of(a, o, o.row0 / p.group) / kKv4Tile;
-    o.t1 = max(o.t0, (hi_of(a, o, (o.row0 + o.rows - 1) / p.group) + kKv4Tile - 1) / kKv4Tile);
+    const int hi = hi_of(a, o, (o.row0 + o.rows - 1) / p.group);
+    o.w0 = o.t0 = lo_of(a, o, o.row0 / p.group) / kKv4Tile;
+    o.t1 = max(o.t0, (hi + kKv4Tile - 1) / kKv4Tile);
+    if constexpr (SINK) {
+        const int first = (min(a.sinks, hi) + kKv4Tile - 1) / kKv4Tile;    // tiles of the first tokens
+        if (first < o.w0) o.t0 -= first;
+        else o.w0 = o.t0 = 0;
+    }
     return true;
 }
 

@@ -26,6 +26,7 @@ struct Kv4Args {
     int S, T, q_heads, max_q, max_kv;
     float scale;
     int causal, window;
+    int sinks;                                     // first tokens that a window leaves visible (0 without one)
 };
 
 constexpr int kKv4Rows = 16;                       // query rows of a row tile (one matrix operand)
@@ -61,7 +62,7 @@ inline bool prompt_serves(const Kv4Args& a, int group, int cus) {
     const int64_t all = std::min(a.S * tiles, (int64_t)a.T * group / kKv4Rows + a.S) * a.c.heads;
     double share = 1.0;                            // causal rows: the first ones see less
     if (a.causal && a.max_kv > 0) {
-        const double reach = a.window > 0 ? std::min(a.window, a.max_kv) : a.max_kv;
+        const double reach = a.window > 0 ? std::min<int64_t>((int64_t)a.window + a.sinks, a.max_kv) : a.max_kv;
         const double ramp = std::min<double>(a.max_q, std::max(0.0, reach - (a.max_kv - std::min(a.max_q, a.max_kv))));
         share -= ramp * ramp / (2.0 * a.max_q * reach);
     }
@@ -102,7 +103,8 @@ inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
         const int64_t span = std::min<int64_t>(a.max_q, (p.tile_rows + p.group - 2) / p.group + 1);
         seen = std::min<int64_t>(seen, (int64_t)a.window + span - 1);
     }
-    const int64_t most = std::max<int64_t>(1, (seen + (a.window > 0 ? 2 : 1) * (kKv4Tile - 1)) / kKv4Tile);   // (a window may start inside a tile)
+    const int64_t most = std::max<int64_t>(1, (seen + (a.window > 0 ? 2 : 1) * (kKv4Tile - 1)) / kKv4Tile) +   // (a window may start inside a tile)
+                         (std::min(a.sinks, a.max_kv) + kKv4Tile - 1) / kKv4Tile;
     p.items = (int64_t)a.S * p.row_tiles;
     const int64_t units = p.items * a.c.heads, places = (int64_t)cus * (a.c.dim == 256 ? 2 : kKv4PerCu);
     const int64_t share = std::max<int64_t>(1, cus / units), fill = (most + share - 1) / share;

@@ -66,10 +66,10 @@ __device__ __forceinline__ void load(PrRaw<NB>& x, const uint8_t* rec, int tid) 
 // Values of column d, tokens 8 g + 4 h + c, at place 16 (g / 2) + 8 h + 4 (g % 2) + c
 // of the column; scales of block b at 32 b + 16 h + 4 g + c (keys', then values').
 // top: the range of the values' scales so far (Range), of tokens tb ... in
-// [lo, hi); each wave that holds scales leaves its own beside the record.
-template <int NB>
+// [lo, hi) (and first ones); each wave that holds scales leaves its own beside the record.
+template <int NB, bool SINK>
 __device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint8_t* lds, int tid, uint32_t& top, int tb, int lo,
-                                       int hi) {
+                                       int hi, int sinks) {
     using L = PrLds<NB>;
 #pragma unroll
     for (int i = 0; i < PrRaw<NB>::KW; i++) {
@@ -106,12 +106,12 @@ __device__ __forceinline__ void decode(const Magic& mg, const PrRaw<NB>& x, uint
         uint8_t* to = lds + L::S + 2 * (32 * b + 16 * (e >> 1) + 4 * g + 2 * (e & 1));
         *(uint32_t*)to = x.ks | bad;
         *(uint32_t*)(to + 64 * NB) = x.vs & ~bad;
-        if (__any(larger_half(x.vs & ~bad) > top)) top = top_of(top, larger_seen(x.vs, tb + 8 * g + 2 * e, lo, hi));
+        if (__any(larger_half(x.vs & ~bad) > top)) top = top_of(top, larger_seen<SINK>(x.vs, tb + 8 * g + 2 * e, lo, hi, sinks));
         if ((tid & 63) == 0) *(uint32_t*)(lds + L::Top + (tid >> 4)) = top;
     }
 }
 
-template <int NB>
+template <int NB, bool SINK>
 __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4Args a, Kv4Plan p, int cus) {
     using L = PrLds<NB>;
     constexpr int D = 32 * NB;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
     const int rank = round & 1 ? min((round + 1) * cus, units) - 1 - in : (int)blockIdx.x;
     const int h = rank % a.c.heads, rest = rank / a.c.heads, s = rest % a.S, rt = p.row_tiles - 1 - rest / a.S;
     Row o;
-    if (!row_tile_of(a, p, s * p.row_tiles + rt, o)) return;
+    if (!row_tile_of<SINK>(a, p, s * p.row_tiles + rt, o)) return;
 
     // the lane's query row; rows past the last repeat it
     const int row = o.row0 + min(32 * wave + col, o.rows - 1), iq = row / p.group;
@@ -154,9 +154,9 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
     // Lane n holds the record of the n-th tile of the next 64 (-1: page absent, or no such tile)
     int recs = -1;
     auto look = [&](int n0) {
-        const int tile = o.t0 + n0 + lane;
+        const int at = o.t0 + n0 + lane, tile = o.tile<SINK>(at);
         recs = -1;
-        if (tile < o.t1) {
+        if (at < o.t1) {
             const int pg = tile / per_page, id = tab[pg];
             if (id >= 0 && id < a.c.pages) recs = (id * a.c.heads + h) * per_page + (tile - pg * per_page);
         }
@@ -206,11 +206,11 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
         values(0);
         __builtin_amdgcn_sched_barrier(0);
         // the lane's tokens: register 4 a + c is token 8 a + 4 h2 + c
-        if (tb < free0 || tb + kKv4Tile > free1) {     // hidden from some row of the wave
+        if ((tb < free0 && !(SINK && tb + kKv4Tile <= a.sinks)) || tb + kKv4Tile > free1) {   // hidden from some row of the wave
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const int t = tb + 8 * (e >> 2) + 4 * h2 + (e & 3);
-                x[e] = t >= lo && t < hi ? x[e] : -__builtin_inff();
+                x[e] = sees<SINK>(t, lo, hi, a.sinks) ? x[e] : -__builtin_inff();
             }
         }
         float tm = x[0];
@@ -262,15 +262,17 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
     int rec = -1, next = -1;
     if (walk > 0) {
         rec = fetch(0);
-        decode<NB>(mg, raw, lds, tid, seen_top, o.t0 * kKv4Tile, seen0, rec >= 0 ? seen1 : 0);
+        decode<NB, SINK>(mg, raw, lds, tid, seen_top, o.tile<SINK>(o.t0) * kKv4Tile, seen0, rec >= 0 ? seen1 : 0, a.sinks);
         next = fetch(1);
         __syncthreads();
     }
     for (int n = 0; n < walk; n++) {
-        if (n + 1 < walk) decode<NB>(mg, raw, lds + ((n + 1) & 1) * L::Bytes, tid, seen_top, (o.t0 + n + 1) * kKv4Tile, seen0, next >= 0 ? seen1 : 0);
+        if (n + 1 < walk)
+            decode<NB, SINK>(mg, raw, lds + ((n + 1) & 1) * L::Bytes, tid, seen_top, o.tile<SINK>(o.t0 + n + 1) * kKv4Tile, seen0,
+                             next >= 0 ? seen1 : 0, a.sinks);
         const int after = n + 2 < walk ? fetch(n + 2) : -1;
-        const int tb = (o.t0 + n) * kKv4Tile;
-        if (rec >= 0 && tb < whi && tb + kKv4Tile > wlo) tile_of(lds + (n & 1) * L::Bytes, tb);
+        const int tb = o.tile<SINK>(o.t0 + n) * kKv4Tile;
+        if (rec >= 0 && tb < whi && (tb + kKv4Tile > wlo || (SINK && tb < a.sinks))) tile_of(lds + (n & 1) * L::Bytes, tb);
         rec = next;
         next = after;
         __syncthreads();
@@ -292,9 +294,9 @@ __global__ __launch_bounds__(kPrThreads, NB == 8 ? 1 : 2) void k_kv4_prompt(Kv4A
             l == 0.f ? -__builtin_inff() : (rg.log2_unit(sc) + __builtin_log2f(l)) * 0.693147180559945309f;
 }
 
-template <int NB>
+template <int NB, bool SINK>
 hipError_t launch(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st) {
-    auto k = k_kv4_prompt<NB>;
+    auto k = k_kv4_prompt<NB, SINK>;
     constexpr int lds = 2 * PrLds<NB>::Bytes;
 
     static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
@@ -309,6 +311,11 @@ hipError_t launch(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st) {
     }
     hipLaunchKernelGGL(k, dim3((unsigned)(p.items * a.c.heads)), dim3(kPrThreads), lds, st, a, p, cus);
     return hipGetLastError();
+}
+
+template <int NB>
+hipError_t launch(const Kv4Args& a, const Kv4Plan& p, int cus, hipStream_t st) {
+    return a.sinks > 0 ? launch<NB, true>(a, p, cus, st) : launch<NB, false>(a, p, cus, st);
 }
 
 }  // namespace

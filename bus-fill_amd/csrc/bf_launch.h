@@ -165,4 +165,25 @@ hipError_t quantize_q8(const uint16_t* A, int lda, void* Aq, int M, int K, hipSt
 bool q8_supports(int M, int K);
 hipError_t gemm_q8(const Q8Args& g, hipStream_t st);
 
+// Residual addition and root-mean-square norm (bf_rms_norm).
+struct NormArgs {
+    const void* X;
+    int64_t ldx;
+    int x_f16;
+    const void* D;             // NULL: nothing is added
+    int64_t ldd;
+    int d_f16;
+    void* R;                   // NULL: the sum is not kept
+    int64_t ldr;
+    const void* W;             // NULL: ones
+    int w_f16;
+    float offset, eps;
+    uint16_t* H;               // NULL: no fp16 rows
+    int64_t ldh;
+    void* Aq;                  // NULL: no int8 rows; q8_bytes(T, K) bytes
+    int T, K;
+};
+bool rms_norm_fits(int T, int K);
+hipError_t rms_norm(const NormArgs& a, hipStream_t st);
+
 }  // namespace bf

@@ -22,11 +22,12 @@
  *       * bf_gemm_ws / bf_gemm_batched_ws / bf_busfill_q4_ws: the caller owns
  *         it (size from bf_gemm_workspace_bytes / bf_gemm_batched_workspace_bytes);
  *         the library allocates nothing and keeps no state between calls.
- *         bf_kv4_attention_ws and bf_moe_ffn_ws do the same for their partial
- *         results and intermediates.
+ *         bf_kv4_attention_ws, bf_kv4_attention_sinks_ws, bf_lora_ws and
+ *         bf_moe_ffn_ws do the same for their partial results and
+ *         intermediates.
  *       * bf_gemm_noalloc: a fixed array in device memory per GPU.
  *       * bf_gemm, bf_gemm_batched, bf_busfill_q4, bf_ffn_swiglu,
- *         bf_kv4_attention, bf_moe_ffn: the
+ *         bf_kv4_attention, bf_kv4_attention_sinks, bf_lora, bf_moe_ffn: the
  *         library's workspace for the (device, stream) -- per host thread for
  *         hipStreamPerThread -- allocated by the first call on the stream that
  *         needs it and grown by a later call that needs more (each region that
@@ -498,6 +499,121 @@ bf_status bf_kv4_attention(const bf_kv4_cache* cache, const bf_kv4_attention_arg
 size_t bf_kv4_attention_workspace_bytes(const bf_kv4_cache* cache, const bf_kv4_attention_args* args);
 bf_status bf_kv4_attention_ws(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, void* workspace,
                               size_t workspace_bytes, void* stream);
+
+/* Attention as above with first tokens that stay in sight: a query sees the last
+ * args->window tokens up to its own and, of the first `sinks` tokens (0 and up),
+ * those up to its own.  Without a window every token is in sight already and sinks
+ * changes nothing; with sinks = 0 the calls are bf_kv4_attention's, bit for bit.
+ * Pages that hold neither are not read (their entries in page_table may be
+ * negative). */
+bf_status bf_kv4_attention_sinks(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, int sinks, void* stream);
+size_t bf_kv4_attention_sinks_workspace_bytes(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, int sinks);
+bf_status bf_kv4_attention_sinks_ws(const bf_kv4_cache* cache, const bf_kv4_attention_args* args, int sinks,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which elements of a head's first `rot` turn together: i and i + rot / 2, or 2 i and 2 i + 1. */
+typedef enum { BF_ROPE_HALVES = 0, BF_ROPE_PAIRS = 1 } bf_rope;
+
+/* T tokens' queries and keys rotated by their positions, keys and values stored:
+ * the i-th pair (x, y) of each head becomes
+ *   (x cos t - y sin t, y cos t + x sin t) factor,  t = positions[token] freq[i] radians,
+ * in fp32, rounded once to fp16 (t to 2^-20 of a turn for positions up to 2^31
+ * either way); elements from rot on stay as they are.  Rotated queries go to
+ * Q_out, rotated keys to the cache (as bf_kv4_store of the fp16 rows, bit for bit)
+ * and, where K_out is given, there too; every row is rotated, whatever its slot.
+ * Q_out may be Q and K_out K (the same rows); other overlaps are not allowed. */
+typedef struct {
+    const uint16_t* Q;       /* [T][ldq] fp16, q_heads heads; NULL: no queries (Q_out NULL, q_heads 0) */
+    int64_t ldq;
+    uint16_t* Q_out;         /* [T][ldqo] */
+    int64_t ldqo;
+    const uint16_t* K;       /* [T][ldk], the cache's heads */
+    int64_t ldk;
+    uint16_t* K_out;         /* [T][ldko] or NULL */
+    int64_t ldko;
+    const uint16_t* V;       /* [T][ldv] */
+    int64_t ldv;
+    const int64_t* slots;    /* [T], as bf_kv4_store's */
+    const int64_t* positions;/* [T] */
+    const float* freq;       /* [rot / 2] */
+    int q_heads;
+    int rot;                 /* 16 .. head_dim, a multiple of 16 */
+    bf_rope style;
+    float factor;            /* 1, or what a stretched context's frequencies go with */
+    int T;
+} bf_kv4_append_args;        /* rows 16-byte aligned, ld multiples of 8 */
+bf_status bf_kv4_append(const bf_kv4_cache* cache, const bf_kv4_append_args* args, void* stream);
+
+/* ---------------------------------------------------------------- norm and adapters
+ * What stands before and beside a layer's linears.  No counterpart in the
+ * reference (kernels/busfill_v1a.cu:41-104 multiplies weights only). */
+typedef enum { BF_F32 = 0, BF_F16 = 1 } bf_dtype;
+
+/* The residual's addition and the root-mean-square norm of T rows:
+ *   r = X + delta,  y = r / sqrt(mean(r^2) + eps) (weight + offset);
+ * R = r in X's type (R may be X), H = y rounded once to fp16 (bf_gemm's A; H may
+ * be delta where that is fp16), Aq = y quantized as by bf_quantize_q8 (bf_gemm_q8's
+ * Aq: d = amax / 127 per 32 values, from the unrounded y; a block with an infinity
+ * or NaN has d NaN and codes 0), bf_q8_bytes(T, K) bytes.  Y is computed from the
+ * unrounded sum.  H or Aq may be NULL, not both.  Elements are aligned to their
+ * size, Aq to 16 bytes; rows of whole 16-byte pieces are read as such, others one
+ * by one (slower).  K up to 32768; K % 32 == 0 with Aq. */
+typedef struct {
+    const void* X;           /* [T][ldx] */
+    bf_dtype xtype;
+    int64_t ldx;
+    const void* delta;       /* [T][ldd] or NULL */
+    bf_dtype dtype;
+    int64_t ldd;
+    void* R;                 /* [T][ldr] or NULL: the sum is not kept */
+    int64_t ldr;
+    const void* weight;      /* [K] or NULL: ones */
+    bf_dtype wtype;
+    float offset;            /* 1 where weights are kept less 1 */
+    float eps;               /* >= 0 */
+    uint16_t* H;             /* [T][ldh] */
+    int64_t ldh;
+    void* Aq;
+    int T, K;
+} bf_rms_norm_args;
+bf_status bf_rms_norm(const bf_rms_norm_args* args, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection, whose output is
+ * C and whose input X (fp16, as the projection takes it):
+ *   Y[t][at + n] = C[t][at + n] + scales[e] sum_r B[e][n][r] sum_k A[e][r][k] X[t][k],  e = ids[t],
+ * for every part (a fused projection's slices, each with an A and a B of its own).
+ * A row whose id is negative or not below `adapters` has none: Y = C there.
+ * Columns of no part are left alone.  ranks[e] (cut to 0 .. rank) says how many of
+ * the `rank` rows of A[e] and columns of B[e] are used; the others may hold
+ * anything.  Rows come in any order, each with any adapter; equal neighbours are
+ * faster where there are many.  Inner sums are fp32 and enter the second product to
+ * 2^-22 of the row's largest; Y is rounded once. */
+typedef struct {
+    const uint16_t* A;       /* [adapters][rank][K] fp16 */
+    const uint16_t* B;       /* [adapters][N][rank] fp16 */
+    int N, at;               /* columns at .. at + N - 1 of C and Y; parts do not overlap */
+} bf_lora_part;
+typedef struct {
+    const uint16_t* X;       /* [T][ldx] */
+    int64_t ldx;
+    const int32_t* ids;      /* [T] */
+    const float* scales;     /* [adapters] or NULL: 1 */
+    const int32_t* ranks;    /* [adapters] or NULL: rank */
+    int adapters, rank;      /* rank a multiple of 8 */
+    int parts;               /* 1 .. 4 */
+    const bf_lora_part* part;/* host memory */
+    const void* C;           /* [T][ldc] */
+    int64_t ldc;
+    void* Y;                 /* [T][ldy]; may be C (with ldy = ldc) */
+    int64_t ldy;
+    bf_otype otype;          /* of C and Y */
+    int T, K;                /* K a multiple of 8; X rows, A and B 16-byte aligned */
+} bf_lora_args;
+/* The inner sums live in the library's workspace for the stream, or in the
+ * caller's (_ws, as bf_gemm_ws). */
+bf_status bf_lora(const bf_lora_args* args, void* stream);
+size_t bf_lora_workspace_bytes(const bf_lora_args* args);
+bf_status bf_lora_ws(const bf_lora_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- mixture of experts
  * No counterpart in the reference, whose end-to-end runs drive a dense model
