@@ -869,7 +869,8 @@ bf_status check_lora(const bf_lora_args* a, bf::LoraArgs& o) {
     o.out_f16 = f16;
     o.T = a->T;
     o.K = a->K;
-    if (a->rank > 4096 || a->K > (1 << 24)) return fail(BF_ERR_UNSUPPORTED, "rank=%d K=%d: at most 4096 and 2^24", a->rank, a->K);
+    if (a->rank > bf::kLoraMaxRank || a->K > (1 << 24))
+        return fail(BF_ERR_UNSUPPORTED, "rank=%d K=%d: at most %d and 2^24", a->rank, a->K, bf::kLoraMaxRank);
     for (int i = 0; i < a->parts; i++)
         if (a->part[i].N > (1 << 24)) return fail(BF_ERR_UNSUPPORTED, "part %d: N=%d: at most 2^24", i, a->part[i].N);
     if (!bf::lora_fits(o)) return fail(BF_ERR_UNSUPPORTED, "T=%d rank=%d: more workgroups than a launch takes", a->T, a->rank);

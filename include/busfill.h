@@ -599,7 +599,7 @@ typedef struct {
     const int32_t* ids;      /* [T] */
     const float* scales;     /* [adapters] or NULL: 1 */
     const int32_t* ranks;    /* [adapters] or NULL: rank */
-    int adapters, rank;      /* rank a multiple of 8 */
+    int adapters, rank;      /* rank a multiple of 8, up to 1024 */
     int parts;               /* 1 .. 4 */
     const bf_lora_part* part;/* host memory */
     const void* C;           /* [T][ldc] */

@@ -147,8 +147,8 @@ LORA = [
     ([(FAKE, FAKE, 64, -1)], "at=-1", 1), ([(FAKE, FAKE, 64, 0), (FAKE, FAKE, 8, 63)], "overlap", 1),
     ([(FAKE, FAKE, 8, 40), (FAKE, FAKE, 64, 0)], "overlap", 1), ([(FAKE, FAKE, 64, 33)], "columns 33", 1),
     ([(FAKE, FAKE, 2 ** 31 - 1, 2 ** 31 - 1)], "columns", 1),
-    (dict(rank=4104), "rank=4104", 2), (dict(K=(1 << 24) + 8, ldx=1 << 25), "K=16777224", 2),
-    (dict(T=(1 << 31) - 1, rank=4096), "workgroups", 2)]
+    (dict(rank=1032), "rank=1032", 2), (dict(K=(1 << 24) + 8, ldx=1 << 25), "K=16777224", 2),
+    (dict(T=(1 << 31) - 1, rank=1024), "workgroups", 2)]
 
 
 def test_lora_refuses():
