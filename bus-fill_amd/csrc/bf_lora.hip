@@ -10,10 +10,16 @@
 // adapters' bytes whatever the products do, and in prompts neighbouring rows are
 // of one adapter.
 //
-// Down: operands go from memory to registers; x and A are fp16, their products
-// exact, sums fp32.  K is cut between a workgroup's waves, whose sums meet in LDS,
-// and into pieces (partial sums in the workspace, added by the up products in
-// their order), so that a few rows fill the chip.
+// Both kernels' matrices come to LDS by direct loads, eight neighbouring lanes 128 bytes
+// of a row, with the row's 16-byte pieces in an order that spreads an operand's
+// reads over the banks.  (Operands straight from memory, a lane's 16 bytes in
+// another row than its neighbours', take the load path a cycle a lane: 23 us where
+// the down products of 32 rows take ....)
+//
+// Down: x and A are fp16, their products exact, sums fp32.  K is cut between a
+// workgroup's waves, whose sums meet in LDS, and into pieces (partial sums in the
+// workspace, added by the up products in their order), so that a few rows fill the
+// chip.
 // Up: s, times a power of two that brings the row's largest to 2^14..2^15, is
 // taken as two fp16 numbers (rounded, and the rest rounded: 2^-22 of the largest), so
 // the products lose nothing that fp32 would keep; sums fp32, one rounding of Y.
@@ -22,6 +28,7 @@
 #include "bf_device.h"
 #include "bf_grid.h"
 #include "bf_launch.h"
+#include "bf_lds.h"
 #include "bf_lora_launch.h"
 
 namespace bf {
@@ -34,8 +41,10 @@ __device__ __forceinline__ int adapter_of(const LoraArgs& a, int64_t t0, int row
     return id < 0 || id >= a.adapters ? -1 : id;
 }
 
-__device__ __forceinline__ int rank_of(const LoraArgs& a, int e) {
-    return a.ranks ? min(max(a.ranks[e], 0), a.rank) : a.rank;
+// ... and how many ranks of it count (0: none).
+__device__ __forceinline__ int ranks_of(const LoraArgs& a, int id) {
+    if (id < 0) return 0;
+    return a.ranks ? min(max(a.ranks[id], 0), a.rank) : a.rank;
 }
 
 __device__ __forceinline__ h8 masked(h8 v, bool in) {
@@ -43,301 +52,733 @@ __device__ __forceinline__ h8 masked(h8 v, bool in) {
     return in ? v : zero;
 }
 
-// Steps [s0, s1) of K: acc[sub][i] += ranks' operand i times rows' operand sub.
-template <int SUBS, int NT, int U>
-__device__ __forceinline__ void dot(f4 (&acc)[SUBS][4], const uint16_t* const (&x)[SUBS], const uint16_t* const (&w)[4], int s0,
-                                    int s1, int K, int g) {
-    for (int s = s0; s < s1; s += U) {
-        h8 xv[U][SUBS], wv[U][NT];
-#pragma unroll
-        for (int j = 0; j < U; j++) {              // (past the last step: the last one again, not used)
-            const int k = min(kLoraStep * min(s + j, s1 - 1) + 8 * g, K - 8);
-#pragma unroll
-            for (int i = 0; i < SUBS; i++) xv[j][i] = *(const h8*)(x[i] + k);
-#pragma unroll
-            for (int i = 0; i < NT; i++) wv[j][i] = *(const h8*)(w[i] + k);
-        }
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            if (s + j >= s1) break;
-            if (kLoraStep * (s + j + 1) > K) {     // the last step of a K off 32
-                const bool in = kLoraStep * (s + j) + 8 * g < K;
-#pragma unroll
-                for (int i = 0; i < SUBS; i++) xv[j][i] = masked(xv[j][i], in);
-#pragma unroll
-                for (int i = 0; i < NT; i++) wv[j][i] = masked(wv[j][i], in);
-            }
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int b = 0; b < SUBS; b++) acc[b][i] = mfma16x16x32(wv[j][i], xv[j][b], acc[b][i]);
-        }
+// The workgroup's tile and which of the tile's it is; false where there is none.
+__device__ __forceinline__ bool place_of(const LoraGrid& q, int& tile, int& in) {
+    const int b = blockIdx.x;
+    if (q.per_xcd) {
+        const int turn = b / kLoraXcds;
+        tile = b % kLoraXcds * q.per_xcd + turn / q.inner;
+        in = turn % q.inner;
+    } else {
+        tile = b % q.tiles;
+        in = b / q.tiles;
     }
+    return tile < q.tiles;
 }
 
-// Grid x: tile and sharer (the fastest), y: piece of K, z: part and ranks.
-template <int SUBS, int NT, int WV>
-__global__ __launch_bounds__(64 * WV) void k_lora_down(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
-    constexpr int ROWS = kLoraSub * SUBS, U = SUBS == 1 ? 4 : 2;
-    __shared__ f4 meet[WV - 1][SUBS * NT][64];
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int tile = blockIdx.x / p.sharers, share = blockIdx.x - tile * p.sharers, piece = blockIdx.y;
-    const int part = blockIdx.z / p.rank_parts, r0 = (blockIdx.z - part * p.rank_parts) * kLoraRanks;
-    const int64_t t0 = (int64_t)tile * ROWS;
-    const int id = adapter_of(a, t0, ROWS, lane);
-    const int64_t steps = (a.K + kLoraStep - 1) / kLoraStep, shares = (int64_t)p.pieces * WV, mine = (int64_t)piece * WV + wave;
-    const int s0 = (int)(steps * mine / shares), s1 = (int)(steps * (mine + 1) / shares);
-    const uint16_t* x[SUBS];
+// A unit in LDS: operands of 16 rows of 128 bytes, those of A first, piece c of row r at place c ^ (r % 8).
+template <int NT> constexpr int kUnitBytes = 2048 * (1 + NT);
+__device__ __forceinline__ h8 piece_of(const uint8_t* unit, int operand, int r, int c) {
+    return *(const h8*)(unit + 2048 * operand + 128 * r + 16 * (c ^ (r & 7)));
+}
+
+// Units [u0, u1) of K: acc[i] += ranks' operand i times the rows.
+template <int NT>
+__device__ __forceinline__ void dot(f4 (&acc)[4], const uint16_t* x, int64_t ldx, int64_t rows_left, const uint16_t* A, int ranks,
+                                    int K, int u0, int u1, const uint8_t* ring, int lane) {
+    constexpr int LOADS = 2 * (1 + NT), BYTES = kUnitBytes<NT>;
+    const int r = lane & 15, g = lane >> 4, row = lane >> 3, piece = (lane & 7) ^ row;   // (as lanes load: eight rows at once)
+    const uint16_t *wp[2 * NT], *xp[2];
 #pragma unroll
-    for (int b = 0; b < SUBS; b++) x[b] = a.X + min(t0 + 16 * b + r, (int64_t)a.T - 1) * a.ldx;
-    float* const out = ws + ((int64_t)part * p.pieces + piece) * a.T * a.rank;
-    int nth = 0;
-    for (uint64_t left = __ballot(id >= 0); left;) {
-        const int e = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const uint64_t rows = __ballot(id == e);
-        left &= ~rows;
-        if (p.sharers > 1 && nth++ != share) continue;
-        const int ranks = rank_of(a, e);
-        if (r0 >= ranks) continue;
-        const uint16_t* const A = a.part[part].A + (int64_t)e * a.rank * a.K;
-        const uint16_t* w[4];
+    for (int i = 0; i < 2 * NT; i++) wp[i] = A + (int64_t)min(8 * i + row, ranks - 1) * K;   // (rows past the rank: not kept)
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = A + (int64_t)min(r0 + 16 * i + r, ranks - 1) * a.K;   // (rows past the rank: not kept)
-        const int tiles = min(NT, (ranks - r0 + 15) / 16);
-        f4 acc[SUBS][4];
+    for (int i = 0; i < 2; i++) xp[i] = x + min((int64_t)(8 * i + row), rows_left - 1) * ldx;
+    const uint32_t ring0 = lds_addr(ring);
+    auto fetch = [&](int u) {
+        const uint32_t to = ring0 + (u & 1) * BYTES;
+        const int k = min(kLoraUnit * u + 8 * piece, K - 8);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                  // what was read there has been read
 #pragma unroll
-        for (int b = 0; b < SUBS; b++)
+        for (int i = 0; i < 2 * NT; i++) dma16(wp[i] + k, to + 1024 * i);
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[b][i] = f4{0.f, 0.f, 0.f, 0.f};
-        if (NT == 1 || tiles == 1) dot<SUBS, 1, U>(acc, x, w, s0, s1, a.K, g);
-        else if (NT == 2 || tiles == 2) dot<SUBS, 2, U>(acc, x, w, s0, s1, a.K, g);
-        else dot<SUBS, 4, U>(acc, x, w, s0, s1, a.K, g);
-        // the waves' sums, added in their order: register set m of all by wave m % WV
-        __syncthreads();                           // the last adapter's are read
-        if (wave > 0)
+        for (int i = 0; i < 2; i++) dma16(xp[i] + k, to + 2048 * NT + 1024 * i);
+    };
+    if (u0 < u1) fetch(u0);
+    for (int u = u0; u < u1; u++) {
+        if (u + 1 < u1) {
+            fetch(u + 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const uint8_t* const unit = ring + (u & 1) * BYTES;
 #pragma unroll
-            for (int b = 0; b < SUBS; b++)
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-                    if (i < tiles) meet[wave - 1][b * NT + i][lane] = acc[b][i];
-        __syncthreads();
-        if (wave > 0) continue;
-        // lane: row 16 b + r of the tile, ranks r0 + 16 i + 4 g ..
-#pragma unroll
-        for (int b = 0; b < SUBS; b++) {
-            if (!((rows >> (16 * b + r)) & 1)) continue;
+        for (int s = 0; s < 2; s++) {
+            const bool in = kLoraUnit * u + 32 * s + 8 * g < K, off = kLoraUnit * (u + 1) > K;   // (the last unit of a K off 64)
+            h8 v = piece_of(unit, NT, r, 4 * s + g);
+            if (off) v = masked(v, in);
 #pragma unroll
             for (int i = 0; i < NT; i++) {
-                const int at = r0 + 16 * i + 4 * g;
-                if (i >= tiles || at >= a.rank) continue;                  // (rank % 8 == 0)
-                f4 s = acc[b][i];
-                for (int v = 0; v < WV - 1; v++) s += meet[v][b * NT + i][lane];
-                *(f4*)(out + (t0 + 16 * b + r) * a.rank + at) = s;
+                h8 w = piece_of(unit, i, r, 4 * s + g);
+                if (off) w = masked(w, in);
+                acc[i] = mfma16x16x32(w, v, acc[i]);
             }
         }
     }
 }
 
-// Sixteen neighbouring columns of a row, n of them inside: Y = C + f d.
-__device__ __forceinline__ void add16(const LoraArgs& a, int64_t ci, int64_t yi, const f4 (&d)[4], float f, int n) {
-    if (a.wide && n >= 16) {
-        if (a.out_f16) {
+// What a workgroup takes of its tile: piece of K (the fastest), ranks, part, sharer.
+struct Share {
+    int piece, r0, part, share;
+};
+__device__ __forceinline__ Share share_of(const LoraArgs& a, const LoraPlan& p, int in) {
+    Share s;
+    s.piece = in % p.pieces;
+    in /= p.pieces;
+    s.r0 = in % p.rank_parts * kLoraRanks;
+    in /= p.rank_parts;
+    s.part = in % a.parts;
+    s.share = in / a.parts;
+    return s;
+}
+
+template <int NT>
+__global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    constexpr int WV = kLoraDownWaves;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // a ring of two units a wave, then the waves' sums
+    f4 (*const meet)[NT][64] = (f4 (*)[NT][64])lds;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int tile, in;
+    if (!place_of(p.down, tile, in)) return;
+    const Share q = share_of(a, p, in);
+    const int64_t t0 = (int64_t)tile * kLoraSub;
+    const int id = adapter_of(a, t0, kLoraSub, lane), rk = ranks_of(a, id);
+    const int64_t units = (a.K + kLoraUnit - 1) / kLoraUnit, shares = (int64_t)p.pieces * WV, mine = (int64_t)q.piece * WV + wave;
+    const int u0 = (int)(units * mine / shares), u1 = (int)(units * (mine + 1) / shares);
+    float* const out = ws + ((int64_t)q.part * p.pieces + q.piece) * a.T * a.rank;
+    const uint8_t* const ring = lds + wave * 2 * kUnitBytes<NT>;
+    int nth = 0;
+    for (uint64_t left = __ballot(id >= 0); left; nth++) {
+        const int first = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(id, first), ranks = __builtin_amdgcn_readlane(rk, first);
+        const uint64_t rows = __ballot(id == e);
+        left &= ~rows;
+        if (nth != q.share) continue;              // (as many sharers as a tile can have adapters)
+        if (q.r0 >= ranks) return;
+        const uint16_t* const A = a.part[q.part].A + ((int64_t)e * a.rank + q.r0) * a.K;
+        const uint16_t* const x = a.X + t0 * a.ldx;
+        const int tiles = min(NT, (ranks - q.r0 + 15) / 16);
+        f4 acc[4];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const h8 c = *(const h8*)((const _Float16*)a.C + ci + 8 * i);
-                f4 lo, hi;
+        for (int i = 0; i < 4; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+        if (NT == 1 || tiles == 1) dot<1>(acc, x, a.ldx, a.T - t0, A, ranks - q.r0, a.K, u0, u1, ring, lane);
+        else if (NT == 2 || tiles == 2) dot<2>(acc, x, a.ldx, a.T - t0, A, ranks - q.r0, a.K, u0, u1, ring, lane);
+        else dot<NT>(acc, x, a.ldx, a.T - t0, A, ranks - q.r0, a.K, u0, u1, ring, lane);
+        // the waves' sums, added in their order
+        __syncthreads();                           // every wave is done with its ring
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    lo[e] = __builtin_fmaf(f, d[2 * i][e], (float)c[e]);
-                    hi[e] = __builtin_fmaf(f, d[2 * i + 1][e], (float)c[4 + e]);
-                }
-                *(u4*)((_Float16*)a.Y + yi + 8 * i) = f32x8_to_f16(lo, hi);
+        for (int i = 0; i < NT; i++) meet[wave][i][lane] = acc[i];
+        __syncthreads();
+        // wave i: lane's row r of the tile, ranks r0 + 16 i + 4 g ..
+        const int at = q.r0 + 16 * wave + 4 * g;
+        if (wave < tiles && ((rows >> r) & 1) && at < a.rank) {            // (rank % 8 == 0)
+            f4 s = meet[0][wave][lane];
+#pragma unroll
+            for (int v = 1; v < WV; v++) s += meet[v][wave][lane];
+            *(f4*)(out + (t0 + r) * a.rank + at) = s;
+        }
+        return;
+    }
+}
+
+// Many rows: a wave takes 16 of 64 rows, whose x it keeps in registers; A's rows, a
+// slab of K at a time, two by turns, are in LDS for all four.
+template <int NT>
+__global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    constexpr int WV = kLoraDownWaves, STEPS = kLoraSlab / kLoraStep, UNITS = kLoraSlab / kLoraUnit, BYTES = UNITS * NT * 2048;
+    constexpr int LOADS = UNITS * NT * 2;          // direct loads of a slab, eight rows of 128 bytes each: wave w does every WV-th
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // two slabs: [unit][operand][16 rows of 128 bytes]
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, row = lane >> 3, piece = (lane & 7) ^ row;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int tile, in;
+    if (!place_of(p.down, tile, in)) return;
+    const Share q = share_of(a, p, in);
+    const int64_t t0 = (int64_t)tile * (4 * kLoraSub), mine = t0 + 16 * wave + r;
+    const int id = adapter_of(a, t0, 4 * kLoraSub, lane), rk = ranks_of(a, id);
+    const int64_t units = (a.K + kLoraUnit - 1) / kLoraUnit;
+    const int k0 = kLoraUnit * (int)(units * q.piece / p.pieces), k1 = min(a.K, kLoraUnit * (int)(units * (q.piece + 1) / p.pieces));
+    float* const out = ws + ((int64_t)q.part * p.pieces + q.piece) * a.T * a.rank;
+    const uint16_t* const x = a.X + min(mine, (int64_t)a.T - 1) * a.ldx;
+
+    // Adapter and slab, in turn: where one's products run, the next one is on its way
+    struct At {
+        int k, ranks;
+        uint64_t rows;
+        const uint16_t* A;
+    };
+    uint64_t left = __ballot(id >= 0 && rk > q.r0);
+    auto next = [&](At& o) -> bool {
+        o.k += kLoraSlab;
+        if (o.k < k1) return true;
+        if (!left) return false;
+        const int first = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(id, first);
+        o.ranks = __builtin_amdgcn_readlane(rk, first) - q.r0;
+        o.rows = __ballot(id == e);
+        left &= ~o.rows;
+        o.A = a.part[q.part].A + ((int64_t)e * a.rank + q.r0) * a.K;
+        o.k = k0;
+        return true;
+    };
+    auto mine_in = [&](const At& o) -> bool { return (o.rows >> (16 * wave)) & 0xFFFFu; };
+    h8 xv[2][STEPS];
+    // (the buffer's readers have passed a barrier)
+    auto fetch = [&](const At& o, int buf, h8 (&v)[STEPS]) {
+#pragma unroll
+        for (int i = 0; i < (LOADS + WV - 1) / WV; i++) {
+            const int n = WV * i + wave;           // unit, eight rows
+            if (n >= LOADS) break;
+            const int u = n / (2 * NT), m = n % (2 * NT), at = min(o.k + kLoraUnit * u + 8 * piece, a.K - 8);
+            dma16(o.A + (int64_t)min(8 * m + row, o.ranks - 1) * a.K + at, lds_addr(lds) + buf * BYTES + 1024 * n);
+        }
+        if (mine_in(o))
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) v[i] = *(const h8*)(x + min(o.k + kLoraStep * i + 8 * g, a.K - 8));
+    };
+    f4 acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const At& o, int buf, const h8 (&v)[STEPS]) {
+        if (!mine_in(o)) return;
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            const int at = o.k + kLoraStep * i;
+            if (at >= k1) break;
+            const uint8_t* const unit = lds + buf * BYTES + (i >> 1) * (2048 * NT);
+            const bool off = at + kLoraStep > k1, ok = at + 8 * g < k1;
+            const h8 b = off ? masked(v[i], ok) : v[i];
+#pragma unroll
+            for (int m = 0; m < NT; m++) {
+                h8 w = piece_of(unit, m, r, 4 * (i & 1) + g);
+                if (off) w = masked(w, ok);
+                acc[m] = mfma16x16x32(w, b, acc[m]);
             }
-        } else {
+        }
+        if (o.k + kLoraSlab < k1) return;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                f4 c = *(const f4*)((const float*)a.C + ci + 4 * i);
+        for (int i = 0; i < NT; i++) {             // the adapter's last slab
+            const int at = q.r0 + 16 * i + 4 * g;
+            if (((o.rows >> (16 * wave + r)) & 1) && at < a.rank) *(f4*)(out + mine * a.rank + at) = acc[i];
+            acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    // one turn; false after the last
+    auto turn = [&](const At& here, int buf, const h8 (&v)[STEPS], At& after, h8 (&w)[STEPS]) -> bool {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                           // this slab is here, the other one has been read
+        after = here;
+        const bool more = next(after);
+        if (more) fetch(after, 1 - buf, w);
+        multiply(here, buf, v);
+        return more;
+    };
+    At one, two;
+    one.k = k1;
+    if (!next(one)) return;
+    fetch(one, 0, xv[0]);
+    while (turn(one, 0, xv[0], two, xv[1]) && turn(two, 1, xv[1], one, xv[0])) {
+    }
+}
+
+// Of a row with `ranks` ranks, at s0 the pieces' sums (`step` apart): the sum of ranks k .. k + 3, pieces in their order.
+__device__ __forceinline__ f4 sum4(const float* s0, int64_t step, int pieces, int k, int ranks) {
+    f4 s = f4{0.f, 0.f, 0.f, 0.f};
+    if (k < ranks) {
+        f4 v[kLoraPieces];                         // (loads of all pieces at once)
 #pragma unroll
-                for (int e = 0; e < 4; e++) c[e] = __builtin_fmaf(f, d[i][e], c[e]);
-                *(f4*)((float*)a.Y + yi + 4 * i) = c;
-            }
+        for (int i = 0; i < kLoraPieces; i++) v[i] = *(const f4*)(s0 + min(i, pieces - 1) * step + k);
+        s = v[0];
+#pragma unroll
+        for (int i = 1; i < kLoraPieces; i++)
+            if (i < pieces) s += v[i];
+#pragma unroll
+        for (int j = 1; j < 4; j++)
+            if (k + j >= ranks) s[j] = 0.f;
+    }
+    return s;
+}
+
+// A row's sums, fours of ranks by PER neighbouring lanes in turn (this one `me`), to
+// two fp16 numbers each, times 2^shift: at hi + k and lo + k, k below `padded`.
+// Returns the shift.
+template <int PER>
+__device__ __forceinline__ int split_row(const float* s0, int64_t step, int pieces, int ranks, int me, int padded, _Float16* hi,
+                                         _Float16* lo) {
+    f4 held[2];
+    float top = 0.f;
+    for (int i = 0, k = 4 * me; k < padded; k += 4 * PER, i++) {
+        const f4 s = sum4(s0, step, pieces, k, ranks);
+        if (i == 0) held[0] = s;
+        if (i == 1) held[1] = s;
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = __builtin_fmaxf(top, __builtin_fabsf(s[j]));
+    }
+#pragma unroll
+    for (int x = 1; x < PER; x <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+    // (s is a sum of products of fp16 numbers, a multiple of 2^-48: the shift is at most 63)
+    const int shift = top > 0.f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+    const float up = __builtin_ldexpf(1.f, shift);
+    for (int i = 0, k = 4 * me; k < padded; k += 4 * PER, i++) {
+        const f4 s = i == 0 ? held[0] : i == 1 ? held[1] : sum4(s0, step, pieces, k, ranks);
+        _Float16 h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float v = s[j] * up;
+            h[j] = (_Float16)v;
+            l[j] = (_Float16)(v - (float)h[j]);
+        }
+        *(uint2*)(hi + k) = uint2{as_u32(h2{h[0], h[1]}), as_u32(h2{h[2], h[3]})};
+        *(uint2*)(lo + k) = uint2{as_u32(h2{l[0], l[1]}), as_u32(h2{l[2], l[3]})};
+    }
+    return shift;
+}
+
+// The joined sums of many rows in the workspace.
+struct Joined {
+    _Float16 *hi, *lo;                             // [part][T][padded]
+    float* factor;                                 // [part][T]: scale 2^-shift (0: no adapter)
+};
+__device__ __forceinline__ Joined joined_of(const LoraArgs& a, const LoraPlan& p, float* ws) {
+    Joined j;
+    const int64_t n = (int64_t)a.parts * a.T * p.padded;
+    j.hi = (_Float16*)(ws + p.joined);
+    j.lo = j.hi + n;
+    j.factor = (float*)(j.lo + n);
+    return j;
+}
+
+// Sixteen lanes a row; grid y: part.
+constexpr int kJoinRows = 16;
+__global__ __launch_bounds__(16 * kJoinRows) void k_lora_join(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    const int64_t t = (int64_t)blockIdx.x * kJoinRows + threadIdx.x / 16;
+    if (t >= a.T) return;
+    const int part = blockIdx.y, me = threadIdx.x % 16;
+    int id = a.ids[t];
+    if (id < 0 || id >= a.adapters) id = -1;
+    const int ranks = ranks_of(a, id);
+    const Joined j = joined_of(a, p, ws);
+    const int64_t row = (int64_t)part * a.T + t;
+    const int shift = split_row<16>(ws + ((int64_t)part * p.pieces * a.T + t) * a.rank, (int64_t)a.T * a.rank, p.pieces, ranks, me,
+                                    p.padded, j.hi + row * p.padded, j.lo + row * p.padded);
+    if (me == 0) j.factor[row] = id < 0 ? 0.f : __builtin_ldexpf(a.scales ? a.scales[id] : 1.f, -shift);
+}
+
+// Four neighbouring columns of a row, n of them inside, as they are held.
+template <bool F16> struct Held {
+    typedef f4 type;
+};
+template <> struct Held<true> {
+    typedef uint2 type;
+};
+template <bool F16> __device__ __forceinline__ typename Held<F16>::type load_c(const LoraArgs& a, int64_t i, int n) {
+    typename Held<F16>::type c = {};
+    if constexpr (F16) {
+        const uint16_t* const p = (const uint16_t*)a.C + i;
+        if (a.wide && n >= 4) c = *(const uint2*)p;
+        else {
+            if (n > 0) c.x = p[0];
+            if (n > 1) c.x |= (uint32_t)p[1] << 16;
+            if (n > 2) c.y = p[2];
+            if (n > 3) c.y |= (uint32_t)p[3] << 16;
         }
     } else {
+        const float* const p = (const float*)a.C + i;
+        if (a.wide && n >= 4) c = *(const f4*)p;
+        else {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            if (e >= n) break;
-            const float v = f * d[e >> 2][e & 3];
-            if (a.out_f16) ((_Float16*)a.Y)[yi + e] = (_Float16)((float)((const _Float16*)a.C)[ci + e] + v);
-            else ((float*)a.Y)[yi + e] = ((const float*)a.C)[ci + e] + v;
+            for (int e = 0; e < 4; e++)
+                if (e < n) c[e] = p[e];
         }
     }
+    return c;
 }
-
-__device__ __forceinline__ void copy16(const LoraArgs& a, int64_t ci, int64_t yi, int n) {
-    if (a.wide && n >= 16) {
-        const int size = a.out_f16 ? 2 : 4;
-        for (int i = 0; i < size; i++) ((u4*)((char*)a.Y + yi * size))[i] = ((const u4*)((const char*)a.C + ci * size))[i];
+template <bool F16> __device__ __forceinline__ void store_y(const LoraArgs& a, int64_t i, typename Held<F16>::type y, int n) {
+    if constexpr (F16) {
+        uint16_t* const p = (uint16_t*)a.Y + i;
+        if (a.wide && n >= 4) *(uint2*)p = y;
+        else {
+            if (n > 0) p[0] = (uint16_t)y.x;
+            if (n > 1) p[1] = (uint16_t)(y.x >> 16);
+            if (n > 2) p[2] = (uint16_t)y.y;
+            if (n > 3) p[3] = (uint16_t)(y.y >> 16);
+        }
     } else {
-        for (int e = 0; e < min(n, 16); e++) {
-            if (a.out_f16) ((uint16_t*)a.Y)[yi + e] = ((const uint16_t*)a.C)[ci + e];
-            else ((uint32_t*)a.Y)[yi + e] = ((const uint32_t*)a.C)[ci + e];
+        float* const p = (float*)a.Y + i;
+        if (a.wide && n >= 4) *(f4*)p = y;
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < n) p[e] = y[e];
         }
     }
 }
+// c + f d
+__device__ __forceinline__ f4 add(f4 c, float f, f4 d) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) c[e] = __builtin_fmaf(f, d[e], c[e]);
+    return c;
+}
+__device__ __forceinline__ uint2 add(uint2 c, float f, f4 d) {
+    const h2 lo = as_h2(c.x), hi = as_h2(c.y);
+    const f4 y = add(f4{(float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]}, f, d);
+    return uint2{as_u32(h2{(_Float16)y[0], (_Float16)y[1]}), as_u32(h2{(_Float16)y[2], (_Float16)y[3]})};
+}
 
-// Grid: tile (the fastest), steps of columns of the parts.
-template <int SUBS>
-__global__ __launch_bounds__(64 * kLoraUpWaves) void k_lora_up(LoraArgs a, LoraPlan p, const float* __restrict__ ws) {
-    constexpr int ROWS = kLoraSub * SUBS, NTH = 64 * kLoraUpWaves, PER = NTH / ROWS;   // threads a row of sums
-    constexpr int HELD = 2;                        // fours of sums that a thread keeps
-    extern __shared__ __attribute__((aligned(16))) _Float16 sums[];        // [hi, lo][ROWS][ld]
-    __shared__ float factor[ROWS];
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tile = blockIdx.x % p.tiles;
-    int at = blockIdx.x / p.tiles, part = 0;
+// 16 neighbouring bytes of a row, n of their elements inside.
+template <bool F16> struct Run {
+    typedef f4 type;
+};
+template <> struct Run<true> {
+    typedef u4 type;
+};
+template <bool F16> __device__ __forceinline__ typename Run<F16>::type load_run(const LoraArgs& a, int64_t i, int n) {
+    typename Run<F16>::type c = {};
+    if constexpr (F16) {
+        const uint16_t* const p = (const uint16_t*)a.C + i;
+        if (a.wide && n >= 8) c = *(const u4*)p;
+        else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < n) c[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+        }
+        return c;
+    } else {
+        return load_c<false>(a, i, n);
+    }
+}
+template <bool F16> __device__ __forceinline__ void store_run(const LoraArgs& a, int64_t i, typename Run<F16>::type y, int n) {
+    if constexpr (F16) {
+        uint16_t* const p = (uint16_t*)a.Y + i;
+        if (a.wide && n >= 8) *(u4*)p = y;
+        else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < n) p[e] = (uint16_t)(y[e >> 1] >> (16 * (e & 1)));
+        }
+    } else {
+        store_y<false>(a, i, y, n);
+    }
+}
+__device__ __forceinline__ f4 add_run(f4 c, float f, const float (&d)[4]) { return add(c, f, f4{d[0], d[1], d[2], d[3]}); }
+__device__ __forceinline__ u4 add_run(u4 c, float f, const float (&d)[8]) {
+    const uint2 lo = add(uint2{c.x, c.y}, f, f4{d[0], d[1], d[2], d[3]}), hi = add(uint2{c.z, c.w}, f, f4{d[4], d[5], d[6], d[7]});
+    return u4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// Step `at` of the parts' columns, `steps` operands' blocks of 64 each.
+__device__ __forceinline__ int part_of(const LoraArgs& a, int steps, int& at) {
+    int part = 0;
     for (; part < a.parts - 1; part++) {
-        const int n = ((a.part[part].N + kLoraCols - 1) / kLoraCols + p.up_steps - 1) / p.up_steps;
+        const int n = ((a.part[part].N + kLoraCols - 1) / kLoraCols + steps - 1) / steps;
         if (at < n) break;
         at -= n;
     }
+    return part;
+}
+
+// A block of B in LDS, columns of RC ranks: the place of a column's piece of eight ranks, such that neighbouring lanes, which
+// read columns 2^SH apart, meet different banks.
+template <int RC, int SH> __device__ __forceinline__ int place(int col, int piece) { return piece ^ ((col >> SH) & (RC / 8 - 1)); }
+// Column c's ranks k0 + k .. of a block that holds k0 .., of which `ranks` count (what lies past them may be anything).
+template <int RC, int SH> __device__ __forceinline__ h8 block_at(const uint8_t* block, int c, int k0, int k, int ranks) {
+    h8 b = *(const h8*)(block + 2 * RC * c + 16 * place<RC, SH>(c, (k / 8) & (RC / 8 - 1)));
+    if (k0 + (k & ~31) + 32 > ranks || RC < 32)
+#pragma unroll
+        for (int i = 0; i < 8; i++) b[i] = k < RC && k0 + k + i < ranks ? b[i] : (_Float16)0.f;
+    return b;
+}
+
+// Few rows.  RC: ranks of B that come to LDS at once.
+template <int RC, int WV, bool F16>
+__global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, const float* __restrict__ ws) {
+    constexpr int ROWS = kLoraSub, PER = 64 * WV / ROWS < 64 ? 64 * WV / ROWS : 64;   // lanes a row of sums
+    constexpr int PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * kLoraCols * RC;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // a block of B a wave, then the sums: fp16 [hi, lo][ROWS][ld]
+    __shared__ f4 factor4[ROWS / 4];
+    float* const factor = (float*)factor4;
+    _Float16* const sums = (_Float16*)(lds + WV * BYTES);
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tile, at;
+    if (!place_of(p.up, tile, at)) return;
+    const int part = part_of(a, p.up_steps, at);
     const LoraPart& w = a.part[part];
     const int n0 = at * p.up_steps * kLoraCols, n1 = min(w.N, n0 + p.up_steps * kLoraCols);
     const int64_t t0 = (int64_t)tile * ROWS;
-    const int id = adapter_of(a, t0, ROWS, lane);
-    const int ld = lora_lds_ranks(a.rank), ranks32 = ld - 8;
+    const int id = adapter_of(a, t0, ROWS, lane), rk = ranks_of(a, id);
+    const float sc = id < 0 ? 0.f : a.scales ? a.scales[id] : 1.f;
+    const int ld = lora_lds_ranks(a.rank), padded = ld - 8;
 
-    // s of row tid / PER, fours of ranks in turn: the pieces' sums, as two fp16 numbers times 2^shift
-    {
-        const int row = tid / PER, e = row < 64 ? __shfl(id, row) : -2;
-        const int ranks = e >= 0 ? rank_of(a, e) : 0;
-        const float* const s0 = ws + ((int64_t)part * p.pieces * a.T + t0 + row) * a.rank;
-        auto sum = [&](int k) {
-            f4 s = f4{0.f, 0.f, 0.f, 0.f};
-            if (k < ranks) {
-                for (int i = 0; i < p.pieces; i++) s += *(const f4*)(s0 + (int64_t)i * a.T * a.rank + k);
-#pragma unroll
-                for (int j = 1; j < 4; j++)
-                    if (k + j >= ranks) s[j] = 0.f;
+    // The wave's pairs of adapter and step, in turn
+    uint64_t left = __ballot(id != -2), rows = 0;
+    int nth = -1, n = n1, e = -1, ranks = 0;
+    auto next = [&]() -> bool {
+        for (;;) {
+            n += kLoraCols;
+            if (n >= n1) {
+                if (!left) return false;
+                const int first = __builtin_ctzll(left);
+                e = __builtin_amdgcn_readlane(id, first);
+                ranks = __builtin_amdgcn_readlane(rk, first);
+                rows = __ballot(id == e);
+                left &= ~rows;
+                n = n0;
             }
-            return s;
-        };
-        f4 held[HELD];
-        float top = 0.f;
-        for (int i = 0, k = 4 * (tid % PER); k < ranks32; k += 4 * PER, i++) {
-            const f4 s = sum(k);
-            if (i == 0) held[0] = s;
-            if (i == 1) held[1] = s;
-#pragma unroll
-            for (int j = 0; j < 4; j++) top = __builtin_fmaxf(top, __builtin_fabsf(s[j]));
+            if (++nth % WV == wave) return true;
         }
+    };
+    // Columns n .. n + 63, ranks k0 .. k0 + RC - 1 of B
+    const uint8_t* const block = lds + wave * BYTES;
+    auto fetch = [&](int k0) {
+        const uint16_t* const B = w.B + (int64_t)e * w.N * a.rank;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // what was read there has been read
 #pragma unroll
-        for (int x = 1; x < PER; x <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
-        // (s is a sum of products of fp16 numbers, a multiple of 2^-48: the shift is at most 63)
-        const int shift = top > 0.f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-        const float up = __builtin_ldexpf(1.f, shift);
-        if (tid % PER == 0) factor[row] = ranks > 0 ? __builtin_ldexpf(a.scales ? a.scales[e] : 1.f, -shift) : 0.f;
-        for (int i = 0, k = 4 * (tid % PER); k < ranks32; k += 4 * PER, i++) {
-            const f4 s = i == 0 ? held[0] : i == 1 ? held[1] : sum(k);
-            _Float16 hi[4], lo[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float v = s[j] * up;
-                hi[j] = (_Float16)v;
-                lo[j] = (_Float16)(v - (float)hi[j]);
-            }
-            _Float16* const to = sums + row * ld + k;
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                *(h2*)(to + j) = h2{hi[j], hi[j + 1]};
-                *(h2*)(to + ROWS * ld + j) = h2{lo[j], lo[j + 1]};
-            }
+        for (int i = 0; i < PIECES; i++) {
+            const int q = 64 * i + lane, col = q / PIECES, k = k0 + 8 * place<RC, 2>(col, q % PIECES);
+            dma16(B + (int64_t)min(n + col, w.N - 1) * a.rank + min(k, a.rank - 8), lds_addr(block) + 1024 * i);
         }
+    };
+    // ... and what it adds to: columns n + 4 r .. of rows 4 g + i
+    typename Held<F16>::type cnext[4];
+    auto start = [&]() -> bool {
+        if (!next()) return false;
+        const int col = n + 4 * r;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            cnext[i] = load_c<F16>(a, (t0 + 4 * g + i) * a.ldc + w.at + col, (rows >> (4 * g + i)) & 1 ? n1 - col : 0);
+        if (ranks > 0) fetch(0);
+        return true;
+    };
+    bool more = start();
+
+    if (tid < PER * ROWS) {                        // (whole waves)
+        const int row = tid / PER, mr = __shfl(rk, row);
+        const float scale = __shfl(sc, row);
+        const int shift = split_row<PER>(ws + ((int64_t)part * p.pieces * a.T + t0 + row) * a.rank, (int64_t)a.T * a.rank, p.pieces, mr,
+                                         tid % PER, padded, sums + row * ld, sums + (ROWS + row) * ld);
+        if (tid % PER == 0) factor[row] = __builtin_ldexpf(scale, -shift);
     }
     __syncthreads();
 
-    int nth = 0;                                   // pairs of adapter and step
-    for (uint64_t left = __ballot(id != -2); left;) {
-        const int e = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const uint64_t rows = __ballot(id == e);
-        left &= ~rows;
-        const int ranks = e < 0 ? 0 : rank_of(a, e);
-        const uint16_t* const B = ranks > 0 ? w.B + (int64_t)e * w.N * a.rank : nullptr;
-        for (int n = n0; n < n1; n += kLoraCols, nth++) {
-            if (nth % kLoraUpWaves != wave) continue;
-            const int first = n + 16 * g, inside = n1 - first;             // the lane's columns
-            f4 acc[SUBS][4];
+    while (more) {
+        // this pair; the next one's block comes while this one's products run
+        const int cn = n, cr = ranks;
+        const uint64_t crows = rows;
+        const int col = cn + 4 * r, inside = n1 - col;                     // the lane's four columns, of rows 4 g + i
+        typename Held<F16>::type c[4];
 #pragma unroll
-            for (int b = 0; b < SUBS; b++)
+        for (int i = 0; i < 4; i++) c[i] = cnext[i];
+        f4 acc[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[b][j] = f4{0.f, 0.f, 0.f, 0.f};
-            for (int k0 = 0; k0 < ranks; k0 += kLoraStep) {
-                const int k = k0 + 8 * g;
-                h8 bv[4];
-                // column n + 16 (i / 4) + 4 j + i % 4 is row i of operand j: a lane's sums are of 16 neighbouring columns
+        for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < cr; k0 += RC) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            h8 bv[KS][4];
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) bv[s][j] = block_at<RC, 2>(block, 4 * r + j, k0, 32 * s + 8 * g, cr);   // operand j: columns 4 i + j
+            if (k0 + RC < cr) fetch(k0 + RC);
+            else more = start();
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                if (k0 + 32 * s >= cr) break;
+                const _Float16* const v = sums + r * ld + k0 + 32 * s + 8 * g;
+                const h8 hi = *(const h8*)v, lo = *(const h8*)(v + ROWS * ld);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int col = min(n + 16 * (r >> 2) + 4 * j + (r & 3), w.N - 1);
-                    bv[j] = *(const h8*)(B + (int64_t)col * a.rank + min(k, a.rank - 8));
-                }
-                if (k0 + kLoraStep > ranks) {      // what lies past the rank may be anything
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) bv[j][i] = k + i < ranks ? bv[j][i] : (_Float16)0.f;
-                }
-#pragma unroll
-                for (int b = 0; b < SUBS; b++) {
-                    if (!((rows >> (16 * b)) & 0xFFFFu)) continue;
-                    const _Float16* const s = sums + (16 * b + r) * ld + k;
-                    const h8 hi = *(const h8*)s, lo = *(const h8*)(s + ROWS * ld);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        acc[b][j] = mfma16x16x32(bv[j], hi, acc[b][j]);
-                        acc[b][j] = mfma16x16x32(bv[j], lo, acc[b][j]);
-                    }
+                    acc[j] = mfma16x16x32(hi, bv[s][j], acc[j]);
+                    acc[j] = mfma16x16x32(lo, bv[s][j], acc[j]);
                 }
             }
-            if (inside <= 0) continue;
+        }
+        if (cr == 0) more = start();
+        if (cr == 0 && a.Y == a.C) continue;       // (no adapter, in place)
+        const f4 f = factor4[g];
 #pragma unroll
-            for (int b = 0; b < SUBS; b++) {
-                if (!((rows >> (16 * b + r)) & 1)) continue;
-                const int64_t row = t0 + 16 * b + r, ci = row * a.ldc + w.at + first, yi = row * a.ldy + w.at + first;
-                if (ranks > 0) add16(a, ci, yi, acc[b], factor[16 * b + r], inside);
-                else if (a.Y != a.C) copy16(a, ci, yi, inside);
-            }
+        for (int i = 0; i < 4; i++) {
+            if (cr > 0) c[i] = add(c[i], f[i], f4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]});   // (no adapter: a copy, through no arithmetic)
+            store_y<F16>(a, (t0 + 4 * g + i) * a.ldy + w.at + col, c[i], (crows >> (4 * g + i)) & 1 ? inside : 0);
         }
     }
 }
 
-template <int SUBS, int NT> void down(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
-    constexpr int WV = SUBS == 1 ? 8 : 4;
-    const dim3 grid((unsigned)(p.tiles * (int64_t)p.sharers), (unsigned)p.pieces, (unsigned)(a.parts * p.rank_parts));
-    hipLaunchKernelGGL((k_lora_down<SUBS, NT, WV>), grid, dim3(64 * WV), 0, st, a, p, ws);
+// Many rows: wave w takes rows 16 (w % 4) .. and columns 128 (w / 4) .. of 64 by 256.
+// Operand j of its eight holds the columns that leave a lane 16 neighbouring bytes
+// of a row of C (8 i + j in fp16, 64 (j / 4) + 4 i + j % 4 in fp32), so that a wave
+// reads and writes runs of 256 bytes.  Everything it needs is on its way at once; a
+// tile of several adapters takes them in turn.
+template <int RC, bool F16>
+__global__ __launch_bounds__(64 * kLoraManyWaves, 4) void k_lora_up_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    constexpr int WV = kLoraManyWaves, ROWS = 64, COLS = 128, PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * COLS * RC;
+    constexpr int SH = F16 ? 3 : 2, PER = F16 ? 1 : 2, W = F16 ? 8 : 4;    // runs of a lane in a row, their columns
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BYTES + 2 * 2 * ROWS * RC];   // two blocks of B, the sums' hi and lo
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), sub = wave & 3;
+    int tile, at;
+    if (!place_of(p.up, tile, at)) return;
+    const int part = part_of(a, p.up_steps, at);
+    const LoraPart& w = a.part[part];
+    const int n = at * p.up_steps * kLoraCols + COLS * (wave >> 2), col = n + W * r;         // (the lane's second run: col + 64)
+    const int64_t t0 = (int64_t)tile * ROWS;
+    const int id = adapter_of(a, t0, ROWS, lane), rk = ranks_of(a, id);
+    const Joined sums = joined_of(a, p, ws);
+    uint8_t* const block = lds + (wave >> 2) * BYTES;
+    uint8_t* const rows_lds = lds + 2 * BYTES;                             // [hi, lo][64 rows][RC]
+
+    // the wave's quarter of its block: ranks k0 .. of adapter e
+    auto fetch_b = [&](int e, int k0) {
+        const uint16_t* const B = w.B + (int64_t)e * w.N * a.rank;
+#pragma unroll
+        for (int i = 0; i < PIECES / 2; i++) {
+            const int m = 4 * i + sub, q = 64 * m + lane, c = q / PIECES, k = k0 + 8 * place<RC, SH>(c, q % PIECES);
+            dma16(B + (int64_t)min(n + c, w.N - 1) * a.rank + min(k, a.rank - 8), lds_addr(block) + 1024 * m);
+        }
+    };
+    // the wave's share of the rows' sums
+    auto fetch_s = [&](int k0) {
+        constexpr int LOADS = 2 * PIECES;          // (of both planes)
+#pragma unroll
+        for (int i = 0; i < (LOADS + WV - 1) / WV; i++) {
+            const int m = WV * i + wave;
+            if (m >= LOADS) break;
+            const int q = 64 * (m % PIECES) + lane, row = q / PIECES, k = k0 + 8 * place<RC, 0>(row, q % PIECES);
+            const _Float16* const s = (m < PIECES ? sums.hi : sums.lo) + ((int64_t)part * a.T + min(t0 + row, (int64_t)a.T - 1)) * p.padded;
+            dma16(s + k, lds_addr(rows_lds) + 1024 * m);
+        }
+    };
+    uint64_t left = __ballot(id != -2), rows = 0;
+    int e = -1, ranks = 0;
+    auto next = [&]() {
+        const int first = __builtin_ctzll(left);
+        e = __builtin_amdgcn_readlane(id, first);
+        ranks = __builtin_amdgcn_readlane(rk, first);
+        rows = __ballot(id == e);
+        left &= ~rows;
+    };
+    next();
+    if (ranks > 0) {
+        fetch_b(e, 0);
+        fetch_s(0);
+    }
+    // the lane's rows 4 g + i: what is added to, and the factors
+    const int64_t lt = t0 + 16 * sub + 4 * g;
+    typename Run<F16>::type c[4][PER];
+    f4 f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int h = 0; h < PER; h++)
+            c[i][h] = load_run<F16>(a, (lt + i) * a.ldc + w.at + col + 64 * h, lt + i < a.T ? w.N - col - 64 * h : 0);
+        f[i] = sums.factor[(int64_t)part * a.T + min(lt + i, (int64_t)a.T - 1)];
+    }
+    bool held = ranks > 0;                         // the sums in LDS are of ranks 0 ..
+    for (;;) {
+        f4 acc[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+        const bool mine = (rows >> (16 * sub)) & 0xFFFFu;
+        for (int k0 = 0; k0 < ranks; k0 += RC) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (mine) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    if (k0 + 32 * s >= ranks) break;
+                    const int row = 16 * sub + r, k = 32 * s + 8 * g;
+                    h8 v[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        v[h] = *(const h8*)(rows_lds + (h * ROWS + row) * (2 * RC) + 16 * place<RC, 0>(row, (k / 8) & (PIECES - 1)));
+                        if (RC < 32) v[h] = masked(v[h], k < RC);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const h8 b = block_at<RC, SH>(block, F16 ? 8 * r + j : 64 * (j >> 2) + 4 * r + (j & 3), k0, k, ranks);
+                        acc[j] = mfma16x16x32(v[0], b, acc[j]);
+                        acc[j] = mfma16x16x32(v[1], b, acc[j]);
+                    }
+                }
+            }
+            if (k0 + RC < ranks) {
+                __syncthreads();                   // the blocks have been read
+                fetch_b(e, k0 + RC);
+                fetch_s(k0 + RC);
+                held = false;
+            }
+        }
+        if (mine && (ranks > 0 || a.Y != a.C)) {   // (no adapter: a copy, through no arithmetic)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int h = 0; h < PER; h++) {
+                    typename Run<F16>::type y = c[i][h];
+                    if (ranks > 0) {
+                        float d[W];
+#pragma unroll
+                        for (int j = 0; j < W; j++) d[j] = acc[4 * h + j][i];
+                        y = add_run(y, f[i], d);
+                    }
+                    const bool in = (rows >> (16 * sub + 4 * g + i)) & 1;
+                    store_run<F16>(a, (lt + i) * a.ldy + w.at + col + 64 * h, y, in ? w.N - col - 64 * h : 0);
+                }
+        }
+        if (!left) return;
+        next();
+        if (ranks > 0) {
+            __syncthreads();                       // the blocks have been read
+            fetch_b(e, 0);
+            if (!held) fetch_s(0);
+            held = true;
+        }
+    }
 }
 
-template <int SUBS> hipError_t go(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
-    auto k = k_lora_up<SUBS>;
-    const size_t lds = (size_t)4 * kLoraSub * SUBS * lora_lds_ranks(a.rank);
-    static std::atomic<uint64_t> attr_set{0};      // one bit per device: LDS limit raised
+template <class K> hipError_t raise_lds(K k, std::atomic<uint64_t>& set, int bytes) {
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
-    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
-        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                4 * kLoraSub * SUBS * lora_lds_ranks(SUBS == 1 ? kLoraMaxRank : 256));
-        if (e != hipSuccess) return e;
-        attr_set.fetch_or(bit, std::memory_order_acq_rel);
-    }
-    if (p.rank_tiles == 1) down<SUBS, 1>(a, p, ws, st);
-    else if (p.rank_tiles == 2) down<SUBS, 2>(a, p, ws, st);
-    else down<SUBS, 4>(a, p, ws, st);
-    e = hipGetLastError();
+    if (set.load(std::memory_order_acquire) & bit) return hipSuccess;
+    e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) set.fetch_or(bit, std::memory_order_acq_rel);
+    return e;
+}
+
+template <int NT> hipError_t down(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
+    constexpr int few = kLoraDownWaves * 2 * kUnitBytes<NT>, many = 2 * kLoraSlab / kLoraUnit * NT * 2048;
+    static std::atomic<uint64_t> set{0}, set_many{0};                      // one bit per device: LDS limit raised
+    auto k = p.many ? k_lora_down_many<NT> : k_lora_down<NT>;
+    const int lds = p.many ? many : few;
+    const hipError_t e = raise_lds(k, p.many ? set_many : set, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, dim3((unsigned)p.up_groups), dim3(64 * kLoraUpWaves), lds, st, a, p, ws);
+    hipLaunchKernelGGL(k, dim3((unsigned)p.down.groups), dim3(64 * kLoraDownWaves), lds, st, a, p, ws);
     return hipGetLastError();
+}
+
+template <int RC, int WV, bool F16> hipError_t up(const LoraArgs& a, const LoraPlan& p, const float* ws, hipStream_t st) {
+    constexpr int blocks = WV * 2 * kLoraCols * RC;
+    const auto sums = [](int rank) { return 4 * kLoraSub * lora_lds_ranks(rank); };
+    static std::atomic<uint64_t> set{0};
+    auto k = k_lora_up<RC, WV, F16>;
+    const hipError_t e = raise_lds(k, set, blocks + sums(RC < 64 ? RC : WV == 8 ? kLoraMaxRank : 256));
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k, dim3((unsigned)p.up.groups), dim3(64 * WV), (size_t)(blocks + sums(a.rank)), st, a, p, ws);
+    return hipGetLastError();
+}
+
+template <int RC, bool F16> hipError_t up(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
+    if (!p.many) return p.up_waves == 16 ? up<RC, 16, F16>(a, p, ws, st) : up<RC, 8, F16>(a, p, ws, st);
+    hipLaunchKernelGGL(k_lora_join, dim3((unsigned)((a.T + kJoinRows - 1) / kJoinRows), (unsigned)a.parts), dim3(16 * kJoinRows), 0, st, a, p, ws);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_lora_up_many<RC, F16>), dim3((unsigned)p.up.groups), dim3(64 * kLoraManyWaves), 0, st, a, p, ws);
+    return hipGetLastError();
+}
+
+template <int RC> hipError_t both(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
+    const hipError_t e = down<RC / 16>(a, p, ws, st);
+    if (e != hipSuccess) return e;
+    return a.out_f16 ? up<RC, true>(a, p, ws, st) : up<RC, false>(a, p, ws, st);
 }
 
 LoraPlan plan_of(const LoraArgs& a) { return plan_lora(a, device_cus() > 0 ? device_cus() : 256); }
@@ -346,14 +787,18 @@ LoraPlan plan_of(const LoraArgs& a) { return plan_lora(a, device_cus() > 0 ? dev
 
 bool lora_fits(const LoraArgs& a) {
     const LoraPlan p = plan_of(a);
-    return launch_fits(p.tiles * (int64_t)p.sharers, 64 * p.down_waves) && launch_fits(p.up_groups, 64 * kLoraUpWaves);
+    return launch_fits(p.down.groups, 64 * kLoraDownWaves) && launch_fits(p.up.groups, 64 * p.up_waves) && launch_fits(a.T, 16);
 }
 
 size_t lora_scratch_bytes(const LoraArgs& a) { return plan_of(a).bytes; }
 
 hipError_t lora(const LoraArgs& a, float* ws, hipStream_t st) {
     const LoraPlan p = plan_of(a);
-    return p.subs == 1 ? go<1>(a, p, ws, st) : go<4>(a, p, ws, st);
+    switch (lora_block(a.rank)) {
+        case 16: return both<16>(a, p, ws, st);
+        case 32: return both<32>(a, p, ws, st);
+        default: return both<64>(a, p, ws, st);
+    }
 }
 
 }  // namespace bf
