@@ -488,9 +488,9 @@ template <int RC, int SH> __device__ __forceinline__ h8 block_at(const uint8_t* 
 }
 
 // Few rows.  RC: ranks of B that come to LDS at once.
-template <int RC, int WV, bool F16>
-__global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, const float* __restrict__ ws) {
-    constexpr int ROWS = kLoraSub, PER = 64 * WV / ROWS < 64 ? 64 * WV / ROWS : 64;   // lanes a row of sums
+template <int RC, bool F16>
+__global__ __launch_bounds__(64 * kLoraUpWaves) void k_lora_up(LoraArgs a, LoraPlan p, const float* __restrict__ ws) {
+    constexpr int ROWS = kLoraSub, WV = kLoraUpWaves, PER = 64 * WV / ROWS;   // lanes a row of sums
     constexpr int PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * kLoraCols * RC;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // a block of B a wave, then the sums: fp16 [hi, lo][ROWS][ld]
     __shared__ f4 factor4[ROWS / 4];
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, con
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
             const int q = 64 * i + lane, col = q / PIECES, k = k0 + 8 * place<RC, 2>(col, q % PIECES);
-            dma16(B + (int64_t)min(n + col, w.N - 1) * a.rank + min(k, a.rank - 8), lds_addr(block) + 1024 * i);
+            if (k < ranks) dma16(B + (int64_t)min(n + col, w.N - 1) * a.rank + k, lds_addr(block) + 1024 * i);
         }
     };
     // ... and what it adds to: columns n + 4 r .. of rows 4 g + i
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, con
     };
     bool more = start();
 
-    if (tid < PER * ROWS) {                        // (whole waves)
+    {
         const int row = tid / PER, mr = __shfl(rk, row);
         const float scale = __shfl(sc, row);
         const int shift = split_row<PER>(ws + ((int64_t)part * p.pieces * a.T + t0 + row) * a.rank, (int64_t)a.T * a.rank, p.pieces, mr,
@@ -572,13 +572,6 @@ __global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, con
         for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
         for (int k0 = 0; k0 < cr; k0 += RC) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            h8 bv[KS][4];
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) bv[s][j] = block_at<RC, 2>(block, 4 * r + j, k0, 32 * s + 8 * g, cr);   // operand j: columns 4 i + j
-            if (k0 + RC < cr) fetch(k0 + RC);
-            else more = start();
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 if (k0 + 32 * s >= cr) break;
@@ -586,10 +579,13 @@ __global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, con
                 const h8 hi = *(const h8*)v, lo = *(const h8*)(v + ROWS * ld);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    acc[j] = mfma16x16x32(hi, bv[s][j], acc[j]);
-                    acc[j] = mfma16x16x32(lo, bv[s][j], acc[j]);
+                    const h8 b = block_at<RC, 2>(block, 4 * r + j, k0, 32 * s + 8 * g, cr);   // operand j: columns 4 i + j
+                    acc[j] = mfma16x16x32(hi, b, acc[j]);
+                    acc[j] = mfma16x16x32(lo, b, acc[j]);
                 }
             }
+            if (k0 + RC < cr) fetch(k0 + RC);
+            else more = start();
         }
         if (cr == 0) more = start();
         if (cr == 0 && a.Y == a.C) continue;       // (no adapter, in place)
@@ -608,8 +604,8 @@ __global__ __launch_bounds__(64 * WV) void k_lora_up(LoraArgs a, LoraPlan p, con
 // reads and writes runs of 256 bytes.  Everything it needs is on its way at once; a
 // tile of several adapters takes them in turn.
 template <int RC, bool F16>
-__global__ __launch_bounds__(64 * kLoraManyWaves, 4) void k_lora_up_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
-    constexpr int WV = kLoraManyWaves, ROWS = 64, COLS = 128, PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * COLS * RC;
+__global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    constexpr int WV = kLoraUpWaves, ROWS = 64, COLS = 128, PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * COLS * RC;
     constexpr int SH = F16 ? 3 : 2, PER = F16 ? 1 : 2, W = F16 ? 8 : 4;    // runs of a lane in a row, their columns
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BYTES + 2 * 2 * ROWS * RC];   // two blocks of B, the sums' hi and lo
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -625,13 +621,13 @@ __global__ __launch_bounds__(64 * kLoraManyWaves, 4) void k_lora_up_many(LoraArg
     uint8_t* const block = lds + (wave >> 2) * BYTES;
     uint8_t* const rows_lds = lds + 2 * BYTES;                             // [hi, lo][64 rows][RC]
 
-    // the wave's quarter of its block: ranks k0 .. of adapter e
-    auto fetch_b = [&](int e, int k0) {
+    // the wave's quarter of its block: ranks k0 .. of adapter e, as far as they count
+    auto fetch_b = [&](int e, int ranks, int k0) {
         const uint16_t* const B = w.B + (int64_t)e * w.N * a.rank;
 #pragma unroll
         for (int i = 0; i < PIECES / 2; i++) {
             const int m = 4 * i + sub, q = 64 * m + lane, c = q / PIECES, k = k0 + 8 * place<RC, SH>(c, q % PIECES);
-            dma16(B + (int64_t)min(n + c, w.N - 1) * a.rank + min(k, a.rank - 8), lds_addr(block) + 1024 * m);
+            if (k < ranks) dma16(B + (int64_t)min(n + c, w.N - 1) * a.rank + k, lds_addr(block) + 1024 * m);
         }
     };
     // the wave's share of the rows' sums
@@ -657,7 +653,7 @@ __global__ __launch_bounds__(64 * kLoraManyWaves, 4) void k_lora_up_many(LoraArg
     };
     next();
     if (ranks > 0) {
-        fetch_b(e, 0);
+        fetch_b(e, ranks, 0);
         fetch_s(0);
     }
     // the lane's rows 4 g + i: what is added to, and the factors
@@ -701,7 +697,7 @@ __global__ __launch_bounds__(64 * kLoraManyWaves, 4) void k_lora_up_many(LoraArg
             }
             if (k0 + RC < ranks) {
                 __syncthreads();                   // the blocks have been read
-                fetch_b(e, k0 + RC);
+                fetch_b(e, ranks, k0 + RC);
                 fetch_s(k0 + RC);
                 held = false;
             }
@@ -726,7 +722,7 @@ __global__ __launch_bounds__(64 * kLoraManyWaves, 4) void k_lora_up_many(LoraArg
         next();
         if (ranks > 0) {
             __syncthreads();                       // the blocks have been read
-            fetch_b(e, 0);
+            fetch_b(e, ranks, 0);
             if (!held) fetch_s(0);
             held = true;
         }
@@ -755,23 +751,23 @@ template <int NT> hipError_t down(const LoraArgs& a, const LoraPlan& p, float* w
     return hipGetLastError();
 }
 
-template <int RC, int WV, bool F16> hipError_t up(const LoraArgs& a, const LoraPlan& p, const float* ws, hipStream_t st) {
-    constexpr int blocks = WV * 2 * kLoraCols * RC;
+template <int RC, bool F16> hipError_t up_few(const LoraArgs& a, const LoraPlan& p, const float* ws, hipStream_t st) {
+    constexpr int WV = kLoraUpWaves, blocks = WV * 2 * kLoraCols * RC;
     const auto sums = [](int rank) { return 4 * kLoraSub * lora_lds_ranks(rank); };
     static std::atomic<uint64_t> set{0};
-    auto k = k_lora_up<RC, WV, F16>;
-    const hipError_t e = raise_lds(k, set, blocks + sums(RC < 64 ? RC : WV == 8 ? kLoraMaxRank : 256));
+    auto k = k_lora_up<RC, F16>;
+    const hipError_t e = raise_lds(k, set, blocks + sums(RC < 64 ? RC : kLoraMaxRank));
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k, dim3((unsigned)p.up.groups), dim3(64 * WV), (size_t)(blocks + sums(a.rank)), st, a, p, ws);
     return hipGetLastError();
 }
 
 template <int RC, bool F16> hipError_t up(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
-    if (!p.many) return p.up_waves == 16 ? up<RC, 16, F16>(a, p, ws, st) : up<RC, 8, F16>(a, p, ws, st);
+    if (!p.many) return up_few<RC, F16>(a, p, ws, st);
     hipLaunchKernelGGL(k_lora_join, dim3((unsigned)((a.T + kJoinRows - 1) / kJoinRows), (unsigned)a.parts), dim3(16 * kJoinRows), 0, st, a, p, ws);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_lora_up_many<RC, F16>), dim3((unsigned)p.up.groups), dim3(64 * kLoraManyWaves), 0, st, a, p, ws);
+    hipLaunchKernelGGL((k_lora_up_many<RC, F16>), dim3((unsigned)p.up.groups), dim3(64 * kLoraUpWaves), 0, st, a, p, ws);
     return hipGetLastError();
 }
 
@@ -787,7 +783,7 @@ LoraPlan plan_of(const LoraArgs& a) { return plan_lora(a, device_cus() > 0 ? dev
 
 bool lora_fits(const LoraArgs& a) {
     const LoraPlan p = plan_of(a);
-    return launch_fits(p.down.groups, 64 * kLoraDownWaves) && launch_fits(p.up.groups, 64 * p.up_waves) && launch_fits(a.T, 16);
+    return launch_fits(p.down.groups, 64 * kLoraDownWaves) && launch_fits(p.up.groups, 64 * kLoraUpWaves) && launch_fits(a.T, 16);
 }
 
 size_t lora_scratch_bytes(const LoraArgs& a) { return plan_of(a).bytes; }

@@ -20,7 +20,7 @@ constexpr int kLoraSlab = 320;                     // many rows: ... of A's rows
 constexpr int kLoraPieces = 8;                     // pieces of K at most
 constexpr int kLoraXcds = 8;                       // (a launch's workgroups go round them)
 constexpr int kLoraDownWaves = 4;
-constexpr int kLoraManyWaves = 8;                  // of the up products of many rows: 64 rows, four steps of columns
+constexpr int kLoraUpWaves = 8;                    // ... of the up products (many rows: of 64 rows and four steps of columns)
 
 struct LoraPart {
     const uint16_t* A;                             // [adapters][rank][K]
@@ -63,8 +63,7 @@ inline LoraGrid lora_grid(int tiles, int64_t inner) {
 // Few rows (tiles of 16): down, a workgroup takes a tile, a part, up to 64 ranks, a
 // piece of K (its waves shares of that) and every `sharers`-th of the tile's
 // adapters; up, a workgroup takes a tile, up_steps steps of 64 columns of a part and
-// all of the tile's adapters, its up_waves waves the pairs of adapter and step in
-// turn, and adds the pieces' sums first.  Many rows (tiles of 64): down, a tile, a
+// all of the tile's adapters, its waves the pairs of adapter and step in turn, and adds the pieces' sums first.  Many rows (tiles of 64): down, a tile, a
 // part, up to 64 ranks, and a piece of K; a join of the pieces; up, a tile and four
 // steps of columns.
 struct LoraPlan {
@@ -72,7 +71,7 @@ struct LoraPlan {
     int rank_parts, rank_tiles;                    // rank_tiles: operands of ranks of a down workgroup (1, 2 or 4)
     int padded;                                    // many: ranks of the joined sums, in whole blocks
     int pieces, sharers;
-    int up_steps, up_waves;
+    int up_steps;
     LoraGrid down, up;
     int64_t joined;                                // many: fp32 words of the partial sums, behind which the joined ones lie
     size_t bytes;                                  // [part][piece][T][rank] fp32; many: hi and lo [part][T][padded] fp16, [part][T] factors
@@ -98,9 +97,8 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
     p.down = lora_grid(t, (int64_t)p.rank_parts * a.parts * p.sharers * p.pieces);
     int64_t cols = 0;                              // steps of columns of all parts
     for (int i = 0; i < a.parts; i++) cols += (a.part[i].N + kLoraCols - 1) / kLoraCols;
-    // few: as many steps a workgroup as leave two workgroups a CU, a wave for each pair where that fits
+    // few: as many steps a workgroup as leave two workgroups a CU
     p.up_steps = p.many ? 4 : (int)std::min<int64_t>(16, std::max<int64_t>(1, (t * cols + 2 * cus - 1) / (2 * cus)));
-    p.up_waves = p.many ? kLoraManyWaves : per_tile * p.up_steps > 8 && a.rank <= 256 ? 16 : 8;
     int64_t groups = 0;
     for (int i = 0; i < a.parts; i++) {
         const int64_t n = (a.part[i].N + kLoraCols - 1) / kLoraCols;
