@@ -612,9 +612,17 @@ def kv4_append(cache: Kv4Cache, K, V, slots, positions, freq, T: int, *, Q=None,
     _check(lib().bf_kv4_append(ctypes.byref(cache), ctypes.byref(a), _stream(stream)), "bf_kv4_append")
 
 
+_dtypes = {}
+
+
 def _dtype(t) -> int:
-    import torch
-    return F32 if t is None else {torch.float32: F32, torch.float16: F16}[t.dtype]
+    """F32 or F16 of a tensor (of None: F32)."""
+    if t is None:
+        return F32
+    if not _dtypes:
+        import torch
+        _dtypes.update({torch.float32: F32, torch.float16: F16})
+    return _dtypes[t.dtype]
 
 
 def rms_norm(X, T: int, K: int, *, H=None, Aq=None, delta=None, R=None, weight=None, offset: float = 0.0, eps: float = 1e-6,

@@ -181,19 +181,22 @@ __global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down(LoraArgs a, L
     }
 }
 
-// Many rows: a wave takes 16 of 64 rows, whose x it keeps in registers; A's rows, a
-// slab of K at a time, two by turns, are in LDS for all four.
+// Many rows: a wave takes 16 of 64 rows and half of each slab of K; x comes to its
+// registers, A's rows, two slabs by turns, to LDS for all eight.  (Four waves with whole
+// slabs: 11.1 us for 2000 rows of 5120 and 64 ranks where this takes ....  LDS gives eight
+// waves 1.7 times what it gives four.)
 template <int NT>
-__global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
-    constexpr int WV = kLoraDownWaves, STEPS = kLoraSlab / kLoraStep, UNITS = kLoraSlab / kLoraUnit, BYTES = UNITS * NT * 2048;
+__global__ __launch_bounds__(64 * kLoraManyWaves) void k_lora_down_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    constexpr int WV = kLoraManyWaves, STEPS = kLoraSlab / kLoraStep / 2, UNITS = kLoraSlab / kLoraUnit, BYTES = UNITS * NT * 2048;
     constexpr int LOADS = UNITS * NT * 2;          // direct loads of a slab, eight rows of 128 bytes each: wave w does every WV-th
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // two slabs: [unit][operand][16 rows of 128 bytes]
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // two slabs, [unit][operand][16 rows of 128 bytes]; sums
+    f4 (*const meet)[NT][64] = (f4 (*)[NT][64])(lds + 2 * BYTES);          // [4], of the waves with the second halves
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, row = lane >> 3, piece = (lane & 7) ^ row;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), sub = wave & 3, half = wave >> 2;
     int tile, in;
     if (!place_of(p.down, tile, in)) return;
     const Share q = share_of(a, p, in);
-    const int64_t t0 = (int64_t)tile * (4 * kLoraSub), mine = t0 + 16 * wave + r;
+    const int64_t t0 = (int64_t)tile * (4 * kLoraSub), mine = t0 + 16 * sub + r;
     const int id = adapter_of(a, t0, 4 * kLoraSub, lane), rk = ranks_of(a, id);
     const int64_t units = (a.K + kLoraUnit - 1) / kLoraUnit;
     const int k0 = kLoraUnit * (int)(units * q.piece / p.pieces), k1 = min(a.K, kLoraUnit * (int)(units * (q.piece + 1) / p.pieces));
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down_many(LoraArgs
         o.k = k0;
         return true;
     };
-    auto mine_in = [&](const At& o) -> bool { return (o.rows >> (16 * wave)) & 0xFFFFu; };
+    auto mine_in = [&](const At& o) -> bool { return (o.rows >> (16 * sub)) & 0xFFFFu; };
     h8 xv[2][STEPS];
     // (the buffer's readers have passed a barrier)
     auto fetch = [&](const At& o, int buf, h8 (&v)[STEPS]) {
@@ -232,33 +235,45 @@ __global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down_many(LoraArgs
         }
         if (mine_in(o))
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) v[i] = *(const h8*)(x + min(o.k + kLoraStep * i + 8 * g, a.K - 8));
+            for (int i = 0; i < STEPS; i++) v[i] = *(const h8*)(x + min(o.k + kLoraStep * (STEPS * half + i) + 8 * g, a.K - 8));
     };
     f4 acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const At& o, int buf, const h8 (&v)[STEPS]) {
-        if (!mine_in(o)) return;
+        if (mine_in(o)) {
+            // A's operands are read a step ahead of their products
+            h8 w[2][NT];
+            auto read = [&](int i) {
+                const int n = STEPS * half + i;
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-            const int at = o.k + kLoraStep * i;
-            if (at >= k1) break;
-            const uint8_t* const unit = lds + buf * BYTES + (i >> 1) * (2048 * NT);
-            const bool off = at + kLoraStep > k1, ok = at + 8 * g < k1;
-            const h8 b = off ? masked(v[i], ok) : v[i];
+                for (int m = 0; m < NT; m++)
+                    w[i & 1][m] = piece_of(lds + buf * BYTES + (n >> 1) * (2048 * NT), m, r, 4 * (n & 1) + g);
+            };
+            read(0);
 #pragma unroll
-            for (int m = 0; m < NT; m++) {
-                h8 w = piece_of(unit, m, r, 4 * (i & 1) + g);
-                if (off) w = masked(w, ok);
-                acc[m] = mfma16x16x32(w, b, acc[m]);
+            for (int i = 0; i < STEPS; i++) {
+                const int at = o.k + kLoraStep * (STEPS * half + i);
+                if (at >= k1) break;
+                if (i + 1 < STEPS) read(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                const bool off = at + kLoraStep > k1, ok = at + 8 * g < k1;
+                const h8 b = off ? masked(v[i], ok) : v[i];
+#pragma unroll
+                for (int m = 0; m < NT; m++) acc[m] = mfma16x16x32(off ? masked(w[i & 1][m], ok) : w[i & 1][m], b, acc[m]);
             }
         }
         if (o.k + kLoraSlab < k1) return;
+        // the adapter's last slab (what was here last has been read before this turn's barrier)
+        if (half)
 #pragma unroll
-        for (int i = 0; i < NT; i++) {             // the adapter's last slab
-            const int at = q.r0 + 16 * i + 4 * g;
-            if (((o.rows >> (16 * wave + r)) & 1) && at < a.rank) *(f4*)(out + mine * a.rank + at) = acc[i];
-            acc[i] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int m = 0; m < NT; m++) meet[sub][m][lane] = acc[m];
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < NT; m++) {
+            const int at = q.r0 + 16 * m + 4 * g;
+            if (!half && ((o.rows >> (16 * sub + r)) & 1) && at < a.rank) *(f4*)(out + mine * a.rank + at) = acc[m] + meet[sub][m][lane];
+            acc[m] = f4{0.f, 0.f, 0.f, 0.f};
         }
     };
     // one turn; false after the last
@@ -741,13 +756,13 @@ template <class K> hipError_t raise_lds(K k, std::atomic<uint64_t>& set, int byt
 }
 
 template <int NT> hipError_t down(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
-    constexpr int few = kLoraDownWaves * 2 * kUnitBytes<NT>, many = 2 * kLoraSlab / kLoraUnit * NT * 2048;
+    constexpr int few = kLoraDownWaves * 2 * kUnitBytes<NT>, many = 2 * kLoraSlab / kLoraUnit * NT * 2048 + 4 * NT * 1024;
     static std::atomic<uint64_t> set{0}, set_many{0};                      // one bit per device: LDS limit raised
     auto k = p.many ? k_lora_down_many<NT> : k_lora_down<NT>;
     const int lds = p.many ? many : few;
     const hipError_t e = raise_lds(k, p.many ? set_many : set, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, dim3((unsigned)p.down.groups), dim3(64 * kLoraDownWaves), lds, st, a, p, ws);
+    hipLaunchKernelGGL(k, dim3((unsigned)p.down.groups), dim3(64 * (p.many ? kLoraManyWaves : kLoraDownWaves)), lds, st, a, p, ws);
     return hipGetLastError();
 }
 
@@ -783,7 +798,7 @@ LoraPlan plan_of(const LoraArgs& a) { return plan_lora(a, device_cus() > 0 ? dev
 
 bool lora_fits(const LoraArgs& a) {
     const LoraPlan p = plan_of(a);
-    return launch_fits(p.down.groups, 64 * kLoraDownWaves) && launch_fits(p.up.groups, 64 * kLoraUpWaves) && launch_fits(a.T, 16);
+    return launch_fits(p.down.groups, 64 * kLoraManyWaves) && launch_fits(p.up.groups, 64 * kLoraUpWaves) && launch_fits(a.T, 16);
 }
 
 size_t lora_scratch_bytes(const LoraArgs& a) { return plan_of(a).bytes; }

@@ -19,7 +19,8 @@ constexpr int kLoraUnit = 64;                      // few rows: k of a row that 
 constexpr int kLoraSlab = 320;                     // many rows: ... of A's rows
 constexpr int kLoraPieces = 8;                     // pieces of K at most
 constexpr int kLoraXcds = 8;                       // (a launch's workgroups go round them)
-constexpr int kLoraDownWaves = 4;
+constexpr int kLoraDownWaves = 4;                  // of a workgroup of the down products of few rows
+constexpr int kLoraManyWaves = 8;                  // ... of many
 constexpr int kLoraUpWaves = 8;                    // ... of the up products (many rows: of 64 rows and four steps of columns)
 
 struct LoraPart {
