@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_DIR = os.path.dirname(_HERE)
@@ -96,6 +97,18 @@ class RmsNormArgs(ctypes.Structure):
                 ("weight", ctypes.c_void_p), ("wtype", ctypes.c_int), ("offset", ctypes.c_float), ("eps", ctypes.c_float),
                 ("H", ctypes.c_void_p), ("ldh", ctypes.c_int64), ("Aq", ctypes.c_void_p), ("T", ctypes.c_int),
                 ("K", ctypes.c_int)]
+
+
+def _packer(cls):
+    """A function that packs the values of a structure's fields (0 for NULL) into bytes, in a quarter of the time that its
+    constructor takes: single launches of a few microseconds are bound by the host otherwise."""
+    codes = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_int64: "q", ctypes.c_float: "f"}
+    s = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0P")
+    assert s.size == ctypes.sizeof(cls)
+    return s.pack
+
+
+_pack_append, _pack_norm = _packer(Kv4AppendArgs), _packer(RmsNormArgs)
 
 
 class LoraPart(ctypes.Structure):
@@ -251,8 +264,8 @@ def lib() -> ctypes.CDLL:
         L.bf_kv4_attention_sinks_workspace_bytes.argtypes = [cp, ap, i]
         L.bf_kv4_attention_sinks_ws.argtypes = [cp, ap, i, vp, sz, vp]
         lp = ctypes.POINTER(LoraArgs)
-        L.bf_kv4_append.argtypes = [cp, ctypes.POINTER(Kv4AppendArgs), vp]
-        L.bf_rms_norm.argtypes = [ctypes.POINTER(RmsNormArgs), vp]
+        L.bf_kv4_append.argtypes = [cp, vp, vp]                    # (Kv4AppendArgs and RmsNormArgs by reference, or as bytes)
+        L.bf_rms_norm.argtypes = [vp, vp]
         L.bf_lora.argtypes = [lp, vp]
         L.bf_lora_workspace_bytes.argtypes = [lp]
         L.bf_lora_ws.argtypes = [lp, vp, sz, vp]
@@ -288,6 +301,11 @@ def _ptr(t) -> int | None:
     if isinstance(t, int):
         return t
     return t.data_ptr()
+
+
+def _addr(t) -> int:
+    """A tensor's address (or an address itself); 0 for None."""
+    return 0 if t is None else t if type(t) is int else t.data_ptr()
 
 
 def _first_current_stream() -> int:
@@ -605,11 +623,12 @@ def kv4_append(cache: Kv4Cache, K, V, slots, positions, freq, T: int, *, Q=None,
     """T tokens' queries and keys (fp16 rows) rotated by their positions (int64; freq: fp32 [rot / 2], radians a position;
     rot: the whole head by default), queries to Q_out, keys and values into the cache's slots as by kv4_store, rotated keys
     to K_out too where given."""
-    kv, q = cache.kv_heads * cache.head_dim, q_heads * cache.head_dim
-    a = Kv4AppendArgs(_ptr(Q), q if ldq is None else ldq, _ptr(Q_out), q if ldqo is None else ldqo, _ptr(K),
-                      kv if ldk is None else ldk, _ptr(K_out), kv if ldko is None else ldko, _ptr(V), kv if ldv is None else ldv,
-                      _ptr(slots), _ptr(positions), _ptr(freq), q_heads, cache.head_dim if rot is None else rot, style, factor, T)
-    _check(lib().bf_kv4_append(ctypes.byref(cache), ctypes.byref(a), _stream(stream)), "bf_kv4_append")
+    dim = cache.head_dim
+    kv, q = cache.kv_heads * dim, q_heads * dim
+    a = _pack_append(_addr(Q), q if ldq is None else ldq, _addr(Q_out), q if ldqo is None else ldqo, _addr(K),
+                     kv if ldk is None else ldk, _addr(K_out), kv if ldko is None else ldko, _addr(V), kv if ldv is None else ldv,
+                     _addr(slots), _addr(positions), _addr(freq), q_heads, dim if rot is None else rot, style, factor, T)
+    _check(lib().bf_kv4_append(ctypes.byref(cache), a, _stream(stream)), "bf_kv4_append")
 
 
 _dtypes = {}
@@ -631,11 +650,11 @@ def rms_norm(X, T: int, K: int, *, H=None, Aq=None, delta=None, R=None, weight=N
     """r = X + delta; H (fp16 rows) and, or, Aq (q8_bytes(T, K) bytes, gemm_q8's activations) = r / sqrt(mean(r^2) + eps)
     (weight + offset); R = r where given.  X, delta and weight are fp32 or fp16 (xtype, dtype, wtype: by default from the
     tensors' dtypes)."""
-    a = RmsNormArgs(_ptr(X), _dtype(X) if xtype is None else xtype, K if ldx is None else ldx, _ptr(delta),
-                    _dtype(delta) if dtype is None else dtype, K if ldd is None else ldd, _ptr(R), K if ldr is None else ldr,
-                    _ptr(weight), _dtype(weight) if wtype is None else wtype, offset, eps, _ptr(H), K if ldh is None else ldh,
-                    _ptr(Aq), T, K)
-    _check(lib().bf_rms_norm(ctypes.byref(a), _stream(stream)), "bf_rms_norm")
+    a = _pack_norm(_addr(X), _dtype(X) if xtype is None else xtype, K if ldx is None else ldx, _addr(delta),
+                   _dtype(delta) if dtype is None else dtype, K if ldd is None else ldd, _addr(R), K if ldr is None else ldr,
+                   _addr(weight), _dtype(weight) if wtype is None else wtype, offset, eps, _addr(H), K if ldh is None else ldh,
+                   _addr(Aq), T, K)
+    _check(lib().bf_rms_norm(a, _stream(stream)), "bf_rms_norm")
 
 
 def lora_parts(parts):

@@ -70,10 +70,13 @@ __device__ __forceinline__ Factor factor(float ss, int K, float eps, V values, i
     return f;
 }
 
-// One value's code; dd the block's scale (0: all zero), not finite: 0.
-__device__ __forceinline__ int code(float y, float dd) {
-    if (!(dd > 0.f && dd < __builtin_inff())) return 0;
-    return (int)__builtin_fminf(__builtin_fmaxf(__builtin_roundf(y / dd), -127.f), 127.f);
+// One value's code; dd the block's scale (0: all zero; not finite: codes 0), inv its reciprocal (one division a block; where
+// that or dd is not normal, one a value).
+__device__ __forceinline__ float reciprocal(float dd) { return dd >= 0x1p-125f && dd < 0x1p125f ? 1.f / dd : 0.f; }
+__device__ __forceinline__ int code(float y, float dd, float inv) {
+    float q = y * inv;
+    if (inv == 0.f) q = dd > 0.f && dd < __builtin_inff() ? y / dd : 0.f;
+    return (int)__builtin_fminf(__builtin_fmaxf(__builtin_roundf(q), -127.f), 127.f);
 }
 
 __device__ __forceinline__ float load1(const void* p, int f16, int64_t i) {
@@ -155,11 +158,11 @@ __global__ __launch_bounds__(1024) void k_rms_norm(NormDev p) {
             m = __builtin_fmaxf(m, __shfl_xor(m, 2));
             bad += __shfl_xor(bad, 1);
             bad += __shfl_xor(bad, 2);
-            const float dd = m / 127.0f + bad;
+            const float dd = m / 127.0f + bad, inv = reciprocal(dd);
             int q[8], sum = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                q[e] = code(y[e], dd);
+                q[e] = code(y[e], dd, inv);
                 sum += q[e];
             }
             sum += __shfl_xor(sum, 1);
@@ -216,7 +219,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(NormDev p) {
                 bad += __shfl_xor(bad, x);
             }
             const float dd = m / 127.0f + bad;
-            const int q = code(y, dd);
+            const int q = code(y, dd, reciprocal(dd));
             int sum = q;
 #pragma unroll
             for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor(sum, x);
