@@ -313,11 +313,10 @@ __device__ __forceinline__ f4 sum4(const float* s0, int64_t step, int pieces, in
 }
 
 // A row's sums, fours of ranks by PER neighbouring lanes in turn (this one `me`), to
-// two fp16 numbers each, times 2^shift: at hi + k and lo + k, k below `padded`.
-// Returns the shift.
-template <int PER>
-__device__ __forceinline__ int split_row(const float* s0, int64_t step, int pieces, int ranks, int me, int padded, _Float16* hi,
-                                         _Float16* lo) {
+// two fp16 numbers each, times 2^shift: put(k, hi, lo) of ranks k .. k + 3, k below
+// `padded`.  Returns the shift.
+template <int PER, class P>
+__device__ __forceinline__ int split_row(const float* s0, int64_t step, int pieces, int ranks, int me, int padded, P put) {
     f4 held[2];
     float top = 0.f;
     for (int i = 0, k = 4 * me; k < padded; k += 4 * PER, i++) {
@@ -341,8 +340,7 @@ __device__ __forceinline__ int split_row(const float* s0, int64_t step, int piec
             h[j] = (_Float16)v;
             l[j] = (_Float16)(v - (float)h[j]);
         }
-        *(uint2*)(hi + k) = uint2{as_u32(h2{h[0], h[1]}), as_u32(h2{h[2], h[3]})};
-        *(uint2*)(lo + k) = uint2{as_u32(h2{l[0], l[1]}), as_u32(h2{l[2], l[3]})};
+        put(k, uint2{as_u32(h2{h[0], h[1]}), as_u32(h2{h[2], h[3]})}, uint2{as_u32(h2{l[0], l[1]}), as_u32(h2{l[2], l[3]})});
     }
     return shift;
 }
@@ -373,7 +371,10 @@ __global__ __launch_bounds__(16 * kJoinRows) void k_lora_join(LoraArgs a, LoraPl
     const Joined j = joined_of(a, p, ws);
     const int64_t row = (int64_t)part * a.T + t;
     const int shift = split_row<16>(ws + ((int64_t)part * p.pieces * a.T + t) * a.rank, (int64_t)a.T * a.rank, p.pieces, ranks, me,
-                                    p.padded, j.hi + row * p.padded, j.lo + row * p.padded);
+                                    p.padded, [&](int k, uint2 hi, uint2 lo) {
+                                        *(uint2*)(j.hi + row * p.padded + k) = hi;
+                                        *(uint2*)(j.lo + row * p.padded + k) = lo;
+                                    });
     if (me == 0) j.factor[row] = id < 0 ? 0.f : __builtin_ldexpf(a.scales ? a.scales[id] : 1.f, -shift);
 }
 
@@ -569,7 +570,10 @@ __global__ __launch_bounds__(64 * kLoraUpWaves) void k_lora_up(LoraArgs a, LoraP
         const int row = tid / PER, mr = __shfl(rk, row);
         const float scale = __shfl(sc, row);
         const int shift = split_row<PER>(ws + ((int64_t)part * p.pieces * a.T + t0 + row) * a.rank, (int64_t)a.T * a.rank, p.pieces, mr,
-                                         tid % PER, padded, sums + row * ld, sums + (ROWS + row) * ld);
+                                         tid % PER, padded, [&](int k, uint2 hi, uint2 lo) {
+                                             *(uint2*)(sums + row * ld + k) = hi;
+                                             *(uint2*)(sums + (ROWS + row) * ld + k) = lo;
+                                         });
         if (tid % PER == 0) factor[row] = __builtin_ldexpf(scale, -shift);
     }
     __syncthreads();
@@ -613,48 +617,48 @@ __global__ __launch_bounds__(64 * kLoraUpWaves) void k_lora_up(LoraArgs a, LoraP
     }
 }
 
-// Many rows: wave w takes rows 16 (w % 4) .. and columns 128 (w / 4) .. of 64 by 256.
-// Operand j of its eight holds the columns that leave a lane 16 neighbouring bytes
-// of a row of C (8 i + j in fp16, 64 (j / 4) + 4 i + j % 4 in fp32), so that a wave
-// reads and writes runs of 256 bytes.  Everything it needs is on its way at once; a
-// tile of several adapters takes them in turn.
-template <int RC, bool F16>
+// Many rows: a workgroup takes 64 rows by 256 columns, wave w rows 16 (w % 4) .. and
+// columns 128 (w / 4) .. of those.  Operand j of its eight holds the columns that
+// leave a lane 16 neighbouring bytes of a row of C (8 i + j in fp16, 64 (j / 4) + 4 i
+// + j % 4 in fp32), so that a wave reads and writes runs of 256 bytes (128-byte runs
+// of 8-byte pieces: 25 us where this took 15).  Everything it needs is on its way at
+// once; a tile of several adapters takes them in turn.  JOIN: the pieces' sums are
+// joined here, for ranks that are one block; else k_lora_join did it.
+template <int RC, bool F16, bool JOIN>
 __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
     constexpr int WV = kLoraUpWaves, ROWS = 64, COLS = 128, PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * COLS * RC;
     constexpr int SH = F16 ? 3 : 2, PER = F16 ? 1 : 2, W = F16 ? 8 : 4;    // runs of a lane in a row, their columns
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BYTES + 2 * 2 * ROWS * RC];   // two blocks of B, the sums' hi and lo
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), sub = wave & 3;
+    __shared__ float factor[ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), sub = wave & 3;
     int tile, at;
     if (!place_of(p.up, tile, at)) return;
     const int part = part_of(a, p.up_steps, at);
     const LoraPart& w = a.part[part];
     const int n = at * p.up_steps * kLoraCols + COLS * (wave >> 2), col = n + W * r;         // (the lane's second run: col + 64)
-    const int64_t t0 = (int64_t)tile * ROWS;
+    const int64_t t0 = (int64_t)tile * ROWS, lt = t0 + 16 * sub + 4 * g;   // (the lane's rows: lt + i)
     const int id = adapter_of(a, t0, ROWS, lane), rk = ranks_of(a, id);
     const Joined sums = joined_of(a, p, ws);
     uint8_t* const block = lds + (wave >> 2) * BYTES;
     uint8_t* const rows_lds = lds + 2 * BYTES;                             // [hi, lo][64 rows][RC]
 
-    // the wave's quarter of its block: ranks k0 .. of adapter e, as far as they count
-    auto fetch_b = [&](int e, int ranks, int k0) {
+    // the wave's quarter of its block: ranks k0 .. of adapter e, as far as they count; and its share of the sums
+    auto fetch = [&](int e, int ranks, int k0) {
         const uint16_t* const B = w.B + (int64_t)e * w.N * a.rank;
 #pragma unroll
         for (int i = 0; i < PIECES / 2; i++) {
             const int m = 4 * i + sub, q = 64 * m + lane, c = q / PIECES, k = k0 + 8 * place<RC, SH>(c, q % PIECES);
             if (k < ranks) dma16(B + (int64_t)min(n + c, w.N - 1) * a.rank + k, lds_addr(block) + 1024 * m);
         }
-    };
-    // the wave's share of the rows' sums
-    auto fetch_s = [&](int k0) {
-        constexpr int LOADS = 2 * PIECES;          // (of both planes)
+        if (JOIN) return;
 #pragma unroll
-        for (int i = 0; i < (LOADS + WV - 1) / WV; i++) {
+        for (int i = 0; i < (2 * PIECES + WV - 1) / WV; i++) {             // (of both planes)
             const int m = WV * i + wave;
-            if (m >= LOADS) break;
+            if (m >= 2 * PIECES) break;
             const int q = 64 * (m % PIECES) + lane, row = q / PIECES, k = k0 + 8 * place<RC, 0>(row, q % PIECES);
             const _Float16* const s = (m < PIECES ? sums.hi : sums.lo) + ((int64_t)part * a.T + min(t0 + row, (int64_t)a.T - 1)) * p.padded;
-            dma16(s + k, lds_addr(rows_lds) + 1024 * m);
+            if (k < p.padded) dma16(s + k, lds_addr(rows_lds) + 1024 * m);
         }
     };
     uint64_t left = __ballot(id != -2), rows = 0;
@@ -667,22 +671,26 @@ __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs 
         left &= ~rows;
     };
     next();
-    if (ranks > 0) {
-        fetch_b(e, ranks, 0);
-        fetch_s(0);
-    }
-    // the lane's rows 4 g + i: what is added to, and the factors
-    const int64_t lt = t0 + 16 * sub + 4 * g;
-    typename Run<F16>::type c[4][PER];
-    f4 f;
+    if (ranks > 0) fetch(e, ranks, 0);
+    typename Run<F16>::type c[4][PER];             // what is added to
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int h = 0; h < PER; h++)
             c[i][h] = load_run<F16>(a, (lt + i) * a.ldc + w.at + col + 64 * h, lt + i < a.T ? w.N - col - 64 * h : 0);
-        f[i] = sums.factor[(int64_t)part * a.T + min(lt + i, (int64_t)a.T - 1)];
+    if (JOIN) {
+        const int row = tid / 8, mr = __shfl(rk, row), me = __shfl(id, row);
+        const int shift = split_row<8>(ws + ((int64_t)part * p.pieces * a.T + t0 + row) * a.rank, (int64_t)a.T * a.rank, p.pieces, mr,
+                                       tid % 8, RC, [&](int k, uint2 hi, uint2 lo) {
+                                           uint8_t* const to = rows_lds + row * (2 * RC) + 16 * place<RC, 0>(row, k / 8) + 2 * (k & 7);
+                                           *(uint2*)to = hi;
+                                           *(uint2*)(to + 2 * ROWS * RC) = lo;
+                                       });
+        if (tid % 8 == 0) factor[row] = me < 0 ? 0.f : __builtin_ldexpf(a.scales ? a.scales[me] : 1.f, -shift);
+    } else if (tid < ROWS) {
+        factor[tid] = t0 + tid < a.T ? sums.factor[(int64_t)part * a.T + t0 + tid] : 0.f;
     }
-    bool held = ranks > 0;                         // the sums in LDS are of ranks 0 ..
+    __syncthreads();
     for (;;) {
         f4 acc[8];
 #pragma unroll
@@ -692,10 +700,11 @@ __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs 
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (mine) {
+                const int row = 16 * sub + r;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
                     if (k0 + 32 * s >= ranks) break;
-                    const int row = 16 * sub + r, k = 32 * s + 8 * g;
+                    const int k = 32 * s + 8 * g;
                     h8 v[2];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -712,35 +721,38 @@ __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs 
             }
             if (k0 + RC < ranks) {
                 __syncthreads();                   // the blocks have been read
-                fetch_b(e, ranks, k0 + RC);
-                fetch_s(k0 + RC);
-                held = false;
+                fetch(e, ranks, k0 + RC);
             }
         }
-        if (mine && (ranks > 0 || a.Y != a.C)) {   // (no adapter: a copy, through no arithmetic)
+        const uint64_t these = rows;
+        const int had = ranks;
+        if (left) {                                // the tile's next adapter
+            next();
+            if (ranks > 0) {
+                __syncthreads();
+                fetch(e, ranks, 0);
+            }
+        } else {
+            e = -2;
+        }
+        if (mine && (had > 0 || a.Y != a.C)) {     // (no adapter: a copy, through no arithmetic)
+            const f4 f = *(const f4*)(factor + 16 * sub + 4 * g);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int h = 0; h < PER; h++) {
                     typename Run<F16>::type y = c[i][h];
-                    if (ranks > 0) {
+                    if (had > 0) {
                         float d[W];
 #pragma unroll
                         for (int j = 0; j < W; j++) d[j] = acc[4 * h + j][i];
                         y = add_run(y, f[i], d);
                     }
-                    const bool in = (rows >> (16 * sub + 4 * g + i)) & 1;
+                    const bool in = (these >> (16 * sub + 4 * g + i)) & 1;
                     store_run<F16>(a, (lt + i) * a.ldy + w.at + col + 64 * h, y, in ? w.N - col - 64 * h : 0);
                 }
         }
-        if (!left) return;
-        next();
-        if (ranks > 0) {
-            __syncthreads();                       // the blocks have been read
-            fetch_b(e, ranks, 0);
-            if (!held) fetch_s(0);
-            held = true;
-        }
+        if (e == -2) return;
     }
 }
 
@@ -777,13 +789,23 @@ template <int RC, bool F16> hipError_t up_few(const LoraArgs& a, const LoraPlan&
     return hipGetLastError();
 }
 
+template <int RC, bool F16, bool JOIN> hipError_t up_many(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
+    if (!JOIN) {
+        hipLaunchKernelGGL(k_lora_join, dim3((unsigned)((a.T + kJoinRows - 1) / kJoinRows), (unsigned)a.parts), dim3(16 * kJoinRows), 0, st,
+                           a, p, ws);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((k_lora_up_many<RC, F16, JOIN>), dim3((unsigned)p.up.groups), dim3(64 * kLoraUpWaves), 0, st, a, p, ws);
+    return hipGetLastError();
+}
+
 template <int RC, bool F16> hipError_t up(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
     if (!p.many) return up_few<RC, F16>(a, p, ws, st);
-    hipLaunchKernelGGL(k_lora_join, dim3((unsigned)((a.T + kJoinRows - 1) / kJoinRows), (unsigned)a.parts), dim3(16 * kJoinRows), 0, st, a, p, ws);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_lora_up_many<RC, F16>), dim3((unsigned)p.up.groups), dim3(64 * kLoraUpWaves), 0, st, a, p, ws);
-    return hipGetLastError();
+    if constexpr (RC == 64) {
+        if (a.rank > RC) return up_many<RC, F16, false>(a, p, ws, st);
+    }
+    return up_many<RC, F16, true>(a, p, ws, st);
 }
 
 template <int RC> hipError_t both(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {

@@ -108,7 +108,7 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
     p.up = lora_grid(t, groups);
     p.joined = (int64_t)a.parts * p.pieces * a.T * a.rank;
     p.bytes = (size_t)p.joined * sizeof(float);
-    if (p.many) p.bytes += (size_t)a.parts * a.T * (4 * (size_t)p.padded + 4);
+    if (p.many && a.rank > rc) p.bytes += (size_t)a.parts * a.T * (4 * (size_t)p.padded + 4);
     return p;
 }
 

@@ -141,6 +141,22 @@ def test_prompts(T, ids):
     Case(T, 512, [200, 56], 12, 16 if T == 2000 else 64, ids=which, otype=bf.OUT_F16).run(workspace=True)
 
 
+@pytest.mark.parametrize("T,widths,rank,otype", [
+    (1100, [4200], 16, bf.OUT_F16), (1100, [4200], 64, bf.OUT_F32), (700, [3000, 1030], 32, bf.OUT_F32), (300, [260], 136, bf.OUT_F16),
+    (600, [4100, 7], 72, bf.OUT_F32), (257, [64], 8, bf.OUT_F16)])
+def test_many_rows_and_columns(T, widths, rank, otype):
+    """Workgroups that take several blocks of columns, blocks of ranks and adapters in turn; tiles of one adapter, of several
+    and of none."""
+    ids = [min(3, t * 4 // T) if t % 230 < 200 else (t % 5) - 1 for t in range(T)]
+    c = Case(T, 96, widths, 4, rank, ids=ids, ranks=[rank, rank - 3, max(1, rank // 3), rank], otype=otype, pad=8)
+    c.run()
+
+
+def test_many_rows_in_place():
+    ids = [t // 100 - 1 for t in range(900)]
+    Case(900, 64, [3500], 7, 16, ids=ids, otype=bf.OUT_F16).run(place="in")
+
+
 def test_one_row_among_many_of_another():
     """Tiles whose rows are of one adapter but for the last."""
     Case(48, 96, [40], 3, 8, ids=([1] * 15 + [2]) * 3).run()
