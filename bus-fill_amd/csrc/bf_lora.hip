@@ -2,27 +2,36 @@
 //   Y[t] = C[t] + scale_e B_e (A_e x[t]),  e = ids[t]  (no adapter: Y[t] = C[t]),
 // for up to four parts (a fused projection's slices), each with its A and B.
 //
-// Two launches: s = A x in fp32 (k_lora_down), then C + scale B s (k_lora_up).
-// Rows are taken in tiles of 16 (few rows) or 64, operands of 16x16x32 MFMAs; a
-// tile's rows may be of as many adapters, and each adapter of a tile is multiplied
-// with the operands that hold rows of it, of which its own are kept.  So nothing
-// is sorted and no row moves: single tokens of many requests are bound by the
-// adapters' bytes whatever the products do, and in prompts neighbouring rows are
-// of one adapter.
+// Two launches: s = A x in fp32 (k_lora_down), then C + scale B s (k_lora_up); for
+// many rows k_lora_down_many and k_lora_up_many, with k_lora_join between them where
+// an adapter has more than 64 ranks.  Rows are taken in tiles of 16, or of 64 from
+// 257 rows on; a tile's rows may be of as many adapters, and each adapter of a tile is
+// multiplied with the operands (of 16x16x32 MFMAs) that hold rows of it, of which its
+// own are kept.  So nothing is sorted and no row moves: single tokens of many requests
+// are bound by the adapters' bytes whatever the products do, and in prompts
+// neighbouring rows are of one adapter.
 //
-// Both kernels' matrices come to LDS by direct loads, eight neighbouring lanes 128 bytes
-// of a row, with the row's 16-byte pieces in an order that spreads an operand's
-// reads over the banks.  (Operands straight from memory, a lane's 16 bytes in
-// another row than its neighbours', take the load path a cycle a lane: 23 us where
-// the down products of 32 rows take ....)
+// Matrices come to LDS by direct loads, eight neighbouring lanes 128 bytes of a row,
+// the row's 16-byte pieces in an order that spreads an operand's reads over the banks.
+// (Operands straight from memory, a lane's 16 bytes in another row than its
+// neighbours', take the load path a cycle a lane: 23 us for the down products of 32
+// rows below, 10 through LDS.)
 //
 // Down: x and A are fp16, their products exact, sums fp32.  K is cut between a
 // workgroup's waves, whose sums meet in LDS, and into pieces (partial sums in the
-// workspace, added by the up products in their order), so that a few rows fill the
+// workspace, added in their order by the next kernel), so that a few rows fill the
 // chip.
 // Up: s, times a power of two that brings the row's largest to 2^14..2^15, is
 // taken as two fp16 numbers (rounded, and the rest rounded: 2^-22 of the largest), so
 // the products lose nothing that fp32 would keep; sums fp32, one rounding of Y.
+//
+// Measured, K = 5120, fp16 C and Y.  One row, rank 16, parts of 5120, 1024 and 1024
+// columns: 10.2 us, 4.1 down and 5.9 up; a launch that does nothing is 2.5, the rest
+// is the chain of ids, operands, sums and outputs.  32 rows of 32 adapters of ranks
+// 16 to 64, the same parts: 20.8 us, 9.5 and 11.5, for 33 MB of adapters (1.6 TB/s; 2.8
+// TB/s of down products with all ranks 64).  2000 rows of six adapters of rank 64, one
+// part of 5120 columns: 36 us, 13.6 and 20, for 69 MB; tiles of two adapters, which take them
+// in turn, are 8 us of that.
 #include <atomic>
 
 #include "bf_device.h"
@@ -50,20 +59,6 @@ __device__ __forceinline__ int ranks_of(const LoraArgs& a, int id) {
 __device__ __forceinline__ h8 masked(h8 v, bool in) {
     const h8 zero = {};
     return in ? v : zero;
-}
-
-// The workgroup's tile and which of the tile's it is; false where there is none.
-__device__ __forceinline__ bool place_of(const LoraGrid& q, int& tile, int& in) {
-    const int b = blockIdx.x;
-    if (q.per_xcd) {
-        const int turn = b / kLoraXcds;
-        tile = b % kLoraXcds * q.per_xcd + turn / q.inner;
-        in = turn % q.inner;
-    } else {
-        tile = b % q.tiles;
-        in = b / q.tiles;
-    }
-    return tile < q.tiles;
 }
 
 // A unit in LDS: operands of 16 rows of 128 bytes, those of A first, piece c of row r at place c ^ (r % 8).
@@ -140,7 +135,7 @@ __global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down(LoraArgs a, L
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     int tile, in;
-    if (!place_of(p.down, tile, in)) return;
+    if (!lora_place(p.down, blockIdx.x, tile, in)) return;
     const Share q = share_of(a, p, in);
     const int64_t t0 = (int64_t)tile * kLoraSub;
     const int id = adapter_of(a, t0, kLoraSub, lane), rk = ranks_of(a, id);
@@ -183,8 +178,8 @@ __global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down(LoraArgs a, L
 
 // Many rows: a wave takes 16 of 64 rows and half of each slab of K; x comes to its
 // registers, A's rows, two slabs by turns, to LDS for all eight.  (Four waves with whole
-// slabs: 11.1 us for 2000 rows of 5120 and 64 ranks where this takes ....  LDS gives eight
-// waves 1.7 times what it gives four.)
+// slabs: 11.1 us for 2000 rows of one adapter, K = 5120, 64 ranks, where this takes 9.9; LDS
+// gives eight waves 1.7 times what it gives four.)
 template <int NT>
 __global__ __launch_bounds__(64 * kLoraManyWaves) void k_lora_down_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
     constexpr int WV = kLoraManyWaves, STEPS = kLoraSlab / kLoraStep / 2, UNITS = kLoraSlab / kLoraUnit, BYTES = UNITS * NT * 2048;
@@ -194,7 +189,7 @@ __global__ __launch_bounds__(64 * kLoraManyWaves) void k_lora_down_many(LoraArgs
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, row = lane >> 3, piece = (lane & 7) ^ row;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), sub = wave & 3, half = wave >> 2;
     int tile, in;
-    if (!place_of(p.down, tile, in)) return;
+    if (!lora_place(p.down, blockIdx.x, tile, in)) return;
     const Share q = share_of(a, p, in);
     const int64_t t0 = (int64_t)tile * (4 * kLoraSub), mine = t0 + 16 * sub + r;
     const int id = adapter_of(a, t0, 4 * kLoraSub, lane), rk = ranks_of(a, id);
@@ -515,7 +510,7 @@ __global__ __launch_bounds__(64 * kLoraUpWaves) void k_lora_up(LoraArgs a, LoraP
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tile, at;
-    if (!place_of(p.up, tile, at)) return;
+    if (!lora_place(p.up, blockIdx.x, tile, at)) return;
     const int part = part_of(a, p.up_steps, at);
     const LoraPart& w = a.part[part];
     const int n0 = at * p.up_steps * kLoraCols, n1 = min(w.N, n0 + p.up_steps * kLoraCols);
@@ -633,7 +628,7 @@ __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs 
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), sub = wave & 3;
     int tile, at;
-    if (!place_of(p.up, tile, at)) return;
+    if (!lora_place(p.up, blockIdx.x, tile, at)) return;
     const int part = part_of(a, p.up_steps, at);
     const LoraPart& w = a.part[part];
     const int n = at * p.up_steps * kLoraCols + COLS * (wave >> 2), col = n + W * r;         // (the lane's second run: col + 64)

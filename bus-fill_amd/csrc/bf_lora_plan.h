@@ -61,6 +61,22 @@ inline LoraGrid lora_grid(int tiles, int64_t inner) {
     return g;
 }
 
+// Workgroup b's tile and which of the tile's it is; false where there is none.
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+inline bool lora_place(const LoraGrid& g, int b, int& tile, int& in) {
+    if (g.per_xcd) {
+        const int turn = b / kLoraXcds;
+        tile = b % kLoraXcds * g.per_xcd + turn / g.inner;
+        in = turn % g.inner;
+    } else {
+        tile = b % g.tiles;
+        in = b / g.tiles;
+    }
+    return tile < g.tiles;
+}
+
 // Few rows (tiles of 16): down, a workgroup takes a tile, a part, up to 64 ranks, a
 // piece of K (its waves shares of that) and every `sharers`-th of the tile's
 // adapters; up, a workgroup takes a tile, up_steps steps of 64 columns of a part and
