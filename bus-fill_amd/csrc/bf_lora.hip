@@ -2,14 +2,20 @@
 //   Y[t] = C[t] + scale_e B_e (A_e x[t]),  e = ids[t]  (no adapter: Y[t] = C[t]),
 // for up to four parts (a fused projection's slices), each with its A and B.
 //
-// Two launches: s = A x in fp32 (k_lora_down), then C + scale B s (k_lora_up); for
-// many rows k_lora_down_many and k_lora_up_many, with k_lora_join between them where
-// an adapter has more than 64 ranks.  Rows are taken in tiles of 16, or of 64 from
-// 257 rows on; a tile's rows may be of as many adapters, and each adapter of a tile is
-// multiplied with the operands (of 16x16x32 MFMAs) that hold rows of it, of which its
-// own are kept.  So nothing is sorted and no row moves: single tokens of many requests
-// are bound by the adapters' bytes whatever the products do, and in prompts
-// neighbouring rows are of one adapter.
+// Up to 256 rows, two launches: s = A x in fp32 (k_lora_down), then C + scale B s
+// (k_lora_up).  Rows are taken as they come, in tiles of 16, which may be of as many
+// adapters; each adapter of a tile is multiplied with the whole tile (an operand of
+// 16x16x32 MFMAs), of which its own rows are kept.  Single tokens of many requests are
+// bound by the adapters' bytes whatever the products do.
+// More rows are sorted by adapter first (k_lora_order), then taken in tiles of up to 64
+// of one adapter (k_lora_down_many, k_lora_up_many, with k_lora_join between them where
+// an adapter has more than 64 ranks).  Without the order, tiles of 64 rows as they
+// come: 2000 rows of 64 adapters in no order, rank 16, 322 us instead of 34, of 8
+// adapters, rank 64, 104 instead of 37; in runs of an adapter it saved nothing (36).
+// Every adapter of the pool may have a tile of its own, so that more workgroups are
+// launched than have work: 0.5 us for 64 adapters, 12 for 1000.  Above 2047 adapters, or with
+// fewer than two rows an adapter, rows are taken as they come (2000 rows, rank 16: 207 to
+// 243 us with as many adapters as rows, 37 with one).
 //
 // Matrices come to LDS by direct loads, eight neighbouring lanes 128 bytes of a row,
 // the row's 16-byte pieces in an order that spreads an operand's reads over the banks.
@@ -28,10 +34,9 @@
 // Measured, K = 5120, fp16 C and Y.  One row, rank 16, parts of 5120, 1024 and 1024
 // columns: 10.2 us, 4.1 down and 5.9 up; a launch that does nothing is 2.5, the rest
 // is the chain of ids, operands, sums and outputs.  32 rows of 32 adapters of ranks
-// 16 to 64, the same parts: 20.8 us, 9.5 and 11.5, for 33 MB of adapters (1.6 TB/s; 2.8
+// 16 to 64, the same parts: 20.6 to 21.9 us, 9.5 and 11.5, for 33 MB of adapters (1.6 TB/s; 2.8
 // TB/s of down products with all ranks 64).  2000 rows of six adapters of rank 64, one
-// part of 5120 columns: 36 us, 13.6 and 20, for 69 MB; tiles of two adapters, which take them
-// in turn, are 8 us of that.
+// part of 5120 columns: 34 to 37 us, 4.2 the order, 12 down and 20 up, for 69 MB.
 #include <atomic>
 
 #include "bf_device.h"
@@ -176,116 +181,187 @@ __global__ __launch_bounds__(64 * kLoraDownWaves) void k_lora_down(LoraArgs a, L
     }
 }
 
+// Many rows' order by adapter and its tiles of up to 64, by one workgroup: rows are
+// counted, adapters' tiles summed up, rows placed (in which order within an adapter
+// changes no result: a row's sums depend on no other row).  2000 rows: 4.2 us, of which
+// a launch that does nothing is 2.  (Every workgroup of the down products for itself, up
+// to 4096 rows: 5.7 us more there.)
+constexpr int kOrderThreads = 1024, kOrderRows = 4;                        // rows a thread and turn
+// Increments bins[id] for the lanes with live; the value before (of lane after lane where a wave's lanes are of one adapter).
+__device__ __forceinline__ int claim(int* bins, int id, bool live, int lane) {
+    const int first = __builtin_amdgcn_readfirstlane(id);
+    const uint64_t all = __ballot(live);
+    if (__ballot(live && id == first) != all) return live ? atomicAdd(&bins[id], 1) : 0;
+    int at = 0;
+    if (lane == 0 && all) at = atomicAdd(&bins[first], __builtin_popcountll(all));
+    return __builtin_amdgcn_readfirstlane(at) + lane;                      // (live lanes come first)
+}
+__global__ __launch_bounds__(kOrderThreads) void k_lora_order(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+    __shared__ int bins[kLoraBins];                // a counter an adapter, and one for rows without
+    __shared__ int part[kOrderThreads / 64];
+    LoraTile* const tiles = (LoraTile*)(ws + p.tiles);
+    int* const rows = (int*)(ws + p.rows);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.adapters + 1;
+    int ids[kOrderRows];
+    auto load = [&](int64_t t0) {
+#pragma unroll
+        for (int i = 0; i < kOrderRows; i++) {
+            const int id = a.ids[min(t0 + kOrderThreads * i + tid, (int64_t)a.T - 1)];
+            ids[i] = id < 0 || id >= a.adapters ? a.adapters : id;
+        }
+    };
+    // (waits for LDS only, not for stores)
+    auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    const int64_t turn = kOrderThreads * kOrderRows;
+    load(0);
+    // a thread's adapters: b0 .. b1 - 1
+    const int per = (n + kOrderThreads - 1) / kOrderThreads, b0 = min(tid * per, n), b1 = min(b0 + per, n);
+    const int rk0 = b0 < a.adapters ? ranks_of(a, b0) : 0;
+    for (int i = tid; i < n; i += kOrderThreads) bins[i] = 0;
+    meet();
+    for (int64_t t0 = 0; t0 < a.T; t0 += turn) {
+        if (t0) load(t0);
+#pragma unroll
+        for (int i = 0; i < kOrderRows; i++)
+            if (t0 + kOrderThreads * i < a.T) claim(bins, ids[i], t0 + kOrderThreads * i + tid < a.T, lane);
+    }
+    meet();
+    // the tiles before them; from here on a counter holds the place, 64 a tile, of its adapter's next row
+    int count = 0;
+    for (int b = b0; b < b1; b++) count += (bins[b] + 63) / 64;
+    int before = count;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        const int c = __shfl_up(before, x);
+        if (lane >= x) before += c;
+    }
+    if (lane == 63) part[wave] = before;
+    before -= count;
+    meet();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kOrderThreads / 64; w++) {
+        before += w < wave ? part[w] : 0;
+        total += part[w];
+    }
+    for (int b = b0; b < b1; b++) {
+        const int here = bins[b];
+        bins[b] = 64 * before;
+        const int e = b < a.adapters ? b : -1, rk = !here || e < 0 ? 0 : b == b0 ? rk0 : ranks_of(a, e);
+        for (int i = 0; i < here; i += 64) tiles[before++] = LoraTile{e, min(64, here - i), rk, 0};
+    }
+    if (tid == 0) tiles[p.most].adapter = total;
+    meet();
+    for (int64_t t0 = 0; t0 < a.T; t0 += turn) {
+        if (a.T > turn) load(t0);
+#pragma unroll
+        for (int i = 0; i < kOrderRows; i++) {
+            if (t0 + kOrderThreads * i >= a.T) break;
+            const int64_t t = t0 + kOrderThreads * i + tid;
+            const int at = claim(bins, ids[i], t < a.T, lane);
+            if (t < a.T) rows[at] = (int)t;
+        }
+    }
+}
+
+// Workgroup's tile of many rows, its rows, and which of the tile's workgroups it is.
+__device__ __forceinline__ bool tile_of(const LoraPlan& p, const LoraGrid& g, const float* ws, LoraTile& o, const int*& rows, int& in) {
+    const LoraTile* const tiles = (const LoraTile*)(ws + p.tiles);
+    int tile;
+    if (!lora_place(lora_grid(tiles[p.most].adapter, g.inner), blockIdx.x, tile, in)) return false;
+    o = tiles[tile];
+    rows = (const int*)(ws + p.rows) + 64 * (int64_t)tile;
+    return true;
+}
+
 // Many rows: a wave takes 16 of 64 rows and half of each slab of K; x comes to its
 // registers, A's rows, two slabs by turns, to LDS for all eight.  (Four waves with whole
-// slabs: 11.1 us for 2000 rows of one adapter, K = 5120, 64 ranks, where this takes 9.9; LDS
+// slabs: 11.1 us for 2000 rows of one adapter, K = 5120, 64 ranks, where this took 9.9; LDS
 // gives eight waves 1.7 times what it gives four.)
 template <int NT>
 __global__ __launch_bounds__(64 * kLoraManyWaves) void k_lora_down_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
     constexpr int WV = kLoraManyWaves, STEPS = kLoraSlab / kLoraStep / 2, UNITS = kLoraSlab / kLoraUnit, BYTES = UNITS * NT * 2048;
     constexpr int LOADS = UNITS * NT * 2;          // direct loads of a slab, eight rows of 128 bytes each: wave w does every WV-th
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // two slabs, [unit][operand][16 rows of 128 bytes]; sums
-    f4 (*const meet)[NT][64] = (f4 (*)[NT][64])(lds + 2 * BYTES);          // [4], of the waves with the second halves
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];        // two slabs, [unit][operand][16 rows of 128 bytes]
+    f4 (*const meet)[NT][64] = (f4 (*)[NT][64])lds;                        // at the end: [4], sums of the waves with the second halves
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, row = lane >> 3, piece = (lane & 7) ^ row;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), sub = wave & 3, half = wave >> 2;
-    int tile, in;
-    if (!lora_place(p.down, blockIdx.x, tile, in)) return;
+    LoraTile o;
+    const int* rows;
+    int in;
+    if (!tile_of(p, p.down, ws, o, rows, in)) return;
     const Share q = share_of(a, p, in);
-    const int64_t t0 = (int64_t)tile * (4 * kLoraSub), mine = t0 + 16 * sub + r;
-    const int id = adapter_of(a, t0, 4 * kLoraSub, lane), rk = ranks_of(a, id);
+    const int ranks = o.ranks - q.r0;
+    if (ranks <= 0) return;
+    const int64_t mine = rows[min(16 * sub + r, o.rows - 1)];
+    const bool busy = 16 * sub < o.rows;           // the wave has rows
     const int64_t units = (a.K + kLoraUnit - 1) / kLoraUnit;
     const int k0 = kLoraUnit * (int)(units * q.piece / p.pieces), k1 = min(a.K, kLoraUnit * (int)(units * (q.piece + 1) / p.pieces));
-    float* const out = ws + ((int64_t)q.part * p.pieces + q.piece) * a.T * a.rank;
-    const uint16_t* const x = a.X + min(mine, (int64_t)a.T - 1) * a.ldx;
+    const uint16_t* const x = a.X + mine * a.ldx;
+    const uint16_t* const A = a.part[q.part].A + ((int64_t)o.adapter * a.rank + q.r0) * a.K;
 
-    // Adapter and slab, in turn: where one's products run, the next one is on its way
-    struct At {
-        int k, ranks;
-        uint64_t rows;
-        const uint16_t* A;
-    };
-    uint64_t left = __ballot(id >= 0 && rk > q.r0);
-    auto next = [&](At& o) -> bool {
-        o.k += kLoraSlab;
-        if (o.k < k1) return true;
-        if (!left) return false;
-        const int first = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(id, first);
-        o.ranks = __builtin_amdgcn_readlane(rk, first) - q.r0;
-        o.rows = __ballot(id == e);
-        left &= ~o.rows;
-        o.A = a.part[q.part].A + ((int64_t)e * a.rank + q.r0) * a.K;
-        o.k = k0;
-        return true;
-    };
-    auto mine_in = [&](const At& o) -> bool { return (o.rows >> (16 * sub)) & 0xFFFFu; };
     h8 xv[2][STEPS];
     // (the buffer's readers have passed a barrier)
-    auto fetch = [&](const At& o, int buf, h8 (&v)[STEPS]) {
+    auto fetch = [&](int k, int buf, h8 (&v)[STEPS]) {
 #pragma unroll
         for (int i = 0; i < (LOADS + WV - 1) / WV; i++) {
             const int n = WV * i + wave;           // unit, eight rows
             if (n >= LOADS) break;
-            const int u = n / (2 * NT), m = n % (2 * NT), at = min(o.k + kLoraUnit * u + 8 * piece, a.K - 8);
-            dma16(o.A + (int64_t)min(8 * m + row, o.ranks - 1) * a.K + at, lds_addr(lds) + buf * BYTES + 1024 * n);
+            const int u = n / (2 * NT), m = n % (2 * NT), at = min(k + kLoraUnit * u + 8 * piece, a.K - 8);
+            dma16(A + (int64_t)min(8 * m + row, ranks - 1) * a.K + at, lds_addr(lds) + buf * BYTES + 1024 * n);
         }
-        if (mine_in(o))
+        if (busy)
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) v[i] = *(const h8*)(x + min(o.k + kLoraStep * (STEPS * half + i) + 8 * g, a.K - 8));
+            for (int i = 0; i < STEPS; i++) v[i] = *(const h8*)(x + min(k + kLoraStep * (STEPS * half + i) + 8 * g, a.K - 8));
     };
     f4 acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i] = f4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const At& o, int buf, const h8 (&v)[STEPS]) {
-        if (mine_in(o)) {
-            // A's operands are read a step ahead of their products
-            h8 w[2][NT];
-            auto read = [&](int i) {
-                const int n = STEPS * half + i;
+    auto multiply = [&](int k, int buf, const h8 (&v)[STEPS]) {
+        // A's operands are read a step ahead of their products
+        h8 w[2][NT];
+        auto read = [&](int i) {
+            const int n = STEPS * half + i;
 #pragma unroll
-                for (int m = 0; m < NT; m++)
-                    w[i & 1][m] = piece_of(lds + buf * BYTES + (n >> 1) * (2048 * NT), m, r, 4 * (n & 1) + g);
-            };
-            read(0);
+            for (int m = 0; m < NT; m++)
+                w[i & 1][m] = piece_of(lds + buf * BYTES + (n >> 1) * (2048 * NT), m, r, 4 * (n & 1) + g);
+        };
+        read(0);
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) {
-                const int at = o.k + kLoraStep * (STEPS * half + i);
-                if (at >= k1) break;
-                if (i + 1 < STEPS) read(i + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                const bool off = at + kLoraStep > k1, ok = at + 8 * g < k1;
-                const h8 b = off ? masked(v[i], ok) : v[i];
+        for (int i = 0; i < STEPS; i++) {
+            const int at = k + kLoraStep * (STEPS * half + i);
+            if (at >= k1) break;
+            if (i + 1 < STEPS) read(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool off = at + kLoraStep > k1, ok = at + 8 * g < k1;
+            const h8 b = off ? masked(v[i], ok) : v[i];
 #pragma unroll
-                for (int m = 0; m < NT; m++) acc[m] = mfma16x16x32(off ? masked(w[i & 1][m], ok) : w[i & 1][m], b, acc[m]);
-            }
-        }
-        if (o.k + kLoraSlab < k1) return;
-        // the adapter's last slab (what was here last has been read before this turn's barrier)
-        if (half)
-#pragma unroll
-            for (int m = 0; m < NT; m++) meet[sub][m][lane] = acc[m];
-        __syncthreads();
-#pragma unroll
-        for (int m = 0; m < NT; m++) {
-            const int at = q.r0 + 16 * m + 4 * g;
-            if (!half && ((o.rows >> (16 * sub + r)) & 1) && at < a.rank) *(f4*)(out + mine * a.rank + at) = acc[m] + meet[sub][m][lane];
-            acc[m] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int m = 0; m < NT; m++) acc[m] = mfma16x16x32(off ? masked(w[i & 1][m], ok) : w[i & 1][m], b, acc[m]);
         }
     };
-    // one turn; false after the last
-    auto turn = [&](const At& here, int buf, const h8 (&v)[STEPS], At& after, h8 (&w)[STEPS]) -> bool {
+    // one slab; false after the last
+    auto turn = [&](int k, int buf, const h8 (&v)[STEPS], h8 (&w)[STEPS]) -> bool {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();                           // this slab is here, the other one has been read
-        after = here;
-        const bool more = next(after);
-        if (more) fetch(after, 1 - buf, w);
-        multiply(here, buf, v);
+        const bool more = k + kLoraSlab < k1;
+        if (more) fetch(k + kLoraSlab, 1 - buf, w);
+        if (busy) multiply(k, buf, v);
         return more;
     };
-    At one, two;
-    one.k = k1;
-    if (!next(one)) return;
-    fetch(one, 0, xv[0]);
-    while (turn(one, 0, xv[0], two, xv[1]) && turn(two, 1, xv[1], one, xv[0])) {
+    fetch(k0, 0, xv[0]);
+    for (int k = k0; turn(k, 0, xv[0], xv[1]) && turn(k + kLoraSlab, 1, xv[1], xv[0]); k += 2 * kLoraSlab) {
+    }
+    __syncthreads();
+    if (half && busy)
+#pragma unroll
+        for (int m = 0; m < NT; m++) meet[sub][m][lane] = acc[m];
+    __syncthreads();
+    if (half || 16 * sub + r >= o.rows) return;
+    float* const out = ws + (((int64_t)q.part * p.pieces + q.piece) * a.T + mine) * a.rank;
+#pragma unroll
+    for (int m = 0; m < NT; m++) {
+        const int at = q.r0 + 16 * m + 4 * g;
+        if (at < a.rank) *(f4*)(out + at) = acc[m] + meet[sub][m][lane];
     }
 }
 
@@ -323,8 +399,9 @@ __device__ __forceinline__ int split_row(const float* s0, int64_t step, int piec
     }
 #pragma unroll
     for (int x = 1; x < PER; x <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
-    // (s is a sum of products of fp16 numbers, a multiple of 2^-48: the shift is at most 63)
-    const int shift = top > 0.f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+    // (s is a sum of products of fp16 numbers, a multiple of 2^-48 and below 2^57 where x is finite: the shift is -42 to 63;
+    // beside an infinity no number's value matters, but all stay finite)
+    const int shift = !(top > 0.f) ? 0 : top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : -48;
     const float up = __builtin_ldexpf(1.f, shift);
     for (int i = 0, k = 4 * me; k < padded; k += 4 * PER, i++) {
         const f4 s = i == 0 ? held[0] : i == 1 ? held[1] : sum4(s0, step, pieces, k, ranks);
@@ -333,7 +410,8 @@ __device__ __forceinline__ int split_row(const float* s0, int64_t step, int piec
         for (int j = 0; j < 4; j++) {
             const float v = s[j] * up;
             h[j] = (_Float16)v;
-            l[j] = (_Float16)(v - (float)h[j]);
+            const float rest = v - (float)h[j];
+            l[j] = (_Float16)(rest == rest ? rest : 0.f);                  // (an infinity has no rest)
         }
         put(k, uint2{as_u32(h2{h[0], h[1]}), as_u32(h2{h[2], h[3]})}, uint2{as_u32(h2{l[0], l[1]}), as_u32(h2{l[2], l[3]})});
     }
@@ -612,35 +690,39 @@ __global__ __launch_bounds__(64 * kLoraUpWaves) void k_lora_up(LoraArgs a, LoraP
     }
 }
 
-// Many rows: a workgroup takes 64 rows by 256 columns, wave w rows 16 (w % 4) .. and
-// columns 128 (w / 4) .. of those.  Operand j of its eight holds the columns that
-// leave a lane 16 neighbouring bytes of a row of C (8 i + j in fp16, 64 (j / 4) + 4 i
-// + j % 4 in fp32), so that a wave reads and writes runs of 256 bytes (128-byte runs
-// of 8-byte pieces: 25 us where this took 15).  Everything it needs is on its way at
-// once; a tile of several adapters takes them in turn.  JOIN: the pieces' sums are
-// joined here, for ranks that are one block; else k_lora_join did it.
+// Many rows: a workgroup takes a tile of 64 rows of one adapter by 256 columns, wave w
+// rows 16 (w % 4) .. and columns 128 (w / 4) .. of those.  Operand j of its eight holds
+// the columns that leave a lane 16 neighbouring bytes of a row of C (8 i + j in fp16, 64
+// (j / 4) + 4 i + j % 4 in fp32), so that a wave reads and writes runs of 256 bytes
+// (128-byte runs of 8-byte pieces: 25 us where this took 15).  JOIN: the pieces' sums are
+// joined here, for ranks that are one block; else k_lora_join did it.  Three workgroups a
+// CU where registers allow it without going to memory (2000 rows, rank 16: 25.5 us for all,
+// with two 27.0; rank 64, whose sums need more: 44 with three, 38 with two).
 template <int RC, bool F16, bool JOIN>
-__global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
+__global__ __launch_bounds__(64 * kLoraUpWaves, RC < 64 && F16 ? 6 : 4) void k_lora_up_many(LoraArgs a, LoraPlan p, float* __restrict__ ws) {
     constexpr int WV = kLoraUpWaves, ROWS = 64, COLS = 128, PIECES = RC / 8, KS = (RC + 31) / 32, BYTES = 2 * COLS * RC;
     constexpr int SH = F16 ? 3 : 2, PER = F16 ? 1 : 2, W = F16 ? 8 : 4;    // runs of a lane in a row, their columns
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BYTES + 2 * 2 * ROWS * RC];   // two blocks of B, the sums' hi and lo
     __shared__ float factor[ROWS];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), sub = wave & 3;
-    int tile, at;
-    if (!lora_place(p.up, blockIdx.x, tile, at)) return;
+    LoraTile o;
+    const int* rows;
+    int at;
+    if (!tile_of(p, p.up, ws, o, rows, at)) return;
+    const int ranks = o.ranks;
+    if (ranks == 0 && a.Y == a.C) return;          // (no adapter, in place)
     const int part = part_of(a, p.up_steps, at);
     const LoraPart& w = a.part[part];
     const int n = at * p.up_steps * kLoraCols + COLS * (wave >> 2), col = n + W * r;         // (the lane's second run: col + 64)
-    const int64_t t0 = (int64_t)tile * ROWS, lt = t0 + 16 * sub + 4 * g;   // (the lane's rows: lt + i)
-    const int id = adapter_of(a, t0, ROWS, lane), rk = ranks_of(a, id);
+    const int t = rows[min(lane, o.rows - 1)];                // lane l: the tile's row l
     const Joined sums = joined_of(a, p, ws);
     uint8_t* const block = lds + (wave >> 2) * BYTES;
     uint8_t* const rows_lds = lds + 2 * BYTES;                             // [hi, lo][64 rows][RC]
 
-    // the wave's quarter of its block: ranks k0 .. of adapter e, as far as they count; and its share of the sums
-    auto fetch = [&](int e, int ranks, int k0) {
-        const uint16_t* const B = w.B + (int64_t)e * w.N * a.rank;
+    // the wave's quarter of its block: ranks k0 .., as far as they count; and its share of the sums
+    auto fetch = [&](int k0) {
+        const uint16_t* const B = w.B + (int64_t)o.adapter * w.N * a.rank;
 #pragma unroll
         for (int i = 0; i < PIECES / 2; i++) {
             const int m = 4 * i + sub, q = 64 * m + lane, c = q / PIECES, k = k0 + 8 * place<RC, SH>(c, q % PIECES);
@@ -652,49 +734,31 @@ __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs 
             const int m = WV * i + wave;
             if (m >= 2 * PIECES) break;
             const int q = 64 * (m % PIECES) + lane, row = q / PIECES, k = k0 + 8 * place<RC, 0>(row, q % PIECES);
-            const _Float16* const s = (m < PIECES ? sums.hi : sums.lo) + ((int64_t)part * a.T + min(t0 + row, (int64_t)a.T - 1)) * p.padded;
+            const _Float16* const s = (m < PIECES ? sums.hi : sums.lo) + ((int64_t)part * a.T + __shfl(t, row)) * p.padded;
             if (k < p.padded) dma16(s + k, lds_addr(rows_lds) + 1024 * m);
         }
     };
-    uint64_t left = __ballot(id != -2), rows = 0;
-    int e = -1, ranks = 0;
-    auto next = [&]() {
-        const int first = __builtin_ctzll(left);
-        e = __builtin_amdgcn_readlane(id, first);
-        ranks = __builtin_amdgcn_readlane(rk, first);
-        rows = __ballot(id == e);
-        left &= ~rows;
-    };
-    next();
-    if (ranks > 0) fetch(e, ranks, 0);
-    typename Run<F16>::type c[4][PER];             // what is added to
+    if (ranks > 0) fetch(0);
+    f4 acc[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int h = 0; h < PER; h++)
-            c[i][h] = load_run<F16>(a, (lt + i) * a.ldc + w.at + col + 64 * h, lt + i < a.T ? w.N - col - 64 * h : 0);
-    if (JOIN) {
-        const int row = tid / 8, mr = __shfl(rk, row), me = __shfl(id, row);
-        const int shift = split_row<8>(ws + ((int64_t)part * p.pieces * a.T + t0 + row) * a.rank, (int64_t)a.T * a.rank, p.pieces, mr,
-                                       tid % 8, RC, [&](int k, uint2 hi, uint2 lo) {
-                                           uint8_t* const to = rows_lds + row * (2 * RC) + 16 * place<RC, 0>(row, k / 8) + 2 * (k & 7);
-                                           *(uint2*)to = hi;
-                                           *(uint2*)(to + 2 * ROWS * RC) = lo;
-                                       });
-        if (tid % 8 == 0) factor[row] = me < 0 ? 0.f : __builtin_ldexpf(a.scales ? a.scales[me] : 1.f, -shift);
-    } else if (tid < ROWS) {
-        factor[tid] = t0 + tid < a.T ? sums.factor[(int64_t)part * a.T + t0 + tid] : 0.f;
-    }
-    __syncthreads();
-    for (;;) {
-        f4 acc[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
-        const bool mine = (rows >> (16 * sub)) & 0xFFFFu;
+    for (int j = 0; j < 8; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+    if (ranks > 0) {
+        if (JOIN) {
+            const int row = tid / 8, mr = row < o.rows ? ranks : 0;
+            const int shift = split_row<8>(ws + ((int64_t)part * p.pieces * a.T + __shfl(t, row)) * a.rank, (int64_t)a.T * a.rank,
+                                           p.pieces, mr, tid % 8, RC, [&](int k, uint2 hi, uint2 lo) {
+                                               uint8_t* const to = rows_lds + row * (2 * RC) + 16 * place<RC, 0>(row, k / 8) + 2 * (k & 7);
+                                               *(uint2*)to = hi;
+                                               *(uint2*)(to + 2 * ROWS * RC) = lo;
+                                           });
+            if (tid % 8 == 0) factor[row] = __builtin_ldexpf(a.scales ? a.scales[o.adapter] : 1.f, -shift);
+        } else if (tid < ROWS) {
+            factor[tid] = sums.factor[(int64_t)part * a.T + t];
+        }
         for (int k0 = 0; k0 < ranks; k0 += RC) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (mine) {
+            if (16 * sub < o.rows) {
                 const int row = 16 * sub + r;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
@@ -716,39 +780,36 @@ __global__ __launch_bounds__(64 * kLoraUpWaves, 4) void k_lora_up_many(LoraArgs 
             }
             if (k0 + RC < ranks) {
                 __syncthreads();                   // the blocks have been read
-                fetch(e, ranks, k0 + RC);
+                fetch(k0 + RC);
             }
         }
-        const uint64_t these = rows;
-        const int had = ranks;
-        if (left) {                                // the tile's next adapter
-            next();
-            if (ranks > 0) {
-                __syncthreads();
-                fetch(e, ranks, 0);
-            }
-        } else {
-            e = -2;
-        }
-        if (mine && (had > 0 || a.Y != a.C)) {     // (no adapter: a copy, through no arithmetic)
-            const f4 f = *(const f4*)(factor + 16 * sub + 4 * g);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int h = 0; h < PER; h++) {
-                    typename Run<F16>::type y = c[i][h];
-                    if (had > 0) {
-                        float d[W];
-#pragma unroll
-                        for (int j = 0; j < W; j++) d[j] = acc[4 * h + j][i];
-                        y = add_run(y, f[i], d);
-                    }
-                    const bool in = (these >> (16 * sub + 4 * g + i)) & 1;
-                    store_run<F16>(a, (lt + i) * a.ldy + w.at + col + 64 * h, y, in ? w.N - col - 64 * h : 0);
-                }
-        }
-        if (e == -2) return;
     }
+    typename Run<F16>::type c[4][PER];             // what is added to, of rows 16 sub + 4 g + i
+    int64_t tr[4];
+    bool in[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        tr[i] = __shfl(t, 16 * sub + 4 * g + i);
+        in[i] = 16 * sub + 4 * g + i < o.rows;
+#pragma unroll
+        for (int h = 0; h < PER; h++)
+            c[i][h] = load_run<F16>(a, tr[i] * a.ldc + w.at + col + 64 * h, in[i] ? w.N - col - 64 * h : 0);
+    }
+    f4 f = f4{0.f, 0.f, 0.f, 0.f};
+    if (ranks > 0) f = *(const f4*)(factor + 16 * sub + 4 * g);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int h = 0; h < PER; h++) {
+            typename Run<F16>::type y = c[i][h];
+            if (ranks > 0) {                       // (no adapter: a copy, through no arithmetic)
+                float d[W];
+#pragma unroll
+                for (int j = 0; j < W; j++) d[j] = acc[4 * h + j][i];
+                y = add_run(y, f[i], d);
+            }
+            store_run<F16>(a, tr[i] * a.ldy + w.at + col + 64 * h, y, in[i] ? w.N - col - 64 * h : 0);
+        }
 }
 
 template <class K> hipError_t raise_lds(K k, std::atomic<uint64_t>& set, int bytes) {
@@ -763,7 +824,7 @@ template <class K> hipError_t raise_lds(K k, std::atomic<uint64_t>& set, int byt
 }
 
 template <int NT> hipError_t down(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
-    constexpr int few = kLoraDownWaves * 2 * kUnitBytes<NT>, many = 2 * kLoraSlab / kLoraUnit * NT * 2048 + 4 * NT * 1024;
+    constexpr int few = kLoraDownWaves * 2 * kUnitBytes<NT>, many = 2 * kLoraSlab / kLoraUnit * NT * 2048;
     static std::atomic<uint64_t> set{0}, set_many{0};                      // one bit per device: LDS limit raised
     auto k = p.many ? k_lora_down_many<NT> : k_lora_down<NT>;
     const int lds = p.many ? many : few;
@@ -803,8 +864,14 @@ template <int RC, bool F16> hipError_t up(const LoraArgs& a, const LoraPlan& p, 
     return up_many<RC, F16, true>(a, p, ws, st);
 }
 
+hipError_t order(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
+    hipLaunchKernelGGL(k_lora_order, dim3(1), dim3(kOrderThreads), 0, st, a, p, ws);
+    return hipGetLastError();
+}
+
 template <int RC> hipError_t both(const LoraArgs& a, const LoraPlan& p, float* ws, hipStream_t st) {
-    const hipError_t e = down<RC / 16>(a, p, ws, st);
+    hipError_t e = p.many ? order(a, p, ws, st) : hipSuccess;
+    if (e == hipSuccess) e = down<RC / 16>(a, p, ws, st);
     if (e != hipSuccess) return e;
     return a.out_f16 ? up<RC, true>(a, p, ws, st) : up<RC, false>(a, p, ws, st);
 }

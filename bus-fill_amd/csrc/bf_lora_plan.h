@@ -11,7 +11,8 @@ namespace bf {
 constexpr int kLoraParts = 4;
 constexpr int kLoraMaxRank = 1024;
 constexpr int kLoraSub = 16;                       // rows of a matrix operand, and of a tile of few rows
-constexpr int kLoraMany = 256;                     // rows from which on tiles are of 64
+constexpr int kLoraMany = 256;                     // more rows, two an adapter or more: sorted by adapter, tiles of 64
+constexpr int kLoraBins = 2048;                    // ... with fewer adapters than that
 constexpr int kLoraRanks = 64;                     // ranks of a workgroup of the down products (four operands)
 constexpr int kLoraCols = 64;                      // columns of a wave of the up products
 constexpr int kLoraStep = 32;                      // k of a matrix instruction
@@ -45,6 +46,11 @@ struct LoraArgs {
     int T, K;
 };
 
+#ifdef __HIPCC__
+#define BF_BOTH __host__ __device__
+#else
+#define BF_BOTH
+#endif
 // Workgroups of a launch: `inner` for each of `tiles` tiles of rows.  Where there
 // are many tiles, each XCD takes a run of them, whose adapters and sums its L2
 // then holds; few are spread over all.
@@ -52,7 +58,7 @@ struct LoraGrid {
     int tiles, inner, per_xcd;                     // per_xcd: tiles of an XCD (0: spread)
     int64_t groups;
 };
-inline LoraGrid lora_grid(int tiles, int64_t inner) {
+BF_BOTH inline LoraGrid lora_grid(int tiles, int64_t inner) {
     LoraGrid g;
     g.tiles = tiles;
     g.inner = (int)inner;
@@ -61,37 +67,44 @@ inline LoraGrid lora_grid(int tiles, int64_t inner) {
     return g;
 }
 
-// Workgroup b's tile and which of the tile's it is; false where there is none.
-#ifdef __HIPCC__
-__host__ __device__
-#endif
-inline bool lora_place(const LoraGrid& g, int b, int& tile, int& in) {
+// Workgroup b's tile and which of the tile's it is; false where there is none (b may be past the grid: one made for more tiles).
+BF_BOTH inline bool lora_place(const LoraGrid& g, int b, int& tile, int& in) {
+    if (g.tiles < 1) return false;
     if (g.per_xcd) {
-        const int turn = b / kLoraXcds;
-        tile = b % kLoraXcds * g.per_xcd + turn / g.inner;
+        const int turn = b / kLoraXcds, nth = turn / g.inner;
+        tile = b % kLoraXcds * g.per_xcd + nth;
         in = turn % g.inner;
-    } else {
-        tile = b % g.tiles;
-        in = b / g.tiles;
+        return nth < g.per_xcd && tile < g.tiles;
     }
-    return tile < g.tiles;
+    tile = b % g.tiles;
+    in = b / g.tiles;
+    return in < g.inner;
 }
+#undef BF_BOTH
+
+// Many rows: `rows` rows of an adapter (-1: rows without one) and the ranks that count.
+struct LoraTile {
+    int adapter, rows, ranks, unused;
+};
 
 // Few rows (tiles of 16): down, a workgroup takes a tile, a part, up to 64 ranks, a
 // piece of K (its waves shares of that) and every `sharers`-th of the tile's
 // adapters; up, a workgroup takes a tile, up_steps steps of 64 columns of a part and
-// all of the tile's adapters, its waves the pairs of adapter and step in turn, and adds the pieces' sums first.  Many rows (tiles of 64): down, a tile, a
-// part, up to 64 ranks, and a piece of K; a join of the pieces; up, a tile and four
-// steps of columns.
+// all of the tile's adapters, its waves the pairs of adapter and step in turn, and
+// adds the pieces' sums first.  Many rows: an order of the rows by adapter, then
+// down, a workgroup takes a tile of 64 rows of one adapter, a part, up to 64 ranks and a piece
+// of K; up, a tile and four steps of columns, with the pieces' sums (of more than 64
+// ranks: joined in a launch of its own).
 struct LoraPlan {
     int many;
     int rank_parts, rank_tiles;                    // rank_tiles: operands of ranks of a down workgroup (1, 2 or 4)
     int padded;                                    // many: ranks of the joined sums, in whole blocks
     int pieces, sharers;
     int up_steps;
-    LoraGrid down, up;
-    int64_t joined;                                // many: fp32 words of the partial sums, behind which the joined ones lie
-    size_t bytes;                                  // [part][piece][T][rank] fp32; many: hi and lo [part][T][padded] fp16, [part][T] factors
+    int most;                                      // many: as many tiles as there can be (how many there are is found on the device)
+    LoraGrid down, up;                             // many: of `most` tiles
+    int64_t tiles, rows, joined;                   // many: where [most + 1] tiles (the last: their number), their rows [most][64] and the joined sums lie, in words
+    size_t bytes;                                  // [part][piece][T][rank] fp32; many: also the above, joined: hi and lo [part][T][padded] fp16, [part][T] factors
 };
 
 // Ranks of B that come to LDS at once.
@@ -101,17 +114,21 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
     LoraPlan p;
     const auto tiles = [&](int rows) { return a.T / rows + (a.T % rows ? 1 : 0); };
     const int rc = lora_block(a.rank);
-    p.many = a.T > kLoraMany;
+    p.many = a.T > kLoraMany && a.adapters <= a.T / 2 && a.adapters < kLoraBins;
     const int t = tiles(p.many ? 4 * kLoraSub : kLoraSub), per_tile = std::min(std::min(a.T, kLoraSub), a.adapters);
+    p.most = p.many ? a.T / (4 * kLoraSub) + std::min(a.adapters + 1, a.T) : t;    // (each adapter's last tile may hold fewer rows)
     p.rank_parts = (a.rank + kLoraRanks - 1) / kLoraRanks;
     p.rank_tiles = rc / 16;
     p.padded = (a.rank + rc - 1) / rc * rc;
-    p.sharers = p.many ? 1 : per_tile;             // (of many rows, neighbours are mostly of one adapter)
+    p.sharers = p.many ? 1 : per_tile;
     const int64_t base = (int64_t)t * p.rank_parts * a.parts * p.sharers;
     // at least two units a wave, or a slab
     const int64_t least = p.many ? kLoraSlab : 2 * kLoraDownWaves * kLoraUnit, most = std::min<int64_t>(kLoraPieces, a.K / least);
-    p.pieces = (int)std::min(std::max<int64_t>(1, most), std::max<int64_t>(1, 2 * cus / base));
-    p.down = lora_grid(t, (int64_t)p.rank_parts * a.parts * p.sharers * p.pieces);
+    // few: two workgroups a CU; many: one, with as many short tiles as a handful of adapters make, or two where that leaves one
+    // piece (2000 rows of six adapters, rank 64: 6 pieces 34.3 us, 8, which are more workgroups than CUs, 38.5; 4000: 3 pieces 47, 8 54)
+    const int64_t one = p.many ? cus / (base + 8) : 0;
+    p.pieces = (int)std::min(std::max<int64_t>(1, most), one >= 2 ? one : std::max<int64_t>(1, 2 * cus / base));
+    p.down = lora_grid(p.most, (int64_t)p.rank_parts * a.parts * p.sharers * p.pieces);
     int64_t cols = 0;                              // steps of columns of all parts
     for (int i = 0; i < a.parts; i++) cols += (a.part[i].N + kLoraCols - 1) / kLoraCols;
     // few: as many steps a workgroup as leave two workgroups a CU
@@ -121,8 +138,10 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
         const int64_t n = (a.part[i].N + kLoraCols - 1) / kLoraCols;
         groups += (n + p.up_steps - 1) / p.up_steps;
     }
-    p.up = lora_grid(t, groups);
-    p.joined = (int64_t)a.parts * p.pieces * a.T * a.rank;
+    p.up = lora_grid(p.most, groups);
+    p.tiles = (int64_t)a.parts * p.pieces * a.T * a.rank;
+    p.rows = p.tiles + (p.many ? 4 * ((int64_t)p.most + 1) : 0);
+    p.joined = p.rows + (p.many ? 64 * (int64_t)p.most : 0);
     p.bytes = (size_t)p.joined * sizeof(float);
     if (p.many && a.rank > rc) p.bytes += (size_t)a.parts * a.T * (4 * (size_t)p.padded + 4);
     return p;

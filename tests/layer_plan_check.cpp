@@ -21,10 +21,11 @@ void expect(bool ok, const char* what, int64_t a = 0, int64_t b = 0, int64_t c =
     std::printf("FAIL %s (%lld, %lld, %lld)\n", what, (long long)a, (long long)b, (long long)c);
 }
 
-// Every (tile, share) has one workgroup.
-void check_grid(const LoraGrid& g, int tiles, int64_t inner) {
+// Every (tile, share) of `tiles` tiles has one of the grid's workgroups (a grid may be made for more tiles than there are).
+void check_grid(const LoraGrid& made, int tiles, int64_t inner) {
     std::vector<int> seen((size_t)(tiles * inner), 0);
-    for (int64_t b = 0; b < g.groups; b++) {
+    const LoraGrid g = lora_grid(tiles, inner);
+    for (int64_t b = 0; b < made.groups; b++) {
         int tile = -1, in = -1;
         if (!lora_place(g, (int)b, tile, in)) continue;
         expect(tile >= 0 && tile < tiles && in >= 0 && in < inner, "workgroup in its tile", b, tile, in);
@@ -38,7 +39,7 @@ void check_lora() {
         for (int T : {1, 5, 16, 17, 100, 256, 257, 600, 2000, 5000})
             for (int K : {8, 64, 1000, 5120, 17408})
                 for (int rank : {8, 16, 24, 64, 72, 256, 1024})
-                    for (int E : {1, 3, 64})
+                    for (int E : {1, 3, 64, 700, 5000})
                         for (int N : {1, 64, 300, 5120}) {
                             LoraArgs a;
                             std::memset(&a, 0, sizeof a);
@@ -53,7 +54,9 @@ void check_lora() {
                             expect(p.pieces >= 1 && p.pieces <= kLoraPieces, "pieces", p.pieces);
                             expect((int64_t)p.rank_parts * kLoraRanks >= rank && (int64_t)(p.rank_parts - 1) * kLoraRanks < rank, "ranks", rank);
                             expect(p.padded >= rank && p.padded % lora_block(rank) == 0, "padded ranks", rank, p.padded);
-                            const int most = E < rows ? E : rows;          // adapters that a tile can have
+                            const int most = E < rows ? E : rows;          // adapters that a tile of few rows can have
+                            expect(p.many == (T > 256 && E <= T / 2 && E < 2048), "many", T, p.many);
+                            expect(p.most >= tiles && (!p.many || p.most >= tiles + (E + 1 < T ? E : T - tiles)), "tiles", T, E, p.most);
                             expect(p.many ? p.sharers == 1 : p.sharers >= (most < T ? most : T), "sharers", T, E, p.sharers);
                             // pieces of K: units of 64, none empty of all waves' shares
                             const int64_t units = (K + kLoraUnit - 1) / kLoraUnit;
@@ -63,13 +66,18 @@ void check_lora() {
                             for (int i = 0; i < a.parts; i++)
                                 groups += ((a.part[i].N + kLoraCols - 1) / kLoraCols + p.up_steps - 1) / p.up_steps;
                             if (cus == 256 && K == 5120) {
-                                check_grid(p.down, tiles, (int64_t)p.rank_parts * a.parts * p.sharers * p.pieces);
-                                check_grid(p.up, tiles, groups);
+                                for (int n : {tiles, p.most, (tiles + p.most) / 2, 31, 32, 33}) {
+                                    if (n < tiles || n > p.most) continue;
+                                    check_grid(p.down, n, (int64_t)p.rank_parts * a.parts * p.sharers * p.pieces);
+                                    check_grid(p.up, n, groups);
+                                }
                             }
                             const int64_t sums = (int64_t)a.parts * p.pieces * T * rank;
-                            expect(p.joined == sums, "partial sums", p.joined, sums);
+                            expect(p.tiles == sums && p.tiles % 4 == 0, "partial sums", p.tiles, sums);
+                            expect(p.rows - p.tiles == (p.many ? 4 * (p.most + 1) : 0), "tiles' place", p.rows, p.tiles, p.most);
+                            expect(p.joined - p.rows == (p.many ? 64 * (int64_t)p.most : 0) && p.joined % 4 == 0, "rows' place", p.joined, p.rows, T);
                             const int64_t joined = p.many && rank > 64 ? (int64_t)a.parts * T * (4 * p.padded + 4) : 0;
-                            expect((int64_t)p.bytes == 4 * sums + joined, "bytes", (int64_t)p.bytes, 4 * sums + joined);
+                            expect((int64_t)p.bytes == 4 * p.joined + joined, "bytes", (int64_t)p.bytes, 4 * p.joined + joined);
                             expect(p.many || 8 * 2 * kLoraCols * lora_block(rank) + 64 * lora_lds_ranks(rank) <= 159 * 1024, "LDS", rank);
                         }
 }

@@ -267,3 +267,68 @@ def test_other_stream_and_graph():
         with pytest.raises(bf.BusfillError) as err:
             bf.lora(big.dx, big.dids, big.parts, big.dc, out, **kw)
     assert err.value.status == bf.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("T,adapters,rank,otype", [
+    (300, 64, 16, bf.OUT_F16), (700, 9, 64, bf.OUT_F32), (257, 128, 72, bf.OUT_F16), (4097, 3, 8, bf.OUT_F16),
+    (9000, 40, 16, bf.OUT_F32), (4160, 2047, 8, bf.OUT_F32)])
+@pytest.mark.parametrize("place", ["in", "out"])
+def test_many_rows_in_no_order(T, adapters, rank, otype, place):
+    """Rows that are sorted by adapter: more than the sort takes at once, adapters with one row, many, none, rows without one."""
+    g = torch.Generator().manual_seed(T)
+    ids = torch.randint(-1, adapters + 1, (T,), generator=g)
+    ids[torch.rand(T, generator=g) < 0.3] = adapters // 2                  # many of one
+    if adapters > 5:
+        ids[ids == 3] = 4                                                  # none of another
+    Case(T, 40, [70], adapters, rank, ids=ids.tolist(), ranks=[(7 * e) % (rank + 1) for e in range(adapters)], otype=otype,
+         pad=2).run(place=place, workspace=True)
+
+
+@pytest.mark.parametrize("T,adapters", [(300, 151), (300, 2500), (5000, 2048)])
+def test_many_rows_of_as_many_adapters(T, adapters):
+    """Fewer than two rows an adapter, or more adapters than the sort counts: rows as they come."""
+    Case(T, 24, [20], adapters, 8).run()
+
+
+def test_sorted_rows_give_the_same_bits():
+    """The order that rows come in, and the one that the sort gives an adapter's rows, change no bits."""
+    c = Case(1500, 640, [260], 7, 32, otype=bf.OUT_F32)
+    kw = c.device()
+
+    def call(x, ids, into):
+        y = torch.empty_like(into)
+        bf.lora(x, ids, c.parts, into, y, **kw)
+        torch.cuda.synchronize()
+        return y
+
+    first = call(c.dx, c.dids, c.dc)
+    for i in range(4):
+        p = torch.randperm(1500, generator=torch.Generator().manual_seed(i)).cuda() if i else c.dids.argsort(stable=True)
+        assert torch.equal(call(c.dx[p].contiguous(), c.dids[p].contiguous(), c.dc[p].contiguous()), first[p])
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_rank_1024(T):
+    Case(T, 128, [90], 2, 1024, ranks=[1024, 777]).run()
+
+
+@pytest.mark.parametrize("T", [20, 300])
+def test_infinities_reach_the_output_as_the_formula_has_them(T):
+    """An infinity in a row of X: every output infinite with the sign of the sum, or NaN where infinities of both signs meet."""
+    c = Case(T, 64, [48], 2, 16, ids=[0] * T)
+    c.x[3, 5], c.x[7, 9] = float("inf"), float("-inf")
+    kw = c.device()
+    y = torch.empty_like(c.dc)
+    bf.lora(c.dx, c.dids, c.parts, c.dc, y, **kw)
+    torch.cuda.synchronize()
+    (a, b), s = c.ab[0], float(c.scales[0])
+    for t, r in ((3, 16), (7, 16)):
+        want = c.c[t].double() + s * (b[0].double() @ (a[0].double() @ c.x[t].double()))
+        assert torch.equal(torch.isnan(y[t].cpu()), torch.isnan(want))
+    # one rank: no infinities of both signs
+    kw["ranks"] = torch.ones(2, dtype=torch.int32, device="cuda")
+    bf.lora(c.dx, c.dids, c.parts, c.dc, y, **kw)
+    torch.cuda.synchronize()
+    for t in (3, 7):
+        want = c.c[t].double() + s * (b[0, :, :1].double() @ (a[0, :1].double() @ c.x[t].double()))
+        assert torch.isinf(want).any() and torch.equal(y[t].cpu().double(), want)
