@@ -9,6 +9,12 @@
 // registers (LDS where rows are not of whole 16-byte pieces) between the sum of
 // squares and the product.  Sums are fp32 over at most 32 values a thread, then
 // across lanes; where squares leave fp32's range they are summed again in 64 bits.
+//
+// Measured, fp32 residual, fp16 addend, rows of 5120: 2000 rows 26.7 us for 123 MB
+// (4.6 TB/s; a copy of 2 GiB reaches 4.9); 32 rows 4.0 us in the kernel and 4.8 to 5.0 a
+// call from Python, 16 rows to int8 4.7 in the kernel: load, two barriers of a workgroup's
+// sums, store, and the launch.  Codes: one division a block and a product a value
+// (a division a value: 0.3 us more).
 #include <atomic>
 
 #include "bf_device.h"
