@@ -332,3 +332,52 @@ def test_infinities_reach_the_output_as_the_formula_has_them(T):
     for t in (3, 7):
         want = c.c[t].double() + s * (b[0, :, :1].double() @ (a[0, :1].double() @ c.x[t].double()))
         assert torch.isinf(want).any() and torch.equal(y[t].cpu().double(), want)
+
+
+@pytest.mark.parametrize("T", [30, 400])
+@pytest.mark.parametrize("otype", [bf.OUT_F32, bf.OUT_F16])
+def test_rows_apart(T, otype):
+    """X, C and Y with strides of their own; what lies between the rows is left alone."""
+    c = Case(T, 88, [60, 20], 5, 24, ids=[(3 * t) % 7 - 1 for t in range(T)], otype=otype)
+    kw = c.device()
+    x = torch.full((T, 104), float("nan"), dtype=F16, device="cuda")
+    x[:, :88] = c.dx
+    into = torch.full((T, 96), float("nan"), dtype=c.dc.dtype, device="cuda")
+    into[:, :80] = c.dc
+    y = torch.full((T, 85), 9.0, dtype=c.dc.dtype, device="cuda")
+    kw.update(ldx=104, ldc=96, ldy=85)
+    torch.cuda.synchronize()
+    bf.lora(x, c.dids, c.parts, into, y, **kw)
+    torch.cuda.synchronize()
+    c.check(y[:, :80])
+    assert (y[:, 80:] == 9.0).all()
+
+
+def test_many_rows_in_a_graph_and_on_two_streams():
+    """Replays sort the ids of the moment; calls at once on two streams have workspaces of their own."""
+    c = Case(700, 640, [260], 9, 32, otype=bf.OUT_F16)
+    kw = c.device()
+    y, z, w = (torch.empty_like(c.dc) for _ in range(3))
+    a = bf.lora_args(c.dx, c.dids, c.parts, c.dc, y, **kw)
+    n = bf.lora_workspace_bytes(a)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=one):
+        bf.lora_ws(a, ws, n)
+    other = torch.empty_like(c.dids)
+    for i in range(4):
+        c.dids.copy_((c.dids * 5 + 1 + i) % 11 - 1)                        # (some without an adapter)
+        other.copy_(c.dids.flip(0))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        bf.lora(c.dx, c.dids, c.parts, c.dc, z, stream=one.cuda_stream, **kw)
+        bf.lora(c.dx, other, c.parts, c.dc, w, stream=two.cuda_stream, **kw)
+        torch.cuda.synchronize()
+        c.ids = c.dids.cpu()
+        c.check(y)
+        assert torch.equal(y, z)
+        c.ids = other.cpu()
+        c.check(w)
