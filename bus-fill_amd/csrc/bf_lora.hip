@@ -2,7 +2,7 @@
 //   Y[t] = C[t] + scale_e B_e (A_e x[t]),  e = ids[t]  (no adapter: Y[t] = C[t]),
 // for up to four parts (a fused projection's slices), each with its A and B.
 //
-// Up to 256 rows, two launches: s = A x in fp32 (k_lora_down), then C + scale B s
+// Up to 128 rows (256 of fewer than eight adapters), two launches: s = A x in fp32 (k_lora_down), then C + scale B s
 // (k_lora_up).  Rows are taken as they come, in tiles of 16, which may be of as many
 // adapters; each adapter of a tile is multiplied with the whole tile (an operand of
 // 16x16x32 MFMAs), of which its own rows are kept.  Single tokens of many requests are

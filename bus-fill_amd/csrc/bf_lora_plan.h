@@ -11,7 +11,8 @@ namespace bf {
 constexpr int kLoraParts = 4;
 constexpr int kLoraMaxRank = 1024;
 constexpr int kLoraSub = 16;                       // rows of a matrix operand, and of a tile of few rows
-constexpr int kLoraMany = 256;                     // more rows, two an adapter or more: sorted by adapter, tiles of 64
+constexpr int kLoraMany = 128;                     // more rows, two an adapter or more: sorted by adapter, tiles of 64
+constexpr int kLoraManyFew = 256;                  // ... with fewer than eight adapters
 constexpr int kLoraBins = 2048;                    // ... with fewer adapters than that
 constexpr int kLoraRanks = 64;                     // ranks of a workgroup of the down products (four operands)
 constexpr int kLoraCols = 64;                      // columns of a wave of the up products
@@ -114,7 +115,9 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
     LoraPlan p;
     const auto tiles = [&](int rows) { return a.T / rows + (a.T % rows ? 1 : 0); };
     const int rc = lora_block(a.rank);
-    p.many = a.T > kLoraMany && a.adapters <= a.T / 2 && a.adapters < kLoraBins;
+    // (192 rows in no order, as they come and sorted: 8 adapters of rank 64 26 and 19 us, 64 of rank 16 29 and 24, 4 of rank 16
+    // 14 and 18; in runs 14 and 19, 18 and 24, 11 and 18.  At 100 rows the first two meet.)
+    p.many = a.T > (a.adapters < 8 ? kLoraManyFew : kLoraMany) && a.adapters <= a.T / 2 && a.adapters < kLoraBins;
     const int t = tiles(p.many ? 4 * kLoraSub : kLoraSub), per_tile = std::min(std::min(a.T, kLoraSub), a.adapters);
     p.most = p.many ? a.T / (4 * kLoraSub) + std::min(a.adapters + 1, a.T) : t;    // (each adapter's last tile may hold fewer rows)
     p.rank_parts = (a.rank + kLoraRanks - 1) / kLoraRanks;

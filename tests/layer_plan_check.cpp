@@ -36,7 +36,7 @@ void check_grid(const LoraGrid& made, int tiles, int64_t inner) {
 
 void check_lora() {
     for (int cus : {64, 256, 304})
-        for (int T : {1, 5, 16, 17, 100, 256, 257, 600, 2000, 5000})
+        for (int T : {1, 5, 16, 17, 100, 128, 129, 256, 257, 600, 2000, 5000})
             for (int K : {8, 64, 1000, 5120, 17408})
                 for (int rank : {8, 16, 24, 64, 72, 256, 1024})
                     for (int E : {1, 3, 64, 700, 5000})
@@ -55,7 +55,7 @@ void check_lora() {
                             expect((int64_t)p.rank_parts * kLoraRanks >= rank && (int64_t)(p.rank_parts - 1) * kLoraRanks < rank, "ranks", rank);
                             expect(p.padded >= rank && p.padded % lora_block(rank) == 0, "padded ranks", rank, p.padded);
                             const int most = E < rows ? E : rows;          // adapters that a tile of few rows can have
-                            expect(p.many == (T > 256 && E <= T / 2 && E < 2048), "many", T, p.many);
+                            expect(p.many == ((T > 256 || (T > 128 && E >= 8)) && E <= T / 2 && E < 2048), "many", T, p.many);
                             expect(p.most >= tiles && (!p.many || p.most >= tiles + (E + 1 < T ? E : T - tiles)), "tiles", T, E, p.most);
                             expect(p.many ? p.sharers == 1 : p.sharers >= (most < T ? most : T), "sharers", T, E, p.sharers);
                             // pieces of K: units of 64, none empty of all waves' shares

@@ -381,3 +381,9 @@ def test_many_rows_in_a_graph_and_on_two_streams():
         assert torch.equal(y, z)
         c.ids = other.cpu()
         c.check(w)
+
+
+@pytest.mark.parametrize("T,adapters", [(128, 8), (129, 7), (129, 8), (129, 64), (129, 65), (256, 7), (257, 7)])
+@pytest.mark.parametrize("rank", [16, 96])
+def test_where_the_sort_begins(T, adapters, rank):
+    Case(T, 72, [90, 6], adapters, rank, otype=bf.OUT_F16).run()
