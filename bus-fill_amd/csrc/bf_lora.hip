@@ -28,8 +28,10 @@
 // workspace, added in their order by the next kernel), so that a few rows fill the
 // chip.
 // Up: s, times a power of two that brings the row's largest to 2^14..2^15, is
-// taken as two fp16 numbers (rounded, and the rest rounded: 2^-22 of the largest), so
-// the products lose nothing that fp32 would keep; sums fp32, one rounding of Y.
+// taken as two fp16 numbers of its sign (cut, and the rest rounded: 2^-22 of the
+// largest), neither 0 unless s is: times an infinity of B both give the infinity
+// that s gives, where a rest of 0 or of the other sign would give NaN.  Sums fp32,
+// one rounding of Y.
 //
 // Measured, K = 5120, fp16 C and Y.  One row, rank 16, parts of 5120, 1024 and 1024
 // columns: 10.2 us, 4.1 down and 5.9 up; a launch that does nothing is 2.5, the rest
@@ -383,6 +385,25 @@ __device__ __forceinline__ f4 sum4(const float* s0, int64_t step, int pieces, in
     return s;
 }
 
+// A pair of numbers to two fp16 numbers each: hi the largest below it in magnitude, lo the rest rounded, both of at least
+// 2^-24 and of its sign (0 of 0).  NaN: hi NaN; infinite: hi infinite.  Magnitudes 0, or 2^-100 and up, to below 2^15.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float v[2] = {__builtin_fabsf(a), __builtin_fabsf(b)};
+    float least[2], low[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        least[i] = __builtin_fminf(v[i] * 0x1p100f, 0x1p-24f);
+        const float cut = v[i] * (1.f - 0x1p-24f);                         // (the fp32 number below)
+        low[i] = cut < least[i] ? least[i] : cut;
+    }
+    const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(low[0], low[1]));
+#pragma unroll
+    for (int i = 0; i < 2; i++) low[i] = __builtin_fmaxf(v[i] - (float)h[i], least[i]);   // (an infinity's rest: the least)
+    const uint32_t sign = (__builtin_bit_cast(uint32_t, a) >> 16 & 0x8000u) | (__builtin_bit_cast(uint32_t, b) & 0x80000000u);
+    hi = as_u32(h) | sign;
+    lo = as_u32(h2{(_Float16)low[0], (_Float16)low[1]}) | sign;
+}
+
 // A row's sums, fours of ranks by PER neighbouring lanes in turn (this one `me`), to
 // two fp16 numbers each, times 2^shift: put(k, hi, lo) of ranks k .. k + 3, k below
 // `padded`.  Returns the shift.
@@ -405,15 +426,10 @@ __device__ __forceinline__ int split_row(const float* s0, int64_t step, int piec
     const float up = __builtin_ldexpf(1.f, shift);
     for (int i = 0, k = 4 * me; k < padded; k += 4 * PER, i++) {
         const f4 s = i == 0 ? held[0] : i == 1 ? held[1] : sum4(s0, step, pieces, k, ranks);
-        _Float16 h[4], l[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float v = s[j] * up;
-            h[j] = (_Float16)v;
-            const float rest = v - (float)h[j];
-            l[j] = (_Float16)(rest == rest ? rest : 0.f);                  // (an infinity has no rest)
-        }
-        put(k, uint2{as_u32(h2{h[0], h[1]}), as_u32(h2{h[2], h[3]})}, uint2{as_u32(h2{l[0], l[1]}), as_u32(h2{l[2], l[3]})});
+        uint2 hi, lo;
+        split2(s[0] * up, s[1] * up, hi.x, lo.x);
+        split2(s[2] * up, s[3] * up, hi.y, lo.y);
+        put(k, hi, lo);
     }
     return shift;
 }

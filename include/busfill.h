@@ -586,7 +586,8 @@ bf_status bf_rms_norm(const bf_rms_norm_args* args, void* stream);
  * Columns of no part are left alone.  ranks[e] (cut to 0 .. rank) says how many of
  * the `rank` rows of A[e] and columns of B[e] are used; the others may hold
  * anything.  Rows come in any order, each with any adapter.  Inner sums are fp32 and
- * enter the second product to 2^-22 of the row's largest; Y is rounded once. */
+ * enter the second product to 2^-22 of the row's largest; Y is rounded once.
+ * Infinities and NaN of X, A, B and C are those of the formula in Y. */
 typedef struct {
     const uint16_t* A;       /* [adapters][rank][K] fp16 */
     const uint16_t* B;       /* [adapters][N][rank] fp16 */
