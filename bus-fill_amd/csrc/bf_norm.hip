@@ -14,7 +14,7 @@
 // (4.6 TB/s; a copy of 2 GiB reaches 4.9); 32 rows 4.0 us in the kernel and 4.8 to 5.0 a
 // call from Python, 16 rows to int8 4.7 in the kernel: load, two barriers of a workgroup's
 // sums, store, and the launch.  Codes: one division a block and a product a value
-// (a division a value: 0.3 us more).
+// (a division a value: 0.3 us more), with a division for those near half way.
 #include <atomic>
 
 #include "bf_device.h"
@@ -76,13 +76,22 @@ __device__ __forceinline__ Factor factor(float ss, int K, float eps, V values, i
     return f;
 }
 
-// One value's code; dd the block's scale (0: all zero; not finite: codes 0), inv its reciprocal (one division a block; where
-// that or dd is not normal, one a value).
-__device__ __forceinline__ float reciprocal(float dd) { return dd >= 0x1p-125f && dd < 0x1p125f ? 1.f / dd : 0.f; }
-__device__ __forceinline__ int code(float y, float dd, float inv) {
-    float q = y * inv;
-    if (inv == 0.f) q = dd > 0.f && dd < __builtin_inff() ? y / dd : 0.f;
-    return (int)__builtin_fminf(__builtin_fmaxf(__builtin_roundf(q), -127.f), 127.f);
+// Codes of N values of a block whose scale is dd (0: all zero; not finite: codes 0).  One division a block, and one a value
+// where some value of a lane is next to half way between two codes (its product with the reciprocal is within 2^-15 of the
+// rounded quotient, whose code counts) or where dd or its reciprocal is not normal.
+template <int N> __device__ __forceinline__ void codes(int (&q)[N], const float (&y)[N], float dd) {
+    const float inv = dd >= 0x1p-125f && dd < 0x1p125f ? 1.f / dd : 0.f;
+    float v[N], near = 1.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        v[e] = y[e] * inv;
+        near = __builtin_fminf(near, __builtin_fabsf(__builtin_amdgcn_fractf(v[e]) - 0.5f));
+    }
+    if (near < 0x1p-14f || inv == 0.f)
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = dd > 0.f && dd < __builtin_inff() ? y[e] / dd : 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = (int)__builtin_fminf(__builtin_fmaxf(__builtin_roundf(v[e]), -127.f), 127.f);
 }
 
 __device__ __forceinline__ float load1(const void* p, int f16, int64_t i) {
@@ -164,13 +173,11 @@ __global__ __launch_bounds__(1024) void k_rms_norm(NormDev p) {
             m = __builtin_fmaxf(m, __shfl_xor(m, 2));
             bad += __shfl_xor(bad, 1);
             bad += __shfl_xor(bad, 2);
-            const float dd = m / 127.0f + bad, inv = reciprocal(dd);
+            const float dd = m / 127.0f + bad;
             int q[8], sum = 0;
+            codes(q, y, dd);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                q[e] = code(y[e], dd, inv);
-                sum += q[e];
-            }
+            for (int e = 0; e < 8; e++) sum += q[e];
             sum += __shfl_xor(sum, 1);
             sum += __shfl_xor(sum, 2);
             if (live) {
@@ -225,7 +232,10 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(NormDev p) {
                 bad += __shfl_xor(bad, x);
             }
             const float dd = m / 127.0f + bad;
-            const int q = code(y, dd, reciprocal(dd));
+            const float v[1] = {y};
+            int qs[1];
+            codes(qs, v, dd);
+            const int q = qs[0];
             int sum = q;
 #pragma unroll
             for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor(sum, x);
