@@ -892,7 +892,8 @@ template <int RC> hipError_t both(const LoraArgs& a, const LoraPlan& p, float* w
     return a.out_f16 ? up<RC, true>(a, p, ws, st) : up<RC, false>(a, p, ws, st);
 }
 
-LoraPlan plan_of(const LoraArgs& a) { return plan_lora(a, device_cus() > 0 ? device_cus() : 256); }
+int cus() { return device_cus() > 0 ? device_cus() : 256; }
+LoraPlan plan_of(const LoraArgs& a) { return plan_lora(a, cus()); }
 
 }  // namespace
 
@@ -901,7 +902,7 @@ bool lora_fits(const LoraArgs& a) {
     return launch_fits(p.down.groups, 64 * kLoraManyWaves) && launch_fits(p.up.groups, 64 * kLoraUpWaves) && launch_fits(a.T, 16);
 }
 
-size_t lora_scratch_bytes(const LoraArgs& a) { return plan_of(a).bytes; }
+size_t lora_scratch_bytes(const LoraArgs& a) { return lora_reserve(a, plan_of(a), cus()); }
 
 hipError_t lora(const LoraArgs& a, float* ws, hipStream_t st) {
     const LoraPlan p = plan_of(a);

@@ -150,6 +150,20 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
     return p;
 }
 
+// Bytes of workspace that a call takes hold of: never fewer than one of fewer rows with the same adapters, ranks, parts and K
+// needs, so that the largest call's workspace serves all.  (More rows have fewer pieces of K, and so may need less themselves.)
+// Of few rows, pieces rows <= rows or <= 2 cus rows / (tiles rank_parts parts sharers), where rows / (tiles sharers) is at most
+// 16 / min(16, adapters); of many, rows or 2 cus rows / (tiles rank_parts parts), rows / tiles at most 64.
+inline size_t lora_reserve(const LoraArgs& a, const LoraPlan& p, int cus) {
+    const auto most = [&](int least, int64_t shared) {
+        return std::max<int64_t>(a.T, std::min(std::max<int64_t>(1, std::min(kLoraPieces, a.K / least)) * a.T, shared));
+    };
+    const int64_t each = (int64_t)p.rank_parts * a.parts;
+    int64_t rows = most(2 * kLoraDownWaves * kLoraUnit, 2 * cus * kLoraSub / (each * std::min(kLoraSub, a.adapters)));
+    if (p.many) rows = std::max(rows, most(kLoraSlab, 2 * cus * 4 * kLoraSub / each));
+    return p.bytes + (size_t)a.parts * a.rank * (rows - (int64_t)p.pieces * a.T) * sizeof(float);
+}
+
 // LDS rows of the inner sums (two planes of fp16): whole steps of 32, 16 bytes past a multiple of 64.
 constexpr int lora_lds_ranks(int rank) { return (rank + kLoraStep - 1) / kLoraStep * kLoraStep + 8; }
 

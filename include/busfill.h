@@ -610,7 +610,8 @@ typedef struct {
     int T, K;                /* K a multiple of 8; X rows, A and B 16-byte aligned */
 } bf_lora_args;
 /* The inner sums live in the library's workspace for the stream, or in the
- * caller's (_ws, as bf_gemm_ws). */
+ * caller's (_ws, as bf_gemm_ws).  Its size never falls as T grows with the rest
+ * the same: what serves T rows serves fewer. */
 bf_status bf_lora(const bf_lora_args* args, void* stream);
 size_t bf_lora_workspace_bytes(const bf_lora_args* args);
 bf_status bf_lora_ws(const bf_lora_args* args, void* workspace, size_t workspace_bytes, void* stream);
