@@ -103,8 +103,11 @@ inline Kv4Plan plan_kv4(const Kv4Args& a, int cus) {
         const int64_t span = std::min<int64_t>(a.max_q, (p.tile_rows + p.group - 2) / p.group + 1);
         seen = std::min<int64_t>(seen, (int64_t)a.window + span - 1);
     }
-    const int64_t most = std::max<int64_t>(1, (seen + (a.window > 0 ? 2 : 1) * (kKv4Tile - 1)) / kKv4Tile) +   // (a window may start inside a tile)
-                         (std::min(a.sinks, a.max_kv) + kKv4Tile - 1) / kKv4Tile;
+    int64_t most = std::max<int64_t>(1, (seen + (a.window > 0 ? 2 : 1) * (kKv4Tile - 1)) / kKv4Tile);   // (a window may start inside a tile)
+    // first tokens' tiles, but no more in all than there are
+    if (a.sinks > 0)
+        most = std::max(most, std::min(most + (std::min<int64_t>(a.sinks, a.max_kv) + kKv4Tile - 1) / kKv4Tile,
+                                       ((int64_t)a.max_kv + kKv4Tile - 1) / kKv4Tile));
     p.items = (int64_t)a.S * p.row_tiles;
     const int64_t units = p.items * a.c.heads, places = (int64_t)cus * (a.c.dim == 256 ? 2 : kKv4PerCu);
     const int64_t share = std::max<int64_t>(1, cus / units), fill = (most + share - 1) / share;
