@@ -77,22 +77,27 @@ __device__ __forceinline__ Factor factor(float ss, int K, float eps, V values, i
     return f;
 }
 
-// Codes of N values of a block whose scale is dd (0: all zero; not finite: codes 0).  One division a block, and one a value
-// where some value of a lane is next to half way between two codes (its product with the reciprocal is within 2^-15 of the
-// rounded quotient, whose code counts) or where dd or its reciprocal is not normal.
-template <int N> __device__ __forceinline__ void codes(int (&q)[N], const float (&y)[N], float dd) {
+// A value's code: its quotient by the block's scale (0: all zero; not finite: codes 0), rounded.
+__device__ __forceinline__ float quotient(float y, float dd) { return dd > 0.f && dd < __builtin_inff() ? y / dd : 0.f; }
+__device__ __forceinline__ int code(float v) {
+    return (int)__builtin_fminf(__builtin_fmaxf(__builtin_roundf(v), -127.f), 127.f);
+}
+// Codes of a lane's eight values.  One division a block, and one a value where one of them is next to half way between two
+// codes (its product with the reciprocal is within 2^-15 of the rounded quotient, whose code counts) or where dd or its
+// reciprocal is not normal.
+__device__ __forceinline__ void codes(int (&q)[8], const float (&y)[8], float dd) {
     const float inv = dd >= 0x1p-125f && dd < 0x1p125f ? 1.f / dd : 0.f;
-    float v[N], near = 1.f;
+    float v[8], near = 1.f;
 #pragma unroll
-    for (int e = 0; e < N; e++) {
+    for (int e = 0; e < 8; e++) {
         v[e] = y[e] * inv;
         near = __builtin_fminf(near, __builtin_fabsf(__builtin_amdgcn_fractf(v[e]) - 0.5f));
     }
     if (near < 0x1p-14f || inv == 0.f)
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] = dd > 0.f && dd < __builtin_inff() ? y[e] / dd : 0.f;
+        for (int e = 0; e < 8; e++) v[e] = quotient(y[e], dd);
 #pragma unroll
-    for (int e = 0; e < N; e++) q[e] = (int)__builtin_fminf(__builtin_fmaxf(__builtin_roundf(v[e]), -127.f), 127.f);
+    for (int e = 0; e < 8; e++) q[e] = code(v[e]);
 }
 
 __device__ __forceinline__ float load1(const void* p, int f16, int64_t i) {
@@ -237,10 +242,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(NormDev p) {
                 bad += __shfl_xor(bad, x);
             }
             const float dd = m / 127.0f + bad;
-            const float v[1] = {y};
-            int qs[1];
-            codes(qs, v, dd);
-            const int q = qs[0];
+            const int q = code(quotient(y, dd));
             int sum = q;
 #pragma unroll
             for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor(sum, x);
