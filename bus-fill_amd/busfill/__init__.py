@@ -635,13 +635,13 @@ _dtypes = {}
 
 
 def _dtype(t) -> int:
-    """F32 or F16 of a tensor (of None: F32)."""
+    """F32 or F16 of a tensor (of None: F32), -1 of one of another type or of an address: the library refuses that."""
     if t is None:
         return F32
     if not _dtypes:
         import torch
         _dtypes.update({torch.float32: F32, torch.float16: F16})
-    return _dtypes[t.dtype]
+    return _dtypes.get(getattr(t, "dtype", None), -1)
 
 
 def rms_norm(X, T: int, K: int, *, H=None, Aq=None, delta=None, R=None, weight=None, offset: float = 0.0, eps: float = 1e-6,
