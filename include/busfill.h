@@ -586,7 +586,9 @@ bf_status bf_rms_norm(const bf_rms_norm_args* args, void* stream);
  * Columns of no part are left alone.  ranks[e] (cut to 0 .. rank) says how many of
  * the `rank` rows of A[e] and columns of B[e] are used; the others may hold
  * anything.  Rows come in any order, each with any adapter.  Inner sums are fp32 and
- * enter the second product to 2^-22 of the row's largest; Y is rounded once.
+ * enter the second product to 2^-22 of the row's largest, its products are held and
+ * summed as fp32 (those of an element of B below 2^-14 only as exactly as those of
+ * 2^-14: they may lose up to 10 bits); Y is rounded once.
  * Infinities and NaN of X, A, B and C are those of the formula in Y. */
 typedef struct {
     const uint16_t* A;       /* [adapters][rank][K] fp16 */
