@@ -18,7 +18,7 @@ constexpr int kLoraRanks = 64;                     // ranks of a workgroup of th
 constexpr int kLoraCols = 64;                      // columns of a wave of the up products
 constexpr int kLoraStep = 32;                      // k of a matrix instruction
 constexpr int kLoraUnit = 64;                      // few rows: k of a row that comes to LDS at once (128 bytes)
-constexpr int kLoraSlab = 320;                     // many rows: ... of A's rows
+constexpr int kLoraSlab = 320;                     // many rows: ... of A's rows (two of 64 ranks take 80 KB: two workgroups a CU)
 constexpr int kLoraPieces = 8;                     // pieces of K at most
 constexpr int kLoraXcds = 8;                       // (a launch's workgroups go round them)
 constexpr int kLoraDownWaves = 4;                  // of a workgroup of the down products of few rows
@@ -127,8 +127,10 @@ inline LoraPlan plan_lora(const LoraArgs& a, int cus) {
     const int64_t base = (int64_t)t * p.rank_parts * a.parts * p.sharers;
     // at least two units a wave, or a slab
     const int64_t least = p.many ? kLoraSlab : 2 * kLoraDownWaves * kLoraUnit, most = std::min<int64_t>(kLoraPieces, a.K / least);
-    // few: two workgroups a CU; many: one, with as many short tiles as a handful of adapters make, or two where that leaves one
-    // piece (2000 rows of six adapters, rank 64: 6 pieces 34.3 us, 8, which are more workgroups than CUs, 38.5; 4000: 3 pieces 47, 8 54)
+    // few: two workgroups a CU; many: one, with as many short tiles as a handful of adapters make (how many there are the host does
+    // not know), or two where that leaves one piece (2000 rows of six adapters, rank 64: 6 pieces 34.3 us, 8, which are more workgroups
+    // than CUs, 38.5; 4000: 3 pieces 47, 8 54.  64 adapters in no order make up to 96 tiles of those 2000 rows, with 6 pieces
+    // each still: not measured otherwise)
     const int64_t one = p.many ? cus / (base + 8) : 0;
     p.pieces = (int)std::min(std::max<int64_t>(1, most), one >= 2 ? one : std::max<int64_t>(1, 2 * cus / base));
     p.down = lora_grid(p.most, (int64_t)p.rank_parts * a.parts * p.sharers * p.pieces);

@@ -37,8 +37,10 @@
  *         from other host threads keep valid memory.  Nothing is allocated
  *         while the stream is being captured into a graph: a call that would
  *         need to returns BF_ERR_UNSUPPORTED and enqueues nothing; make one
- *         uncaptured call of the largest shape on the stream first, or use a
- *         caller-owned workspace.  The one-launch feed-forward block
+ *         uncaptured call of each shape on the stream first, or use a
+ *         caller-owned workspace.  (A larger shape may need less: attention over
+ *         more sequences is cut into fewer chunks.  Of bf_lora, the call of the
+ *         most rows serves all.)  The one-launch feed-forward block
  *         (bf_ffn_swiglu_ex, BF_FFN_ONE_LAUNCH) keeps its hand-over words in
  *         the same workspace.  A captured graph holds the buffer of the
  *         stream it was captured on: replaying it while other exchanging work
@@ -472,7 +474,9 @@ bf_status bf_kv4_load(const bf_kv4_cache* cache, const int64_t* slots, uint16_t*
  * upper bounds of the queries of a sequence and of kv_len (larger ones are cut
  * to them); max_kv <= ldt page_size.  Rows of no sequence are left alone.
  * The arrays q_start, kv_len and page_table are device memory: nothing is read
- * back, so a captured call serves every length up to max_kv. */
+ * back, so a captured call serves every length up to max_kv.  Scores, maxima,
+ * probabilities and sums are fp32; a probability times the scale of 32 values is
+ * rounded once to fp16 (2^-11) for the second product. */
 typedef struct {
     const uint16_t* Q;       /* [T][ldq] fp16, head h at column h head_dim; rows 16-byte aligned */
     int64_t ldq;
@@ -518,7 +522,7 @@ typedef enum { BF_ROPE_HALVES = 0, BF_ROPE_PAIRS = 1 } bf_rope;
  * the i-th pair (x, y) of each head becomes
  *   (x cos t - y sin t, y cos t + x sin t) factor,  t = positions[token] freq[i] radians,
  * in fp32, rounded once to fp16 (t to 2^-20 of a turn for positions up to 2^31
- * either way); elements from rot on stay as they are.  Rotated queries go to
+ * either way and frequencies up to 2 pi); elements from rot on stay as they are.  Rotated queries go to
  * Q_out, rotated keys to the cache (as bf_kv4_store of the fp16 rows, bit for bit)
  * and, where K_out is given, there too; every row is rotated, whatever its slot.
  * Q_out may be Q and K_out K (the same rows); other overlaps are not allowed. */
