@@ -111,3 +111,20 @@ def test_an_infinity_meets_a_sum_far_below_the_largest(T):
     want, size = formula(x.half(), a.half(), b.half(), c, ids, scales)
     assert (want[::2, 3:] == INF).all() and (want[1::2, 3:] == -INF).all() and torch.isfinite(want[:, :3]).all()
     check(call(x.half(), a.half(), b.half(), c, ids, scales), want, size, rank)
+
+
+@pytest.mark.parametrize("rank", [16, 72])
+@pytest.mark.parametrize("T", [20, 300])
+def test_infinite_sums_and_the_smallest_b(T, rank):
+    """An infinity of X times a B of 2^-24 or of 65504, and of 0 (NaN); a scale of 0 (NaN)."""
+    x = torch.ones(T, 8)
+    x[::2, 0], x[1::4, 0] = INF, -INF
+    a, b = torch.ones(2, rank, 8), torch.ones(2, 40, rank)
+    b[:, ::4], b[:, 1::4], b[:, 2::4] = 2.0 ** -24, -(2.0 ** -24), 65504.0
+    b[:, 3::8, rank - 1] = 0.0
+    ids = (torch.arange(T) % 3 == 1).int()
+    scales = torch.tensor([2.0, 0.0])
+    c = torch.randn(T, 40, generator=torch.Generator().manual_seed(T))
+    want, size = formula(x.half(), a.half(), b.half(), c, ids, scales)
+    assert torch.isinf(want).any() and torch.isnan(want).any() and torch.isfinite(want).any()
+    check(call(x.half(), a.half(), b.half(), c, ids, scales), want, size, rank)
