@@ -960,8 +960,7 @@ bf_status take_workspace(const char* who, size_t bytes, const bf::Scratch* scrat
     const hipError_t e = bf::split_workspace(scratch, hs, 0, bytes, &counters, out);
     if (e == hipErrorStreamCaptureUnsupported)
         return fail(BF_ERR_UNSUPPORTED, "%s: the workspace for this stream is allocated on first use, which cannot happen "
-                                        "during stream capture; make one uncaptured call of this size (or a larger one) on the "
-                                        "stream first", who);
+                                        "during stream capture; make one uncaptured call of this shape on the stream first", who);
     return from_hip(e, who);
 }
 
